@@ -274,6 +274,62 @@ int moe_q2_grouped_switch_glu(const void* x, int n_tokens, const int32_t* row_to
 int moe_pair_combine(const void* y, const void* scores, const void* residual, int n_tokens, int k,
                      int hidden, float* out, void* stream);
 
+/* ---- Part 2b: unquantised experts and adapters (no counterpart in the reference) ------------ */
+/* The reference multiplies 2-bit experts only (prefill_qproj.py:18-40); these are its sorted products
+ * for fp16 or bf16 weights (dtype 0 or 1, inputs, weights and outputs alike), with their gradients, the
+ * row plan they take, and low-rank adapters.  Pointers are device memory, 16-byte aligned; ld* are
+ * elements from row to row and *_stride elements from matrix to matrix, both multiples of 8, as all row
+ * lengths are; within a matrix rows follow each other.  Row numbers and sizes are 32-bit, offsets
+ * 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).  Nothing is allocated,
+ * kept between calls or synchronised.  Sums are fp32, rounded once. */
+
+/* The rows of a batch sorted by expert, as prefill.resident_plan (loader.py:583-591) makes them on the
+ * host: ids i32 [n_ids], pair p = token * k + j.  Sorted row r is pair row_out[r] of token row_token[r];
+ * expert e's rows are seg_start[e] .. seg_start[e + 1] - 1 (seg_start: n_exp + 1 entries) in the order
+ * of their pairs.  Pairs whose id is outside 0 .. n_exp - 1 come behind the last segment, in order.
+ * n_exp in 1..1024, n_ids a multiple of k. */
+int moe_expert_plan(const int32_t* ids, int n_ids, int k, int n_exp, int32_t* row_token, int32_t* row_out,
+                    int32_t* seg_start, void* stream);
+/* y[row_out[r]] = scale[u] W_u x[row_in[r]] for the rows r of segment u: seg_start[u] .. seg_start[u + 1]
+ * - 1, W_u [n][k] = w + seg_slot[u] * w_stride (seg_slot null: u), scale fp32 per slot or null; row_in /
+ * row_out null: row r.  n_seg in 0..1024.  A row_in outside x gives a row of zeros; a row_out outside y
+ * is not written.  Rows of no segment, and of one whose slot is outside 0 .. n_slots - 1, are written as
+ * zeros if fill != 0 and left as they are if not. */
+int moe_grouped_mm(const void* x, int64_t ldx, int n_x, const int32_t* row_in, const int32_t* seg_start,
+                   const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots, int n,
+                   int k, const float* scale, void* y, int64_t ldy, int n_y, const int32_t* row_out, int dtype, int fill,
+                   void* stream);
+/* h[r] = silu(g) * u with (g, u) = W x[row_in[r]], W [2 * inter][hidden]: inter gate rows, then inter up
+ * rows.  gu (or null): receives (g, u), [n_rows][2 * inter], for moe_grouped_mm_dx.  Other arguments as
+ * moe_grouped_mm; h and gu have row r at r. */
+int moe_grouped_gate_up(const void* x, int64_t ldx, int n_x, const int32_t* row_in, const int32_t* seg_start,
+                        const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots,
+                        int inter, int hidden, void* h, int64_t ldh, void* gu, int64_t ldgu, int dtype, int fill,
+                        void* stream);
+/* dx[row_out[r]] = scale[u] W_u^T dy[row_in[r]], W_u [n][k]: the gradient of moe_grouped_mm in x, with
+ * row_in and row_out in each other's place (a row of x that several rows read gets their sum from the
+ * caller).  gu != null: W_u's input was moe_grouped_gate_up's h (k = inter) and dx [..][2 * k] receives
+ * the gradient of (g, u) instead; gu has sorted row r at r. */
+int moe_grouped_mm_dx(const void* dy, int64_t lddy, int n_dy, const int32_t* row_in, const int32_t* seg_start,
+                      const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots, int n,
+                      int k, const float* scale, const void* gu, int64_t ldgu, void* dx, int64_t lddx, int n_dx,
+                      const int32_t* row_out, int dtype, int fill, void* stream);
+/* dw + u * dw_stride [n][k] = scale[u] * sum over the rows r of segment u of dy[row_dy[r]] x[row_x[r]]^T:
+ * the gradient of moe_grouped_mm in the weights, for every segment (zeros where it has no rows), fp32 if
+ * out_f32 != 0.  Rows whose row_dy or row_x is outside dy or x add nothing. */
+int moe_grouped_mm_dw(const void* dy, int64_t lddy, int n_dy, const int32_t* row_dy, const void* x, int64_t ldx, int n_x,
+                      const int32_t* row_x, const int32_t* seg_start, int n_seg, int n_rows, int n, int k,
+                      const float* scale, void* dw, int64_t dw_stride, int out_f32, int dtype, void* stream);
+/* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scale[i] B_i (A_i x[t]),
+ * i = ids[t]; A_i [rank][n_in] = a + i * a_stride, B_i [n_out][rank] = b + i * b_stride, scale fp32 per
+ * adapter or null.  An id outside 0 .. n_ad - 1 gives out[t] = base[t].  out may be base.  rank: a
+ * multiple of 8 up to 256.  workspace: moe_lora_workspace_bytes bytes, any contents, one per call in
+ * flight. */
+uint64_t moe_lora_workspace_bytes(int n_tok, int rank);
+int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, const void* a, int64_t a_stride,
+                 const void* b, int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in,
+                 int n_out, int rank, int dtype, void* workspace, void* out, int64_t ld_out, void* stream);
+
 /* 2-bit codebook experts: the Nemotron model of README.md:37 (IQ2_XXS GGUF, 240 experts, top-9),
  * run by the reference only inside llama.cpp's Metal backend (llama-moe-cache.patch:1-12 adds the
  * mul_mm_id map for 9 experts per token; format in csrc/moe_common.h CbLayout): non-gated up ->

@@ -16,6 +16,7 @@ SRC_DIR = PKG_DIR.parent
 
 _c_int, _c_u32, _c_i32, _c_u64, _c_f, _c_vp = (ctypes.c_int, ctypes.c_uint32, ctypes.c_int32,
                                               ctypes.c_uint64, ctypes.c_float, ctypes.c_void_p)
+_c_i64 = ctypes.c_int64
 _u32p, _i32p, _u64p = (ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_int32),
                        ctypes.POINTER(ctypes.c_uint64))
 
@@ -105,6 +106,20 @@ SIGNATURES: dict[str, tuple] = {
     "moe_cb_moe_norm": (_c_int, [_c_vp, _c_vp, _c_f, _c_vp, _c_vp, _c_u64, _c_int, _c_vp, _c_vp, _c_int,
                                  _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
     "moe_pair_combine": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    # unquantised experts and adapters
+    "moe_expert_plan": (_c_int, [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "moe_grouped_mm": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64, _c_int, _c_int,
+                                _c_int, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_int, _c_vp]),
+    "moe_grouped_gate_up": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64, _c_int,
+                                     _c_int, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_int, _c_vp]),
+    "moe_grouped_mm_dx": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64, _c_int,
+                                   _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_int,
+                                   _c_vp]),
+    "moe_grouped_mm_dw": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_int, _c_int,
+                                   _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_vp]),
+    "moe_lora_workspace_bytes": (_c_u64, [_c_int, _c_int]),
+    "moe_lora_add": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_int,
+                              _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp]),
     # no reference counterpart
     "c_last_error": (ctypes.c_char_p, []),
     "c_clear_error": (None, []),

@@ -203,3 +203,323 @@ def cb_up(x, pool, slots, grid, hidden, inter, h_out=None):
                               _p(h_out), _stream())
     _lib.check(rc, "moe_cb_up")
     return h_out
+
+
+# ---- unquantised experts (fp16 / bf16): sorted rows, their products and gradients ---------------
+
+_HALF = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_gpu(who: str, **tensors) -> torch.device:
+    """The one GPU that every given tensor is on."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{who}: {name} must be a tensor, not {type(t).__name__}")
+        _need(t.is_cuda, f"{who}: {name} is on {t.device}, not on a GPU")
+        _need(dev is None or t.device == dev, f"{who}: {name} is on {t.device}, others on {dev}")
+        dev = t.device
+    return dev
+
+
+def _rows(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, width: int | None) -> int:
+    """Checks a matrix with contiguous rows; returns the elements from row to row."""
+    if t.dtype != dtype:
+        raise TypeError(f"{who}: {name} is {t.dtype}, not {dtype}")
+    _need(t.dim() == 2 and (rows is None or t.shape[0] == rows) and (width is None or t.shape[1] == width),
+          f"{who}: {name} has shape {tuple(t.shape)}, not ({'*' if rows is None else rows}, {'*' if width is None else width})")
+    _need(t.shape[1] % 8 == 0 and t.shape[1] > 0, f"{who}: {name}: rows of {t.shape[1]} elements (a multiple of 8 wanted)")
+    _need(t.stride(1) == 1 or t.numel() == 0, f"{who}: {name}'s rows are not contiguous")
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    _need(t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0, f"{who}: {name}'s rows are {t.stride(0)} elements apart")
+    return t.stride(0)
+
+
+def _mats(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> int:
+    """Checks a stack of contiguous matrices; returns the elements from one to the next."""
+    if t.dtype != dtype:
+        raise TypeError(f"{who}: {name} is {t.dtype}, not {dtype}")
+    _need(t.dim() == 3 and all(s is None or s == d for s, d in zip(shape, t.shape)),
+          f"{who}: {name} has shape {tuple(t.shape)}, not {tuple('*' if s is None else s for s in shape)}")
+    n, k = t.shape[1:]
+    _need(n > 0 and n % 8 == 0 and k > 0 and k % 8 == 0, f"{who}: {name}: matrices of {n} x {k} (multiples of 8 wanted)")
+    _need(t.numel() == 0 or (t.stride(2) == 1 and t.stride(1) == k), f"{who}: {name}'s matrices are not contiguous")
+    if t.shape[0] <= 1:
+        return n * k
+    _need(t.stride(0) >= n * k and t.stride(0) % 8 == 0, f"{who}: {name}'s matrices are {t.stride(0)} elements apart")
+    return t.stride(0)
+
+
+def _index(who: str, name: str, t: torch.Tensor | None, n: int | None = None) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.int32:
+        raise TypeError(f"{who}: {name} is {t.dtype}, not torch.int32")
+    _need(t.is_contiguous() and (n is None or t.numel() == n), f"{who}: {name} must be contiguous" +
+          ("" if n is None else f" with {n} entries, not {t.numel()}"))
+
+
+def _scale(who: str, t: torch.Tensor | None, n: int) -> None:
+    if t is None:
+        return
+    if t.dtype != torch.float32:
+        raise TypeError(f"{who}: scale is {t.dtype}, not torch.float32")
+    _need(t.is_contiguous() and t.numel() == n, f"{who}: scale must be contiguous with {n} entries")
+
+
+def _half(who: str, t: torch.Tensor) -> int:
+    if t.dtype not in _HALF:
+        raise TypeError(f"{who}: {t.dtype} (torch.float16 and torch.bfloat16 are supported)")
+    return _HALF[t.dtype]
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """Calls an entry point on the tensors' own GPU and its current stream."""
+    with torch.cuda.device(dev):
+        rc = getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, name)
+
+
+def _fresh_rows(n_out_rows: int | None, n_rows: int, width: int, like: torch.Tensor) -> torch.Tensor:
+    """A new output.  With a row for each sorted row the kernels write all of them themselves."""
+    make = torch.empty if n_out_rows is None else torch.zeros
+    return make((n_rows if n_out_rows is None else n_out_rows, width), dtype=like.dtype, device=like.device)
+
+
+def expert_plan(ids: torch.Tensor, n_exp: int, row_token: torch.Tensor | None = None, row_out: torch.Tensor | None = None,
+                seg_start: torch.Tensor | None = None):
+    """The row plan of prefill.resident_plan, made on the GPU: the (token, k) pairs sorted by expert.
+
+    ids: int32 [n_tok, k] (or [n_tok]: k = 1).  Returns int32 (row_token [M], row_out [M], seg_start
+    [n_exp + 1]): sorted row r is pair row_out[r] (= token * k + j) of token row_token[r]; expert e has
+    rows seg_start[e]:seg_start[e + 1], in pair order.  One segment per expert, empty ones too, so the
+    slot is the expert id and no seg_slot is needed.  Pairs with an id outside 0 .. n_exp - 1 come
+    behind the last segment.  n_exp up to 1024.
+    """
+    dev = _on_gpu("expert_plan", ids=ids, row_token=row_token, row_out=row_out, seg_start=seg_start)
+    _index("expert_plan", "ids", ids)
+    _need(ids.dim() in (1, 2), f"expert_plan: ids has {ids.dim()} dimensions")
+    k = ids.shape[1] if ids.dim() == 2 else 1
+    m = ids.numel()
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
+    row_token = row_token if row_token is not None else new(m)
+    row_out = row_out if row_out is not None else new(m)
+    _need(1 <= n_exp <= 1024, f"expert_plan: n_exp={n_exp} (1..1024)")
+    seg_start = seg_start if seg_start is not None else new(n_exp + 1)
+    for name, t, n in (("row_token", row_token, m), ("row_out", row_out, m), ("seg_start", seg_start, n_exp + 1)):
+        _index("expert_plan", name, t, n)
+    _call("moe_expert_plan", dev, _p(ids), m, max(k, 1), n_exp, _p(row_token), _p(row_out), _p(seg_start))
+    return row_token, row_out, seg_start
+
+
+def _segments(who, seg_start, seg_slot):
+    _index(who, "seg_start", seg_start)
+    _need(1 <= seg_start.numel() <= 1025, f"{who}: seg_start has {seg_start.numel()} entries (1..1025)")
+    n_seg = seg_start.numel() - 1
+    _index(who, "seg_slot", seg_slot, n_seg)
+    return n_seg
+
+
+def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_slot=None, scale=None, out=None):
+    """y[row_out[r]] = scale[s] * (w[s] @ x[row_in[r]]) for rows r sorted into segments, s the segment's slot.
+
+    x: fp16 or bf16 [*, K]; w: same type [n_slots, N, K]; segment u is rows seg_start[u]:seg_start[u + 1]
+    with slot seg_slot[u] (u when None).  row_in / row_out None: row r.  The number of sorted rows is
+    row_in's or row_out's, else x's.  A new output has n_out_rows rows, or as many as there are sorted rows
+    (row_out is then one place for each, as expert_plan's); rows of no segment, or of one whose slot is
+    outside w, are zeros in it and left as they are in a given `out`.  A row_in outside x gives a row of
+    zeros, a row_out outside the output is dropped.
+    """
+    who = "grouped_mm"
+    dev = _on_gpu(who, x=x, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, out=out)
+    dt = _half(who, x)
+    n_seg = _segments(who, seg_start, seg_slot)
+    w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
+    n_slots, N, K = w.shape
+    ldx = _rows(who, "x", x, x.dtype, None, K)
+    n_rows = row_in.numel() if row_in is not None else row_out.numel() if row_out is not None else x.shape[0]
+    _index(who, "row_in", row_in, n_rows)
+    _index(who, "row_out", row_out, n_rows)
+    _scale(who, scale, n_slots)
+    fill = out is None
+    if fill:
+        out = _fresh_rows(n_out_rows, n_rows, N, x)
+    _need(n_out_rows is None or out.shape[0] == n_out_rows, f"{who}: out has {out.shape[0]} rows, not {n_out_rows}")
+    ldy = _rows(who, "out", out, x.dtype, None, N)
+    _need((row_in is not None or n_rows <= x.shape[0]) and (row_out is not None or n_rows <= out.shape[0]),
+          f"{who}: {n_rows} sorted rows, x has {x.shape[0]} and out {out.shape[0]}")
+    _call("moe_grouped_mm", dev, _p(x), ldx, x.shape[0], _p(row_in), _p(seg_start), _p(seg_slot), n_seg, n_rows, _p(w),
+          w_stride, n_slots, N, K, _p(scale), _p(out), ldy, out.shape[0], _p(row_out), dt, int(fill))
+    return out
+
+
+def grouped_gate_up(x, row_token, seg_start, w, seg_slot=None, h_out=None, gu_out=None):
+    """h[r] = silu(g) * u, (g, u) = w[slot] @ x[row_token[r]], for rows sorted by expert (row_token None: row r).
+
+    x: fp16 or bf16 [n_tok, hidden]; w: same type [n_slots, 2 * inter, hidden], a slot's inter gate rows
+    before its inter up rows; seg_start, seg_slot as grouped_mm.  gu_out ([M, 2 * inter], optional)
+    receives (g, u) for grouped_mm_dx.  Returns [M, inter]; rows of no valid segment are zeros in a new
+    output and left as they are in a given one.
+    """
+    who = "grouped_gate_up"
+    dev = _on_gpu(who, x=x, row_token=row_token, seg_start=seg_start, w=w, seg_slot=seg_slot, h_out=h_out, gu_out=gu_out)
+    dt = _half(who, x)
+    n_seg = _segments(who, seg_start, seg_slot)
+    w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
+    n_slots, N, K = w.shape
+    _need(N % 16 == 0, f"{who}: w has {N} rows per slot: twice a multiple of 8 wanted")
+    ldx = _rows(who, "x", x, x.dtype, None, K)
+    M = row_token.numel() if row_token is not None else x.shape[0]
+    _index(who, "row_token", row_token, M)
+    fill = h_out is None
+    if fill:
+        h_out = torch.empty((M, N // 2), dtype=x.dtype, device=dev)
+    ldh = _rows(who, "h_out", h_out, x.dtype, M, N // 2)
+    ldgu = _rows(who, "gu_out", gu_out, x.dtype, M, N) if gu_out is not None else 0
+    _call("moe_grouped_gate_up", dev, _p(x), ldx, x.shape[0], _p(row_token), _p(seg_start), _p(seg_slot), n_seg, M, _p(w),
+          w_stride, n_slots, N // 2, K, _p(h_out), ldh, _p(gu_out), ldgu, dt, int(fill))
+    return h_out
+
+
+def grouped_switch_glu(x, row_token, seg_start, w_gate_up, w_down, row_out=None, n_out_rows=None, seg_slot=None, h_ws=None,
+                       out=None):
+    """Both projections of unquantised experts, as q2_grouped_switch_glu has them for 2-bit ones:
+    [n_out_rows, hidden] per-(token, k) SwitchGLU outputs, sorted row r written at row_out[r]."""
+    h = grouped_gate_up(x, row_token, seg_start, w_gate_up, seg_slot=seg_slot, h_out=h_ws)
+    return grouped_mm(h, seg_start, w_down, row_out=row_out, n_out_rows=n_out_rows, seg_slot=seg_slot, out=out)
+
+
+def grouped_mm_dx(dy, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_slot=None, scale=None, gu=None, out=None):
+    """dx[row_out[r]] = scale[s] * (w[s]^T @ dy[row_in[r]]): grouped_mm's gradient in x, one row per sorted row.
+
+    Where grouped_mm read x[a[r]] and wrote y[b[r]], this takes row_in=b and writes one row per sorted
+    row; rows of x read several times get the sum of theirs from the caller (row_out = the pairs' order,
+    then a sum over k).  gu: w's input was grouped_gate_up's h, and gu the (g, u) it kept, [M, 2 * K] in
+    sorted order; the result is then the gradient of (g, u), [*, 2 * K].  Other arguments as grouped_mm.
+    """
+    who = "grouped_mm_dx"
+    dev = _on_gpu(who, dy=dy, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, gu=gu,
+                  out=out)
+    dt = _half(who, dy)
+    n_seg = _segments(who, seg_start, seg_slot)
+    w_stride = _mats(who, "w", w, dy.dtype, (None, None, None))
+    n_slots, N, K = w.shape
+    width = K if gu is None else 2 * K
+    lddy = _rows(who, "dy", dy, dy.dtype, None, N)
+    n_rows = row_in.numel() if row_in is not None else row_out.numel() if row_out is not None else dy.shape[0]
+    _index(who, "row_in", row_in, n_rows)
+    _index(who, "row_out", row_out, n_rows)
+    _scale(who, scale, n_slots)
+    ldgu = _rows(who, "gu", gu, dy.dtype, n_rows, width) if gu is not None else 0
+    fill = out is None
+    if fill:
+        out = _fresh_rows(n_out_rows, n_rows, width, dy)
+    _need(n_out_rows is None or out.shape[0] == n_out_rows, f"{who}: out has {out.shape[0]} rows, not {n_out_rows}")
+    lddx = _rows(who, "out", out, dy.dtype, None, width)
+    _need((row_in is not None or n_rows <= dy.shape[0]) and (row_out is not None or n_rows <= out.shape[0]),
+          f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and out {out.shape[0]}")
+    _call("moe_grouped_mm_dx", dev, _p(dy), lddy, dy.shape[0], _p(row_in), _p(seg_start), _p(seg_slot), n_seg, n_rows,
+          _p(w), w_stride, n_slots, N, K, _p(scale), _p(gu), ldgu, _p(out), lddx, out.shape[0], _p(row_out), dt, int(fill))
+    return out
+
+
+def grouped_mm_dw(dy, x, seg_start, row_dy=None, row_x=None, scale=None, dtype=None, out=None):
+    """dw[u] = scale[u] * sum over the rows r of segment u of dy[row_dy[r]] (outer) x[row_x[r]]: [n_seg, N, K].
+
+    grouped_mm's gradient in the weights, one matrix per segment (zeros for an empty one; segments that
+    shared a slot are summed by the caller).  dtype: the inputs' (default) or torch.float32.  Where
+    grouped_mm took row_in and row_out, this takes row_x=row_in and row_dy=row_out.
+    """
+    who = "grouped_mm_dw"
+    dev = _on_gpu(who, dy=dy, x=x, seg_start=seg_start, row_dy=row_dy, row_x=row_x, scale=scale, out=out)
+    dt = _half(who, dy)
+    n_seg = _segments(who, seg_start, None)
+    lddy, ldx = _rows(who, "dy", dy, dy.dtype, None, None), _rows(who, "x", x, dy.dtype, None, None)
+    N, K = dy.shape[1], x.shape[1]
+    n_rows = row_dy.numel() if row_dy is not None else row_x.numel() if row_x is not None else dy.shape[0]
+    _index(who, "row_dy", row_dy, n_rows)
+    _index(who, "row_x", row_x, n_rows)
+    _need((row_dy is not None or n_rows <= dy.shape[0]) and (row_x is not None or n_rows <= x.shape[0]),
+          f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and x {x.shape[0]}")
+    _scale(who, scale, n_seg)
+    dtype = dtype if dtype is not None else out.dtype if out is not None else dy.dtype
+    if dtype not in (dy.dtype, torch.float32):
+        raise TypeError(f"{who}: gradients of {dy.dtype} come as {dy.dtype} or torch.float32, not {dtype}")
+    if out is None:
+        out = torch.empty((n_seg, N, K), dtype=dtype, device=dev)
+    stride = _mats(who, "out", out, dtype, (n_seg, N, K))
+    _call("moe_grouped_mm_dw", dev, _p(dy), lddy, dy.shape[0], _p(row_dy), _p(x), ldx, x.shape[0], _p(row_x), _p(seg_start),
+          n_seg, n_rows, N, K, _p(scale), _p(out), stride, int(dtype == torch.float32), dt)
+    return out
+
+
+# ---- low-rank adapters -------------------------------------------------------------------------
+
+def _lora_args(who, x, a, b, ids, scale):
+    dt = _half(who, x)
+    a_stride = _mats(who, "a", a, x.dtype, (None, None, x.shape[-1]))
+    n_ad, rank, n_in = a.shape
+    _need(rank <= 256, f"{who}: rank {rank} (up to 256)")
+    b_stride = _mats(who, "b", b, x.dtype, (n_ad, None, rank))
+    _index(who, "ids", ids, x.shape[0])
+    _scale(who, scale, n_ad)
+    return dt, n_ad, rank, n_in, b.shape[1], a_stride, b_stride
+
+
+def lora_add(base, x, a, b, ids, scale=None, out=None, workspace=None):
+    """out[t] = base[t] + scale[i] * (b[i] @ (a[i] @ x[t])), i = ids[t]: each token's own request's adapter
+    beside a projection that all share.
+
+    base: fp16 or bf16 [n_tok, n_out], the shared projection's output; x: same type [n_tok, n_in]; a [n_ad,
+    rank, n_in], b [n_ad, n_out, rank] (rank a multiple of 8 up to 256); ids: int32 [n_tok], an id outside
+    the adapters leaves base[t]; scale: fp32 [n_ad] or None.  out=base adds in place.  workspace: uint8
+    scratch of moe_lora_workspace_bytes, for callers that keep one per call in flight.
+    """
+    who = "lora_add"
+    dev = _on_gpu(who, base=base, x=x, a=a, b=b, ids=ids, scale=scale, out=out, workspace=workspace)
+    _need(x.dim() == 2, f"{who}: x has {x.dim()} dimensions")
+    dt, n_ad, rank, n_in, n_out, a_stride, b_stride = _lora_args(who, x, a, b, ids, scale)
+    n_tok = x.shape[0]
+    ldx = _rows(who, "x", x, x.dtype, n_tok, n_in)
+    ld_base = _rows(who, "base", base, x.dtype, n_tok, n_out)
+    if out is None:
+        out = torch.empty((n_tok, n_out), dtype=x.dtype, device=dev)
+    ld_out = _rows(who, "out", out, x.dtype, n_tok, n_out)
+    nb = 4 * n_tok * rank
+    if workspace is None:
+        workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _need(workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= nb,
+          f"{who}: workspace of {workspace.numel() * workspace.element_size()} bytes, {nb} wanted")
+    _call("moe_lora_add", dev, _p(base), ld_base, _p(x), ldx, _p(a), a_stride, _p(b), b_stride, _p(ids), _p(scale), n_tok,
+          n_ad, n_in, n_out, rank, dt, _p(workspace), _p(out), ld_out)
+    return out
+
+
+def lora_grad(dy, x, a, b, ids, scale=None):
+    """The gradients of lora_add in x (the adapter's part; base's is dy itself), a and b: (dx, da, db).
+
+    With the tokens sorted by adapter: v = a x, dv = scale b^T dy, dx = a^T dv, da = sum dv x^T, db = scale
+    sum dy v^T.  v and dv are rounded to the inputs' type, as activations between two layers are.  Tokens
+    without an adapter get dx = 0, adapters without tokens da = db = 0.  At most 1024 adapters.
+    """
+    who = "lora_grad"
+    _on_gpu(who, dy=dy, x=x, a=a, b=b, ids=ids, scale=scale)
+    _need(x.dim() == 2 and dy.dim() == 2 and dy.shape[0] == x.shape[0], f"{who}: dy {tuple(dy.shape)}, x {tuple(x.shape)}")
+    _, n_ad, _, _, n_out, _, _ = _lora_args(who, x, a, b, ids, scale)
+    _rows(who, "dy", dy, x.dtype, x.shape[0], n_out)
+    _need(1 <= n_ad <= 1024, f"{who}: {n_ad} adapters (1..1024)")
+    _, order, seg = expert_plan(ids.reshape(-1), n_ad)
+    v = grouped_mm(x, seg, a, row_in=order)
+    dv = grouped_mm_dx(dy, seg, b, row_in=order, scale=scale)
+    dx = grouped_mm_dx(dv, seg, a, row_out=order)
+    da = grouped_mm_dw(dv, x, seg, row_x=order)
+    db = grouped_mm_dw(dy, v, seg, row_dy=order, scale=scale)
+    return dx, da, db
