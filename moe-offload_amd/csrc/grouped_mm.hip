@@ -57,196 +57,388 @@ __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
 }
 
 template <typename T>
-__device__ __forceinline__ uint2 round4(const float* v) {
+__device__ __forceinline__ uint2 round4(f32x4 v) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const t4 r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     return __builtin_bit_cast(uint2, r);
 }
 
 template <typename T>
-__device__ __forceinline__ void widen4(uint2 w, float* v) {
+__device__ __forceinline__ f32x4 widen4(uint2 w) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const t4 r = __builtin_bit_cast(t4, w);
-    for (int i = 0; i < 4; ++i) v[i] = (float)r[i];
+    return (f32x4){(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
 }
 
-constexpr int kBP = 64, kBQ = 64, kBC = 32, kLd = kBC + 8;
+// What an operand's lanes read where it has nothing: contraction indexes past the end.
+__device__ uint4 g_zero16;
 
-template <typename T, int OP>
-__global__ __launch_bounds__(256) void k_grouped(Args a) {
-    __shared__ __attribute__((aligned(16))) uint16_t lp[kBP * kLd];
-    __shared__ __attribute__((aligned(16))) uint16_t lq[kBQ * kLd];
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-    const int qstep = OP == kGateUp ? kBQ / 2 : kBQ;          // output columns of a tile
-    const int inter = a.nq;                                    // gate_up, and mm_dx with gu
+// 16 bytes per lane from global memory straight into LDS: lane l's land at lds + 16 l (lds wave-uniform).
+// The issuing code waits for them itself (vmcnt), and no register receives data.
+__device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+
+constexpr int kBC = 64;                                       // contraction indexes per step
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// Row of a step's image, along which the other index runs -> which 32-byte block trades places with block 0:
+// the rows that one transposing read touches (4 of each of two or four lane groups) get eight different ones.
+__device__ __forceinline__ int turn(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
+
+// One operand's fragments for v_mfma_f32_16x16x32: lane (n, kq) holds c = 32 ks + 8 kq .. + 7 of row / column n.
+// ALONG false: the image has a row per tile row, kBC values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
+// ALONG true: a row per c, W values each, read transposed by ds_read_b64_tr_b16 (lane i of 16 gives the address of
+// 4 columns of row i / 4 and receives column i of 4 rows).
+template <bool ALONG, int W, int SUBS>
+struct Frags {
+    uint32_t at[ALONG ? SUBS : 2];
+
+    __device__ __forceinline__ void init(uint32_t base, int first, int lane) {
+        const int n = lane & 15, kq = lane >> 4;
+        if constexpr (ALONG) {
+            const int row = kq * 8 + (n >> 2);
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s)
+                at[s] = base + row * (W * 2) + (((first >> 4) + s) ^ turn(row)) * 32 + (n & 3) * 8;
+        } else {
+            at[0] = base + (first + n) * 128 + (kq ^ (n & 7)) * 16;
+            at[1] = base + (first + n) * 128 + ((kq + 4) ^ (n & 7)) * 16;
+        }
+    }
+
+    __device__ __forceinline__ uint4 read(uint32_t stage, int s, int ks) const {
+        if constexpr (ALONG) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* ptr;
+            const uint32_t p = at[s] + stage + ks * 32 * (W * 2);
+            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)p));
+            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(p + 4 * (W * 2))));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) const u32x4* ptr;
+            const u32x4 v = *(ptr)(uintptr_t)(at[ks] + stage + s * 2048);
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+};
+
+// Two subtiles' 4 adjacent 16-bit results per lane -> 8 adjacent: lanes 16-31 and 48-63 take the second
+// subtile.  Returns the 16 bytes and which subtile (0, 1) and half (0, 1) of its 16 columns they are.
+__device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+    return make_uint4(x[0], y[0], x[1], y[1]);
+}
+
+// BP x BQ results per block of WP x WQ waves.  A step of 64 contraction indexes goes from global memory to LDS
+// without passing registers while the step before it is multiplied: two images, one barrier per step.
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
+__global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
+    constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
+    constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
+    constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;      // 1 KiB each
+    constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
+    constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
+    static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
+    static_assert(!kAlongQ || BQ >= 128, "the image's turns take 8 blocks of 32 bytes");
+    static_assert(!kAlongP || BP >= 128, "");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int inter = a.nq;                                                    // gate_up, and mm_dx with gu
     int r0, r1, slot, q0, p0 = 0, nc = a.nc, seg = 0;
     if constexpr (OP == kDw) {
-        const int tq = (a.nq + kBQ - 1) / kBQ, tp = (a.np + kBP - 1) / kBP;
+        const int tq = (a.nq + BQ - 1) / BQ, tp = (a.np + BP - 1) / BP;
         const uint32_t item = gmm::xcd_order(blockIdx.x, gridDim.x);
         seg = item / (tq * tp);
-        p0 = (int)(item / tq % tp) * kBP;
-        q0 = (int)(item % tq) * kBQ;
-        Segs S = a.S;
-        gmm::seg_rows(S, seg + 1, r0, r1, slot);
+        p0 = (int)(item / tq % tp) * BP;
+        q0 = (int)(item % tq) * BQ;
+        gmm::seg_rows(a.S, seg + 1, r0, r1, slot);
         nc = r1 - r0;
     } else {
         Tile tile;
-        if (!gmm::find_tile<256>(a.S, kBP, (a.nq + qstep - 1) / qstep, tile)) return;
+        if (!gmm::find_tile<64 * kWaves>(a.S, BP, (a.nq + kQStep - 1) / kQStep, tile)) return;
         r0 = tile.r0;
         r1 = tile.r1;
         slot = tile.slot;
-        q0 = tile.col * qstep;
-        if (slot < 0) nc = 0;
+        q0 = tile.col * kQStep;
+        if (slot < 0 || a.n_p == 0) nc = 0;
     }
     const T* P = (const T*)a.p;
     const T* Q = (const T*)a.q;
     if constexpr (OP != kDw) Q += (int64_t)(slot < 0 ? 0 : slot) * a.ldq;
 
-    // this thread's 16 bytes of each operand per step
-    const int crow = t >> 2, cch = (t & 3) * 8;                // contiguous in c: row, first c
-    const int trow = t >> 3, tch = (t & 7) * 8;                // c along the rows: c, first column
-    const T* prow = nullptr;
-    const T* qrow = nullptr;
-    if constexpr (OP != kDw) {
-        const int r = r0 + crow;
-        if (r < r1) {
-            const int v = a.row_p ? a.row_p[r] : r;
-            if (v >= 0 && v < a.n_p) prow = P + (int64_t)v * a.ldp;
+    // this lane's 16 bytes of each of its wave's loads.  Rows past the tile, and rows that do not exist, read some
+    // row that does: their results are not stored, or replaced by zeros.
+    const T* pp[kLoadsP];
+    const T* qp[kLoadsQ];
+    const int cu = ((lane & 7) ^ (lane >> 3)) * 8;                             // not ALONG: first c of the 16 bytes
+    if constexpr (!kAlongP) {
+#pragma unroll
+        for (int j = 0; j < kLoadsP; ++j) {
+            int r = r0 + (wv * kLoadsP + j) * 8 + (lane >> 3);
+            r = r < r1 ? r : r1 - 1;
+            int v = a.row_p ? a.row_p[r] : r;
+            v = v >= 0 && v < a.n_p ? v : 0;
+            pp[j] = P + (int64_t)v * a.ldp + cu;
         }
     }
-    if constexpr (OP == kMM) {
-        if (q0 + crow < a.nq) qrow = Q + (int64_t)(q0 + crow) * a.nc;
+    if constexpr (!kAlongQ) {
+#pragma unroll
+        for (int j = 0; j < kLoadsQ; ++j) {
+            const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
+            int64_t q;
+            if constexpr (OP == kGateUp) {
+                // a wave's first SQ / 2 subtiles are gate rows, the others the up rows of the same outputs
+                const int sub = row / 16 % SQ;
+                int c = q0 + row / (SQ * 16) * (SQ * 8) + sub % (SQ / 2) * 16 + row % 16;
+                c = c < inter ? c : inter - 1;
+                q = c + (sub < SQ / 2 ? 0 : inter);
+            } else {
+                q = q0 + row < a.nq ? q0 + row : a.nq - 1;
+            }
+            qp[j] = Q + q * a.nc + cu;
+        }
     }
-    if constexpr (OP == kGateUp) {
-        // the tile's 64 weight rows: per wave column 16 gate rows, then the 16 up rows of the same outputs
-        const int c = q0 + (crow >> 5) * 16 + (crow & 15);
-        if (c < inter) qrow = Q + (int64_t)(c + ((crow >> 4) & 1) * inter) * a.nc;
+    constexpr int kUnitsP = BP / 8, kUnitsQ = BQ / 8;                          // ALONG: 16-byte units per row of the image
+    auto along_row = [&](int j, int loads, int units) { return (wv * loads + j) * (64 / units) + lane / units; };
+    auto along_col = [&](int row, int units) { return (lane % units ^ 2 * turn(row)) * 8; };
+    if constexpr (OP == kDx || OP == kDxGlu) {
+#pragma unroll
+        for (int j = 0; j < kLoadsQ; ++j) {
+            const int row = along_row(j, kLoadsQ, kUnitsQ);
+            const int q = q0 + along_col(row, kUnitsQ);
+            qp[j] = Q + (int64_t)row * a.nq + (q < a.nq ? q : 0);
+        }
     }
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    f32x4 acc[2][2] = {};
-    const int wp = (wv >> 1) * 32, wq = (wv & 1) * 32, n = lane & 15, kq = lane >> 4;
-    for (int c0 = 0; c0 < nc; c0 += kBC) {
-        uint4 vp = zero, vq = zero;
+    // mm_dw: which rows of dy and x the next step reads (-1: none).  A row that is missing on one side is left out on
+    // both: zeros would still meet an infinity there.
+    int rp[kLoadsP], rq[kLoadsQ];
+    auto next_rows = [&](int c0) {
+        static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
+#pragma unroll
+        for (int j = 0; j < kLoadsP; ++j) {
+            const int c = c0 + along_row(j, kLoadsP, kUnitsP);
+            int v = -1, x = -1;
+            if (c < nc) {
+                v = a.row_p ? a.row_p[r0 + c] : r0 + c;
+                x = a.row_q ? a.row_q[r0 + c] : r0 + c;
+            }
+            const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
+            rp[j] = both ? v : -1;
+            rq[j] = both ? x : -1;
+        }
+    };
+    auto issue = [&](int c0, uint32_t stage) {
+        const uint32_t lp = lds0 + stage + wv * kLoadsP * 1024, lq = lds0 + stage + kStageP + wv * kLoadsQ * 1024;
+        const bool whole = c0 + kBC <= nc;                                     // wave-uniform
         if constexpr (OP == kDw) {
-            const int r = r0 + c0 + trow;
-            if (r < r1) {
-                const int v = a.row_p ? a.row_p[r] : r, x = a.row_q ? a.row_q[r] : r;
-                if (v >= 0 && v < a.n_p && x >= 0 && x < a.n_q) {
-                    if (p0 + tch < a.np) vp = *(const uint4*)(P + (int64_t)v * a.ldp + p0 + tch);
-                    if (q0 + tch < a.nq) vq = *(const uint4*)(Q + (int64_t)x * a.ldq + q0 + tch);
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) {
+                const int row = along_row(j, kLoadsP, kUnitsP), q = p0 + along_col(row, kUnitsP);
+                load_to_lds(rp[j] >= 0 ? P + (int64_t)rp[j] * a.ldp + (q < a.np ? q : 0) : (const T*)&g_zero16, lp + j * 1024);
+            }
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) {
+                const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
+                load_to_lds(rq[j] >= 0 ? Q + (int64_t)rq[j] * a.ldq + (q < a.nq ? q : 0) : (const T*)&g_zero16, lq + j * 1024);
+            }
+            next_rows(c0 + kBC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) {
+                load_to_lds(whole || c0 + cu < nc ? pp[j] : (const T*)&g_zero16, lp + j * 1024);
+                pp[j] += kBC;
+            }
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) {
+                if constexpr (kAlongQ) {
+                    load_to_lds(whole || c0 + along_row(j, kLoadsQ, kUnitsQ) < nc ? qp[j] : (const T*)&g_zero16, lq + j * 1024);
+                    qp[j] += (int64_t)kBC * a.nq;
+                } else {
+                    load_to_lds(whole || c0 + cu < nc ? qp[j] : (const T*)&g_zero16, lq + j * 1024);
+                    qp[j] += kBC;
                 }
             }
-        } else {
-            if (prow && c0 + cch < nc) vp = *(const uint4*)(prow + c0 + cch);
-            if constexpr (OP == kDx || OP == kDxGlu) {
-                if (c0 + trow < nc && q0 + tch < a.nq) vq = *(const uint4*)(Q + (int64_t)(c0 + trow) * a.nq + q0 + tch);
-            } else {
-                if (qrow && c0 + cch < nc) vq = *(const uint4*)(qrow + c0 + cch);
-            }
         }
-        __syncthreads();
-        auto put = [&](uint16_t* l, uint4 v, bool along) {
-            if (along) {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    };
+
+    const int wp = wv / WQ, wq = wv % WQ, n = lane & 15, kq = lane >> 4;
+    Frags<kAlongP, BP, SP> fp;
+    Frags<kAlongQ, BQ, SQ> fq;
+    fp.init(lds0, wp * SP * 16, lane);
+    fq.init(lds0 + kStageP, wq * SQ * 16, lane);
+    f32x4 acc[SP][SQ] = {};
+    if constexpr (OP == kDw) next_rows(0);
+    if (nc > 0) issue(0, 0);
+    for (int c0 = 0; c0 < nc; c0 += kBC) {
+        const uint32_t stage = c0 / kBC % 2 * kStage;
+        // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so
+        // are everyone's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (c0 + kBC < nc) issue(c0 + kBC, kStage - stage);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) l[(tch + i) * kLd + trow] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-            } else {
-                *(uint4*)(l + crow * kLd + cch) = v;
-            }
-        };
-        put(lp, vp, OP == kDw);
-        put(lq, vq, OP >= kDx);
-        __syncthreads();
-        uint4 fp[2], fq[2];
+        for (int ks = 0; ks < 2; ++ks) {
+            uint4 vp[SP], vq[SQ];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fp[i] = *(const uint4*)(lp + (wp + i * 16 + n) * kLd + kq * 8);
-            fq[i] = *(const uint4*)(lq + (wq + i * 16 + n) * kLd + kq * 8);
+            for (int j = 0; j < SQ; ++j) vq[j] = fq.read(stage, j, ks);
+#pragma unroll
+            for (int i = 0; i < SP; ++i) vp[i] = fp.read(stage, i, ks);
+#pragma unroll
+            for (int i = 0; i < SP; ++i)
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[j], vp[i], acc[i][j]);
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = mfma<T>(fq[j], fp[i], acc[i][j]);
     }
     const float s = a.scale && slot >= 0 ? a.scale[slot] : 1.0f;
+    // 16-byte stores: lane (n, kq) of a pair of subtiles holds columns 8 (kq / 2) .. + 7 of subtile kq % 2
+    const int pair_col = (kq & 1) * 16 + (kq >> 1) * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int m = wp + i * 16 + n;
+    for (int i = 0; i < SP; ++i) {
+        const int m = wp * SP * 16 + i * 16 + n;
         if constexpr (OP == kDw) {
-            if (p0 + m >= a.np) continue;
-            for (int j = 0; j < 2; ++j) {
-                const int q = q0 + wq + j * 16 + kq * 4;
-                if (q >= a.nq) continue;
-                float v[4];
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * s;
-                const int64_t at = (int64_t)seg * a.ldo + (int64_t)(p0 + m) * a.nq + q;
-                if (a.out_f32) *(float4*)((float*)a.out + at) = make_float4(v[0], v[1], v[2], v[3]);
-                else *(uint2*)((T*)a.out + at) = round4<T>(v);
+            const int64_t row = (int64_t)seg * a.ldo + (int64_t)(p0 + m) * a.nq;
+            const bool live = p0 + m < a.np;
+            if (a.out_f32) {
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) {
+                    const int q = q0 + wq * SQ * 16 + j * 16 + kq * 4;
+                    if (live && q < a.nq)
+                        *(float4*)((float*)a.out + row + q) = make_float4(acc[i][j][0] * s, acc[i][j][1] * s, acc[i][j][2] * s, acc[i][j][3] * s);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < SQ; j += 2) {
+                    const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
+                    const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
+                    if (live && q < a.nq) *(uint4*)((T*)a.out + row + q) = v;
+                }
             }
             continue;
         }
         const int r = r0 + m;
-        if (r >= r1) continue;
-        if constexpr (OP == kGateUp) {
-            const int c = q0 + (wv & 1) * 16 + kq * 4;
-            if (c >= inter) continue;
-            float g[4], u[4], h[4];
-            for (int e = 0; e < 4; ++e) {
-                g[e] = acc[i][0][e];
-                u[e] = acc[i][1][e];
-                h[e] = g[e] / (1.0f + __expf(-g[e])) * u[e];
+        bool live = r < r1, dead = slot < 0;
+        int o = r;
+        if (live) {
+            if (a.row_p) {
+                const int v = a.row_p[r];
+                dead |= v < 0 || v >= a.n_p;
             }
-            *(uint2*)((T*)a.out + (int64_t)r * a.ldo + c) = round4<T>(h);
-            if (a.gu_out) {
-                *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = round4<T>(g);
-                *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = round4<T>(u);
+            if (OP != kGateUp && a.row_out) o = a.row_out[r];
+            if (OP != kGateUp) live = o >= 0 && o < a.n_out;
+        }
+        if constexpr (OP == kGateUp) {
+            uint2 h[SQ / 2], g2[SQ / 2], u2[SQ / 2];
+#pragma unroll
+            for (int j = 0; j < SQ / 2; ++j) {
+                f32x4 g = acc[i][j], u = acc[i][j + SQ / 2], hv;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    g[e] = dead ? 0.f : g[e];
+                    u[e] = dead ? 0.f : u[e];
+                    hv[e] = g[e] / (1.0f + __expf(-g[e])) * u[e];
+                }
+                h[j] = round4<T>(hv);
+                g2[j] = round4<T>(g);
+                u2[j] = round4<T>(u);
+            }
+            if constexpr (SQ / 2 == 1) {
+                const int c = q0 + wq * 16 + kq * 4;
+                if (live && c < inter) {
+                    *(uint2*)((T*)a.out + (int64_t)r * a.ldo + c) = h[0];
+                    if (a.gu_out) {
+                        *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = g2[0];
+                        *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = u2[0];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < SQ / 2; j += 2) {
+                    const int c = q0 + wq * SQ * 8 + j * 16 + pair_col;
+                    const uint4 vh = pair8(h[j], h[j + 1]);
+                    if (live && c < inter) *(uint4*)((T*)a.out + (int64_t)r * a.ldo + c) = vh;
+                    if (a.gu_out) {
+                        const uint4 vg = pair8(g2[j], g2[j + 1]), vu = pair8(u2[j], u2[j + 1]);
+                        if (live && c < inter) {
+                            *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = vg;
+                            *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = vu;
+                        }
+                    }
+                }
+            }
+        } else if constexpr (OP == kDxGlu) {
+#pragma unroll
+            for (int j = 0; j < SQ; j += 2) {
+                uint2 dg[2], du[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int q = q0 + wq * SQ * 16 + (j + b) * 16 + kq * 4;
+                    f32x4 g = {}, u = {}, vg, vu;
+                    if (live && !dead && q < inter) {
+                        const T* gr = (const T*)a.gu + (int64_t)r * a.ldgu + q;
+                        g = widen4<T>(*(const uint2*)gr);
+                        u = widen4<T>(*(const uint2*)(gr + inter));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float dh = dead ? 0.f : acc[i][j + b][e] * s, sg = 1.0f / (1.0f + __expf(-g[e]));
+                        vg[e] = dh * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
+                        vu[e] = dh * g[e] * sg;
+                    }
+                    dg[b] = round4<T>(vg);
+                    du[b] = round4<T>(vu);
+                }
+                const uint4 vg = pair8(dg[0], dg[1]), vu = pair8(du[0], du[1]);
+                const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
+                if (live && q < inter) {
+                    T* d = (T*)a.out + (int64_t)o * a.ldo + q;
+                    *(uint4*)d = vg;
+                    *(uint4*)(d + inter) = vu;
+                }
             }
         } else {
-            const int o = a.row_out ? a.row_out[r] : r;
-            if (o < 0 || o >= a.n_out) continue;
-            for (int j = 0; j < 2; ++j) {
-                const int q = q0 + wq + j * 16 + kq * 4;
-                if (q >= a.nq) continue;
-                float v[4];
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * s;
-                T* d = (T*)a.out + (int64_t)o * a.ldo + q;
-                if constexpr (OP == kDxGlu) {
-                    float g[4], u[4], dg[4], du[4];
-                    const T* gr = (const T*)a.gu + (int64_t)r * a.ldgu + q;
-                    widen4<T>(*(const uint2*)gr, g);
-                    widen4<T>(*(const uint2*)(gr + inter), u);
-                    for (int e = 0; e < 4; ++e) {
-                        const float sg = 1.0f / (1.0f + __expf(-g[e]));
-                        dg[e] = slot < 0 ? 0.f : v[e] * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
-                        du[e] = slot < 0 ? 0.f : v[e] * g[e] * sg;
-                    }
-                    *(uint2*)d = round4<T>(dg);
-                    *(uint2*)(d + inter) = round4<T>(du);
-                } else {
-                    *(uint2*)d = round4<T>(v);
-                }
+#pragma unroll
+            for (int j = 0; j < SQ; j += 2) {
+                const f32x4 zero = {};
+                const uint4 v = pair8(round4<T>(dead ? zero : acc[i][j] * s), round4<T>(dead ? zero : acc[i][j + 1] * s));
+                const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
+                if (live && q < a.nq) *(uint4*)((T*)a.out + (int64_t)o * a.ldo + q) = v;
             }
         }
     }
 }
 
-template <typename T, int OP>
-int launch(const Args& a, hipStream_t s) {
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
+int launch_tiles(const Args& a, hipStream_t s) {
     uint64_t blocks;
     if constexpr (OP == kDw) {
-        blocks = (uint64_t)a.S.n_seg * ((a.nq + kBQ - 1) / kBQ) * ((a.np + kBP - 1) / kBP);
+        blocks = (uint64_t)a.S.n_seg * ((a.nq + BQ - 1) / BQ) * ((a.np + BP - 1) / BP);
     } else {
-        const int qstep = OP == kGateUp ? kBQ / 2 : kBQ;
+        const int qstep = OP == kGateUp ? BQ / 2 : BQ;
         const uint64_t segs = (uint64_t)(a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
-        blocks = ((uint64_t)a.S.n_rows / kBP + segs) * ((a.nq + qstep - 1) / qstep);
+        blocks = ((uint64_t)a.S.n_rows / BP + segs) * ((a.nq + qstep - 1) / qstep);
     }
     if (blocks > 0x7FFFFFFFu) {
         moe_set_error("grouped product: %llu tiles are more than one launch takes", (unsigned long long)blocks);
         return -1;
     }
-    hipLaunchKernelGGL((k_grouped<T, OP>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
+}
+
+template <typename T, int OP>
+int launch(const Args& a, hipStream_t s) {
+    if constexpr (OP == kDw) return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
+    else {
+        const int64_t per_seg = a.S.n_seg ? a.S.n_rows / a.S.n_seg : 0;
+        if (per_seg <= 96) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
+        return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
+    }
 }
 
 template <int OP>

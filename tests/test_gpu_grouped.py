@@ -230,6 +230,14 @@ def test_infinities_and_nan_stay_in_their_rows(dtype):
     rows = torch.ones(n, dtype=torch.bool, device=DEV)
     rows[3] = False
     assert torch.equal(dw[1][rows], cdw[1][rows]) and not bool(dw[1][3].isfinite().any())
+    # a row left out of the weights' gradient on one side does not meet the other side's infinity
+    out = list(range(100))
+    out[40], out[41] = -1, 100
+    x2, dy2 = x.clone(), rnd((100, n), dtype, 4)
+    x2[40:42], dy2[50] = float("inf"), float("nan")
+    xin = list(range(100))
+    xin[50] = 200
+    assert bool(ops.grouped_mm_dw(dy2, x2, seg, row_dy=i32(out), row_x=i32(xin)).isfinite().all())
     w2 = w.clone()
     w2[1, 7, 9] = float("nan")
     y = ops.grouped_mm(x, seg, w2)
