@@ -287,9 +287,11 @@ int moe_pair_combine(const void* y, const void* scores, const void* residual, in
  * host: ids i32 [n_ids], pair p = token * k + j.  Sorted row r is pair row_out[r] of token row_token[r];
  * expert e's rows are seg_start[e] .. seg_start[e + 1] - 1 (seg_start: n_exp + 1 entries) in the order
  * of their pairs.  Pairs whose id is outside 0 .. n_exp - 1 come behind the last segment, in order.
- * n_exp in 1..1024, n_ids a multiple of k. */
-int moe_expert_plan(const int32_t* ids, int n_ids, int k, int n_exp, int32_t* row_token, int32_t* row_out,
-                    int32_t* seg_start, void* stream);
+ * n_exp in 1..1024, n_ids a multiple of k.  workspace: moe_expert_plan_workspace_bytes bytes (0: may be
+ * null), any contents, one per call in flight. */
+uint64_t moe_expert_plan_workspace_bytes(int n_ids, int n_exp);
+int moe_expert_plan(const int32_t* ids, int n_ids, int k, int n_exp, void* workspace, int32_t* row_token,
+                    int32_t* row_out, int32_t* seg_start, void* stream);
 /* y[row_out[r]] = scale[u] W_u x[row_in[r]] for the rows r of segment u: seg_start[u] .. seg_start[u + 1]
  * - 1, W_u [n][k] = w + seg_slot[u] * w_stride (seg_slot null: u), scale fp32 per slot or null; row_in /
  * row_out null: row r.  n_seg in 0..1024.  A row_in outside x gives a row of zeros; a row_out outside y
@@ -329,6 +331,15 @@ uint64_t moe_lora_workspace_bytes(int n_tok, int rank);
 int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, const void* a, int64_t a_stride,
                  const void* b, int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in,
                  int n_out, int rank, int dtype, void* workspace, void* out, int64_t ld_out, void* stream);
+/* The gradients of moe_lora_add, given dy [n_tok][n_out] (base's own is dy):  dx[t] = A_i^T dv[t] (zeros without
+ * an adapter), da_i [rank][n_in] = sum of dv[t] x[t]^T and db_i [n_out][rank] = scale[i] * sum of dy[t] v[t]^T over
+ * adapter i's tokens (zeros without any), v = A_i x[t], dv = scale[i] * B_i^T dy[t], both rounded to dtype.  da and
+ * db are contiguous; n_ad in 1..1024.  workspace: moe_lora_grad_workspace_bytes bytes, 16-byte aligned, any
+ * contents, one per call in flight. */
+uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank);
+int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* a, int64_t a_stride, const void* b,
+                  int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out,
+                  int rank, int dtype, void* workspace, void* dx, int64_t lddx, void* da, void* db, void* stream);
 
 /* 2-bit codebook experts: the Nemotron model of README.md:37 (IQ2_XXS GGUF, 240 experts, top-9),
  * run by the reference only inside llama.cpp's Metal backend (llama-moe-cache.patch:1-12 adds the

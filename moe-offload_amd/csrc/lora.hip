@@ -4,11 +4,34 @@
 // A_i [rank][n_in], B_i [n_out][rank]; an id outside the adapters leaves out[t] = base[t].  base is the
 // shared projection's output (a grouped product, the 2-bit experts' rows, a router's logits) and may be
 // out itself.  v = A_i x stays in fp32 between the two products, and out is rounded once.
+//
+// Two launches.  k_lora_v: 16 tokens and up to 32 ranks per block, the contraction split over its waves, both
+// operands from global memory straight in the matrix unit's layout (each byte of x is used for 16 ranks at a
+// time, so staging would gain nothing).  k_lora_out: 16 tokens and 64 output columns per block, v and B in the
+// fp32 matrix unit, so v keeps its bits and its range.  The tokens of a tile may have different adapters: the
+// tile is multiplied by each adapter that occurs in it and every token keeps its own adapter's result.  In a
+// batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks of
+// their own.
 #include <hip/hip_bf16.h>
 
-#include "moe_common.h"
+#include <initializer_list>
+
+#include "../../include/moe_offload.h"
+#include "grouped_mm.h"
 
 namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 
 template <typename T>
 __device__ __forceinline__ void widen8(uint4 w, float* v) {
@@ -18,67 +41,182 @@ __device__ __forceinline__ void widen8(uint4 w, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = (float)r[i];
 }
 
-// v[t][j] = s_i A_i[j] x[t]: one wave per (t, j).
 template <typename T>
+__device__ __forceinline__ uint4 round8(const float* v) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const t8 r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
+    return __builtin_bit_cast(uint4, r);
+}
+
+// The adapters of a tile of 16 tokens, each once in the order of their first tokens: calls f(adapter, whether this
+// lane's token has it) for the ones numbered first, first + step, ...  Wave-uniform.
+template <typename F>
+__device__ __forceinline__ void each_adapter(int id, bool has, int first, int step, F f) {
+    uint32_t todo = (uint32_t)__ballot(has) & 0xFFFFu;
+    for (int j = 0; todo; ++j) {
+        const int i = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+        const bool mine = has && id == i;
+        todo &= ~(uint32_t)__ballot(mine);
+        if (j >= first && (j - first) % step == 0) f(i, mine);
+    }
+}
+
+// v[t][j] = s_i A_i[j] x[t] for 16 tokens (blockIdx.x) and 16 SR ranks (blockIdx.y).
+template <typename T, int SR>
 __global__ __launch_bounds__(256) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A, int64_t a_stride,
                                                 const int32_t* __restrict__ ids, const float* __restrict__ scale, int n_tok,
                                                 int n_ad, int n_in, int rank, float* __restrict__ v) {
-    const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(w / rank), j = (int)(w % rank);
-    if (t >= n_tok) return;
-    const int i = ids[t];
-    if (i < 0 || i >= n_ad) return;
-    const T* a = A + (int64_t)i * a_stride + (int64_t)j * n_in;
-    const T* xr = x + (int64_t)t * ldx;
-    float sum = 0.f;
-    for (int c = lane * 8; c < n_in; c += 512) {
-        float av[8], xv[8];
-        widen8<T>(*(const uint4*)(a + c), av);
-        widen8<T>(*(const uint4*)(xr + c), xv);
+    __shared__ f32x4 part[3][SR][64];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
+    const int64_t t = (int64_t)blockIdx.x * 16 + n;
+    const int id = t < n_tok ? ids[t] : -1, j0 = blockIdx.y * (16 * SR);
+    const bool has = id >= 0 && id < n_ad;
+    const T* xr = x + (t < n_tok ? t : (int64_t)n_tok - 1) * ldx + kq * 8;
+    const int steps = (n_in + 31) / 32, per = (steps + 3) / 4;
+    const int c0 = wv * per * 32, c1 = c0 + per * 32 < n_in ? c0 + per * 32 : n_in;
+    each_adapter(id, has, blockIdx.z, gridDim.z, [&](int i, bool mine) {
+        const T* ar[SR];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(av[e], xv[e], sum);
-    }
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    if (lane == 0) v[(int64_t)t * rank + j] = (scale ? scale[i] : 1.0f) * sum;
+        for (int s = 0; s < SR; ++s) {
+            const int j = j0 + s * 16 + n;
+            ar[s] = A + (int64_t)i * a_stride + (int64_t)(j < rank ? j : rank - 1) * n_in + kq * 8;
+        }
+        f32x4 acc[SR] = {};
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        int c = c0;
+#pragma unroll 1
+        for (; c + 256 <= c1; c += 256) {
+            uint4 xv[8], av[SR][8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                xv[u] = *(const uint4*)(xr + c + u * 32);
+#pragma unroll
+                for (int s = 0; s < SR; ++s) av[s][u] = *(const uint4*)(ar[s] + c + u * 32);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int s = 0; s < SR; ++s) acc[s] = mfma<T>(av[s][u], xv[u], acc[s]);
+        }
+        if (c < c1) {
+            uint4 xv[8], av[SR][8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const bool in = c + u * 32 + kq * 8 < c1;
+                xv[u] = in ? *(const uint4*)(xr + c + u * 32) : zero;
+#pragma unroll
+                for (int s = 0; s < SR; ++s) av[s][u] = in ? *(const uint4*)(ar[s] + c + u * 32) : zero;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int s = 0; s < SR; ++s) acc[s] = mfma<T>(av[s][u], xv[u], acc[s]);
+        }
+        if (wv > 0)
+            for (int s = 0; s < SR; ++s) part[wv - 1][s][lane] = acc[s];
+        __syncthreads();
+        if (wv == 0) {
+            const float si = scale ? scale[i] : 1.0f;
+            for (int s = 0; s < SR; ++s) {
+                const f32x4 sum = ((acc[s] + part[0][s][lane]) + (part[1][s][lane] + part[2][s][lane])) * si;
+                const int j = j0 + s * 16 + kq * 4;
+                if (mine && j < rank) *(f32x4*)(v + t * rank + j) = sum;
+            }
+        }
+        __syncthreads();
+    });
 }
 
+// out = base + B_i v for 16 tokens (blockIdx.x) and 64 columns (blockIdx.y), 16 to a wave.
 template <typename T>
 __global__ __launch_bounds__(256) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
                                                   const T* __restrict__ B, int64_t b_stride, const int32_t* __restrict__ ids,
-                                                  int n_ad, int n_out, int rank, T* out, int64_t ldo) {
-    const int64_t t = blockIdx.x;
-    const int n = blockIdx.y * 256 + threadIdx.x;
-    if (n >= n_out) return;
-    const int i = ids[t];
-    float sum = 0.f;
-    if (i >= 0 && i < n_ad) {
-        const T* b = B + (int64_t)i * b_stride + (int64_t)n * rank;
-        for (int j = 0; j < rank; j += 8) {
-            float bv[8];
-            widen8<T>(*(const uint4*)(b + j), bv);
+                                                  int n_tok, int n_ad, int n_out, int rank, T* out, int64_t ldo) {
+    const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
+    const int q0 = blockIdx.y * 64 + (threadIdx.x >> 6) * 16;
+    if (q0 >= n_out) return;
+    const int64_t t = (int64_t)blockIdx.x * 16 + n;
+    const int id = t < n_tok ? ids[t] : -1;
+    const bool has = id >= 0 && id < n_ad;
+    const float* vr = v + (t < n_tok ? t : 0) * rank;
+    f32x4 acc = {};
+    bool got = false;
+    each_adapter(id, has, blockIdx.z, gridDim.z, [&](int i, bool mine) {
+        const T* br = B + (int64_t)i * b_stride + (int64_t)(q0 + n < n_out ? q0 + n : n_out - 1) * rank;
+        f32x4 one = {};
+        for (int k0 = 0; k0 < rank; k0 += 32) {
+            float bv[8] = {}, vv[8] = {};
+            if (k0 + kq * 8 < rank) {
+                widen8<T>(*(const uint4*)(br + k0 + kq * 8), bv);
+                if (mine) {
+                    const f32x4 lo = *(const f32x4*)(vr + k0 + kq * 8), hi = *(const f32x4*)(vr + k0 + kq * 8 + 4);
+                    for (int e = 0; e < 4; ++e) vv[e] = lo[e], vv[4 + e] = hi[e];
+                }
+            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(bv[e], v[t * rank + j + e], sum);
+            for (int e = 0; e < 8; ++e) one = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[e], vv[e], one, 0, 0, 0);
         }
-    } else if (base == out) {
-        return;
-    }
-    out[t * ldo + n] = (T)((float)base[t * ldb + n] + sum);
+        if (mine) acc = one, got = true;
+    });
+    // lane (n, kq): columns 4 kq .. + 3 of token n.  Tokens without an adapter are the first block's.
+    const int q = q0 + kq * 4;
+    if (t >= n_tok || q >= n_out || !(got || (!has && blockIdx.z == 0 && base != out))) return;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 r = *(const t4*)(base + t * ldb + q);
+    if (got)
+        for (int e = 0; e < 4; ++e) r[e] = (T)((float)r[e] + acc[e]);
+    *(t4*)(out + t * ldo + q) = r;
 }
 
 template <typename T>
 int lora_add(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* B,
              int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
              float* v, void* out, int64_t ldo, hipStream_t s) {
-    const int64_t waves = (int64_t)n_tok * rank;
-    hipLaunchKernelGGL((k_lora_v<T>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, (const T*)x, ldx, (const T*)A,
-                       a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((k_lora_out<T>), dim3(n_tok, (n_out + 255) / 256), dim3(256), 0, s, (const T*)base, ldb, v,
-                       (const T*)B, b_stride, ids, n_ad, n_out, rank, (T*)out, ldo);
+    const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 15) / 16);
+    // up to 256 tokens a tile's adapters get blocks of their own (16 tokens have 16 at most)
+    const uint32_t split = n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
+    if (n_ad > 0) {
+        if (rank <= 16)
+            hipLaunchKernelGGL((k_lora_v<T, 1>), dim3(tiles, 1, split), dim3(256), 0, s, (const T*)x, ldx, (const T*)A,
+                               a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
+        else
+            hipLaunchKernelGGL((k_lora_v<T, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(256), 0, s, (const T*)x, ldx,
+                               (const T*)A, a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
+        HIP_TRY(hipGetLastError());
+    }
+    hipLaunchKernelGGL((k_lora_out<T>), dim3(tiles, (n_out + 63) / 64, split), dim3(256), 0, s, (const T*)base, ldb, v,
+                       (const T*)B, b_stride, ids, n_tok, n_ad, n_out, rank, (T*)out, ldo);
     HIP_TRY(hipGetLastError());
     return 0;
 }
+
+// The shapes and strides that both entry points take; base or dy is [n_tok][n_out].
+bool bad_shapes(const char* who, int dtype, int n_tok, int n_ad, int n_in, int n_out, int rank, int64_t ldx, int64_t ldy,
+                int64_t a_stride, int64_t b_stride) {
+    if ((dtype != 0 && dtype != 1) || n_tok < 0 || n_ad < 0 || n_in <= 0 || n_out <= 0 || rank <= 0 || n_in % 8 ||
+        n_out % 8 || rank % 8 || rank > 256 || (n_out + 63) / 64 > 65535) {
+        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^22)",
+                      who, dtype, n_tok, n_ad, n_in, n_out, rank);
+        return true;
+    }
+    if (ldx % 8 || ldy % 8 || a_stride % 8 || b_stride % 8 || (n_tok > 1 && (ldx < n_in || ldy < n_out)) ||
+        (n_ad > 1 && (a_stride < (int64_t)rank * n_in || b_stride < (int64_t)rank * n_out))) {
+        moe_set_error("%s: strides must be multiples of 8 and not less than a row or matrix", who);
+        return true;
+    }
+    return false;
+}
+
+bool bad_pointers(const char* who, std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (!p || (uintptr_t)p % 16) {
+            moe_set_error("%s: a pointer is null or not 16-byte aligned", who);
+            return true;
+        }
+    return false;
+}
+
+uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 }  // namespace
 
@@ -90,32 +228,68 @@ extern "C" int moe_lora_add(const void* base, int64_t ld_base, const void* x, in
                             const void* b, int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad,
                             int n_in, int n_out, int rank, int dtype, void* workspace, void* out, int64_t ld_out,
                             void* stream) {
-    if ((dtype != 0 && dtype != 1) || n_tok < 0 || n_ad < 0 || n_in <= 0 || n_out <= 0 || rank <= 0 || n_in % 8 ||
-        n_out % 8 || rank % 8 || rank > 256) {
-        moe_set_error("lora_add: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256)", dtype,
-                      n_tok, n_ad, n_in, n_out, rank);
-        return -1;
-    }
-    if (ldx % 8 || ld_base % 8 || ld_out % 8 || a_stride % 8 || b_stride % 8 ||
-        (n_tok > 1 && (ldx < n_in || ld_base < n_out || ld_out < n_out)) ||
-        (n_ad > 1 && (a_stride < (int64_t)rank * n_in || b_stride < (int64_t)rank * n_out))) {
-        moe_set_error("lora_add: strides must be multiples of 8 and not less than a row or matrix");
+    const char* who = "lora_add";
+    if (bad_shapes(who, dtype, n_tok, n_ad, n_in, n_out, rank, ldx, ld_base, a_stride, b_stride)) return -1;
+    if (ld_out % 8 || (n_tok > 1 && (ld_out < n_out || (out == base && ld_out != ld_base)))) {
+        moe_set_error("%s: ld_out=%lld (ld_base=%lld)", who, (long long)ld_out, (long long)ld_base);
         return -1;
     }
     if (n_tok == 0) return 0;
-    if (!base || !x || !ids || !out || !workspace || (n_ad > 0 && (!a || !b))) {
-        moe_set_error("lora_add: null pointer");
+    if (!ids) {
+        moe_set_error("%s: ids is null", who);
         return -1;
     }
-    if (((uintptr_t)base | (uintptr_t)x | (uintptr_t)a | (uintptr_t)b | (uintptr_t)out | (uintptr_t)workspace) % 16) {
-        moe_set_error("lora_add: pointers must be 16-byte aligned");
-        return -1;
-    }
-    if (((int64_t)n_tok * rank + 3) / 4 > 0x7FFFFFFF || (n_out + 255) / 256 > 65535) {
-        moe_set_error("lora_add: n_tok=%d x rank=%d or n_out=%d is more than one launch takes", n_tok, rank, n_out);
-        return -1;
-    }
+    if (bad_pointers(who, {base, x, out, workspace}) || (n_ad > 0 && bad_pointers(who, {a, b}))) return -1;
     auto f = dtype ? lora_add<__bf16> : lora_add<_Float16>;
     return f(base, ld_base, x, ldx, a, a_stride, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, (float*)workspace,
              out, ld_out, (hipStream_t)stream);
+}
+
+extern "C" uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank) {
+    if (n_tok < 0 || n_ad < 1 || rank <= 0) return 0;
+    return 2 * up16((uint64_t)n_tok * rank * 2) + 2 * up16((uint64_t)n_tok * 4) + up16((uint64_t)(n_ad + 1) * 4) +
+           moe_expert_plan_workspace_bytes(n_tok, n_ad);
+}
+
+extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* a, int64_t a_stride,
+                             const void* b, int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad,
+                             int n_in, int n_out, int rank, int dtype, void* workspace, void* dx, int64_t lddx, void* da,
+                             void* db, void* stream) {
+    const char* who = "lora_grad";
+    if (bad_shapes(who, dtype, n_tok, n_ad, n_in, n_out, rank, ldx, lddy, a_stride, b_stride)) return -1;
+    if (n_ad < 1 || n_ad > gmm::kMaxSeg || lddx % 8 || (n_tok > 1 && lddx < n_in)) {
+        moe_set_error("%s: n_ad=%d (1..%d) lddx=%lld", who, n_ad, gmm::kMaxSeg, (long long)lddx);
+        return -1;
+    }
+    if (n_tok > 0 && !ids) {
+        moe_set_error("%s: ids is null", who);
+        return -1;
+    }
+    if (bad_pointers(who, {a, b, da, db, workspace}) || (n_tok > 0 && bad_pointers(who, {dy, x, dx}))) return -1;
+    uint8_t* p = (uint8_t*)workspace;
+    auto take = [&](uint64_t bytes) {
+        uint8_t* q = p;
+        p += up16(bytes);
+        return q;
+    };
+    const int64_t mat = (int64_t)rank * n_in;
+    void* v = take((uint64_t)n_tok * rank * 2);
+    void* dv = take((uint64_t)n_tok * rank * 2);
+    int32_t* order = (int32_t*)take((uint64_t)n_tok * 4);
+    int32_t* same = (int32_t*)take((uint64_t)n_tok * 4);
+    int32_t* seg = (int32_t*)take((uint64_t)(n_ad + 1) * 4);
+    // rows sorted by adapter; v and dv are in that order.  Without tokens da and db are the products over empty segments
+    if (moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
+        moe_grouped_mm(x, ldx, n_tok, order, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, v, rank, n_tok,
+                       nullptr, dtype, 1, stream) ||
+        moe_grouped_mm_dx(dy, lddy, n_tok, order, seg, nullptr, n_ad, n_tok, b, b_stride, n_ad, n_out, rank, scale, nullptr, 0,
+                          dv, rank, n_tok, nullptr, dtype, 1, stream) ||
+        moe_grouped_mm_dx(dv, rank, n_tok, nullptr, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, nullptr,
+                          0, dx, lddx, n_tok, order, dtype, 1, stream) ||
+        moe_grouped_mm_dw(dv, rank, n_tok, nullptr, x, ldx, n_tok, order, seg, n_ad, n_tok, rank, n_in, nullptr, da, mat, 0,
+                          dtype, stream) ||
+        moe_grouped_mm_dw(dy, lddy, n_tok, order, v, rank, n_tok, nullptr, seg, n_ad, n_tok, n_out, rank, scale, db,
+                          (int64_t)rank * n_out, 0, dtype, stream))
+        return -1;
+    return 0;
 }

@@ -107,7 +107,8 @@ SIGNATURES: dict[str, tuple] = {
                                  _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
     "moe_pair_combine": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
     # unquantised experts and adapters
-    "moe_expert_plan": (_c_int, [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "moe_expert_plan_workspace_bytes": (_c_u64, [_c_int, _c_int]),
+    "moe_expert_plan": (_c_int, [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
     "moe_grouped_mm": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64, _c_int, _c_int,
                                 _c_int, _c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_int, _c_vp]),
     "moe_grouped_gate_up": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64, _c_int,
@@ -120,6 +121,9 @@ SIGNATURES: dict[str, tuple] = {
     "moe_lora_workspace_bytes": (_c_u64, [_c_int, _c_int]),
     "moe_lora_add": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_int,
                               _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "moe_lora_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int]),
+    "moe_lora_grad": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_int,
+                               _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp]),
     # no reference counterpart
     "c_last_error": (ctypes.c_char_p, []),
     "c_clear_error": (None, []),

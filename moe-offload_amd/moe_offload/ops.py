@@ -210,52 +210,59 @@ def cb_up(x, pool, slots, grid, hidden, inter, h_out=None):
 _HALF = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _on_gpu(who: str, **tensors) -> torch.device:
-    """The one GPU that every given tensor is on."""
+def _one_gpu(who: str, **tensors) -> int:
+    """The index of the one GPU that every given tensor is on."""
     dev = None
     for name, t in tensors.items():
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{who}: {name} must be a tensor, not {type(t).__name__}")
-        _need(t.is_cuda, f"{who}: {name} is on {t.device}, not on a GPU")
-        _need(dev is None or t.device == dev, f"{who}: {name} is on {t.device}, others on {dev}")
-        dev = t.device
+        at = t.get_device()
+        if at < 0:
+            raise ValueError(f"{who}: {name} is on {t.device}, not on a GPU")
+        if dev is None:
+            dev = at
+        elif at != dev:
+            raise ValueError(f"{who}: {name} is on GPU {at}, others on GPU {dev}")
     return dev
 
 
 def _rows(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, width: int | None) -> int:
     """Checks a matrix with contiguous rows; returns the elements from row to row."""
+    shape = t.shape
     if t.dtype != dtype:
         raise TypeError(f"{who}: {name} is {t.dtype}, not {dtype}")
-    _need(t.dim() == 2 and (rows is None or t.shape[0] == rows) and (width is None or t.shape[1] == width),
-          f"{who}: {name} has shape {tuple(t.shape)}, not ({'*' if rows is None else rows}, {'*' if width is None else width})")
-    _need(t.shape[1] % 8 == 0 and t.shape[1] > 0, f"{who}: {name}: rows of {t.shape[1]} elements (a multiple of 8 wanted)")
-    _need(t.stride(1) == 1 or t.numel() == 0, f"{who}: {name}'s rows are not contiguous")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    _need(t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0, f"{who}: {name}'s rows are {t.stride(0)} elements apart")
-    return t.stride(0)
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (width is not None and shape[1] != width):
+        raise ValueError(f"{who}: {name} has shape {tuple(shape)}, not ({'*' if rows is None else rows}, "
+                         f"{'*' if width is None else width})")
+    n, w = shape
+    step, inner = t.stride()
+    if w % 8 or w == 0:
+        raise ValueError(f"{who}: {name}: rows of {w} elements (a multiple of 8 wanted)")
+    if n == 0 or (n == 1 and inner == 1):
+        return w
+    if inner != 1 or step < w or step % 8:
+        raise ValueError(f"{who}: {name}: rows must be contiguous and a multiple of 8 elements apart, not {t.stride()}")
+    return step
 
 
 def _mats(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> int:
     """Checks a stack of contiguous matrices; returns the elements from one to the next."""
+    have = t.shape
     if t.dtype != dtype:
         raise TypeError(f"{who}: {name} is {t.dtype}, not {dtype}")
-    _need(t.dim() == 3 and all(s is None or s == d for s, d in zip(shape, t.shape)),
-          f"{who}: {name} has shape {tuple(t.shape)}, not {tuple('*' if s is None else s for s in shape)}")
-    n, k = t.shape[1:]
-    _need(n > 0 and n % 8 == 0 and k > 0 and k % 8 == 0, f"{who}: {name}: matrices of {n} x {k} (multiples of 8 wanted)")
-    _need(t.numel() == 0 or (t.stride(2) == 1 and t.stride(1) == k), f"{who}: {name}'s matrices are not contiguous")
-    if t.shape[0] <= 1:
+    if len(have) != 3 or any(s is not None and s != d for s, d in zip(shape, have)):
+        raise ValueError(f"{who}: {name} has shape {tuple(have)}, not {tuple('*' if s is None else s for s in shape)}")
+    m, n, k = have
+    if n % 8 or n == 0 or k % 8 or k == 0:
+        raise ValueError(f"{who}: {name}: matrices of {n} x {k} (multiples of 8 wanted)")
+    if m == 0:
         return n * k
-    _need(t.stride(0) >= n * k and t.stride(0) % 8 == 0, f"{who}: {name}'s matrices are {t.stride(0)} elements apart")
-    return t.stride(0)
+    step, row, inner = t.stride()
+    if inner != 1 or row != k or (m > 1 and (step < n * k or step % 8)):
+        raise ValueError(f"{who}: {name}: matrices must be contiguous and a multiple of 8 elements apart, not {t.stride()}")
+    return step if m > 1 else n * k
 
 
 def _index(who: str, name: str, t: torch.Tensor | None, n: int | None = None) -> None:
@@ -263,8 +270,8 @@ def _index(who: str, name: str, t: torch.Tensor | None, n: int | None = None) ->
         return
     if t.dtype != torch.int32:
         raise TypeError(f"{who}: {name} is {t.dtype}, not torch.int32")
-    _need(t.is_contiguous() and (n is None or t.numel() == n), f"{who}: {name} must be contiguous" +
-          ("" if n is None else f" with {n} entries, not {t.numel()}"))
+    if not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{who}: {name} must be contiguous" + ("" if n is None else f" with {n} entries, not {t.numel()}"))
 
 
 def _scale(who: str, t: torch.Tensor | None, n: int) -> None:
@@ -272,20 +279,36 @@ def _scale(who: str, t: torch.Tensor | None, n: int) -> None:
         return
     if t.dtype != torch.float32:
         raise TypeError(f"{who}: scale is {t.dtype}, not torch.float32")
-    _need(t.is_contiguous() and t.numel() == n, f"{who}: scale must be contiguous with {n} entries")
+    if not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{who}: scale must be contiguous with {n} entries")
 
 
 def _half(who: str, t: torch.Tensor) -> int:
-    if t.dtype not in _HALF:
+    dt = _HALF.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{who}: {t.dtype} (torch.float16 and torch.bfloat16 are supported)")
-    return _HALF[t.dtype]
+    return dt
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
-    """Calls an entry point on the tensors' own GPU and its current stream."""
-    with torch.cuda.device(dev):
-        rc = getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _call(name: str, dev: int, *args) -> None:
+    """Calls an entry point on the tensors' own GPU and that GPU's current stream."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, name)
+
+
+def _scratch(nbytes: int, like: torch.Tensor, given: torch.Tensor | None, who: str) -> torch.Tensor:
+    """A call's own scratch: given, or new from torch's allocator (which keeps it for the stream, or the graph)."""
+    if given is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    have = given.numel() * given.element_size()
+    if not given.is_contiguous() or have < nbytes:
+        raise ValueError(f"{who}: a contiguous workspace of {nbytes} bytes is wanted, not {have}")
+    return given
 
 
 def _fresh_rows(n_out_rows: int | None, n_rows: int, width: int, like: torch.Tensor) -> torch.Tensor:
@@ -304,26 +327,32 @@ def expert_plan(ids: torch.Tensor, n_exp: int, row_token: torch.Tensor | None = 
     slot is the expert id and no seg_slot is needed.  Pairs with an id outside 0 .. n_exp - 1 come
     behind the last segment.  n_exp up to 1024.
     """
-    dev = _on_gpu("expert_plan", ids=ids, row_token=row_token, row_out=row_out, seg_start=seg_start)
-    _index("expert_plan", "ids", ids)
-    _need(ids.dim() in (1, 2), f"expert_plan: ids has {ids.dim()} dimensions")
+    who = "expert_plan"
+    dev = _one_gpu(who, ids=ids, row_token=row_token, row_out=row_out, seg_start=seg_start)
+    _index(who, "ids", ids)
+    if ids.dim() not in (1, 2) or not 1 <= n_exp <= 1024:
+        raise ValueError(f"{who}: ids of shape {tuple(ids.shape)}, n_exp={n_exp} (ids [n_tok, k] or [n_tok], n_exp 1..1024)")
     k = ids.shape[1] if ids.dim() == 2 else 1
     m = ids.numel()
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
-    row_token = row_token if row_token is not None else new(m)
-    row_out = row_out if row_out is not None else new(m)
-    _need(1 <= n_exp <= 1024, f"expert_plan: n_exp={n_exp} (1..1024)")
-    seg_start = seg_start if seg_start is not None else new(n_exp + 1)
+    if row_token is None:
+        row_token = torch.empty(m, dtype=torch.int32, device=ids.device)
+    if row_out is None:
+        row_out = torch.empty(m, dtype=torch.int32, device=ids.device)
+    if seg_start is None:
+        seg_start = torch.empty(n_exp + 1, dtype=torch.int32, device=ids.device)
     for name, t, n in (("row_token", row_token, m), ("row_out", row_out, m), ("seg_start", seg_start, n_exp + 1)):
-        _index("expert_plan", name, t, n)
-    _call("moe_expert_plan", dev, _p(ids), m, max(k, 1), n_exp, _p(row_token), _p(row_out), _p(seg_start))
+        _index(who, name, t, n)
+    nb = _lib.lib().moe_expert_plan_workspace_bytes(m, n_exp)
+    ws = _scratch(nb, ids, None, who) if nb else None
+    _call("moe_expert_plan", dev, _p(ids), m, max(k, 1), n_exp, _p(ws), _p(row_token), _p(row_out), _p(seg_start))
     return row_token, row_out, seg_start
 
 
 def _segments(who, seg_start, seg_slot):
     _index(who, "seg_start", seg_start)
-    _need(1 <= seg_start.numel() <= 1025, f"{who}: seg_start has {seg_start.numel()} entries (1..1025)")
     n_seg = seg_start.numel() - 1
+    if not 0 <= n_seg <= 1024:
+        raise ValueError(f"{who}: seg_start has {n_seg + 1} entries (1..1025)")
     _index(who, "seg_slot", seg_slot, n_seg)
     return n_seg
 
@@ -339,7 +368,7 @@ def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_
     zeros, a row_out outside the output is dropped.
     """
     who = "grouped_mm"
-    dev = _on_gpu(who, x=x, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, out=out)
+    dev = _one_gpu(who, x=x, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, out=out)
     dt = _half(who, x)
     n_seg = _segments(who, seg_start, seg_slot)
     w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
@@ -352,10 +381,9 @@ def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_
     fill = out is None
     if fill:
         out = _fresh_rows(n_out_rows, n_rows, N, x)
-    _need(n_out_rows is None or out.shape[0] == n_out_rows, f"{who}: out has {out.shape[0]} rows, not {n_out_rows}")
-    ldy = _rows(who, "out", out, x.dtype, None, N)
-    _need((row_in is not None or n_rows <= x.shape[0]) and (row_out is not None or n_rows <= out.shape[0]),
-          f"{who}: {n_rows} sorted rows, x has {x.shape[0]} and out {out.shape[0]}")
+    ldy = _rows(who, "out", out, x.dtype, n_out_rows, N)
+    if (row_in is None and n_rows > x.shape[0]) or (row_out is None and n_rows > out.shape[0]):
+        raise ValueError(f"{who}: {n_rows} sorted rows, x has {x.shape[0]} and out {out.shape[0]}")
     _call("moe_grouped_mm", dev, _p(x), ldx, x.shape[0], _p(row_in), _p(seg_start), _p(seg_slot), n_seg, n_rows, _p(w),
           w_stride, n_slots, N, K, _p(scale), _p(out), ldy, out.shape[0], _p(row_out), dt, int(fill))
     return out
@@ -370,18 +398,19 @@ def grouped_gate_up(x, row_token, seg_start, w, seg_slot=None, h_out=None, gu_ou
     output and left as they are in a given one.
     """
     who = "grouped_gate_up"
-    dev = _on_gpu(who, x=x, row_token=row_token, seg_start=seg_start, w=w, seg_slot=seg_slot, h_out=h_out, gu_out=gu_out)
+    dev = _one_gpu(who, x=x, row_token=row_token, seg_start=seg_start, w=w, seg_slot=seg_slot, h_out=h_out, gu_out=gu_out)
     dt = _half(who, x)
     n_seg = _segments(who, seg_start, seg_slot)
     w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
     n_slots, N, K = w.shape
-    _need(N % 16 == 0, f"{who}: w has {N} rows per slot: twice a multiple of 8 wanted")
+    if N % 16:
+        raise ValueError(f"{who}: w has {N} rows per slot: twice a multiple of 8 wanted")
     ldx = _rows(who, "x", x, x.dtype, None, K)
     M = row_token.numel() if row_token is not None else x.shape[0]
     _index(who, "row_token", row_token, M)
     fill = h_out is None
     if fill:
-        h_out = torch.empty((M, N // 2), dtype=x.dtype, device=dev)
+        h_out = torch.empty((M, N // 2), dtype=x.dtype, device=x.device)
     ldh = _rows(who, "h_out", h_out, x.dtype, M, N // 2)
     ldgu = _rows(who, "gu_out", gu_out, x.dtype, M, N) if gu_out is not None else 0
     _call("moe_grouped_gate_up", dev, _p(x), ldx, x.shape[0], _p(row_token), _p(seg_start), _p(seg_slot), n_seg, M, _p(w),
@@ -406,7 +435,7 @@ def grouped_mm_dx(dy, seg_start, w, row_in=None, row_out=None, n_out_rows=None, 
     sorted order; the result is then the gradient of (g, u), [*, 2 * K].  Other arguments as grouped_mm.
     """
     who = "grouped_mm_dx"
-    dev = _on_gpu(who, dy=dy, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, gu=gu,
+    dev = _one_gpu(who, dy=dy, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, gu=gu,
                   out=out)
     dt = _half(who, dy)
     n_seg = _segments(who, seg_start, seg_slot)
@@ -422,10 +451,9 @@ def grouped_mm_dx(dy, seg_start, w, row_in=None, row_out=None, n_out_rows=None, 
     fill = out is None
     if fill:
         out = _fresh_rows(n_out_rows, n_rows, width, dy)
-    _need(n_out_rows is None or out.shape[0] == n_out_rows, f"{who}: out has {out.shape[0]} rows, not {n_out_rows}")
-    lddx = _rows(who, "out", out, dy.dtype, None, width)
-    _need((row_in is not None or n_rows <= dy.shape[0]) and (row_out is not None or n_rows <= out.shape[0]),
-          f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and out {out.shape[0]}")
+    lddx = _rows(who, "out", out, dy.dtype, n_out_rows, width)
+    if (row_in is None and n_rows > dy.shape[0]) or (row_out is None and n_rows > out.shape[0]):
+        raise ValueError(f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and out {out.shape[0]}")
     _call("moe_grouped_mm_dx", dev, _p(dy), lddy, dy.shape[0], _p(row_in), _p(seg_start), _p(seg_slot), n_seg, n_rows,
           _p(w), w_stride, n_slots, N, K, _p(scale), _p(gu), ldgu, _p(out), lddx, out.shape[0], _p(row_out), dt, int(fill))
     return out
@@ -439,7 +467,7 @@ def grouped_mm_dw(dy, x, seg_start, row_dy=None, row_x=None, scale=None, dtype=N
     grouped_mm took row_in and row_out, this takes row_x=row_in and row_dy=row_out.
     """
     who = "grouped_mm_dw"
-    dev = _on_gpu(who, dy=dy, x=x, seg_start=seg_start, row_dy=row_dy, row_x=row_x, scale=scale, out=out)
+    dev = _one_gpu(who, dy=dy, x=x, seg_start=seg_start, row_dy=row_dy, row_x=row_x, scale=scale, out=out)
     dt = _half(who, dy)
     n_seg = _segments(who, seg_start, None)
     lddy, ldx = _rows(who, "dy", dy, dy.dtype, None, None), _rows(who, "x", x, dy.dtype, None, None)
@@ -447,14 +475,14 @@ def grouped_mm_dw(dy, x, seg_start, row_dy=None, row_x=None, scale=None, dtype=N
     n_rows = row_dy.numel() if row_dy is not None else row_x.numel() if row_x is not None else dy.shape[0]
     _index(who, "row_dy", row_dy, n_rows)
     _index(who, "row_x", row_x, n_rows)
-    _need((row_dy is not None or n_rows <= dy.shape[0]) and (row_x is not None or n_rows <= x.shape[0]),
-          f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and x {x.shape[0]}")
+    if (row_dy is None and n_rows > dy.shape[0]) or (row_x is None and n_rows > x.shape[0]):
+        raise ValueError(f"{who}: {n_rows} sorted rows, dy has {dy.shape[0]} and x {x.shape[0]}")
     _scale(who, scale, n_seg)
     dtype = dtype if dtype is not None else out.dtype if out is not None else dy.dtype
     if dtype not in (dy.dtype, torch.float32):
         raise TypeError(f"{who}: gradients of {dy.dtype} come as {dy.dtype} or torch.float32, not {dtype}")
     if out is None:
-        out = torch.empty((n_seg, N, K), dtype=dtype, device=dev)
+        out = torch.empty((n_seg, N, K), dtype=dtype, device=dy.device)
     stride = _mats(who, "out", out, dtype, (n_seg, N, K))
     _call("moe_grouped_mm_dw", dev, _p(dy), lddy, dy.shape[0], _p(row_dy), _p(x), ldx, x.shape[0], _p(row_x), _p(seg_start),
           n_seg, n_rows, N, K, _p(scale), _p(out), stride, int(dtype == torch.float32), dt)
@@ -465,9 +493,12 @@ def grouped_mm_dw(dy, x, seg_start, row_dy=None, row_x=None, scale=None, dtype=N
 
 def _lora_args(who, x, a, b, ids, scale):
     dt = _half(who, x)
-    a_stride = _mats(who, "a", a, x.dtype, (None, None, x.shape[-1]))
+    if x.dim() != 2:
+        raise ValueError(f"{who}: x has {x.dim()} dimensions")
+    a_stride = _mats(who, "a", a, x.dtype, (None, None, x.shape[1]))
     n_ad, rank, n_in = a.shape
-    _need(rank <= 256, f"{who}: rank {rank} (up to 256)")
+    if rank > 256:
+        raise ValueError(f"{who}: rank {rank} (up to 256)")
     b_stride = _mats(who, "b", b, x.dtype, (n_ad, None, rank))
     _index(who, "ids", ids, x.shape[0])
     _scale(who, scale, n_ad)
@@ -480,46 +511,44 @@ def lora_add(base, x, a, b, ids, scale=None, out=None, workspace=None):
 
     base: fp16 or bf16 [n_tok, n_out], the shared projection's output; x: same type [n_tok, n_in]; a [n_ad,
     rank, n_in], b [n_ad, n_out, rank] (rank a multiple of 8 up to 256); ids: int32 [n_tok], an id outside
-    the adapters leaves base[t]; scale: fp32 [n_ad] or None.  out=base adds in place.  workspace: uint8
-    scratch of moe_lora_workspace_bytes, for callers that keep one per call in flight.
+    the adapters leaves base[t]; scale: fp32 [n_ad] or None.  out=base adds in place.  workspace: scratch of
+    moe_lora_workspace_bytes, for callers that keep one per call in flight.
     """
     who = "lora_add"
-    dev = _on_gpu(who, base=base, x=x, a=a, b=b, ids=ids, scale=scale, out=out, workspace=workspace)
-    _need(x.dim() == 2, f"{who}: x has {x.dim()} dimensions")
+    dev = _one_gpu(who, base=base, x=x, a=a, b=b, ids=ids, scale=scale, out=out, workspace=workspace)
     dt, n_ad, rank, n_in, n_out, a_stride, b_stride = _lora_args(who, x, a, b, ids, scale)
     n_tok = x.shape[0]
     ldx = _rows(who, "x", x, x.dtype, n_tok, n_in)
     ld_base = _rows(who, "base", base, x.dtype, n_tok, n_out)
     if out is None:
-        out = torch.empty((n_tok, n_out), dtype=x.dtype, device=dev)
+        out = torch.empty((n_tok, n_out), dtype=x.dtype, device=x.device)
     ld_out = _rows(who, "out", out, x.dtype, n_tok, n_out)
-    nb = 4 * n_tok * rank
-    if workspace is None:
-        workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _need(workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= nb,
-          f"{who}: workspace of {workspace.numel() * workspace.element_size()} bytes, {nb} wanted")
+    workspace = _scratch(4 * n_tok * rank, x, workspace, who)
     _call("moe_lora_add", dev, _p(base), ld_base, _p(x), ldx, _p(a), a_stride, _p(b), b_stride, _p(ids), _p(scale), n_tok,
           n_ad, n_in, n_out, rank, dt, _p(workspace), _p(out), ld_out)
     return out
 
 
-def lora_grad(dy, x, a, b, ids, scale=None):
+def lora_grad(dy, x, a, b, ids, scale=None, workspace=None):
     """The gradients of lora_add in x (the adapter's part; base's is dy itself), a and b: (dx, da, db).
 
     With the tokens sorted by adapter: v = a x, dv = scale b^T dy, dx = a^T dv, da = sum dv x^T, db = scale
     sum dy v^T.  v and dv are rounded to the inputs' type, as activations between two layers are.  Tokens
-    without an adapter get dx = 0, adapters without tokens da = db = 0.  At most 1024 adapters.
+    without an adapter get dx = 0, adapters without tokens da = db = 0.  At most 1024 adapters.  workspace:
+    scratch of moe_lora_grad_workspace_bytes.
     """
     who = "lora_grad"
-    _on_gpu(who, dy=dy, x=x, a=a, b=b, ids=ids, scale=scale)
-    _need(x.dim() == 2 and dy.dim() == 2 and dy.shape[0] == x.shape[0], f"{who}: dy {tuple(dy.shape)}, x {tuple(x.shape)}")
-    _, n_ad, _, _, n_out, _, _ = _lora_args(who, x, a, b, ids, scale)
-    _rows(who, "dy", dy, x.dtype, x.shape[0], n_out)
-    _need(1 <= n_ad <= 1024, f"{who}: {n_ad} adapters (1..1024)")
-    _, order, seg = expert_plan(ids.reshape(-1), n_ad)
-    v = grouped_mm(x, seg, a, row_in=order)
-    dv = grouped_mm_dx(dy, seg, b, row_in=order, scale=scale)
-    dx = grouped_mm_dx(dv, seg, a, row_out=order)
-    da = grouped_mm_dw(dv, x, seg, row_x=order)
-    db = grouped_mm_dw(dy, v, seg, row_dy=order, scale=scale)
+    dev = _one_gpu(who, dy=dy, x=x, a=a, b=b, ids=ids, scale=scale, workspace=workspace)
+    dt, n_ad, rank, n_in, n_out, a_stride, b_stride = _lora_args(who, x, a, b, ids, scale)
+    n_tok = x.shape[0]
+    ldx = _rows(who, "x", x, x.dtype, n_tok, n_in)
+    lddy = _rows(who, "dy", dy, x.dtype, n_tok, n_out)
+    if not 1 <= n_ad <= 1024:
+        raise ValueError(f"{who}: {n_ad} adapters (1..1024)")
+    dx = torch.empty((n_tok, n_in), dtype=x.dtype, device=x.device)
+    da = torch.empty((n_ad, rank, n_in), dtype=x.dtype, device=x.device)
+    db = torch.empty((n_ad, n_out, rank), dtype=x.dtype, device=x.device)
+    workspace = _scratch(_lib.lib().moe_lora_grad_workspace_bytes(n_tok, n_ad, rank), x, workspace, who)
+    _call("moe_lora_grad", dev, _p(dy), lddy, _p(x), ldx, _p(a), a_stride, _p(b), b_stride, _p(ids), _p(scale), n_tok, n_ad,
+          n_in, n_out, rank, dt, _p(workspace), _p(dx), n_in, _p(da), _p(db))
     return dx, da, db

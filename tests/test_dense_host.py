@@ -78,7 +78,7 @@ def refused(name, *args):
     return msg
 
 
-PLAN = dict(ids=P, n_ids=20, k=4, n_exp=8, row_token=P, row_out=P, seg_start=P, stream=None)
+PLAN = dict(ids=P, n_ids=20, k=4, n_exp=8, workspace=None, row_token=P, row_out=P, seg_start=P, stream=None)
 MM = dict(x=P, ldx=64, n_x=10, row_in=None, seg_start=P, seg_slot=None, n_seg=2, n_rows=10, w=P, w_stride=4096, n_slots=2, n=64, k=64,
           scale=None, y=P, ldy=64, n_y=10, row_out=None, dtype=1, fill=0, stream=None)
 UP = dict(x=P, ldx=64, n_x=10, row_in=None, seg_start=P, seg_slot=None, n_seg=2, n_rows=10, w=P, w_stride=4096, n_slots=2, inter=32,
@@ -88,12 +88,14 @@ DX = dict(dy=P, lddy=64, n_dy=10, row_in=None, seg_start=P, seg_slot=None, n_seg
 DW = dict(dy=P, lddy=64, n_dy=10, row_dy=None, x=P, ldx=64, n_x=10, row_x=None, seg_start=P, n_seg=2, n_rows=10, n=64, k=64, scale=None,
           dw=P, dw_stride=4096, out_f32=0, dtype=1, stream=None)
 LORA = dict(base=P, ld_base=64, x=P, ldx=64, a=P, a_stride=512, b=P, b_stride=512, ids=P, scale=None, n_tok=4, n_ad=2, n_in=64, n_out=64,
-            rank=8, dtype=1, workspace=P, out=P, ld_out=64, stream=None)
+            rank=8, dtype=1, workspace=P, out=P + 4096, ld_out=64, stream=None)
+GRAD = dict(dy=P, lddy=64, x=P, ldx=64, a=P, a_stride=512, b=P, b_stride=512, ids=P, scale=None, n_tok=4, n_ad=2, n_in=64, n_out=64,
+            rank=8, dtype=1, workspace=P, dx=P, lddx=64, da=P, db=P, stream=None)
 
 
 @pytest.mark.parametrize("name,good,bad", [
     ("moe_expert_plan", PLAN, [dict(n_ids=-4), dict(k=0), dict(k=3), dict(n_exp=0), dict(n_exp=1025), dict(ids=None), dict(row_token=None),
-                               dict(row_out=None), dict(seg_start=None)]),
+                               dict(row_out=None), dict(seg_start=None), dict(n_ids=4100)]),
     ("moe_grouped_mm", MM, [dict(n_seg=-1), dict(n_seg=1025), dict(n_rows=-1), dict(n_rows=11), dict(n_x=9), dict(n_y=9), dict(dtype=2),
                             dict(k=60), dict(n=0), dict(n=-8), dict(n=12), dict(ldx=60), dict(ldx=56), dict(ldx=-64), dict(ldy=56), dict(w_stride=4088),
                             dict(w_stride=4100), dict(x=None), dict(x=P + 2), dict(w=None), dict(w=P + 8), dict(y=None), dict(y=P + 4),
@@ -106,7 +108,12 @@ LORA = dict(base=P, ld_base=64, x=P, ldx=64, a=P, a_stride=512, b=P, b_stride=51
                                dict(seg_start=None), dict(n_seg=1025)]),
     ("moe_lora_add", LORA, [dict(rank=12), dict(rank=0), dict(rank=264), dict(n_in=60), dict(n_out=60), dict(n_tok=-1), dict(n_ad=-1), dict(dtype=2),
                             dict(ldx=56), dict(ldx=60), dict(ld_base=56), dict(ld_out=56), dict(a_stride=504), dict(b_stride=504), dict(a=None),
-                            dict(b=None), dict(ids=None), dict(out=None), dict(base=None), dict(workspace=None), dict(x=P + 2), dict(out=P + 8)]),
+                            dict(b=None), dict(ids=None), dict(out=None), dict(base=None), dict(workspace=None), dict(x=P + 2), dict(out=P + 8),
+                             dict(out=P, ld_out=72), dict(n_out=1 << 23, ld_base=1 << 23, ld_out=1 << 23, b_stride=1 << 26)]),
+    ("moe_lora_grad", GRAD, [dict(rank=12), dict(rank=264), dict(n_in=60), dict(n_out=60), dict(n_tok=-1), dict(n_ad=0), dict(n_ad=1025),
+                             dict(dtype=2), dict(ldx=56), dict(lddy=56), dict(lddx=56), dict(a_stride=504), dict(b_stride=504), dict(a=None),
+                             dict(b=None), dict(ids=None), dict(dx=None), dict(da=None), dict(db=P + 8), dict(workspace=None), dict(workspace=P + 4),
+                             dict(dy=None), dict(x=P + 2)]),
 ])
 def test_entry_points_refuse(name, good, bad):
     for change in bad:
@@ -120,5 +127,8 @@ def test_nothing_to_do_launches_nothing():
     for name, args in (("moe_grouped_mm", {**MM, "n_rows": 0}), ("moe_grouped_gate_up", {**UP, "n_rows": 0}),
                        ("moe_grouped_mm_dx", {**DX, "n_rows": 0}), ("moe_grouped_mm_dw", {**DW, "n_seg": 0}), ("moe_lora_add", {**LORA, "n_tok": 0})):
         assert getattr(lib, name)(*args.values()) == 0 and not _lib.last_error(), name
+    assert lib.moe_expert_plan_workspace_bytes(4096, 512) == 0 and lib.moe_expert_plan_workspace_bytes(4097, 512) == 5 * 513 * 4
+    assert lib.moe_expert_plan_workspace_bytes(2 ** 31 - 1, 1024) == 256 * 1025 * 4
+    assert lib.moe_lora_grad_workspace_bytes(0, 3, 8) == 16
     assert lib.moe_lora_workspace_bytes(5, 16) == 320 and lib.moe_lora_workspace_bytes(0, 16) == 0
     assert ctypes.sizeof(ctypes.c_int64) == 8

@@ -175,6 +175,15 @@ def test_gradients(dtype, tokens, n_ad, rank, n_in, n_out):
         assert torch.equal(got.grad, want)
 
 
+def test_gradients_without_tokens():
+    from moe_offload import ops
+    base, x, a, b, ids, scale = make(torch.bfloat16, 3, 4, 16, 64, 72)
+    dx, da, db = ops.lora_grad(base[:0], x[:0], a, b, ids[:0], scale=scale)
+    assert dx.shape == (0, 64) and not bool(da.any()) and not bool(db.any())
+    dx, da, db = ops.lora_grad(base, x, a, b, torch.full_like(ids, 4), scale=scale)
+    assert not bool(dx.any()) and not bool(da.any()) and not bool(db.any())
+
+
 def test_gradient_against_differences():
     from moe_offload import ops
     dtype = torch.float16
