@@ -46,6 +46,7 @@ struct Args {
     int n_p, n_q, n_out;         // rows of p, q and out that exist
     int np, nq, nc;              // extents: output columns in p (mm_dw) and q, and the contraction
     int out_f32;
+    int span;                    // column tiles per block
 };
 
 template <typename T>
@@ -79,6 +80,7 @@ __device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
 }
 
+constexpr uint64_t kBlocksWanted = 4096;
 constexpr int kBC = 64;                                       // contraction indexes per step
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
@@ -132,8 +134,9 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
     return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
-// BP x BQ results per block of WP x WQ waves.  A step of 64 contraction indexes goes from global memory to LDS
-// without passing registers while the step before it is multiplied: two images, one barrier per step.
+// A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
+// indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
+// next tile's first step during the last of this one: two images, one barrier per step.
 template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
@@ -148,24 +151,26 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
     const int inter = a.nq;                                                    // gate_up, and mm_dx with gu
-    int r0, r1, slot, q0, p0 = 0, nc = a.nc, seg = 0;
+    const int tiles = (a.nq + kQStep - 1) / kQStep, groups = (tiles + a.span - 1) / a.span;
+    int r0, r1, slot, tile, p0 = 0, nc = a.nc, seg = 0;
     if constexpr (OP == kDw) {
-        const int tq = (a.nq + BQ - 1) / BQ, tp = (a.np + BP - 1) / BP;
+        const int tp = (a.np + BP - 1) / BP;
         const uint32_t item = gmm::xcd_order(blockIdx.x, gridDim.x);
-        seg = item / (tq * tp);
-        p0 = (int)(item / tq % tp) * BP;
-        q0 = (int)(item % tq) * BQ;
+        seg = item / (groups * tp);
+        p0 = (int)(item / groups % tp) * BP;
+        tile = (int)(item % groups) * a.span;
         gmm::seg_rows(a.S, seg + 1, r0, r1, slot);
         nc = r1 - r0;
     } else {
-        Tile tile;
-        if (!gmm::find_tile<64 * kWaves>(a.S, BP, (a.nq + kQStep - 1) / kQStep, tile)) return;
-        r0 = tile.r0;
-        r1 = tile.r1;
-        slot = tile.slot;
-        q0 = tile.col * kQStep;
+        Tile at;
+        if (!gmm::find_tile<64 * kWaves>(a.S, BP, groups, at)) return;
+        r0 = at.r0;
+        r1 = at.r1;
+        slot = at.slot;
+        tile = at.col * a.span;
         if (slot < 0 || a.n_p == 0) nc = 0;
     }
+    const int end = tile + a.span < tiles ? tile + a.span : tiles;
     const T* P = (const T*)a.p;
     const T* Q = (const T*)a.q;
     if constexpr (OP != kDw) Q += (int64_t)(slot < 0 ? 0 : slot) * a.ldq;
@@ -185,67 +190,82 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             pp[j] = P + (int64_t)v * a.ldp + cu;
         }
     }
-    if constexpr (!kAlongQ) {
-#pragma unroll
-        for (int j = 0; j < kLoadsQ; ++j) {
-            const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
-            int64_t q;
-            if constexpr (OP == kGateUp) {
-                // a wave's first SQ / 2 subtiles are gate rows, the others the up rows of the same outputs
-                const int sub = row / 16 % SQ;
-                int c = q0 + row / (SQ * 16) * (SQ * 8) + sub % (SQ / 2) * 16 + row % 16;
-                c = c < inter ? c : inter - 1;
-                q = c + (sub < SQ / 2 ? 0 : inter);
-            } else {
-                q = q0 + row < a.nq ? q0 + row : a.nq - 1;
-            }
-            qp[j] = Q + q * a.nc + cu;
-        }
-    }
     constexpr int kUnitsP = BP / 8, kUnitsQ = BQ / 8;                          // ALONG: 16-byte units per row of the image
     auto along_row = [&](int j, int loads, int units) { return (wv * loads + j) * (64 / units) + lane / units; };
     auto along_col = [&](int row, int units) { return (lane % units ^ 2 * turn(row)) * 8; };
-    if constexpr (OP == kDx || OP == kDxGlu) {
+    // this lane's places in q of tile `at`
+    auto start_q = [&](int at) {
+        const int q0 = at * kQStep;
 #pragma unroll
         for (int j = 0; j < kLoadsQ; ++j) {
-            const int row = along_row(j, kLoadsQ, kUnitsQ);
-            const int q = q0 + along_col(row, kUnitsQ);
-            qp[j] = Q + (int64_t)row * a.nq + (q < a.nq ? q : 0);
+            if constexpr (OP == kDw) {
+                const int q = q0 + along_col(along_row(j, kLoadsQ, kUnitsQ), kUnitsQ);
+                qp[j] = Q + (q < a.nq ? q : 0);
+            } else if constexpr (kAlongQ) {
+                const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
+                qp[j] = Q + (int64_t)row * a.nq + (q < a.nq ? q : 0);
+            } else {
+                const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
+                int64_t q;
+                if constexpr (OP == kGateUp) {
+                    // a wave's first SQ / 2 subtiles are gate rows, the others the up rows of the same outputs
+                    const int sub = row / 16 % SQ;
+                    int c = q0 + row / (SQ * 16) * (SQ * 8) + sub % (SQ / 2) * 16 + row % 16;
+                    c = c < inter ? c : inter - 1;
+                    q = c + (sub < SQ / 2 ? 0 : inter);
+                } else {
+                    q = q0 + row < a.nq ? q0 + row : a.nq - 1;
+                }
+                qp[j] = Q + q * a.nc + cu;
+            }
         }
-    }
-    // mm_dw: which rows of dy and x the next step reads (-1: none).  A row that is missing on one side is left out on
-    // both: zeros would still meet an infinity there.
+    };
+    // mm_dw: which rows of dy and x the next step reads.  Loaded a step ahead and looked at where they are used: a
+    // look here would wait for the loads to LDS as well.
     int rp[kLoadsP], rq[kLoadsQ];
     auto next_rows = [&](int c0) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
 #pragma unroll
         for (int j = 0; j < kLoadsP; ++j) {
-            const int c = c0 + along_row(j, kLoadsP, kUnitsP);
-            int v = -1, x = -1;
-            if (c < nc) {
-                v = a.row_p ? a.row_p[r0 + c] : r0 + c;
-                x = a.row_q ? a.row_q[r0 + c] : r0 + c;
-            }
-            const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
-            rp[j] = both ? v : -1;
-            rq[j] = both ? x : -1;
+            int c = c0 + along_row(j, kLoadsP, kUnitsP);
+            c = r0 + (c < nc ? c : nc - 1);
+            rp[j] = a.row_p ? a.row_p[c] : c;
+            rq[j] = a.row_q ? a.row_q[c] : c;
         }
     };
-    auto issue = [&](int c0, uint32_t stage) {
+    if constexpr (kAlongP) {
+#pragma unroll
+        for (int j = 0; j < kLoadsP; ++j) {
+            const int q = p0 + along_col(along_row(j, kLoadsP, kUnitsP), kUnitsP);
+            pp[j] = P + (q < a.np ? q : 0);
+        }
+    }
+    // the step to be loaded next: tile and first contraction index
+    int load_tile = tile, load_c = 0;
+    auto issue = [&](uint32_t stage) {
         const uint32_t lp = lds0 + stage + wv * kLoadsP * 1024, lq = lds0 + stage + kStageP + wv * kLoadsQ * 1024;
+        const int c0 = load_c;
         const bool whole = c0 + kBC <= nc;                                     // wave-uniform
+        load_c += kBC;
+        if (load_c >= nc) {
+            load_c = 0;
+            ++load_tile;
+        }
         if constexpr (OP == kDw) {
+            // a row that is missing on one side is left out on both: zeros would still meet an infinity there
+            int64_t op[kLoadsP], oq[kLoadsQ];
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) {
-                const int row = along_row(j, kLoadsP, kUnitsP), q = p0 + along_col(row, kUnitsP);
-                load_to_lds(rp[j] >= 0 ? P + (int64_t)rp[j] * a.ldp + (q < a.np ? q : 0) : (const T*)&g_zero16, lp + j * 1024);
+                const bool ok = c0 + along_row(j, kLoadsP, kUnitsP) < nc && rp[j] >= 0 && rp[j] < a.n_p && rq[j] >= 0 && rq[j] < a.n_q;
+                op[j] = ok ? rp[j] * a.ldp : -1;
+                oq[j] = ok ? rq[j] * a.ldq : -1;
             }
 #pragma unroll
-            for (int j = 0; j < kLoadsQ; ++j) {
-                const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
-                load_to_lds(rq[j] >= 0 ? Q + (int64_t)rq[j] * a.ldq + (q < a.nq ? q : 0) : (const T*)&g_zero16, lq + j * 1024);
-            }
-            next_rows(c0 + kBC);
+            for (int j = 0; j < kLoadsP; ++j) load_to_lds(op[j] >= 0 ? pp[j] + op[j] : (const T*)&g_zero16, lp + j * 1024);
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) load_to_lds(oq[j] >= 0 ? qp[j] + oq[j] : (const T*)&g_zero16, lq + j * 1024);
+            if (nc > kBC) next_rows(load_c);
+            if (load_c == 0) start_q(load_tile);
         } else {
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) {
@@ -262,6 +282,11 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
                     qp[j] += kBC;
                 }
             }
+            if (load_c == 0 && load_tile < end) {
+#pragma unroll
+                for (int j = 0; j < kLoadsP; ++j) pp[j] -= c0 + kBC;
+                start_q(load_tile);
+            }
         }
     };
 
@@ -270,158 +295,169 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     Frags<kAlongQ, BQ, SQ> fq;
     fp.init(lds0, wp * SP * 16, lane);
     fq.init(lds0 + kStageP, wq * SQ * 16, lane);
-    f32x4 acc[SP][SQ] = {};
-    if constexpr (OP == kDw) next_rows(0);
-    if (nc > 0) issue(0, 0);
-    for (int c0 = 0; c0 < nc; c0 += kBC) {
-        const uint32_t stage = c0 / kBC % 2 * kStage;
-        // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so
-        // are everyone's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (c0 + kBC < nc) issue(c0 + kBC, kStage - stage);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            uint4 vp[SP], vq[SQ];
-#pragma unroll
-            for (int j = 0; j < SQ; ++j) vq[j] = fq.read(stage, j, ks);
-#pragma unroll
-            for (int i = 0; i < SP; ++i) vp[i] = fp.read(stage, i, ks);
-#pragma unroll
-            for (int i = 0; i < SP; ++i)
-#pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[j], vp[i], acc[i][j]);
-        }
-    }
     const float s = a.scale && slot >= 0 ? a.scale[slot] : 1.0f;
     // 16-byte stores: lane (n, kq) of a pair of subtiles holds columns 8 (kq / 2) .. + 7 of subtile kq % 2
     const int pair_col = (kq & 1) * 16 + (kq >> 1) * 8;
+    uint32_t stage = 0;
+    if (nc > 0) {
+        if constexpr (OP == kDw) next_rows(0);
+        start_q(tile);
+        issue(0);
+    }
+#pragma unroll 1
+    for (; tile < end; ++tile) {
+        const int q0 = tile * kQStep;
+        f32x4 acc[SP][SQ] = {};
+#pragma unroll 1
+        for (int c0 = 0; c0 < nc; c0 += kBC) {
+            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so
+            // are everyone's
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (load_tile < end) issue(kStage - stage);
 #pragma unroll
-    for (int i = 0; i < SP; ++i) {
-        const int m = wp * SP * 16 + i * 16 + n;
-        if constexpr (OP == kDw) {
-            const int64_t row = (int64_t)seg * a.ldo + (int64_t)(p0 + m) * a.nq;
-            const bool live = p0 + m < a.np;
-            if (a.out_f32) {
+            for (int ks = 0; ks < 2; ++ks) {
+                uint4 vp[SP], vq[SQ];
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) {
-                    const int q = q0 + wq * SQ * 16 + j * 16 + kq * 4;
-                    if (live && q < a.nq)
-                        *(float4*)((float*)a.out + row + q) = make_float4(acc[i][j][0] * s, acc[i][j][1] * s, acc[i][j][2] * s, acc[i][j][3] * s);
+                for (int j = 0; j < SQ; ++j) vq[j] = fq.read(stage, j, ks);
+#pragma unroll
+                for (int i = 0; i < SP; ++i) vp[i] = fp.read(stage, i, ks);
+#pragma unroll
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[j], vp[i], acc[i][j]);
+            }
+            stage = kStage - stage;
+        }
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+            const int m = wp * SP * 16 + i * 16 + n;
+            if constexpr (OP == kDw) {
+                const int64_t row = (int64_t)seg * a.ldo + (int64_t)(p0 + m) * a.nq;
+                const bool live = p0 + m < a.np;
+                if (a.out_f32) {
+#pragma unroll
+                    for (int j = 0; j < SQ; ++j) {
+                        const int q = q0 + wq * SQ * 16 + j * 16 + kq * 4;
+                        if (live && q < a.nq)
+                            *(float4*)((float*)a.out + row + q) = make_float4(acc[i][j][0] * s, acc[i][j][1] * s, acc[i][j][2] * s, acc[i][j][3] * s);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < SQ; j += 2) {
+                        const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
+                        const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
+                        if (live && q < a.nq) *(uint4*)((T*)a.out + row + q) = v;
+                    }
+                }
+                continue;
+            }
+            const int r = r0 + m;
+            bool live = r < r1, dead = slot < 0;
+            int o = r;
+            if (live) {
+                if (a.row_p) {
+                    const int v = a.row_p[r];
+                    dead |= v < 0 || v >= a.n_p;
+                }
+                if (OP != kGateUp && a.row_out) o = a.row_out[r];
+                if (OP != kGateUp) live = o >= 0 && o < a.n_out;
+            }
+            if constexpr (OP == kGateUp) {
+                uint2 h[SQ / 2], g2[SQ / 2], u2[SQ / 2];
+#pragma unroll
+                for (int j = 0; j < SQ / 2; ++j) {
+                    f32x4 g = acc[i][j], u = acc[i][j + SQ / 2], hv;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        g[e] = dead ? 0.f : g[e];
+                        u[e] = dead ? 0.f : u[e];
+                        hv[e] = g[e] / (1.0f + __expf(-g[e])) * u[e];
+                    }
+                    h[j] = round4<T>(hv);
+                    g2[j] = round4<T>(g);
+                    u2[j] = round4<T>(u);
+                }
+                if constexpr (SQ / 2 == 1) {
+                    const int c = q0 + wq * 16 + kq * 4;
+                    if (live && c < inter) {
+                        *(uint2*)((T*)a.out + (int64_t)r * a.ldo + c) = h[0];
+                        if (a.gu_out) {
+                            *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = g2[0];
+                            *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = u2[0];
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < SQ / 2; j += 2) {
+                        const int c = q0 + wq * SQ * 8 + j * 16 + pair_col;
+                        const uint4 vh = pair8(h[j], h[j + 1]);
+                        if (live && c < inter) *(uint4*)((T*)a.out + (int64_t)r * a.ldo + c) = vh;
+                        if (a.gu_out) {
+                            const uint4 vg = pair8(g2[j], g2[j + 1]), vu = pair8(u2[j], u2[j + 1]);
+                            if (live && c < inter) {
+                                *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = vg;
+                                *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = vu;
+                            }
+                        }
+                    }
+                }
+            } else if constexpr (OP == kDxGlu) {
+#pragma unroll
+                for (int j = 0; j < SQ; j += 2) {
+                    uint2 dg[2], du[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int q = q0 + wq * SQ * 16 + (j + b) * 16 + kq * 4;
+                        f32x4 g = {}, u = {}, vg, vu;
+                        if (live && !dead && q < inter) {
+                            const T* gr = (const T*)a.gu + (int64_t)r * a.ldgu + q;
+                            g = widen4<T>(*(const uint2*)gr);
+                            u = widen4<T>(*(const uint2*)(gr + inter));
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float dh = dead ? 0.f : acc[i][j + b][e] * s, sg = 1.0f / (1.0f + __expf(-g[e]));
+                            vg[e] = dh * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
+                            vu[e] = dh * g[e] * sg;
+                        }
+                        dg[b] = round4<T>(vg);
+                        du[b] = round4<T>(vu);
+                    }
+                    const uint4 vg = pair8(dg[0], dg[1]), vu = pair8(du[0], du[1]);
+                    const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
+                    if (live && q < inter) {
+                        T* d = (T*)a.out + (int64_t)o * a.ldo + q;
+                        *(uint4*)d = vg;
+                        *(uint4*)(d + inter) = vu;
+                    }
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < SQ; j += 2) {
-                    const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
+                    const f32x4 zero = {};
+                    const uint4 v = pair8(round4<T>(dead ? zero : acc[i][j] * s), round4<T>(dead ? zero : acc[i][j + 1] * s));
                     const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                    if (live && q < a.nq) *(uint4*)((T*)a.out + row + q) = v;
+                    if (live && q < a.nq) *(uint4*)((T*)a.out + (int64_t)o * a.ldo + q) = v;
                 }
-            }
-            continue;
-        }
-        const int r = r0 + m;
-        bool live = r < r1, dead = slot < 0;
-        int o = r;
-        if (live) {
-            if (a.row_p) {
-                const int v = a.row_p[r];
-                dead |= v < 0 || v >= a.n_p;
-            }
-            if (OP != kGateUp && a.row_out) o = a.row_out[r];
-            if (OP != kGateUp) live = o >= 0 && o < a.n_out;
-        }
-        if constexpr (OP == kGateUp) {
-            uint2 h[SQ / 2], g2[SQ / 2], u2[SQ / 2];
-#pragma unroll
-            for (int j = 0; j < SQ / 2; ++j) {
-                f32x4 g = acc[i][j], u = acc[i][j + SQ / 2], hv;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    g[e] = dead ? 0.f : g[e];
-                    u[e] = dead ? 0.f : u[e];
-                    hv[e] = g[e] / (1.0f + __expf(-g[e])) * u[e];
-                }
-                h[j] = round4<T>(hv);
-                g2[j] = round4<T>(g);
-                u2[j] = round4<T>(u);
-            }
-            if constexpr (SQ / 2 == 1) {
-                const int c = q0 + wq * 16 + kq * 4;
-                if (live && c < inter) {
-                    *(uint2*)((T*)a.out + (int64_t)r * a.ldo + c) = h[0];
-                    if (a.gu_out) {
-                        *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = g2[0];
-                        *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = u2[0];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < SQ / 2; j += 2) {
-                    const int c = q0 + wq * SQ * 8 + j * 16 + pair_col;
-                    const uint4 vh = pair8(h[j], h[j + 1]);
-                    if (live && c < inter) *(uint4*)((T*)a.out + (int64_t)r * a.ldo + c) = vh;
-                    if (a.gu_out) {
-                        const uint4 vg = pair8(g2[j], g2[j + 1]), vu = pair8(u2[j], u2[j + 1]);
-                        if (live && c < inter) {
-                            *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = vg;
-                            *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = vu;
-                        }
-                    }
-                }
-            }
-        } else if constexpr (OP == kDxGlu) {
-#pragma unroll
-            for (int j = 0; j < SQ; j += 2) {
-                uint2 dg[2], du[2];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int q = q0 + wq * SQ * 16 + (j + b) * 16 + kq * 4;
-                    f32x4 g = {}, u = {}, vg, vu;
-                    if (live && !dead && q < inter) {
-                        const T* gr = (const T*)a.gu + (int64_t)r * a.ldgu + q;
-                        g = widen4<T>(*(const uint2*)gr);
-                        u = widen4<T>(*(const uint2*)(gr + inter));
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float dh = dead ? 0.f : acc[i][j + b][e] * s, sg = 1.0f / (1.0f + __expf(-g[e]));
-                        vg[e] = dh * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
-                        vu[e] = dh * g[e] * sg;
-                    }
-                    dg[b] = round4<T>(vg);
-                    du[b] = round4<T>(vu);
-                }
-                const uint4 vg = pair8(dg[0], dg[1]), vu = pair8(du[0], du[1]);
-                const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                if (live && q < inter) {
-                    T* d = (T*)a.out + (int64_t)o * a.ldo + q;
-                    *(uint4*)d = vg;
-                    *(uint4*)(d + inter) = vu;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < SQ; j += 2) {
-                const f32x4 zero = {};
-                const uint4 v = pair8(round4<T>(dead ? zero : acc[i][j] * s), round4<T>(dead ? zero : acc[i][j + 1] * s));
-                const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                if (live && q < a.nq) *(uint4*)((T*)a.out + (int64_t)o * a.ldo + q) = v;
             }
         }
     }
 }
 
 template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
-int launch_tiles(const Args& a, hipStream_t s) {
-    uint64_t blocks;
+int launch_tiles(Args a, hipStream_t s) {
+    const int qstep = OP == kGateUp ? BQ / 2 : BQ, tiles = (a.nq + qstep - 1) / qstep;
+    uint64_t rows;                                            // tiles in p, at most
     if constexpr (OP == kDw) {
-        blocks = (uint64_t)a.S.n_seg * ((a.nq + BQ - 1) / BQ) * ((a.np + BP - 1) / BP);
+        rows = (uint64_t)a.S.n_seg * ((a.np + BP - 1) / BP);
     } else {
-        const int qstep = OP == kGateUp ? BQ / 2 : BQ;
-        const uint64_t segs = (uint64_t)(a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
-        blocks = ((uint64_t)a.S.n_rows / BP + segs) * ((a.nq + qstep - 1) / qstep);
+        rows = (uint64_t)a.S.n_rows / BP + (uint64_t)(a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
     }
+    const uint64_t span = rows * tiles / kBlocksWanted;
+    a.span = span < 1 ? 1 : span > (uint64_t)tiles ? tiles : (int)span;
+    const uint64_t blocks = rows * ((tiles + a.span - 1) / a.span);
     if (blocks > 0x7FFFFFFFu) {
         moe_set_error("grouped product: %llu tiles are more than one launch takes", (unsigned long long)blocks);
         return -1;
