@@ -18,6 +18,8 @@
 // so a lane of the result holds four adjacent q of one p.
 #include <hip/hip_bf16.h>
 
+#include <algorithm>
+
 #include "grouped_mm.h"
 
 namespace {
@@ -80,7 +82,6 @@ __device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
 }
 
-constexpr uint64_t kBlocksWanted = 4096;
 constexpr int kBC = 64;                                       // contraction indexes per step
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
@@ -89,7 +90,7 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 __device__ __forceinline__ int turn(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
 
 // One operand's fragments for v_mfma_f32_16x16x32: lane (n, kq) holds c = 32 ks + 8 kq .. + 7 of row / column n.
-// ALONG false: the image has a row per tile row, kBC values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
+// ALONG false: the image has a row per tile row, 64 values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
 // ALONG true: a row per c, W values each, read transposed by ds_read_b64_tr_b16 (lane i of 16 gives the address of
 // 4 columns of row i / 4 and receives column i of 4 rows).
 template <bool ALONG, int W, int SUBS>
@@ -141,7 +142,7 @@ template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
     constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
-    constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;      // 1 KiB each
+    constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;        // 1 KiB each
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
@@ -175,55 +176,21 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     const T* Q = (const T*)a.q;
     if constexpr (OP != kDw) Q += (int64_t)(slot < 0 ? 0 : slot) * a.ldq;
 
-    // this lane's 16 bytes of each of its wave's loads.  Rows past the tile, and rows that do not exist, read some
-    // row that does: their results are not stored, or replaced by zeros.
+    // Where this lane's 16 bytes of each of its wave's next loads are.  Rows past the tile, and rows that do not
+    // exist, read some row that does: their results are not stored, or replaced by zeros.  Contraction indexes past
+    // the end read zeros.
+    const T* zero = (const T*)&g_zero16;
+    asm("" : "+s"(zero));                                                      // kept in registers
     const T* pp[kLoadsP];
     const T* qp[kLoadsQ];
-    const int cu = ((lane & 7) ^ (lane >> 3)) * 8;                             // not ALONG: first c of the 16 bytes
-    if constexpr (!kAlongP) {
-#pragma unroll
-        for (int j = 0; j < kLoadsP; ++j) {
-            int r = r0 + (wv * kLoadsP + j) * 8 + (lane >> 3);
-            r = r < r1 ? r : r1 - 1;
-            int v = a.row_p ? a.row_p[r] : r;
-            v = v >= 0 && v < a.n_p ? v : 0;
-            pp[j] = P + (int64_t)v * a.ldp + cu;
-        }
-    }
     constexpr int kUnitsP = BP / 8, kUnitsQ = BQ / 8;                          // ALONG: 16-byte units per row of the image
+    const int cu = ((lane & 7) ^ (lane >> 3)) * 8;                             // not ALONG: first c of the 16 bytes
     auto along_row = [&](int j, int loads, int units) { return (wv * loads + j) * (64 / units) + lane / units; };
     auto along_col = [&](int row, int units) { return (lane % units ^ 2 * turn(row)) * 8; };
-    // this lane's places in q of tile `at`
-    auto start_q = [&](int at) {
-        const int q0 = at * kQStep;
-#pragma unroll
-        for (int j = 0; j < kLoadsQ; ++j) {
-            if constexpr (OP == kDw) {
-                const int q = q0 + along_col(along_row(j, kLoadsQ, kUnitsQ), kUnitsQ);
-                qp[j] = Q + (q < a.nq ? q : 0);
-            } else if constexpr (kAlongQ) {
-                const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
-                qp[j] = Q + (int64_t)row * a.nq + (q < a.nq ? q : 0);
-            } else {
-                const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
-                int64_t q;
-                if constexpr (OP == kGateUp) {
-                    // a wave's first SQ / 2 subtiles are gate rows, the others the up rows of the same outputs
-                    const int sub = row / 16 % SQ;
-                    int c = q0 + row / (SQ * 16) * (SQ * 8) + sub % (SQ / 2) * 16 + row % 16;
-                    c = c < inter ? c : inter - 1;
-                    q = c + (sub < SQ / 2 ? 0 : inter);
-                } else {
-                    q = q0 + row < a.nq ? q0 + row : a.nq - 1;
-                }
-                qp[j] = Q + q * a.nc + cu;
-            }
-        }
-    };
-    // mm_dw: which rows of dy and x the next step reads.  Loaded a step ahead and looked at where they are used: a
-    // look here would wait for the loads to LDS as well.
+    // mm_dw: the rows of dy and x of a step, loaded two steps ahead of their use in the product.  Otherwise the rows
+    // of x or dy, the same in every step.
     int rp[kLoadsP], rq[kLoadsQ];
-    auto next_rows = [&](int c0) {
+    auto step_rows = [&](int c0) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
 #pragma unroll
         for (int j = 0; j < kLoadsP; ++j) {
@@ -233,62 +200,75 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             rq[j] = a.row_q ? a.row_q[c] : c;
         }
     };
-    if constexpr (kAlongP) {
+    if constexpr (OP != kDw) {
 #pragma unroll
         for (int j = 0; j < kLoadsP; ++j) {
-            const int q = p0 + along_col(along_row(j, kLoadsP, kUnitsP), kUnitsP);
-            pp[j] = P + (q < a.np ? q : 0);
+            int r = r0 + (wv * kLoadsP + j) * 8 + (lane >> 3);
+            r = r < r1 ? r : r1 - 1;
+            const int v = a.row_p ? a.row_p[r] : r;
+            rp[j] = v >= 0 && v < a.n_p ? v : 0;
         }
     }
-    // the step to be loaded next: tile and first contraction index
-    int load_tile = tile, load_c = 0;
-    auto issue = [&](uint32_t stage) {
-        const uint32_t lp = lds0 + stage + wv * kLoadsP * 1024, lq = lds0 + stage + kStageP + wv * kLoadsQ * 1024;
-        const int c0 = load_c;
-        const bool whole = c0 + kBC <= nc;                                     // wave-uniform
+    int load_tile = tile, load_c = 0;                                          // the step that is loaded next
+    auto place = [&]() {
+        const bool any = load_tile < end;
+        const int q0 = load_tile * kQStep;
+        if constexpr (OP == kDw) {
+            // a row that is missing on one side is left out on both: zeros would still meet an infinity there
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) {
+                const int row = along_row(j, kLoadsP, kUnitsP), col = along_col(row, kUnitsP);
+                const bool ok = any && load_c + row < nc && rp[j] >= 0 && rp[j] < a.n_p && rq[j] >= 0 && rq[j] < a.n_q;
+                pp[j] = ok ? P + rp[j] * a.ldp + (p0 + col < a.np ? p0 + col : 0) : zero;
+                qp[j] = ok ? Q + rq[j] * a.ldq + (q0 + col < a.nq ? q0 + col : 0) : zero;
+            }
+        } else {
+            const bool ok = any && load_c + cu < nc;
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) pp[j] = ok ? P + rp[j] * a.ldp + load_c + cu : zero;
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) {
+                if constexpr (kAlongQ) {
+                    const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
+                    qp[j] = any && load_c + row < nc ? Q + (int64_t)(load_c + row) * a.nq + (q < a.nq ? q : 0) : zero;
+                } else {
+                    const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
+                    int64_t q;
+                    if constexpr (OP == kGateUp) {
+                        // a wave's first SQ / 2 subtiles are gate rows, the others the up rows of the same outputs
+                        const int sub = row / 16 % SQ;
+                        int c = q0 + row / (SQ * 16) * (SQ * 8) + sub % (SQ / 2) * 16 + row % 16;
+                        c = c < inter ? c : inter - 1;
+                        q = c + (sub < SQ / 2 ? 0 : inter);
+                    } else {
+                        q = q0 + row < a.nq ? q0 + row : a.nq - 1;
+                    }
+                    qp[j] = ok ? Q + q * a.nc + load_c + cu : zero;
+                }
+            }
+        }
+    };
+    auto advance = [&]() {
         load_c += kBC;
+        if (OP != kDw && load_tile < end && load_c + kBC <= nc) {                // wave-uniform; past the end all stay at zero
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) pp[j] += kBC;
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) qp[j] += kAlongQ ? (int64_t)kBC * a.nq : kBC;
+            return;
+        }
         if (load_c >= nc) {
             load_c = 0;
             ++load_tile;
         }
-        if constexpr (OP == kDw) {
-            // a row that is missing on one side is left out on both: zeros would still meet an infinity there
-            int64_t op[kLoadsP], oq[kLoadsQ];
-#pragma unroll
-            for (int j = 0; j < kLoadsP; ++j) {
-                const bool ok = c0 + along_row(j, kLoadsP, kUnitsP) < nc && rp[j] >= 0 && rp[j] < a.n_p && rq[j] >= 0 && rq[j] < a.n_q;
-                op[j] = ok ? rp[j] * a.ldp : -1;
-                oq[j] = ok ? rq[j] * a.ldq : -1;
-            }
-#pragma unroll
-            for (int j = 0; j < kLoadsP; ++j) load_to_lds(op[j] >= 0 ? pp[j] + op[j] : (const T*)&g_zero16, lp + j * 1024);
-#pragma unroll
-            for (int j = 0; j < kLoadsQ; ++j) load_to_lds(oq[j] >= 0 ? qp[j] + oq[j] : (const T*)&g_zero16, lq + j * 1024);
-            if (nc > kBC) next_rows(load_c);
-            if (load_c == 0) start_q(load_tile);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kLoadsP; ++j) {
-                load_to_lds(whole || c0 + cu < nc ? pp[j] : (const T*)&g_zero16, lp + j * 1024);
-                pp[j] += kBC;
-            }
-#pragma unroll
-            for (int j = 0; j < kLoadsQ; ++j) {
-                if constexpr (kAlongQ) {
-                    load_to_lds(whole || c0 + along_row(j, kLoadsQ, kUnitsQ) < nc ? qp[j] : (const T*)&g_zero16, lq + j * 1024);
-                    qp[j] += (int64_t)kBC * a.nq;
-                } else {
-                    load_to_lds(whole || c0 + cu < nc ? qp[j] : (const T*)&g_zero16, lq + j * 1024);
-                    qp[j] += kBC;
-                }
-            }
-            if (load_c == 0 && load_tile < end) {
-#pragma unroll
-                for (int j = 0; j < kLoadsP; ++j) pp[j] -= c0 + kBC;
-                start_q(load_tile);
-            }
-        }
+        place();
+        if (OP == kDw && nc > kBC) step_rows(load_c + kBC < nc ? load_c + kBC : 0);
     };
+    auto load = [&](int d, uint32_t stage) {
+        if (d < kLoadsP) load_to_lds(pp[d], lds0 + stage + (wv * kLoadsP + d) * 1024);
+        else load_to_lds(qp[d - kLoadsP], lds0 + stage + kStageP + (wv * kLoadsQ + d - kLoadsP) * 1024);
+    };
+    constexpr int kLoads = kLoadsP + kLoadsQ;
 
     const int wp = wv / WQ, wq = wv % WQ, n = lane & 15, kq = lane >> 4;
     Frags<kAlongP, BP, SP> fp;
@@ -298,11 +278,30 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     const float s = a.scale && slot >= 0 ? a.scale[slot] : 1.0f;
     // 16-byte stores: lane (n, kq) of a pair of subtiles holds columns 8 (kq / 2) .. + 7 of subtile kq % 2
     const int pair_col = (kq & 1) * 16 + (kq >> 1) * 8;
+    // the output row of this lane's row in each subtile (-1: none); bit i of dead: its results are zeros
+    int orow[SP];
+    uint32_t dead_rows = 0;
+    if constexpr (OP != kDw) {
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+            const int r = r0 + wp * SP * 16 + i * 16 + n;
+            orow[i] = -1;
+            if (r < r1) {
+                const int v = a.row_p ? a.row_p[r] : 0, o = a.row_out ? a.row_out[r] : r;
+                if (slot < 0 || (a.row_p && (v < 0 || v >= a.n_p))) dead_rows |= 1u << i;
+                orow[i] = o < a.n_out ? o : -1;
+            }
+        }
+    }
     uint32_t stage = 0;
     if (nc > 0) {
-        if constexpr (OP == kDw) next_rows(0);
-        start_q(tile);
-        issue(0);
+        if constexpr (OP == kDw) step_rows(0);
+        place();
+#pragma unroll
+        for (int d = 0; d < kLoads; ++d) load(d, 0);
+        if constexpr (OP == kDw)
+            if (nc > kBC) step_rows(kBC);
+        advance();
     }
 #pragma unroll 1
     for (; tile < end; ++tile) {
@@ -310,24 +309,47 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
         f32x4 acc[SP][SQ] = {};
 #pragma unroll 1
         for (int c0 = 0; c0 < nc; c0 += kBC) {
-            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so
-            // are everyone's
+            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier,
+            // so are everyone's
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (load_tile < end) issue(kStage - stage);
+            if constexpr (OP == kDw) {
+                // here no load is under way that the compiler's wait for these could take in
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                uint4 vp[SP], vq[SQ];
-#pragma unroll
-                for (int j = 0; j < SQ; ++j) vq[j] = fq.read(stage, j, ks);
-#pragma unroll
-                for (int i = 0; i < SP; ++i) vp[i] = fp.read(stage, i, ks);
-#pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[j], vp[i], acc[i][j]);
+                for (int j = 0; j < kLoadsP; ++j) asm volatile("" : "+v"(rp[j]), "+v"(rq[j]));
             }
+            // The step's second half is read from LDS, and the next step's loads are issued, between the first half's
+            // products, row by row (past the last step they fetch zeros that nobody reads)
+            uint4 vp[2][SP], vq[2][SQ];
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) vq[0][j] = fq.read(stage, j, 0);
+#pragma unroll
+            for (int i = 0; i < SP; ++i) vp[0][i] = fp.read(stage, i, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < SP; ++i) {
+                // (of eight rows from the middle on: by then half of the first half's registers are free)
+                constexpr int kFrom = SP > 4 ? SP / 2 : 0, kEach = SP > 4 ? 2 : 1;
+                if (i == kFrom) {
+#pragma unroll
+                    for (int j = 0; j < SQ; ++j) vq[1][j] = fq.read(stage, j, 1);
+                }
+                if (i >= kFrom) {
+#pragma unroll
+                    for (int e = (i - kFrom) * kEach; e < (i - kFrom + 1) * kEach; ++e) vp[1][e] = fp.read(stage, e, 1);
+                }
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+#pragma unroll
+                for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, kStage - stage);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance();
+#pragma unroll
+            for (int i = 0; i < SP; ++i)
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
             stage = kStage - stage;
         }
 #pragma unroll
@@ -353,17 +375,8 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
                 }
                 continue;
             }
-            const int r = r0 + m;
-            bool live = r < r1, dead = slot < 0;
-            int o = r;
-            if (live) {
-                if (a.row_p) {
-                    const int v = a.row_p[r];
-                    dead |= v < 0 || v >= a.n_p;
-                }
-                if (OP != kGateUp && a.row_out) o = a.row_out[r];
-                if (OP != kGateUp) live = o >= 0 && o < a.n_out;
-            }
+            const int r = r0 + m, o = orow[i];
+            const bool live = o >= 0, dead = dead_rows >> i & 1;
             if constexpr (OP == kGateUp) {
                 uint2 h[SQ / 2], g2[SQ / 2], u2[SQ / 2];
 #pragma unroll
@@ -444,35 +457,65 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             }
         }
     }
+    // the last step's loads write LDS that is another block's once this one has ended
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
+
+// Row tiles of a call as far as the host knows it: a segment's last tile is half full on average.
+int64_t row_tiles(const Args& a, int bp) { return (a.S.n_rows + (int64_t)(a.S.n_seg - 1) * (bp / 2) + bp - 1) / bp; }
 
 template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 int launch_tiles(Args a, hipStream_t s) {
     const int qstep = OP == kGateUp ? BQ / 2 : BQ, tiles = (a.nq + qstep - 1) / qstep;
-    uint64_t rows;                                            // tiles in p, at most
+    int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
     if constexpr (OP == kDw) {
-        rows = (uint64_t)a.S.n_seg * ((a.np + BP - 1) / BP);
+        rows = most = (int64_t)a.S.n_seg * ((a.np + BP - 1) / BP);
+        steps = a.S.n_rows / a.S.n_seg / kBC + 1;
     } else {
-        rows = (uint64_t)a.S.n_rows / BP + (uint64_t)(a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
+        rows = row_tiles(a, BP);
+        most = (int64_t)a.S.n_rows / BP + (a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
+        steps = (a.nc + kBC - 1) / kBC;
     }
-    const uint64_t span = rows * tiles / kBlocksWanted;
-    a.span = span < 1 ? 1 : span > (uint64_t)tiles ? tiles : (int)span;
-    const uint64_t blocks = rows * ((tiles + a.span - 1) / a.span);
-    if (blocks > 0x7FFFFFFFu) {
-        moe_set_error("grouped product: %llu tiles are more than one launch takes", (unsigned long long)blocks);
+    // Column tiles per block: short tiles share one block's start (the search for its rows, the first load's way) while
+    // that leaves 1024 blocks.  us per launch at 1, 2, 4 and 16 tiles: weights' gradient 4096 x 1024 of 16 x 256 rows (4
+    // steps) 75, 68, 65, -, 1024 x 2048 of 512 x 40 rows (1 step) 871, -, 632, 606; mm 4096 x 1024 of 16 x 512 rows (16
+    // steps) 85, 80, -, -.  Tiles of 64 rows wait for memory and have three blocks per CU to do so: mm_dx 1024 x 2048 of
+    // 512 x 40 rows (16 steps) 514 and, at 3 tiles, 540.
+    const int64_t target = OP == kDw ? 16 : BP == 64 ? 8 : 32;
+    const int64_t span = std::min(target / steps, rows * tiles / 1024);
+    a.span = (int)std::max<int64_t>(1, std::min<int64_t>(span, tiles));
+    const int64_t groups = (tiles + a.span - 1) / a.span;
+    if (most > 0x7FFFFFFF / groups) {
+        moe_set_error("grouped product: %lld x %lld tiles are more than one launch takes", (long long)most, (long long)groups);
         return -1;
     }
-    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
+    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)(most * groups)), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
 }
 
+// Tiles of 256 x 256 (one block per CU) multiply 1.3 times as fast as tiles of 128 x 128 (two per CU) once every CU has
+// one, but there are a quarter of them: TFLOP/s of 128 and 256, bf16, 16 segments: mm 4096 x 1024 of 2048 rows each 744
+// and 853, of 1024 rows 681 and 951; 1024 x 4096 of 2048 rows 916 and 1179; mm_dx 4096 x 1024 of 1024 rows 892 and 1196;
+// one segment of 2048 rows, 4096 x 2048, (512 and 128 tiles) 920 and 655.
+bool big_tiles(int64_t tiles128, int64_t tiles256) {
+    return (tiles256 + 255) / 256 * 256 * 4 * 10 < (tiles128 + 511) / 512 * 512 * 13;
+}
+
 template <typename T, int OP>
 int launch(const Args& a, hipStream_t s) {
-    if constexpr (OP == kDw) return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
-    else {
-        const int64_t per_seg = a.S.n_seg ? a.S.n_rows / a.S.n_seg : 0;
-        if (per_seg <= 96) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
+    const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
+    auto cols = [&](int bq) { return (a.nq + (OP == kGateUp ? bq / 2 : bq) - 1) / (OP == kGateUp ? bq / 2 : bq); };
+    if constexpr (OP == kDw) {
+        // with few rows the output's bytes bound it, and smaller tiles have more of them under way (512 x 40 rows, 1024 x
+        // 2048: 592 us, and 737 with the large tiles)
+        auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * cols(b); };
+        if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
+        return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
+    } else {
+        if (per_seg <= 48) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
+        if (big_tiles(row_tiles(a, 128) * cols(128), row_tiles(a, 256) * cols(256)))
+            return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
         return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
     }
 }

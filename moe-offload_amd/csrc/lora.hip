@@ -41,153 +41,229 @@ __device__ __forceinline__ void widen8(uint4 w, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = (float)r[i];
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 round8(const float* v) {
-    typedef T t8 __attribute__((ext_vector_type(8)));
-    const t8 r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
-    return __builtin_bit_cast(uint4, r);
-}
-
-// The adapters of a tile of 16 tokens, each once in the order of their first tokens: calls f(adapter, whether this
-// lane's token has it) for the ones numbered first, first + step, ...  Wave-uniform.
-template <typename F>
-__device__ __forceinline__ void each_adapter(int id, bool has, int first, int step, F f) {
-    uint32_t todo = (uint32_t)__ballot(has) & 0xFFFFu;
-    for (int j = 0; todo; ++j) {
-        const int i = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-        const bool mine = has && id == i;
-        todo &= ~(uint32_t)__ballot(mine);
+// The adapters of a tile of 16 ST tokens, each once in the order of their first tokens: calls f(adapter, which of this
+// lane's tokens have it) for the ones numbered first, first + step, ...  Wave-uniform.
+template <int ST, typename F>
+__device__ __forceinline__ void each_adapter(const int (&id)[ST], const bool (&has)[ST], int first, int step, F f) {
+    uint32_t todo[ST];
+    for (int m = 0; m < ST; ++m) todo[m] = (uint32_t)__ballot(has[m]) & 0xFFFFu;
+    for (int j = 0;; ++j) {
+        int i = -1;
+#pragma unroll
+        for (int m = ST - 1; m >= 0; --m)
+            if (todo[m]) i = __builtin_amdgcn_readlane(id[m], __builtin_ctz(todo[m]));
+        if (i < 0) return;
+        bool mine[ST];
+#pragma unroll
+        for (int m = 0; m < ST; ++m) {
+            mine[m] = has[m] && id[m] == i;
+            todo[m] &= ~(uint32_t)__ballot(mine[m]);
+        }
         if (j >= first && (j - first) % step == 0) f(i, mine);
     }
 }
 
-// v[t][j] = s_i A_i[j] x[t] for 16 tokens (blockIdx.x) and 16 SR ranks (blockIdx.y).
-template <typename T, int SR>
-__global__ __launch_bounds__(256) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A, int64_t a_stride,
-                                                const int32_t* __restrict__ ids, const float* __restrict__ scale, int n_tok,
-                                                int n_ad, int n_in, int rank, float* __restrict__ v) {
-    __shared__ f32x4 part[3][SR][64];
+// What lanes past the end of a row read.
+__device__ uint4 g_zero16;
+
+constexpr int kVWaves = 8;
+
+// v[t][j] = s_i A_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), an eighth of the row per wave.
+template <typename T, int SR, int ST>
+__global__ __launch_bounds__(64 * kVWaves, 4) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A,
+                                                            int64_t a_stride, const int32_t* __restrict__ ids,
+                                                            const float* __restrict__ scale, int n_tok, int n_ad, int n_in,
+                                                            int rank, float* __restrict__ v) {
+    constexpr int U = 8 / (SR * ST) < 4 ? 4 : 8 / (SR * ST);                   // steps of 32 whose loads are under way at once
+    __shared__ f32x4 part[kVWaves][SR * ST][64];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
-    const int64_t t = (int64_t)blockIdx.x * 16 + n;
-    const int id = t < n_tok ? ids[t] : -1, j0 = blockIdx.y * (16 * SR);
-    const bool has = id >= 0 && id < n_ad;
-    const T* xr = x + (t < n_tok ? t : (int64_t)n_tok - 1) * ldx + kq * 8;
-    const int steps = (n_in + 31) / 32, per = (steps + 3) / 4;
-    const int c0 = wv * per * 32, c1 = c0 + per * 32 < n_in ? c0 + per * 32 : n_in;
-    each_adapter(id, has, blockIdx.z, gridDim.z, [&](int i, bool mine) {
+    const int j0 = blockIdx.y * (16 * SR);
+    const T* zero = (const T*)&g_zero16;
+    int64_t t[ST];
+    const T* xr[ST];
+    int id[ST];
+    bool has[ST];
+#pragma unroll
+    for (int m = 0; m < ST; ++m) {
+        t[m] = ((int64_t)blockIdx.x * ST + m) * 16 + n;
+        xr[m] = x + (t[m] < n_tok ? t[m] : (int64_t)n_tok - 1) * ldx + kq * 8;
+        id[m] = t[m] < n_tok ? ids[t[m]] : -1;
+        has[m] = id[m] >= 0 && id[m] < n_ad;
+    }
+    const int steps = (n_in + 31) / 32, per = (steps + kVWaves - 1) / kVWaves;
+    const int s0 = wv * per, s1 = s0 + per < steps ? s0 + per : steps;
+    each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
         const T* ar[SR];
 #pragma unroll
         for (int s = 0; s < SR; ++s) {
             const int j = j0 + s * 16 + n;
             ar[s] = A + (int64_t)i * a_stride + (int64_t)(j < rank ? j : rank - 1) * n_in + kq * 8;
         }
-        f32x4 acc[SR] = {};
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        int c = c0;
+        f32x4 acc[SR][ST] = {};
 #pragma unroll 1
-        for (; c + 256 <= c1; c += 256) {
-            uint4 xv[8], av[SR][8];
+        for (int s = s0; s < s1; s += U) {
+            uint4 xv[ST][U], av[SR][U];
+            const bool whole = s + U <= s1 && (s + U) * 32 <= n_in;            // wave-uniform
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                xv[u] = *(const uint4*)(xr + c + u * 32);
+            for (int u = 0; u < U; ++u) {
+                const int c = (s + u) * 32;
+                const bool in = whole || (s + u < s1 && c + kq * 8 < n_in);
 #pragma unroll
-                for (int s = 0; s < SR; ++s) av[s][u] = *(const uint4*)(ar[s] + c + u * 32);
+                for (int m = 0; m < ST; ++m) xv[m][u] = *(const uint4*)(in ? xr[m] + c : zero);
+#pragma unroll
+                for (int r = 0; r < SR; ++r) av[r][u] = *(const uint4*)(in ? ar[r] + c : zero);
             }
+            __builtin_amdgcn_sched_barrier(0);                                 // all of them before the first product
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int s = 0; s < SR; ++s) acc[s] = mfma<T>(av[s][u], xv[u], acc[s]);
+                for (int r = 0; r < SR; ++r)
+#pragma unroll
+                    for (int m = 0; m < ST; ++m) acc[r][m] = mfma<T>(av[r][u], xv[m][u], acc[r][m]);
         }
-        if (c < c1) {
-            uint4 xv[8], av[SR][8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const bool in = c + u * 32 + kq * 8 < c1;
-                xv[u] = in ? *(const uint4*)(xr + c + u * 32) : zero;
+        for (int r = 0; r < SR; ++r)
 #pragma unroll
-                for (int s = 0; s < SR; ++s) av[s][u] = in ? *(const uint4*)(ar[s] + c + u * 32) : zero;
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int s = 0; s < SR; ++s) acc[s] = mfma<T>(av[s][u], xv[u], acc[s]);
-        }
-        if (wv > 0)
-            for (int s = 0; s < SR; ++s) part[wv - 1][s][lane] = acc[s];
+            for (int m = 0; m < ST; ++m) part[wv][r * ST + m][lane] = acc[r][m];
         __syncthreads();
-        if (wv == 0) {
+        if (wv < SR * ST) {
+            const int r = wv / ST, j = j0 + r * 16 + kq * 4;
+            f32x4 sum = part[0][wv][lane];
+#pragma unroll
+            for (int w = 1; w < kVWaves; ++w) sum += part[w][wv][lane];
             const float si = scale ? scale[i] : 1.0f;
-            for (int s = 0; s < SR; ++s) {
-                const f32x4 sum = ((acc[s] + part[0][s][lane]) + (part[1][s][lane] + part[2][s][lane])) * si;
-                const int j = j0 + s * 16 + kq * 4;
-                if (mine && j < rank) *(f32x4*)(v + t * rank + j) = sum;
-            }
+#pragma unroll
+            for (int m = 0; m < ST; ++m)
+                if (wv % ST == m && mine[m] && j < rank) *(f32x4*)(v + t[m] * rank + j) = sum * si;
         }
         __syncthreads();
     });
 }
 
-// out = base + B_i v for 16 tokens (blockIdx.x) and 64 columns (blockIdx.y), 16 to a wave.
-template <typename T>
+// out = base + B_i v for 16 ST tokens (blockIdx.x) and 64 SC columns (blockIdx.y), 16 SC to a wave.
+template <typename T, int SC, int ST>
 __global__ __launch_bounds__(256) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
                                                   const T* __restrict__ B, int64_t b_stride, const int32_t* __restrict__ ids,
                                                   int n_tok, int n_ad, int n_out, int rank, T* out, int64_t ldo) {
-    const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
-    const int q0 = blockIdx.y * 64 + (threadIdx.x >> 6) * 16;
-    if (q0 >= n_out) return;
-    const int64_t t = (int64_t)blockIdx.x * 16 + n;
-    const int id = t < n_tok ? ids[t] : -1;
-    const bool has = id >= 0 && id < n_ad;
-    const float* vr = v + (t < n_tok ? t : 0) * rank;
-    f32x4 acc = {};
-    bool got = false;
-    each_adapter(id, has, blockIdx.z, gridDim.z, [&](int i, bool mine) {
-        const T* br = B + (int64_t)i * b_stride + (int64_t)(q0 + n < n_out ? q0 + n : n_out - 1) * rank;
-        f32x4 one = {};
-        for (int k0 = 0; k0 < rank; k0 += 32) {
-            float bv[8] = {}, vv[8] = {};
-            if (k0 + kq * 8 < rank) {
-                widen8<T>(*(const uint4*)(br + k0 + kq * 8), bv);
-                if (mine) {
-                    const f32x4 lo = *(const f32x4*)(vr + k0 + kq * 8), hi = *(const f32x4*)(vr + k0 + kq * 8 + 4);
-                    for (int e = 0; e < 4; ++e) vv[e] = lo[e], vv[4 + e] = hi[e];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) one = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[e], vv[e], one, 0, 0, 0);
-        }
-        if (mine) acc = one, got = true;
-    });
-    // lane (n, kq): columns 4 kq .. + 3 of token n.  Tokens without an adapter are the first block's.
-    const int q = q0 + kq * 4;
-    if (t >= n_tok || q >= n_out || !(got || (!has && blockIdx.z == 0 && base != out))) return;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 r = *(const t4*)(base + t * ldb + q);
-    if (got)
-        for (int e = 0; e < 4; ++e) r[e] = (T)((float)r[e] + acc[e]);
-    *(t4*)(out + t * ldo + q) = r;
+    const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
+    const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * (16 * SC);
+    if (q0 >= n_out) return;
+    const T* zero = (const T*)&g_zero16;
+    int64_t t[ST];
+    int id[ST];
+    bool has[ST], got[ST];
+    t4 bs[ST][SC];                             // lane (n, kq): columns 4 kq .. + 3 of token n
+    f32x4 acc[ST][SC];
+#pragma unroll
+    for (int m = 0; m < ST; ++m) {
+        t[m] = ((int64_t)blockIdx.x * ST + m) * 16 + n;
+        id[m] = t[m] < n_tok ? ids[t[m]] : -1;
+        has[m] = id[m] >= 0 && id[m] < n_ad;
+        got[m] = false;
+#pragma unroll
+        for (int s = 0; s < SC; ++s) {
+            const int q = q0 + s * 16 + kq * 4;
+            bs[m][s] = *(const t4*)(base + (t[m] < n_tok ? t[m] : 0) * ldb + (q < n_out ? q : 0));
+        }
+    }
+    each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
+        const T* br[SC];
+#pragma unroll
+        for (int s = 0; s < SC; ++s) {
+            const int q = q0 + s * 16 + n;
+            br[s] = B + (int64_t)i * b_stride + (int64_t)(q < n_out ? q : n_out - 1) * rank + kq * 8;
+        }
+        f32x4 one[ST][SC] = {};
+        uint4 bv[SC];
+        f32x4 lo[ST], hi[ST];
+        auto fetch = [&](int k0) {
+            const bool in = k0 + kq * 8 < rank;
+#pragma unroll
+            for (int s = 0; s < SC; ++s) bv[s] = *(const uint4*)(in ? br[s] + k0 : zero);
+#pragma unroll
+            for (int m = 0; m < ST; ++m) {
+                const float* p = v + t[m] * rank + k0 + kq * 8;
+                lo[m] = *(const f32x4*)(in && mine[m] ? p : (const float*)zero);
+                hi[m] = *(const f32x4*)(in && mine[m] ? p + 4 : (const float*)zero);
+            }
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int k0 = 0; k0 < rank; k0 += 32) {
+            float bw[SC][8];
+            f32x4 l[ST], h[ST];
+#pragma unroll
+            for (int s = 0; s < SC; ++s) widen8<T>(bv[s], bw[s]);
+#pragma unroll
+            for (int m = 0; m < ST; ++m) l[m] = lo[m], h[m] = hi[m];
+            if (k0 + 32 < rank) fetch(k0 + 32);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int m = 0; m < ST; ++m)
+#pragma unroll
+                    for (int s = 0; s < SC; ++s)
+                        one[m][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[s][e], e < 4 ? l[m][e] : h[m][e - 4], one[m][s], 0, 0, 0);
+        }
+#pragma unroll
+        for (int m = 0; m < ST; ++m)
+            if (mine[m]) {
+                got[m] = true;
+#pragma unroll
+                for (int s = 0; s < SC; ++s) acc[m][s] = one[m][s];
+            }
+    });
+    // a token without an adapter is written by the first block of its tile
+#pragma unroll
+    for (int m = 0; m < ST; ++m) {
+        if (t[m] >= n_tok || !(got[m] || (!has[m] && blockIdx.z == 0 && base != out))) continue;
+#pragma unroll
+        for (int s = 0; s < SC; ++s) {
+            const int q = q0 + s * 16 + kq * 4;
+            t4 r = bs[m][s];
+            if (got[m])
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = (T)((float)r[e] + acc[m][s][e]);
+            if (q < n_out) *(t4*)(out + t[m] * ldo + q) = r;
+        }
+    }
+}
+
+template <typename T, int ST>
+int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* B, int64_t b_stride,
+             const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, float* v, T* out,
+             int64_t ldo, hipStream_t s) {
+    const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST));
+    // up to 256 tokens a tile's adapters get blocks of their own (16 tokens have 16 at most)
+    const uint32_t split = ST == 1 && n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
+    if (n_ad > 0) {
+        if (rank <= 16)
+            hipLaunchKernelGGL((k_lora_v<T, 1, ST>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A, a_stride, ids,
+                               scale, n_tok, n_ad, n_in, rank, v);
+        else
+            hipLaunchKernelGGL((k_lora_v<T, 2, ST>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+                               a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
+        HIP_TRY(hipGetLastError());
+    }
+    if ((int64_t)tiles * n_out < 512 * 256)
+        hipLaunchKernelGGL((k_lora_out<T, 1, ST>), dim3(tiles, (n_out + 63) / 64, split), dim3(256), 0, s, base, ldb, v, B,
+                           b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
+    else
+        hipLaunchKernelGGL((k_lora_out<T, 4, ST>), dim3(tiles, (n_out + 255) / 256, split), dim3(256), 0, s, base, ldb, v, B,
+                           b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
+    HIP_TRY(hipGetLastError());
+    return 0;
 }
 
 template <typename T>
-int lora_add(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* B,
-             int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
-             float* v, void* out, int64_t ldo, hipStream_t s) {
-    const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 15) / 16);
-    // up to 256 tokens a tile's adapters get blocks of their own (16 tokens have 16 at most)
-    const uint32_t split = n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
-    if (n_ad > 0) {
-        if (rank <= 16)
-            hipLaunchKernelGGL((k_lora_v<T, 1>), dim3(tiles, 1, split), dim3(256), 0, s, (const T*)x, ldx, (const T*)A,
-                               a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
-        else
-            hipLaunchKernelGGL((k_lora_v<T, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(256), 0, s, (const T*)x, ldx,
-                               (const T*)A, a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
-        HIP_TRY(hipGetLastError());
-    }
-    hipLaunchKernelGGL((k_lora_out<T>), dim3(tiles, (n_out + 63) / 64, split), dim3(256), 0, s, (const T*)base, ldb, v,
-                       (const T*)B, b_stride, ids, n_tok, n_ad, n_out, rank, (T*)out, ldo);
-    HIP_TRY(hipGetLastError());
-    return 0;
+int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* B,
+                   int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
+                   float* v, void* out, int64_t ldo, hipStream_t s) {
+    auto f = n_tok <= 1024 ? lora_add<T, 1> : lora_add<T, 2>;
+    return f((const T*)base, ldb, (const T*)x, ldx, (const T*)A, a_stride, (const T*)B, b_stride, ids, scale, n_tok, n_ad, n_in,
+             n_out, rank, v, (T*)out, ldo, s);
 }
 
 // The shapes and strides that both entry points take; base or dy is [n_tok][n_out].
@@ -240,7 +316,7 @@ extern "C" int moe_lora_add(const void* base, int64_t ld_base, const void* x, in
         return -1;
     }
     if (bad_pointers(who, {base, x, out, workspace}) || (n_ad > 0 && bad_pointers(who, {a, b}))) return -1;
-    auto f = dtype ? lora_add<__bf16> : lora_add<_Float16>;
+    auto f = dtype ? lora_add_typed<__bf16> : lora_add_typed<_Float16>;
     return f(base, ld_base, x, ldx, a, a_stride, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, (float*)workspace,
              out, ld_out, (hipStream_t)stream);
 }
