@@ -1,5 +1,5 @@
-// What the grouped products of unquantised experts share: the operands' description, the check of a
-// call's arguments, and the search for a block's tile.
+// What the grouped products of unquantised experts and the adapters share: the search for a block's rows, loads
+// from global memory straight into LDS, and the matrix unit's operands read from there.
 #pragma once
 #include "moe_common.h"
 
@@ -53,12 +53,13 @@ struct Tile {
 };
 
 // The row tile (bm rows of one segment at most) and column tile of this block; false: none is left for it.
+// scratch: THREADS / 64 + 3 words of LDS, free again once every thread is back.
 // Every thread sums the tiles of its own few segments, a scan over the block turns the sums into first
 // tiles, and the thread whose segments hold the block's item publishes it.
 template <int THREADS>
-__device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, Tile& out) {
-    __shared__ uint32_t wave_sum[THREADS / 64];
-    __shared__ int found[3];
+__device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, uint32_t* scratch, Tile& out) {
+    uint32_t* wave_sum = scratch;
+    int* found = (int*)(scratch + THREADS / 64);
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
     const int n_virtual = S.n_seg + 2, per = (n_virtual + THREADS - 1) / THREADS;
     const int v0 = t * per, v1 = v0 + per < n_virtual ? v0 + per : n_virtual;
@@ -106,5 +107,85 @@ __device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, Tile
     out.col = (int)(item % (uint32_t)n_col);
     return true;
 }
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 round4(f32x4 v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const t4 r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    return __builtin_bit_cast(uint2, r);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 widen4(uint2 w) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const t4 r = __builtin_bit_cast(t4, w);
+    return (f32x4){(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
+}
+
+// What an operand's lanes read where it has nothing: contraction indexes past the end.
+static __device__ uint4 g_zero16;
+
+// 16 bytes per lane from global memory straight into LDS: lane l's land at lds + 16 l (lds wave-uniform).
+// The issuing code waits for them itself (vmcnt), and no register receives data.
+__device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+
+constexpr int kBC = 64;                                       // contraction indexes per step
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// Row of a step's image, along which the other index runs -> which 32-byte block trades places with block 0:
+// the rows that one transposing read touches (4 of each of two or four lane groups) get eight different ones.
+__device__ __forceinline__ int turn(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
+
+// One operand's fragments for v_mfma_f32_16x16x32: lane (n, kq) holds c = 32 ks + 8 kq .. + 7 of row / column n.
+// ALONG false: the image has a row per tile row, 64 values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
+// ALONG true: a row per c, W values each, read transposed by ds_read_b64_tr_b16 (lane i of 16 gives the address of
+// 4 columns of row i / 4 and receives column i of 4 rows).
+template <bool ALONG, int W, int SUBS>
+struct Frags {
+    uint32_t at[ALONG ? SUBS : 2];
+
+    __device__ __forceinline__ void init(uint32_t base, int first, int lane) {
+        const int n = lane & 15, kq = lane >> 4;
+        if constexpr (ALONG) {
+            const int row = kq * 8 + (n >> 2);
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s)
+                at[s] = base + row * (W * 2) + (((first >> 4) + s) ^ turn(row)) * 32 + (n & 3) * 8;
+        } else {
+            at[0] = base + (first + n) * 128 + (kq ^ (n & 7)) * 16;
+            at[1] = base + (first + n) * 128 + ((kq + 4) ^ (n & 7)) * 16;
+        }
+    }
+
+    __device__ __forceinline__ uint4 read(uint32_t stage, int s, int ks) const {
+        if constexpr (ALONG) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* ptr;
+            const uint32_t p = at[s] + stage + ks * 32 * (W * 2);
+            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)p));
+            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(p + 4 * (W * 2))));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) const u32x4* ptr;
+            const u32x4 v = *(ptr)(uintptr_t)(at[ks] + stage + s * 2048);
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+};
 
 }  // namespace gmm

@@ -24,12 +24,7 @@
 
 namespace {
 
-using gmm::Segs;
-using gmm::Tile;
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+using namespace gmm;
 
 enum { kMM = 0, kGateUp = 1, kDx = 2, kDxGlu = 3, kDw = 4 };
 
@@ -49,82 +44,6 @@ struct Args {
     int np, nq, nc;              // extents: output columns in p (mm_dw) and q, and the contraction
     int out_f32;
     int span;                    // column tiles per block
-};
-
-template <typename T>
-__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
-    if constexpr (__is_same(T, _Float16))
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <typename T>
-__device__ __forceinline__ uint2 round4(f32x4 v) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    const t4 r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-    return __builtin_bit_cast(uint2, r);
-}
-
-template <typename T>
-__device__ __forceinline__ f32x4 widen4(uint2 w) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    const t4 r = __builtin_bit_cast(t4, w);
-    return (f32x4){(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
-}
-
-// What an operand's lanes read where it has nothing: contraction indexes past the end.
-__device__ uint4 g_zero16;
-
-// 16 bytes per lane from global memory straight into LDS: lane l's land at lds + 16 l (lds wave-uniform).
-// The issuing code waits for them itself (vmcnt), and no register receives data.
-__device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
-}
-
-constexpr int kBC = 64;                                       // contraction indexes per step
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-
-// Row of a step's image, along which the other index runs -> which 32-byte block trades places with block 0:
-// the rows that one transposing read touches (4 of each of two or four lane groups) get eight different ones.
-__device__ __forceinline__ int turn(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
-
-// One operand's fragments for v_mfma_f32_16x16x32: lane (n, kq) holds c = 32 ks + 8 kq .. + 7 of row / column n.
-// ALONG false: the image has a row per tile row, 64 values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
-// ALONG true: a row per c, W values each, read transposed by ds_read_b64_tr_b16 (lane i of 16 gives the address of
-// 4 columns of row i / 4 and receives column i of 4 rows).
-template <bool ALONG, int W, int SUBS>
-struct Frags {
-    uint32_t at[ALONG ? SUBS : 2];
-
-    __device__ __forceinline__ void init(uint32_t base, int first, int lane) {
-        const int n = lane & 15, kq = lane >> 4;
-        if constexpr (ALONG) {
-            const int row = kq * 8 + (n >> 2);
-#pragma unroll
-            for (int s = 0; s < SUBS; ++s)
-                at[s] = base + row * (W * 2) + (((first >> 4) + s) ^ turn(row)) * 32 + (n & 3) * 8;
-        } else {
-            at[0] = base + (first + n) * 128 + (kq ^ (n & 7)) * 16;
-            at[1] = base + (first + n) * 128 + ((kq + 4) ^ (n & 7)) * 16;
-        }
-    }
-
-    __device__ __forceinline__ uint4 read(uint32_t stage, int s, int ks) const {
-        if constexpr (ALONG) {
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4* ptr;
-            const uint32_t p = at[s] + stage + ks * 32 * (W * 2);
-            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)p));
-            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(p + 4 * (W * 2))));
-            return make_uint4(lo.x, lo.y, hi.x, hi.y);
-        } else {
-            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) const u32x4* ptr;
-            const u32x4 v = *(ptr)(uintptr_t)(at[ks] + stage + s * 2048);
-            return make_uint4(v[0], v[1], v[2], v[3]);
-        }
-    }
 };
 
 // Two subtiles' 4 adjacent 16-bit results per lane -> 8 adjacent: lanes 16-31 and 48-63 take the second
@@ -156,15 +75,16 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     int r0, r1, slot, tile, p0 = 0, nc = a.nc, seg = 0;
     if constexpr (OP == kDw) {
         const int tp = (a.np + BP - 1) / BP;
-        const uint32_t item = gmm::xcd_order(blockIdx.x, gridDim.x);
+        const uint32_t item = xcd_order(blockIdx.x, gridDim.x);
         seg = item / (groups * tp);
         p0 = (int)(item / groups % tp) * BP;
         tile = (int)(item % groups) * a.span;
-        gmm::seg_rows(a.S, seg + 1, r0, r1, slot);
+        seg_rows(a.S, seg + 1, r0, r1, slot);
         nc = r1 - r0;
     } else {
         Tile at;
-        if (!gmm::find_tile<64 * kWaves>(a.S, BP, groups, at)) return;
+        __shared__ uint32_t scratch[kWaves + 3];
+        if (!find_tile<64 * kWaves>(a.S, BP, groups, scratch, at)) return;
         r0 = at.r0;
         r1 = at.r1;
         slot = at.slot;
@@ -461,6 +381,99 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// A few rows per segment (decoding): one wave per 16 rows of a segment and 16 weight rows (mm: 16 columns; gate_up: 8
+// gate rows and the 8 up rows of the same outputs), which it streams through an LDS ring of its own, kFewRing steps of
+// 64 ahead, without a barrier.  Loads that put the weights straight into the matrix unit's layout would take 16 bytes
+// per lane from 16 rows at a time, four times the cache accesses.  The steps are k_grouped's, in its order, so a row's
+// result has the same bits whichever of the two a call's size selects.
+constexpr int kFewRing = 8;
+
+template <typename T, int OP>
+__global__ __launch_bounds__(64) void k_grouped_few(Args a) {
+    constexpr int kQStep = OP == kGateUp ? 8 : 16;
+    constexpr uint32_t kStage = 4096;                                          // 16 weight rows, 16 rows of x
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kFewRing * kStage];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
+    const int lane = threadIdx.x, n = lane & 15, kq = lane >> 4;
+    Tile at;
+    if (!find_tile<64>(a.S, 16, (a.nq + kQStep - 1) / kQStep, (uint32_t*)lds, at)) return;
+    const int slot = at.slot, q0 = at.col * kQStep, nc = slot < 0 || a.n_p == 0 ? 0 : a.nc, steps = (nc + kBC - 1) / kBC;
+    const T* zero = (const T*)&g_zero16;
+    const T* Q = (const T*)a.q + (int64_t)(slot < 0 ? 0 : slot) * a.ldq;
+    // this lane's 16 bytes of each load: row lane / 8 of its 8 rows
+    const int cu = ((lane & 7) ^ (lane >> 3)) * 8;
+    const T* pp[2];
+    const T* qp[2];
+    uint32_t live_p = 0;                                                       // rows of x that do not exist read zeros
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = at.r0 + j * 8 + (lane >> 3);
+        int v = -1;
+        if (r < at.r1) v = a.row_p ? a.row_p[r] : r;
+        if (v >= 0 && v < a.n_p) live_p |= 1u << j;
+        pp[j] = (const T*)a.p + (int64_t)(live_p >> j & 1 ? v : 0) * a.ldp + cu;
+        int64_t c = q0 + (OP == kGateUp ? 0 : j * 8) + (lane >> 3);
+        c = c < a.nq ? c : a.nq - 1;
+        qp[j] = Q + (OP == kGateUp ? c + (int64_t)j * a.nq : c) * nc + cu;
+    }
+    auto issue = [&](int s) {
+        const uint32_t to = lds0 + (uint32_t)(s % kFewRing) * kStage;
+        const bool in = s * kBC + cu < nc;                                     // (also past the last step)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) load_to_lds(in ? qp[j] + s * kBC : zero, to + j * 1024);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) load_to_lds(in && live_p >> j & 1 ? pp[j] + s * kBC : zero, to + 2048 + j * 1024);
+    };
+    Frags<false, 16, 1> fp, fq;
+    fq.init(lds0, 0, lane);
+    fp.init(lds0 + 2048, 0, lane);
+    f32x4 acc = {};
+    if (steps > 0) {
+#pragma unroll
+        for (int s = 0; s < kFewRing; ++s) issue(s);
+    }
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+        const uint32_t stage = (uint32_t)(s % kFewRing) * kStage;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kFewRing - 1) * 4) : "memory");     // loads return in order
+        const uint4 q0v = fq.read(stage, 0, 0), p0v = fp.read(stage, 0, 0), q1v = fq.read(stage, 0, 1), p1v = fp.read(stage, 0, 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                            // read before the next load overwrites it
+        issue(s + kFewRing);
+        acc = mfma<T>(q0v, p0v, acc);
+        acc = mfma<T>(q1v, p1v, acc);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                  // LDS is another block's after this one
+    // lane (n, kq): row n, columns 4 kq .. + 3
+    const int r = at.r0 + n;
+    bool live = r < at.r1, dead = slot < 0;
+    int o = r;
+    if (live) {
+        if (a.row_p) {
+            const int v = a.row_p[r];
+            dead |= v < 0 || v >= a.n_p;
+        }
+        if (OP == kMM && a.row_out) o = a.row_out[r];
+        live = o >= 0 && o < a.n_out;
+    }
+    if (dead) acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if constexpr (OP == kGateUp) {
+        // gate columns 4 kq .. + 3 in the lower two lane groups, the same outputs' up values 32 lanes further
+        f32x4 up, h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) up[e] = __shfl_xor(acc[e], 32, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = acc[e] / (1.0f + __expf(-acc[e])) * up[e];
+        const int c = q0 + (kq & 1) * 4;
+        if (!live || c >= a.nq) return;
+        if (kq < 2) *(uint2*)((T*)a.out + (int64_t)r * a.ldo + c) = round4<T>(h);
+        if (a.gu_out) *(uint2*)((T*)a.gu_out + (int64_t)r * a.ldgu + (kq < 2 ? 0 : a.nq) + c) = round4<T>(acc);
+    } else {
+        const int c = q0 + kq * 4;
+        const float s = a.scale && slot >= 0 ? a.scale[slot] : 1.0f;
+        if (live && c < a.nq) *(uint2*)((T*)a.out + (int64_t)o * a.ldo + c) = round4<T>(acc * s);
+    }
+}
+
 // Row tiles of a call as far as the host knows it: a segment's last tile is half full on average.
 int64_t row_tiles(const Args& a, int bp) { return (a.S.n_rows + (int64_t)(a.S.n_seg - 1) * (bp / 2) + bp - 1) / bp; }
 
@@ -502,6 +515,17 @@ bool big_tiles(int64_t tiles128, int64_t tiles256) {
     return (tiles256 + 255) / 256 * 256 * 4 * 10 < (tiles128 + 511) / 512 * 512 * 13;
 }
 
+constexpr int64_t kFewTiles = 1024;
+
+template <typename T, int OP>
+int launch_few(const Args& a, hipStream_t s) {
+    const int qstep = OP == kGateUp ? 8 : 16;
+    const int64_t rows = (int64_t)a.S.n_rows / 16 + std::min(a.S.n_seg + 2, a.S.n_rows), tiles = (a.nq + qstep - 1) / qstep;
+    hipLaunchKernelGGL((k_grouped_few<T, OP>), dim3((uint32_t)(rows * tiles)), dim3(64), 0, s, a);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
 template <typename T, int OP>
 int launch(const Args& a, hipStream_t s) {
     const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
@@ -513,6 +537,9 @@ int launch(const Args& a, hipStream_t s) {
         if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
         return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
     } else {
+        if constexpr (OP == kMM || OP == kGateUp) {
+            if (per_seg <= 16 && std::min(a.S.n_seg, a.S.n_rows) * (int64_t)cols(128) < kFewTiles) return launch_few<T, OP>(a, s);
+        }
         if (per_seg <= 48) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
         if (big_tiles(row_tiles(a, 128) * cols(128), row_tiles(a, 256) * cols(256)))
             return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);

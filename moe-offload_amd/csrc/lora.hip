@@ -7,13 +7,13 @@
 //
 // Two launches.  k_lora_v: 16 tokens and up to 32 ranks per block, the contraction split over its waves, both
 // operands from global memory straight in the matrix unit's layout (each byte of x is used for 16 ranks at a
-// time, so staging would gain nothing).  k_lora_out: 16 tokens and 64 output columns per block, v and B in the
-// fp32 matrix unit, so v keeps its bits and its range.  The tokens of a tile may have different adapters: the
+// TODO  The tokens of a tile may have different adapters: the
 // tile is multiplied by each adapter that occurs in it and every token keeps its own adapter's result.  In a
 // batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks of
 // their own.
 #include <hip/hip_bf16.h>
 
+#include <algorithm>
 #include <initializer_list>
 
 #include "../../include/moe_offload.h"
@@ -21,17 +21,7 @@
 
 namespace {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-template <typename T>
-__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
-    if constexpr (__is_same(T, _Float16))
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
+using namespace gmm;
 
 template <typename T>
 __device__ __forceinline__ void widen8(uint4 w, float* v) {
@@ -63,64 +53,89 @@ __device__ __forceinline__ void each_adapter(const int (&id)[ST], const bool (&h
     }
 }
 
-// What lanes past the end of a row read.
-__device__ uint4 g_zero16;
-
 constexpr int kVWaves = 8;
 
-// v[t][j] = s_i A_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), an eighth of the row per wave.
-template <typename T, int SR, int ST>
-__global__ __launch_bounds__(64 * kVWaves, 4) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A,
-                                                            int64_t a_stride, const int32_t* __restrict__ ids,
-                                                            const float* __restrict__ scale, int n_tok, int n_ad, int n_in,
-                                                            int rank, float* __restrict__ v) {
-    constexpr int U = 8 / (SR * ST) < 4 ? 4 : 8 / (SR * ST);                   // steps of 32 whose loads are under way at once
-    __shared__ f32x4 part[kVWaves][SR * ST][64];
+// v[t][j] = s_i A_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y).  Each wave multiplies every eighth
+// step of 64 along the row, through an LDS ring of its own (D steps of the tokens' and the ranks' rows); the waves'
+// sums are added in their order.
+template <typename T, int SR, int ST, int D>
+__global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A,
+                                                         int64_t a_stride, const int32_t* __restrict__ ids,
+                                                         const float* __restrict__ scale, int n_tok, int n_ad, int n_in,
+                                                         int rank, float* __restrict__ v) {
+    constexpr int kLoads = 2 * (ST + SR);
+    constexpr uint32_t kStage = kLoads * 1024;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kVWaves * D * kStage];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
-    const int j0 = blockIdx.y * (16 * SR);
+    const uint32_t all = (uint32_t)(uintptr_t)(lds_u8*)lds, ring = all + wv * D * kStage;
+    const int j0 = blockIdx.y * (16 * SR), cu = ((lane & 7) ^ (lane >> 3)) * 8;
     const T* zero = (const T*)&g_zero16;
+    asm("" : "+s"(zero));
     int64_t t[ST];
-    const T* xr[ST];
+    const T* xp[2 * ST];
     int id[ST];
     bool has[ST];
 #pragma unroll
     for (int m = 0; m < ST; ++m) {
         t[m] = ((int64_t)blockIdx.x * ST + m) * 16 + n;
-        xr[m] = x + (t[m] < n_tok ? t[m] : (int64_t)n_tok - 1) * ldx + kq * 8;
         id[m] = t[m] < n_tok ? ids[t[m]] : -1;
         has[m] = id[m] >= 0 && id[m] < n_ad;
     }
-    const int steps = (n_in + 31) / 32, per = (steps + kVWaves - 1) / kVWaves;
-    const int s0 = wv * per, s1 = s0 + per < steps ? s0 + per : steps;
+#pragma unroll
+    for (int j = 0; j < 2 * ST; ++j) {
+        const int64_t r = (int64_t)blockIdx.x * 16 * ST + j * 8 + (lane >> 3);
+        xp[j] = x + (r < n_tok ? r : n_tok - 1) * ldx + cu;
+    }
+    Frags<false, 16, ST> fx;
+    Frags<false, 16, SR> fa;
+    fx.init(ring, 0, lane);
+    fa.init(ring + ST * 2048, 0, lane);
+    const int steps = ((n_in + 63) / 64 - wv + kVWaves - 1) / kVWaves;         // wv, wv + 8, ...
     each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
-        const T* ar[SR];
+        const float si = scale ? scale[i] : 1.0f;
+        const T* ap[2 * SR];
 #pragma unroll
-        for (int s = 0; s < SR; ++s) {
-            const int j = j0 + s * 16 + n;
-            ar[s] = A + (int64_t)i * a_stride + (int64_t)(j < rank ? j : rank - 1) * n_in + kq * 8;
+        for (int j = 0; j < 2 * SR; ++j) {
+            const int r = j0 + j * 8 + (lane >> 3);
+            ap[j] = A + (int64_t)i * a_stride + (int64_t)(r < rank ? r : rank - 1) * n_in + cu;
         }
+        auto issue = [&](int s) {
+            const int c = (s * kVWaves + wv) * 64;
+            const uint32_t to = ring + (uint32_t)(s % D) * kStage;
+            const bool in = c + cu < n_in;                                     // (also past the last step)
+#pragma unroll
+            for (int j = 0; j < 2 * ST; ++j) load_to_lds(in ? xp[j] + c : zero, to + j * 1024);
+#pragma unroll
+            for (int j = 0; j < 2 * SR; ++j) load_to_lds(in ? ap[j] + c : zero, to + (2 * ST + j) * 1024);
+        };
         f32x4 acc[SR][ST] = {};
+#pragma unroll
+        for (int s = 0; s < D; ++s) issue(s);
 #pragma unroll 1
-        for (int s = s0; s < s1; s += U) {
-            uint4 xv[ST][U], av[SR][U];
-            const bool whole = s + U <= s1 && (s + U) * 32 <= n_in;            // wave-uniform
+        for (int s = 0; s < steps; ++s) {
+            const uint32_t stage = (uint32_t)(s % D) * kStage;
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");   // loads return in order
+            uint4 xv[2][ST], av[2][SR];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int c = (s + u) * 32;
-                const bool in = whole || (s + u < s1 && c + kq * 8 < n_in);
+            for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-                for (int m = 0; m < ST; ++m) xv[m][u] = *(const uint4*)(in ? xr[m] + c : zero);
+                for (int m = 0; m < ST; ++m) xv[ks][m] = fx.read(stage, m, ks);
 #pragma unroll
-                for (int r = 0; r < SR; ++r) av[r][u] = *(const uint4*)(in ? ar[r] + c : zero);
+                for (int r = 0; r < SR; ++r) av[ks][r] = fa.read(stage, r, ks);
             }
-            __builtin_amdgcn_sched_barrier(0);                                 // all of them before the first product
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                        // read before the next load overwrites it
+            issue(s + D);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int r = 0; r < SR; ++r)
 #pragma unroll
-                    for (int m = 0; m < ST; ++m) acc[r][m] = mfma<T>(av[r][u], xv[m][u], acc[r][m]);
+                    for (int m = 0; m < ST; ++m) acc[r][m] = mfma<T>(av[ks][r], xv[ks][m], acc[r][m]);
         }
+        // the sums trade places through the rings, which are idle once every wave's loads have landed
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        f32x4(*part)[SR * ST][64] = (f32x4(*)[SR * ST][64])lds;
 #pragma unroll
         for (int r = 0; r < SR; ++r)
 #pragma unroll
@@ -131,7 +146,6 @@ __global__ __launch_bounds__(64 * kVWaves, 4) void k_lora_v(const T* __restrict_
             f32x4 sum = part[0][wv][lane];
 #pragma unroll
             for (int w = 1; w < kVWaves; ++w) sum += part[w][wv][lane];
-            const float si = scale ? scale[i] : 1.0f;
 #pragma unroll
             for (int m = 0; m < ST; ++m)
                 if (wv % ST == m && mine[m] && j < rank) *(f32x4*)(v + t[m] * rank + j) = sum * si;
@@ -140,95 +154,196 @@ __global__ __launch_bounds__(64 * kVWaves, 4) void k_lora_v(const T* __restrict_
     });
 }
 
-// out = base + B_i v for 16 ST tokens (blockIdx.x) and 64 SC columns (blockIdx.y), 16 SC to a wave.
-template <typename T, int SC, int ST>
-__global__ __launch_bounds__(256) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
-                                                  const T* __restrict__ B, int64_t b_stride, const int32_t* __restrict__ ids,
-                                                  int n_tok, int n_ad, int n_out, int rank, T* out, int64_t ldo) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    const int lane = threadIdx.x & 63, n = lane & 15, kq = lane >> 4;
-    const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * (16 * SC);
-    if (q0 >= n_out) return;
-    const T* zero = (const T*)&g_zero16;
-    int64_t t[ST];
-    int id[ST];
-    bool has[ST], got[ST];
-    t4 bs[ST][SC];                             // lane (n, kq): columns 4 kq .. + 3 of token n
-    f32x4 acc[ST][SC];
+// fp32 values as sums of values of T that keep their bits: bf16 has fp32's range, three of its 8 bits each are 24 bits;
+// fp16 values are first scaled by a power of two per token, so that the largest is just below 2^15, and two of 11 bits
+// each are 22 bits, or 2^-40 of the token's largest value.  (The fp32 matrix unit takes 8 times as long and wants B
+// widened.)  An infinity or NaN stays in the first part.
+template <typename T>
+constexpr int kParts = __is_same(T, _Float16) ? 2 : 3;
+
+template <typename T>
+__device__ __forceinline__ void split8(const float* v, uint4 (&part)[kParts<T>]) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 p[kParts<T>];
 #pragma unroll
-    for (int m = 0; m < ST; ++m) {
-        t[m] = ((int64_t)blockIdx.x * ST + m) * 16 + n;
-        id[m] = t[m] < n_tok ? ids[t[m]] : -1;
-        has[m] = id[m] >= 0 && id[m] < n_ad;
-        got[m] = false;
+    for (int e = 0; e < 8; ++e) {
+        float rest = v[e];
+        const bool fine = __builtin_fabsf(rest) < __builtin_inff();
 #pragma unroll
-        for (int s = 0; s < SC; ++s) {
-            const int q = q0 + s * 16 + kq * 4;
-            bs[m][s] = *(const t4*)(base + (t[m] < n_tok ? t[m] : 0) * ldb + (q < n_out ? q : 0));
+        for (int k = 0; k < kParts<T>; ++k) {
+            p[k][e] = (T)rest;
+            rest = fine ? rest - (float)p[k][e] : 0.f;
         }
     }
-    each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
-        const T* br[SC];
 #pragma unroll
-        for (int s = 0; s < SC; ++s) {
-            const int q = q0 + s * 16 + n;
-            br[s] = B + (int64_t)i * b_stride + (int64_t)(q < n_out ? q : n_out - 1) * rank + kq * 8;
+    for (int k = 0; k < kParts<T>; ++k) part[k] = __builtin_bit_cast(uint4, p[k]);
+}
+
+// out = base + B_i v for 16 tokens (blockIdx.x) and 128 columns per wave.  The wave's eight subtiles of 16 columns are
+// dealt out so that lane n has the columns 8 n .. 8 n + 7, one of each: 16 bytes per token, and 16 lanes' are one row's
+// 256.
+// out = base + B_i v for 16 ST tokens (blockIdx.x) and 128 columns per wave, W waves.  The wave's eight subtiles of 16
+// columns are dealt out so that lane n has the columns 8 n .. 8 n + 7, one of each: 16 bytes per token, and 16 lanes' are
+// one row's 256.  B's rows and v go through LDS, 64 ranks at a time, in loads of whole lines: loaded straight into the
+// matrix unit's layout every lane's 16 bytes are a cache access of their own, and those set the pace.
+template <typename T, int ST, int W>
+__global__ __launch_bounds__(64 * W, 2) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
+                                                        const T* __restrict__ B, int64_t b_stride, const int32_t* __restrict__ ids,
+                                                        int n_tok, int n_ad, int n_out, int rank, T* out, int64_t ldo) {
+    constexpr int SC = 8, kVLoads = (4 * ST + W - 1) / W;
+    constexpr uint32_t kB = 128 * 128;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kB + kVLoads * W * 1024];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
+    const uint32_t lds_b = (uint32_t)(uintptr_t)(lds_u8*)lds + wv * kB, lds_v = (uint32_t)(uintptr_t)(lds_u8*)lds + W * kB;
+    const int first = ((int)blockIdx.y * W + wv) * 128, q = first + n * 8;
+    const bool in_q = q < n_out;
+    const T* zero = (const T*)&g_zero16;
+    asm("" : "+s"(zero));
+    const int64_t t0 = (int64_t)blockIdx.x * 16 * ST;
+    int id[ST];
+    bool has[ST];
+#pragma unroll
+    for (int m = 0; m < ST; ++m) {
+        const int64_t t = t0 + m * 16 + n;
+        id[m] = t < n_tok ? ids[t] : -1;
+        has[m] = id[m] >= 0 && id[m] < n_ad;
+    }
+    // result lane (n, kq): columns q .. q + 7 of tokens 4 kq .. + 3
+    uint4 bs[ST][4];
+#pragma unroll
+    for (int m = 0; m < ST; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = t0 + m * 16 + kq * 4 + i;
+            bs[m][i] = *(const uint4*)(r < n_tok && in_q ? base + r * ldb + q : zero);
         }
-        f32x4 one[ST][SC] = {};
-        uint4 bv[SC];
-        f32x4 lo[ST], hi[ST];
-        auto fetch = [&](int k0) {
-            const bool in = k0 + kq * 8 < rank;
+    auto put = [&](uint32_t tokens, int m, int i, uint4 r) {
+        if (tokens >> (kq * 4 + i) & 1 && in_q) *(uint4*)(out + (t0 + m * 16 + kq * 4 + i) * ldo + q) = r;
+    };
+    // tokens without an adapter are copied by the first of a tile's blocks
+    if (base != out && blockIdx.z == 0)
 #pragma unroll
-            for (int s = 0; s < SC; ++s) bv[s] = *(const uint4*)(in ? br[s] + k0 : zero);
+        for (int m = 0; m < ST; ++m) {
+            const uint32_t none = (uint32_t)__ballot(t0 + m * 16 + n < n_tok && !has[m]) & 0xFFFFu;
+            if (none)
 #pragma unroll
-            for (int m = 0; m < ST; ++m) {
-                const float* p = v + t[m] * rank + k0 + kq * 8;
-                lo[m] = *(const f32x4*)(in && mine[m] ? p : (const float*)zero);
-                hi[m] = *(const f32x4*)(in && mine[m] ? p + 4 : (const float*)zero);
+                for (int i = 0; i < 4; ++i) put(none, m, i, bs[m][i]);
+        }
+    each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
+        const T* Bi = B + (int64_t)i * b_stride;
+        // columns past the end read the last ones', whose results are not stored (both ends are multiples of 8)
+        auto load_chunk = [&](int k0) {
+            int l = lane;
+            asm volatile("" : "+v"(l));                                        // no addresses are kept over the products
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int top = first + j * 8 < n_out ? first + j * 8 : n_out - 8, u = ((l & 7) ^ (j & 7)) * 8;
+                const T* p = Bi + (int64_t)top * rank + k0 + ((l >> 3) * rank + u);
+                load_to_lds(k0 + u < rank ? p : zero, lds_b + j * 1024);
+            }
+#pragma unroll
+            for (int j = 0; j < kVLoads; ++j) {
+                const int row = (wv * kVLoads + j) * 4 + (l >> 4), k = k0 + ((l & 15) ^ (row & 15)) * 4;
+                const float* p = v + t0 * rank + (row * rank + k);
+                load_to_lds(k < rank && row < 16 * ST && t0 + row < n_tok ? (const void*)p : zero, lds_v + (wv * kVLoads + j) * 1024);
             }
         };
-        fetch(0);
-#pragma unroll 1
-        for (int k0 = 0; k0 < rank; k0 += 32) {
-            float bw[SC][8];
-            f32x4 l[ST], h[ST];
+        auto read_v = [&](int m, int ks, float* w) {
+            typedef __attribute__((address_space(3))) const f32x4* ptr;
+            const uint32_t at = lds_v + (m * 16 + n) * 256;
+            const f32x4 lo = *(ptr)(uintptr_t)(at + ((8 * ks + 2 * kq) ^ n) * 16), hi = *(ptr)(uintptr_t)(at + ((8 * ks + 2 * kq + 1) ^ n) * 16);
 #pragma unroll
-            for (int s = 0; s < SC; ++s) widen8<T>(bv[s], bw[s]);
+            for (int e = 0; e < 4; ++e) w[e] = lo[e], w[4 + e] = hi[e];
+        };
+        auto landed = [&]() {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        load_chunk(0);
+        // fp16: the power of two of this lane's token in each tile, from its largest |v|
+        float up[ST], down[ST];
 #pragma unroll
-            for (int m = 0; m < ST; ++m) l[m] = lo[m], h[m] = hi[m];
-            if (k0 + 32 < rank) fetch(k0 + 32);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
+        for (int m = 0; m < ST; ++m) up[m] = down[m] = 1.f;
+        if constexpr (kParts<T> == 2) {
+            float most[ST] = {};
+            for (int k0 = 64; k0 < rank; k0 += 64)                             // what the first 64 ranks leave
                 for (int m = 0; m < ST; ++m)
+                    for (int k = k0 + kq * 8; k < k0 + 64 && k < rank; k += 32)
+                        for (int e = 0; e < 8; ++e)
+                            most[m] = fmaxf(most[m], mine[m] ? __builtin_fabsf(v[(t0 + m * 16 + n) * rank + k + e]) : 0.f);
+            landed();
 #pragma unroll
-                    for (int s = 0; s < SC; ++s)
-                        one[m][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(bw[s][e], e < 4 ? l[m][e] : h[m][e - 4], one[m][s], 0, 0, 0);
-        }
+            for (int m = 0; m < ST; ++m) {
 #pragma unroll
-        for (int m = 0; m < ST; ++m)
-            if (mine[m]) {
-                got[m] = true;
+                for (int ks = 0; ks < 2; ++ks) {
+                    float w[8];
+                    read_v(m, ks, w);
 #pragma unroll
-                for (int s = 0; s < SC; ++s) acc[m][s] = one[m][s];
+                    for (int e = 0; e < 8; ++e) most[m] = fmaxf(most[m], __builtin_fabsf(w[e]));
+                }
+                most[m] = fmaxf(most[m], __shfl_xor(most[m], 16, 64));
+                most[m] = fmaxf(most[m], __shfl_xor(most[m], 32, 64));
+                if (most[m] > 0.f && most[m] < __builtin_inff()) {
+                    // 2^100 or 2^-113 at most: what is smaller yet than 2^-85 is 0 in the result's type
+                    int e = 15 - __builtin_amdgcn_frexp_expf(most[m]);
+                    e = e > 100 ? 100 : e < -113 ? -113 : e;
+                    up[m] = ldexpf(1.f, e);
+                    down[m] = ldexpf(1.f, -e);
+                }
             }
-    });
-    // a token without an adapter is written by the first block of its tile
-#pragma unroll
-    for (int m = 0; m < ST; ++m) {
-        if (t[m] >= n_tok || !(got[m] || (!has[m] && blockIdx.z == 0 && base != out))) continue;
-#pragma unroll
-        for (int s = 0; s < SC; ++s) {
-            const int q = q0 + s * 16 + kq * 4;
-            t4 r = bs[m][s];
-            if (got[m])
-#pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = (T)((float)r[e] + acc[m][s][e]);
-            if (q < n_out) *(t4*)(out + t[m] * ldo + q) = r;
+        } else {
+            landed();
         }
-    }
+        f32x4 acc[ST][SC] = {};
+#pragma unroll 1
+        for (int k0 = 0;; k0 += 64) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (k0 + ks * 32 >= rank) break;
+                uint4 part[ST][kParts<T>];
+#pragma unroll
+                for (int m = 0; m < ST; ++m) {
+                    float w[8];
+                    read_v(m, ks, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] *= up[m];
+                    split8<T>(w, part[m]);
+                }
+#pragma unroll
+                for (int s = 0; s < SC; ++s) {
+                    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) const u32x4* ptr;
+                    const u32x4 r = *(ptr)(uintptr_t)(lds_b + (8 * n + s) * 128 + ((4 * ks + kq) ^ (n & 7)) * 16);
+                    const uint4 b = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+                    for (int m = 0; m < ST; ++m)
+#pragma unroll
+                        for (int k = 0; k < kParts<T>; ++k) acc[m][s] = mfma<T>(part[m][k], b, acc[m][s]);
+                }
+            }
+            // everyone has read this chunk (and, after the last, the next adapter's may overwrite it)
+            landed();
+            if (k0 + 64 >= rank) break;
+            load_chunk(k0 + 64);
+            landed();
+        }
+#pragma unroll
+        for (int m = 0; m < ST; ++m) {
+            const uint32_t tokens = (uint32_t)__ballot(mine[m]) & 0xFFFFu;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                typedef T t8 __attribute__((ext_vector_type(8)));
+                float w[8];
+                t8 r;
+                widen8<T>(bs[m][e], w);
+                const float back = __shfl(down[m], kq * 4 + e, 64);
+#pragma unroll
+                for (int s = 0; s < SC; ++s) r[s] = (T)fmaf(acc[m][s][e], back, w[s]);
+                put(tokens, m, e, __builtin_bit_cast(uint4, r));
+            }
+        }
+    });
 }
 
 template <typename T, int ST>
@@ -240,19 +355,17 @@ int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, in
     const uint32_t split = ST == 1 && n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
     if (n_ad > 0) {
         if (rank <= 16)
-            hipLaunchKernelGGL((k_lora_v<T, 1, ST>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A, a_stride, ids,
-                               scale, n_tok, n_ad, n_in, rank, v);
+            hipLaunchKernelGGL((k_lora_v<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+                               a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
         else
-            hipLaunchKernelGGL((k_lora_v<T, 2, ST>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+            hipLaunchKernelGGL((k_lora_v<T, 2, ST, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                                a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
         HIP_TRY(hipGetLastError());
     }
-    if ((int64_t)tiles * n_out < 512 * 256)
-        hipLaunchKernelGGL((k_lora_out<T, 1, ST>), dim3(tiles, (n_out + 63) / 64, split), dim3(256), 0, s, base, ldb, v, B,
-                           b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
-    else
-        hipLaunchKernelGGL((k_lora_out<T, 4, ST>), dim3(tiles, (n_out + 255) / 256, split), dim3(256), 0, s, base, ldb, v, B,
-                           b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
+    // few tokens: a wave per block, to reach more of the card
+    constexpr int W = ST == 1 ? 1 : 4;
+    hipLaunchKernelGGL((k_lora_out<T, ST, W>), dim3(tiles, (n_out + 128 * W - 1) / (128 * W), split), dim3(64 * W), 0, s, base, ldb,
+                       v, B, b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -270,8 +383,8 @@ int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, co
 bool bad_shapes(const char* who, int dtype, int n_tok, int n_ad, int n_in, int n_out, int rank, int64_t ldx, int64_t ldy,
                 int64_t a_stride, int64_t b_stride) {
     if ((dtype != 0 && dtype != 1) || n_tok < 0 || n_ad < 0 || n_in <= 0 || n_out <= 0 || rank <= 0 || n_in % 8 ||
-        n_out % 8 || rank % 8 || rank > 256 || (n_out + 63) / 64 > 65535) {
-        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^22)",
+        n_out % 8 || rank % 8 || rank > 256 || (n_out + 127) / 128 > 65535) {
+        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^23)",
                       who, dtype, n_tok, n_ad, n_in, n_out, rank);
         return true;
     }

@@ -97,16 +97,21 @@ def weight_grad(dyr, xr, seg_start, n_seg, scale=None):
 
 
 def lora(base, x, a, b, ids, scale=None):
-    """(base + scale b (a x), bound): both sums in fp32, the second over v with v's own error."""
+    """(base + scale b (a x), bound): both sums in fp32, the second over scale v with v's own error and, where v is
+    taken apart into 16-bit parts, a rest of 2^-22 of each value and 2^-39 of the token's largest."""
     out, xd = base.double().cpu().clone(), x.double().cpu()
     slack = torch.zeros_like(out)
     for j in range(a.shape[0]):
         rows = (ids.cpu() == j).nonzero()[:, 0]
+        if not rows.numel():
+            continue
         aj, bj, s = a[j].double().cpu(), b[j].double().cpu(), 1.0 if scale is None else float(scale[j])
         v = xd[rows] @ aj.T
-        dv = (aj.shape[1] + 2) * F32 * (xd[rows].abs() @ aj.abs().T)
+        dv = (aj.shape[1] + 3) * F32 * (xd[rows].abs() @ aj.abs().T)
+        dv = dv + 2.0 ** -22 * (v.abs() + dv) + 2.0 ** -39 * (v.abs() + dv).amax(1, keepdim=True)
         delta = s * (v @ bj.T)
         out[rows] += delta
         mag = abs(s) * ((v.abs() + dv) @ bj.abs().T)
-        slack[rows] = (aj.shape[0] + 3) * F32 * mag + abs(s) * (dv @ bj.abs().T) + F32 * (out[rows].abs() + mag)
+        # every value comes in up to three parts, each a term of its own in the sum
+        slack[rows] = (3 * aj.shape[0] + 3) * F32 * mag + abs(s) * (dv @ bj.abs().T) + F32 * (out[rows].abs() + mag)
     return out, slack

@@ -246,6 +246,25 @@ def test_infinities_and_nan_stay_in_their_rows(dtype):
     assert torch.equal(y, clean)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_has_the_same_bits_in_every_call(dtype):
+    """Alone, among few, among many, among thousands: the products and their gradients in x add in one order."""
+    from moe_offload import ops
+    n, k, e = 136, 1096, 3
+    w, wu = rnd((e, n, k), dtype, 1, k ** -0.5), rnd((e, 2 * n, k), dtype, 2, k ** -0.5)
+    first = None
+    for lens in ([1, 1, 1], [5, 16, 2], [40, 33, 17], [130, 200, 300], [2100, 1500, 2000]):
+        seg = np.concatenate([[0], np.cumsum(lens)])
+        m = int(seg[-1])
+        x, dy = rnd((m, k), dtype, 3), rnd((m, n), dtype, 4)
+        for i in range(3):                              # the first row of each segment is the same in every call
+            x[seg[i]], dy[seg[i]] = rnd((k,), dtype, 10 + i), rnd((n,), dtype, 20 + i)
+        at = torch.as_tensor(seg[:3], device=DEV)
+        got = [ops.grouped_mm(x, i32(seg), w)[at], ops.grouped_gate_up(x, None, i32(seg), wu)[at], ops.grouped_mm_dx(dy, i32(seg), w)[at]]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got)), lens
+
+
 def test_values_out_of_fp16_range_become_infinite():
     from moe_offload import ops
     x = torch.full((3, 64), 100.0, dtype=torch.float16, device=DEV)
