@@ -147,8 +147,14 @@ constexpr int kBC = 64;                                       // contraction ind
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 // Row of a step's image, along which the other index runs -> which 32-byte block trades places with block 0:
-// the rows that one transposing read touches (4 of each of two or four lane groups) get eight different ones.
-__device__ __forceinline__ int turn(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
+// the rows that one transposing read touches (4 of each of two or four lane groups) get eight different ones, or
+// as many as a row of W values has.
+template <int W>
+__device__ __forceinline__ int turn(int row) {
+    if constexpr (W >= 128) return (row & 3) | ((row >> 3) & 1) << 2;
+    else if constexpr (W == 64) return row & 3;
+    else return W == 32 ? row >> 3 & 1 : 0;              // rows of 64 bytes: 4 rows are 4 places already
+}
 
 // One operand's fragments for v_mfma_f32_16x16x32: lane (n, kq) holds c = 32 ks + 8 kq .. + 7 of row / column n.
 // ALONG false: the image has a row per tile row, 64 values (128 bytes) each, 16-byte unit u of row r at u ^ (r & 7).
@@ -164,7 +170,7 @@ struct Frags {
             const int row = kq * 8 + (n >> 2);
 #pragma unroll
             for (int s = 0; s < SUBS; ++s)
-                at[s] = base + row * (W * 2) + (((first >> 4) + s) ^ turn(row)) * 32 + (n & 3) * 8;
+                at[s] = base + row * (W * 2) + (((first >> 4) + s) ^ turn<W>(row)) * 32 + (n & 3) * 8;
         } else {
             at[0] = base + (first + n) * 128 + (kq ^ (n & 7)) * 16;
             at[1] = base + (first + n) * 128 + ((kq + 4) ^ (n & 7)) * 16;

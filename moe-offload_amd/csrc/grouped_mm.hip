@@ -19,6 +19,7 @@
 #include <hip/hip_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "grouped_mm.h"
 
@@ -56,8 +57,9 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
 
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
-// next tile's first step during the last of this one: two images, one barrier per step.
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
+// next tile's first step during the last of this one: two images, one barrier per step.  Narrow weights' gradients have
+// S = 4 images, three steps under way: their tiles are too few to hide a step's way behind each other's.
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, int S = 2, bool NT = false>
 __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
     constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
@@ -65,9 +67,12 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
-    static_assert(!kAlongQ || BQ >= 128, "the image's turns take 8 blocks of 32 bytes");
-    static_assert(!kAlongP || BP >= 128, "");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    constexpr bool kThroughLds = OP == kDw && BP == 128;
+    static_assert(!kThroughLds || (S == 2 && SP == 4 && SQ == 4 && kStage / kWaves == 8192), "");
+    static_assert(!NT || kThroughLds, "");
+    constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
+    __shared__ int2 idx[OP == kDw ? kIdx : 1];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
     const int inter = a.nq;                                                    // gate_up, and mm_dx with gu
@@ -106,18 +111,15 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kUnitsP = BP / 8, kUnitsQ = BQ / 8;                          // ALONG: 16-byte units per row of the image
     const int cu = ((lane & 7) ^ (lane >> 3)) * 8;                             // not ALONG: first c of the 16 bytes
     auto along_row = [&](int j, int loads, int units) { return (wv * loads + j) * (64 / units) + lane / units; };
-    auto along_col = [&](int row, int units) { return (lane % units ^ 2 * turn(row)) * 8; };
-    // mm_dw: the rows of dy and x of a step, loaded two steps ahead of their use in the product.  Otherwise the rows
-    // of x or dy, the same in every step.
-    int rp[kLoadsP], rq[kLoadsQ];
-    auto step_rows = [&](int c0) {
+    // The rows of x or dy, the same in every step.  mm_dw: numbers of the rows [c0, c1) of dy and x, -1 for one that is
+    // missing on either side: zeros on the one would still meet an infinity on the other.
+    int rp[kLoadsP];
+    auto hold_rows = [&](int c0, int c1) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
-#pragma unroll
-        for (int j = 0; j < kLoadsP; ++j) {
-            int c = c0 + along_row(j, kLoadsP, kUnitsP);
-            c = r0 + (c < nc ? c : nc - 1);
-            rp[j] = a.row_p ? a.row_p[c] : c;
-            rq[j] = a.row_q ? a.row_q[c] : c;
+        for (int c = c0 + t; c < c1; c += 64 * kWaves) {
+            const int v = a.row_p ? a.row_p[r0 + c] : r0 + c, x = a.row_q ? a.row_q[r0 + c] : r0 + c;
+            const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
+            idx[c - c0] = make_int2(both ? v : -1, both ? x : -1);
         }
     };
     if constexpr (OP != kDw) {
@@ -129,18 +131,21 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             rp[j] = v >= 0 && v < a.n_p ? v : 0;
         }
     }
+    // mm_dw of more rows than are held: tile by tile, kIdx rows [part0, part1) at a time
+    const bool parts = OP == kDw && nc > kIdx;
+    int part0 = 0, part1 = nc;
     int load_tile = tile, load_c = 0;                                          // the step that is loaded next
     auto place = [&]() {
         const bool any = load_tile < end;
         const int q0 = load_tile * kQStep;
         if constexpr (OP == kDw) {
-            // a row that is missing on one side is left out on both: zeros would still meet an infinity there
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) {
-                const int row = along_row(j, kLoadsP, kUnitsP), col = along_col(row, kUnitsP);
-                const bool ok = any && load_c + row < nc && rp[j] >= 0 && rp[j] < a.n_p && rq[j] >= 0 && rq[j] < a.n_q;
-                pp[j] = ok ? P + rp[j] * a.ldp + (p0 + col < a.np ? p0 + col : 0) : zero;
-                qp[j] = ok ? Q + rq[j] * a.ldq + (q0 + col < a.nq ? q0 + col : 0) : zero;
+                const int row = along_row(j, kLoadsP, kUnitsP), col = (lane % kUnitsP ^ 2 * turn<BP>(row)) * 8;
+                const int2 v = idx[any && load_c + row < part1 ? load_c + row - part0 : 0];
+                const bool ok = any && load_c + row < part1 && v.x >= 0;
+                pp[j] = ok ? P + v.x * a.ldp + (p0 + col < a.np ? p0 + col : 0) : zero;
+                qp[j] = ok ? Q + v.y * a.ldq + (q0 + col < a.nq ? q0 + col : 0) : zero;
             }
         } else {
             const bool ok = any && load_c + cu < nc;
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
 #pragma unroll
             for (int j = 0; j < kLoadsQ; ++j) {
                 if constexpr (kAlongQ) {
-                    const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + along_col(row, kUnitsQ);
+                    const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + (lane % kUnitsQ ^ 2 * turn<BQ>(row)) * 8;
                     qp[j] = any && load_c + row < nc ? Q + (int64_t)(load_c + row) * a.nq + (q < a.nq ? q : 0) : zero;
                 } else {
                     const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
@@ -177,12 +182,17 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             for (int j = 0; j < kLoadsQ; ++j) qp[j] += kAlongQ ? (int64_t)kBC * a.nq : kBC;
             return;
         }
-        if (load_c >= nc) {
+        if (load_c >= part1) {
             load_c = 0;
-            ++load_tile;
+            load_tile = parts ? end : load_tile + 1;
+            if (kThroughLds && nc <= kBC && load_tile < end && (load_tile + 1) * BQ <= a.nq) {
+                // the same rows again, further right: no row numbers, no multiplications (lanes without a row stay at zero)
+#pragma unroll
+                for (int j = 0; j < kLoadsQ; ++j) qp[j] += qp[j] == zero ? 0 : BQ;
+                return;
+            }
         }
         place();
-        if (OP == kDw && nc > kBC) step_rows(load_c + kBC < nc ? load_c + kBC : 0);
     };
     auto load = [&](int d, uint32_t stage) {
         if (d < kLoadsP) load_to_lds(pp[d], lds0 + stage + (wv * kLoadsP + d) * 1024);
@@ -214,14 +224,26 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
         }
     }
     uint32_t stage = 0;
-    if (nc > 0) {
-        if constexpr (OP == kDw) step_rows(0);
+    bool landed = false;                                                       // the next step's loads have been waited for
+    auto start = [&](int c0) {
+        load_tile = tile;
+        load_c = c0;
         place();
+        uint32_t to = stage;
 #pragma unroll
-        for (int d = 0; d < kLoads; ++d) load(d, 0);
-        if constexpr (OP == kDw)
-            if (nc > kBC) step_rows(kBC);
-        advance();
+        for (int s = 0; s < S - 1; ++s) {
+#pragma unroll
+            for (int d = 0; d < kLoads; ++d) load(d, to);
+            to = to == (S - 1) * kStage ? 0 : to + kStage;
+            advance();
+        }
+    };
+    if (nc > 0 && !parts) {
+        if constexpr (OP == kDw) {
+            hold_rows(0, nc);
+            __syncthreads();
+        }
+        start(0);
     }
 #pragma unroll 1
     for (; tile < end; ++tile) {
@@ -229,16 +251,23 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
         f32x4 acc[SP][SQ] = {};
 #pragma unroll 1
         for (int c0 = 0; c0 < nc; c0 += kBC) {
-            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier,
-            // so are everyone's
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if (OP == kDw && parts && c0 % kIdx == 0) {
+                part0 = c0;
+                part1 = c0 + kIdx < nc ? c0 + kIdx : nc;
+                __syncthreads();                                               // the rows held so far are all placed
+                hold_rows(part0, part1);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the part before's loads past its end
+                __syncthreads();
+                start(part0);
+            }
+            // this wave's loads of the step have landed (they return in order; later steps' may be under way) and its
+            // reads of the step before are done; past the barrier, so are everyone's
+            if (landed) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * kLoads) : "memory");
+            landed = false;
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if constexpr (OP == kDw) {
-                // here no load is under way that the compiler's wait for these could take in
-#pragma unroll
-                for (int j = 0; j < kLoadsP; ++j) asm volatile("" : "+v"(rp[j]), "+v"(rq[j]));
-            }
+            const uint32_t fill = stage == 0 ? (S - 1) * kStage : stage - kStage;
             // The step's second half is read from LDS, and the next step's loads are issued, between the first half's
             // products, row by row (past the last step they fetch zeros that nobody reads)
             uint4 vp[2][SP], vq[2][SQ];
@@ -262,7 +291,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
 #pragma unroll
                 for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
 #pragma unroll
-                for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, kStage - stage);
+                for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
                 __builtin_amdgcn_sched_barrier(0);
             }
             advance();
@@ -270,7 +299,68 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             for (int i = 0; i < SP; ++i)
 #pragma unroll
                 for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
-            stage = kStage - stage;
+            stage = stage == (S - 1) * kStage ? 0 : stage + kStage;
+        }
+        // The next tile's first step is waited for before the stores: in the loop the wait would take them in.
+        if (S == 2 && BP < 256 && nc > 0 && tile + 1 < end) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            landed = !parts;
+        }
+        if constexpr (kThroughLds) {
+            // The results go through the image just multiplied, a part of it for each wave, and out in whole lines: a lane
+            // of the matrix unit's result has 8 or 16 bytes of a row and its neighbour another row's, each a cache access
+            // of its own.  That pays where the output is most of the bytes (weights' gradient over 512 x 40 rows, 1024 x
+            // 2048: 640 us, like this 591, with stores past the caches 520) and costs a barrier where it is not (mm of 777
+            // x 6 rows over 100 segments, 1152 x 320: 20.6 us, like this 24.4).
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                                      // everyone has read the image
+            asm volatile("" ::: "memory");
+            const uint32_t area = lds0 + (kStage - stage) + wv * (kStage / kWaves);
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) u32x4* lds16;
+            const int64_t top = (int64_t)seg * a.ldo;
+            const int first = p0 + wp * SP * 16;                               // output row of the wave's row 0
+            // subtile rows [i0, i0 + kPass) of the wave's 16 SQ columns; unit u of row r is at u ^ (r & 7) in its low bits
+            auto pass = [&](auto bytes_c, int i0, auto put, auto* dst) {
+                constexpr int kBytes = decltype(bytes_c)::value, UNITS = SQ * kBytes, kRowsPer = 64 / UNITS;
+                constexpr int kPass = kStage / kWaves / (UNITS * 256);
+                auto at = [&](int row, int u) { return area + (uint32_t)(row * UNITS + (u ^ (row & 7))) * 16; };
+                put(at);
+#pragma unroll
+                for (int it = 0; it < kPass * 16 / kRowsPer; ++it) {
+                    const int row = it * kRowsPer + lane / UNITS, u = lane % UNITS;
+                    const u32x4 v = *(lds16)(uintptr_t)at(row, u);
+                    const int o = first + i0 * 16 + row, c = q0 + wq * SQ * 16 + u * (16 / kBytes);
+                    if (o < a.np && c < a.nq) {
+                        auto* to = (u32x4*)(dst + top + (int64_t)o * a.nq + c);
+                        if constexpr (NT) __builtin_nontemporal_store(v, to);
+                        else *to = v;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if (a.out_f32) {
+#pragma unroll
+                for (int i0 = 0; i0 < SP; i0 += 2)
+                    pass(std::integral_constant<int, 4>(), i0, [&](auto at) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int j = 0; j < SQ; ++j)
+                                *(lds16)(uintptr_t)at(i * 16 + n, 4 * j + kq) = __builtin_bit_cast(u32x4, acc[i0 + i][j] * s);
+                    }, (float*)a.out);
+            } else {
+                pass(std::integral_constant<int, 2>(), 0, [&](auto at) {
+#pragma unroll
+                    for (int i = 0; i < SP; ++i)
+#pragma unroll
+                        for (int j = 0; j < SQ; j += 2) {
+                            const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
+                            *(lds16)(uintptr_t)at(i * 16 + n, 2 * j + (kq & 1) * 2 + (kq >> 1)) = (u32x4){v.x, v.y, v.z, v.w};
+                        }
+                }, (T*)a.out);
+            }
+            continue;
         }
 #pragma unroll
         for (int i = 0; i < SP; ++i) {
@@ -477,7 +567,7 @@ __global__ __launch_bounds__(64) void k_grouped_few(Args a) {
 // Row tiles of a call as far as the host knows it: a segment's last tile is half full on average.
 int64_t row_tiles(const Args& a, int bp) { return (a.S.n_rows + (int64_t)(a.S.n_seg - 1) * (bp / 2) + bp - 1) / bp; }
 
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, int S = 2, bool NT = false>
 int launch_tiles(Args a, hipStream_t s) {
     const int qstep = OP == kGateUp ? BQ / 2 : BQ, tiles = (a.nq + qstep - 1) / qstep;
     int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
@@ -502,7 +592,7 @@ int launch_tiles(Args a, hipStream_t s) {
         moe_set_error("grouped product: %lld x %lld tiles are more than one launch takes", (long long)most, (long long)groups);
         return -1;
     }
-    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)(most * groups)), dim3(64 * WP * WQ), 0, s, a);
+    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS, S, NT>), dim3((uint32_t)(most * groups)), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -535,6 +625,11 @@ int launch(const Args& a, hipStream_t s) {
         // 2048: 592 us, and 737 with the large tiles)
         auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * cols(b); };
         if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
+        // an output larger than the 256 MB of Infinity Cache only pushes the inputs out of it, and its lines are written
+        // back under the next kernel
+        if (per_seg < 512 && (int64_t)a.S.n_seg * a.np * a.nq * (a.out_f32 ? 4 : 2) > 256 << 20)
+            return launch_tiles<T, OP, 128, 128, 2, 2, 2, 2, true>(a, s);
+        if (a.np <= 64 || a.nq <= 64) return launch_tiles<T, OP, 64, 64, 2, 2, 2, 4>(a, s);
         return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
     } else {
         if constexpr (OP == kMM || OP == kGateUp) {

@@ -1,5 +1,5 @@
-"""Plain 64-bit forms of the grouped products, their gradients and the adapters (CPU), with the bounds their
-tests use.
+"""Plain 64-bit forms of the grouped products, their gradients and the adapters, with the bounds their tests use; on the
+device of the sorted rows they are given (the CPU but for the largest sizes).
 
 Bounds.  Inputs are fp16 or bf16, so a product of two is exact in fp32 (at most 22 significand bits).  A sum of
 c of them in fp32, in any order and with either rounding or truncation per addition, is off by at most
@@ -18,7 +18,7 @@ def half_step(want, dtype):
 
 def check(got, want, slack, what=""):
     """|got - want| <= half a step of got's type + slack, where slack bounds the error before rounding."""
-    got_d, want_d = got.detach().double().cpu(), want.double()
+    got_d, want_d = got.detach().to(want.device).double(), want.double()
     assert got_d.shape == want_d.shape, (what, got_d.shape, want_d.shape)
     # the value that is rounded may be `slack` larger than want, and its step with it
     room = half_step(want_d.abs() + slack, got.dtype) + slack
@@ -50,10 +50,10 @@ def gather(x, rows):
 
 def product(xr, seg_start, w, seg_slot=None, scale=None, transposed=False):
     """(values, bound before rounding, rows that a segment covers) of the sorted rows' products."""
-    w = w.double().cpu()
+    w = w.to(xr.device).double()
     n_out = w.shape[2] if transposed else w.shape[1]
-    y = torch.zeros((xr.shape[0], n_out), dtype=torch.float64)
-    mag, has = y.clone(), torch.zeros(xr.shape[0], dtype=torch.bool)
+    y = torch.zeros((xr.shape[0], n_out), dtype=torch.float64, device=xr.device)
+    mag, has = y.clone(), torch.zeros(xr.shape[0], dtype=torch.bool, device=xr.device)
     for r0, r1, slot in segments(seg_start, seg_slot, w.shape[0], xr.shape[0]):
         m = w[slot] if transposed else w[slot].T
         s = 1.0 if scale is None else float(scale[slot])
@@ -74,7 +74,7 @@ def glu(g, u, slack_g, slack_u):
 
 
 def glu_grad(dh, slack_dh, gu):
-    g, u = gu.double().cpu().chunk(2, 1)
+    g, u = gu.to(dh.device).double().chunk(2, 1)
     sig = torch.sigmoid(g)
     fg, fu = u * sig * (1 + g * (1 - sig)), g * sig
     # 1 + g (1 - sig) may cancel: its parts' roundings count with their magnitude
@@ -87,7 +87,7 @@ def glu_grad(dh, slack_dh, gu):
 
 def weight_grad(dyr, xr, seg_start, n_seg, scale=None):
     n_rows = dyr.shape[0]
-    dw = torch.zeros((n_seg, dyr.shape[1], xr.shape[1]), dtype=torch.float64)
+    dw = torch.zeros((n_seg, dyr.shape[1], xr.shape[1]), dtype=torch.float64, device=xr.device)
     slack = dw.clone()
     for r0, r1, u in segments(seg_start, None, n_seg, n_rows):
         s = 1.0 if scale is None else float(scale[u])

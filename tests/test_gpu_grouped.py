@@ -299,6 +299,52 @@ def test_offsets_past_32_bits(op):
         ref.check(ops.grouped_mm_dx(dy, seg, far), *ref.product(dy.double().cpu(), seg.tolist(), w, transposed=True)[:2])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_products(dtype):
+    """Long segments and wide outputs, where the largest tiles run; sizes that end inside them."""
+    from moe_offload import ops
+    seg = np.array([0, 2100, 2100, 3601, 5602], np.int32)
+    m, e, n, k = 5602, 4, 2056, 200
+    x, w, wu = rnd((m, k), dtype, 1), rnd((e, n, k), dtype, 2, k ** -0.5), rnd((e, 2 * 1048, k), dtype, 3, k ** -0.5)
+    rng = np.random.default_rng(0)
+    order = i32(rng.permutation(m))
+    xr, at = x[order.long()].double(), order.long()
+    y = ops.grouped_mm(x, i32(seg), w, row_in=order, row_out=order)
+    want, slack, _ = ref.product(xr, seg, w)
+    ref.check(y[at], want, slack, "mm")
+    gu = torch.empty((m, 2096), dtype=dtype, device=DEV)
+    h = ops.grouped_gate_up(x, order, i32(seg), wu, gu_out=gu)
+    want, slack, _ = ref.product(xr, seg, wu)
+    ref.check(gu, want, slack, "gu")
+    ref.check(h, *ref.glu(*want.chunk(2, 1), *slack.chunk(2, 1)), "h")
+    dy, wd = rnd((m, k), dtype, 4), rnd((e, k, n), dtype, 5, k ** -0.5)
+    dyr = dy[at].double()
+    want, slack, _ = ref.product(dyr, seg, wd, transposed=True)
+    ref.check(ops.grouped_mm_dx(dy, i32(seg), wd, row_in=order, row_out=order)[at], want, slack, "dx")
+    g2 = rnd((m, 2 * n), dtype, 6)
+    ref.check(ops.grouped_mm_dx(dy, i32(seg), wd, row_in=order, gu=g2), *ref.glu_grad(want, slack, g2), "dgu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k,lens", [(64, 264, [1024, 0, 1025, 2500]), (200, 40, [3000, 1]), (264, 392, [1100, 2049, 64]),
+                                      (1032, 1000, [512] * 10 + [0, 1030, 2600, 511, 700, 3])])
+def test_dw_of_long_segments(dtype, n, k, lens):
+    """More rows than a block holds the numbers of, in each of the tile sizes, some rows missing."""
+    from moe_offload import ops
+    seg = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    m, e = int(seg[-1]), len(lens)
+    rng = np.random.default_rng(n)
+    rows_dy, rows_x = rng.integers(-2, 900, m), rng.integers(0, 1002, m)
+    dy, x = rnd((900, n), dtype, 1), rnd((1000, k), dtype, 2)
+    both = torch.tensor((rows_dy >= 0) & (rows_x < 1000)).unsqueeze(1)
+    dyr, xr = ref.gather(dy, rows_dy) * both, ref.gather(x, rows_x) * both
+    want, slack = ref.weight_grad(dyr.to(DEV), xr.to(DEV), seg, e)
+    ref.check(ops.grouped_mm_dw(dy, x, i32(seg), row_dy=i32(rows_dy), row_x=i32(rows_x)), want, slack, "by index")
+    ref.check(ops.grouped_mm_dw(dy, x, i32(seg), row_dy=i32(rows_dy), row_x=i32(rows_x), dtype=torch.float32), want, slack, "fp32")
+    dy, x = rnd((m, n), dtype, 3), rnd((m, k), dtype, 4)
+    ref.check(ops.grouped_mm_dw(dy, x, i32(seg)), *ref.weight_grad(dy.double(), x.double(), seg, e), "in order")
+
+
 def _layer(dtype, tokens, k, n_exp, hidden, inter, seed=0, drop=False):
     g = torch.Generator().manual_seed(seed)
     ids = torch.stack([torch.randperm(n_exp, generator=g)[:k] for _ in range(tokens)]).to(torch.int32)
