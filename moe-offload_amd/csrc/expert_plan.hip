@@ -24,7 +24,7 @@ constexpr int kPlanThreads = 64 * kPlanWaves;
 constexpr int kPlanMaxExp = 1024;
 constexpr int kPlanOne = 4096;        // pairs that one block takes alone
 constexpr int kPlanBlocks = 256;
-constexpr int kPlanPairs = 1024;      // pairs per block, at least, where there are several
+constexpr int kPlanPairs = 2048;      // pairs per block, at least, where there are several
 
 __host__ __device__ inline int plan_blocks(int n_ids) {
     if (n_ids <= kPlanOne) return 1;
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_place(const int32_t* __re
     // thread c: the pairs of class c in all blocks, and in the blocks before this one
     int all = 0, before = 0;
     if (gridDim.x > 1 && t < classes) {
-#pragma unroll 8
+#pragma unroll 16
         for (int b = 0; b < (int)gridDim.x; ++b) {
             const int c = counts[(size_t)b * classes + t];
             all += c;

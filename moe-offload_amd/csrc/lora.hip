@@ -55,19 +55,19 @@ __device__ __forceinline__ void each_adapter(const int (&id)[ST], const bool (&h
 
 constexpr int kVWaves = 8;
 
-// v[t][j] = s_i A_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y).  Each wave multiplies every eighth
-// step of 64 along the row, through an LDS ring of its own (D steps of the tokens' and the ranks' rows); the waves'
-// sums are added in their order.
-template <typename T, int SR, int ST, int D>
-__global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x, int64_t ldx, const T* __restrict__ A,
-                                                         int64_t a_stride, const int32_t* __restrict__ ids,
-                                                         const float* __restrict__ scale, int n_tok, int n_ad, int n_in,
-                                                         int rank, float* __restrict__ v) {
+// v[t][j] = s_i W_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), where W_i[j] is row j of A_i, or
+// (ALONG) column j of B_i [nc][rank].  Each wave multiplies every eighth step of 64 along the contraction, through an LDS
+// ring of its own (D steps of the tokens' and the ranks' operands); the waves' sums are added in their order.  O: fp32, or
+// T where v is an operand of a product next.
+template <typename T, int SR, int ST, int D, bool ALONG, typename O>
+__device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* __restrict__ x, int64_t ldx,
+                                         const T* __restrict__ W, int64_t w_stride, const int32_t* __restrict__ ids,
+                                         const float* __restrict__ scale, int n_tok, int n_ad, int nc, int rank,
+                                         O* __restrict__ v) {
     constexpr int kLoads = 2 * (ST + SR);
     constexpr uint32_t kStage = kLoads * 1024;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kVWaves * D * kStage];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
-    const uint32_t all = (uint32_t)(uintptr_t)(lds_u8*)lds, ring = all + wv * D * kStage;
+    const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)lds + wv * D * kStage;
     const int j0 = blockIdx.y * (16 * SR), cu = ((lane & 7) ^ (lane >> 3)) * 8;
     const T* zero = (const T*)&g_zero16;
     asm("" : "+s"(zero));
@@ -87,26 +87,34 @@ __global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x
         xp[j] = x + (r < n_tok ? r : n_tok - 1) * ldx + cu;
     }
     Frags<false, 16, ST> fx;
-    Frags<false, 16, SR> fa;
+    Frags<ALONG, 16 * SR, SR> fw;
     fx.init(ring, 0, lane);
-    fa.init(ring + ST * 2048, 0, lane);
-    const int steps = ((n_in + 63) / 64 - wv + kVWaves - 1) / kVWaves;         // wv, wv + 8, ...
-    each_adapter<ST>(id, has, blockIdx.z, gridDim.z, [&](int i, const bool (&mine)[ST]) {
+    fw.init(ring + ST * 2048, 0, lane);
+    const int steps = ((nc + 63) / 64 - wv + kVWaves - 1) / kVWaves;           // wv, wv + 8, ...
+    each_adapter<ST>(id, has, z, n_z, [&](int i, const bool (&mine)[ST]) {
         const float si = scale ? scale[i] : 1.0f;
-        const T* ap[2 * SR];
+        const T* wp[2 * SR];
+        int first_c[2 * SR];                                                   // of the lane's 16 bytes, in a step
 #pragma unroll
         for (int j = 0; j < 2 * SR; ++j) {
-            const int r = j0 + j * 8 + (lane >> 3);
-            ap[j] = A + (int64_t)i * a_stride + (int64_t)(r < rank ? r : rank - 1) * n_in + cu;
+            if constexpr (ALONG) {
+                const int row = j * (32 / SR) + lane / (2 * SR), q = j0 + (lane % (2 * SR) ^ 2 * turn<16 * SR>(row)) * 8;
+                first_c[j] = q < rank ? row : nc;                              // (ranks past the end: zeros)
+                wp[j] = W + (int64_t)i * w_stride + (int64_t)row * rank + q;
+            } else {
+                const int r = j0 + j * 8 + (lane >> 3);
+                first_c[j] = cu;
+                wp[j] = W + (int64_t)i * w_stride + (int64_t)(r < rank ? r : rank - 1) * nc + cu;
+            }
         }
         auto issue = [&](int s) {
-            const int c = (s * kVWaves + wv) * 64;
+            const int c = (s * kVWaves + wv) * 64;                             // (also past the last step)
             const uint32_t to = ring + (uint32_t)(s % D) * kStage;
-            const bool in = c + cu < n_in;                                     // (also past the last step)
 #pragma unroll
-            for (int j = 0; j < 2 * ST; ++j) load_to_lds(in ? xp[j] + c : zero, to + j * 1024);
+            for (int j = 0; j < 2 * ST; ++j) load_to_lds(c + cu < nc ? xp[j] + c : zero, to + j * 1024);
 #pragma unroll
-            for (int j = 0; j < 2 * SR; ++j) load_to_lds(in ? ap[j] + c : zero, to + (2 * ST + j) * 1024);
+            for (int j = 0; j < 2 * SR; ++j)
+                load_to_lds(c + first_c[j] < nc ? wp[j] + (ALONG ? (int64_t)c * rank : c) : zero, to + (2 * ST + j) * 1024);
         };
         f32x4 acc[SR][ST] = {};
 #pragma unroll
@@ -115,13 +123,13 @@ __global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x
         for (int s = 0; s < steps; ++s) {
             const uint32_t stage = (uint32_t)(s % D) * kStage;
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");   // loads return in order
-            uint4 xv[2][ST], av[2][SR];
+            uint4 xv[2][ST], wr[2][SR];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
                 for (int m = 0; m < ST; ++m) xv[ks][m] = fx.read(stage, m, ks);
 #pragma unroll
-                for (int r = 0; r < SR; ++r) av[ks][r] = fa.read(stage, r, ks);
+                for (int r = 0; r < SR; ++r) wr[ks][r] = fw.read(stage, r, ks);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                        // read before the next load overwrites it
             issue(s + D);
@@ -130,7 +138,7 @@ __global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x
 #pragma unroll
                 for (int r = 0; r < SR; ++r)
 #pragma unroll
-                    for (int m = 0; m < ST; ++m) acc[r][m] = mfma<T>(av[ks][r], xv[ks][m], acc[r][m]);
+                    for (int m = 0; m < ST; ++m) acc[r][m] = mfma<T>(wr[ks][r], xv[ks][m], acc[r][m]);
         }
         // the sums trade places through the rings, which are idle once every wave's loads have landed
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -146,12 +154,69 @@ __global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* __restrict__ x
             f32x4 sum = part[0][wv][lane];
 #pragma unroll
             for (int w = 1; w < kVWaves; ++w) sum += part[w][wv][lane];
+            sum *= si;
 #pragma unroll
             for (int m = 0; m < ST; ++m)
-                if (wv % ST == m && mine[m] && j < rank) *(f32x4*)(v + t[m] * rank + j) = sum * si;
+                if (wv % ST == m && mine[m] && j < rank) {
+                    if constexpr (sizeof(O) == 4) *(f32x4*)(v + t[m] * rank + j) = sum;
+                    else *(uint2*)(v + t[m] * rank + j) = round4<T>(sum);
+                }
         }
         __syncthreads();
     });
+}
+
+template <int SR, int ST, int D>
+constexpr uint32_t kRings = kVWaves * D * 2 * (ST + SR) * 1024;
+
+template <typename T, int SR, int ST, int D>
+__global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* x, int64_t ldx, const T* A, int64_t a_stride, const int32_t* ids,
+                                                         const float* scale, int n_tok, int n_ad, int n_in, int rank, float* v) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST, D>];
+    ranks_of<T, SR, ST, D, false, float>(lds, blockIdx.z, gridDim.z, x, ldx, A, a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
+}
+
+// The gradients' v = A_i x[t] and dv = s_i B_i^T dy[t], one in the even blocks of the third dimension, one in the odd.
+template <typename T, int SR, int ST, int D>
+__global__ __launch_bounds__(64 * kVWaves) void k_lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy,
+                                                            int64_t lddy, const T* B, int64_t b_stride, const int32_t* ids,
+                                                            const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
+                                                            T* v, T* dv) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST, D>];
+    const int z = blockIdx.z >> 1, n_z = gridDim.z >> 1;
+    if (blockIdx.z & 1)
+        ranks_of<T, SR, ST, D, true, T>(lds, z, n_z, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_out, rank, dv);
+    else
+        ranks_of<T, SR, ST, D, false, T>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
+}
+
+// Blocks of a tile's adapters: up to 256 tokens each gets its own (16 tokens have 16 at most).
+template <int ST>
+uint32_t split_of(int n_tok) {
+    return ST == 1 && n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
+}
+
+template <typename T, int ST>
+int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy, int64_t lddy, const T* B, int64_t b_stride,
+              const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, T* v, T* dv, hipStream_t s) {
+    const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST)), split = 2 * split_of<ST>(n_tok);
+    if (rank <= 16)
+        hipLaunchKernelGGL((k_lora_v_dv<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+                           a_stride, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv);
+    else
+        hipLaunchKernelGGL((k_lora_v_dv<T, 2, ST, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+                           a_stride, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+template <typename T>
+int lora_v_dv_typed(const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* dy, int64_t lddy, const void* B,
+                    int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
+                    void* v, void* dv, hipStream_t s) {
+    auto f = n_tok <= 1024 ? lora_v_dv<T, 1> : lora_v_dv<T, 2>;
+    return f((const T*)x, ldx, (const T*)A, a_stride, (const T*)dy, lddy, (const T*)B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out,
+             rank, (T*)v, (T*)dv, s);
 }
 
 // fp32 values as sums of values of T that keep their bits: bf16 has fp32's range, three of its 8 bits each are 24 bits;
@@ -351,8 +416,7 @@ int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, in
              const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, float* v, T* out,
              int64_t ldo, hipStream_t s) {
     const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST));
-    // up to 256 tokens a tile's adapters get blocks of their own (16 tokens have 16 at most)
-    const uint32_t split = ST == 1 && n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
+    const uint32_t split = split_of<ST>(n_tok);
     if (n_ad > 0) {
         if (rank <= 16)
             hipLaunchKernelGGL((k_lora_v<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
@@ -467,17 +531,17 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
     int32_t* order = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* same = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* seg = (int32_t*)take((uint64_t)(n_ad + 1) * 4);
-    // rows sorted by adapter; v and dv are in that order.  Without tokens da and db are the products over empty segments
+    auto v_dv = dtype ? lora_v_dv_typed<__bf16> : lora_v_dv_typed<_Float16>;
+    // the tokens sorted by adapter: a token's row number everywhere but in seg is its own.  Without tokens da and db are the
+    // products over empty segments.
     if (moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
-        moe_grouped_mm(x, ldx, n_tok, order, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, v, rank, n_tok,
-                       nullptr, dtype, 1, stream) ||
-        moe_grouped_mm_dx(dy, lddy, n_tok, order, seg, nullptr, n_ad, n_tok, b, b_stride, n_ad, n_out, rank, scale, nullptr, 0,
-                          dv, rank, n_tok, nullptr, dtype, 1, stream) ||
-        moe_grouped_mm_dx(dv, rank, n_tok, nullptr, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, nullptr,
-                          0, dx, lddx, n_tok, order, dtype, 1, stream) ||
-        moe_grouped_mm_dw(dv, rank, n_tok, nullptr, x, ldx, n_tok, order, seg, n_ad, n_tok, rank, n_in, nullptr, da, mat, 0,
+        (n_tok > 0 && v_dv(x, ldx, a, a_stride, dy, lddy, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv,
+                           (hipStream_t)stream)) ||
+        moe_grouped_mm_dx(dv, rank, n_tok, order, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, nullptr, 0,
+                          dx, lddx, n_tok, order, dtype, 1, stream) ||
+        moe_grouped_mm_dw(dv, rank, n_tok, order, x, ldx, n_tok, order, seg, n_ad, n_tok, rank, n_in, nullptr, da, mat, 0,
                           dtype, stream) ||
-        moe_grouped_mm_dw(dy, lddy, n_tok, order, v, rank, n_tok, nullptr, seg, n_ad, n_tok, n_out, rank, scale, db,
+        moe_grouped_mm_dw(dy, lddy, n_tok, order, v, rank, n_tok, order, seg, n_ad, n_tok, n_out, rank, scale, db,
                           (int64_t)rank * n_out, 0, dtype, stream))
         return -1;
     return 0;

@@ -210,21 +210,22 @@ def cb_up(x, pool, slots, grid, hidden, inter, h_out=None):
 _HALF = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _one_gpu(who: str, **tensors) -> int:
-    """The index of the one GPU that every given tensor is on."""
+def _one_gpu(who: str, names: str, *tensors) -> int:
+    """The index of the one GPU that every given tensor is on (names: theirs, in order)."""
     dev = None
-    for name, t in tensors.items():
+    for i, t in enumerate(tensors):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{who}: {name} must be a tensor, not {type(t).__name__}")
+            raise TypeError(f"{who}: {names.split()[i]} must be a tensor, not {type(t).__name__}")
         at = t.get_device()
+        if at == dev:
+            continue
         if at < 0:
-            raise ValueError(f"{who}: {name} is on {t.device}, not on a GPU")
-        if dev is None:
-            dev = at
-        elif at != dev:
-            raise ValueError(f"{who}: {name} is on GPU {at}, others on GPU {dev}")
+            raise ValueError(f"{who}: {names.split()[i]} is on {t.device}, not on a GPU")
+        if dev is not None:
+            raise ValueError(f"{who}: {names.split()[i]} is on GPU {at}, others on GPU {dev}")
+        dev = at
     return dev
 
 
@@ -290,14 +291,18 @@ def _half(who: str, t: torch.Tensor) -> int:
     return dt
 
 
+# the current stream's handle without a Stream object around it, where torch has that (a microsecond per call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _call(name: str, dev: int, *args) -> None:
     """Calls an entry point on the tensors' own GPU and that GPU's current stream."""
     fn = getattr(_lib.lib(), name)
     if torch.cuda.current_device() == dev:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     _lib.check(rc, name)
 
 
@@ -328,12 +333,14 @@ def expert_plan(ids: torch.Tensor, n_exp: int, row_token: torch.Tensor | None = 
     behind the last segment.  n_exp up to 1024.
     """
     who = "expert_plan"
-    dev = _one_gpu(who, ids=ids, row_token=row_token, row_out=row_out, seg_start=seg_start)
+    dev = _one_gpu(who, "ids row_token row_out seg_start", ids, row_token, row_out, seg_start)
     _index(who, "ids", ids)
     if ids.dim() not in (1, 2) or not 1 <= n_exp <= 1024:
         raise ValueError(f"{who}: ids of shape {tuple(ids.shape)}, n_exp={n_exp} (ids [n_tok, k] or [n_tok], n_exp 1..1024)")
     k = ids.shape[1] if ids.dim() == 2 else 1
     m = ids.numel()
+    if row_token is None and row_out is None and seg_start is None:
+        row_token, row_out, seg_start = torch.empty(2 * m + n_exp + 1, dtype=torch.int32, device=ids.device).split((m, m, n_exp + 1))
     if row_token is None:
         row_token = torch.empty(m, dtype=torch.int32, device=ids.device)
     if row_out is None:
@@ -368,7 +375,7 @@ def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_
     zeros, a row_out outside the output is dropped.
     """
     who = "grouped_mm"
-    dev = _one_gpu(who, x=x, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, out=out)
+    dev = _one_gpu(who, "x seg_start w row_in row_out seg_slot scale out", x, seg_start, w, row_in, row_out, seg_slot, scale, out)
     dt = _half(who, x)
     n_seg = _segments(who, seg_start, seg_slot)
     w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
@@ -398,7 +405,7 @@ def grouped_gate_up(x, row_token, seg_start, w, seg_slot=None, h_out=None, gu_ou
     output and left as they are in a given one.
     """
     who = "grouped_gate_up"
-    dev = _one_gpu(who, x=x, row_token=row_token, seg_start=seg_start, w=w, seg_slot=seg_slot, h_out=h_out, gu_out=gu_out)
+    dev = _one_gpu(who, "x row_token seg_start w seg_slot h_out gu_out", x, row_token, seg_start, w, seg_slot, h_out, gu_out)
     dt = _half(who, x)
     n_seg = _segments(who, seg_start, seg_slot)
     w_stride = _mats(who, "w", w, x.dtype, (None, None, None))
@@ -435,8 +442,7 @@ def grouped_mm_dx(dy, seg_start, w, row_in=None, row_out=None, n_out_rows=None, 
     sorted order; the result is then the gradient of (g, u), [*, 2 * K].  Other arguments as grouped_mm.
     """
     who = "grouped_mm_dx"
-    dev = _one_gpu(who, dy=dy, seg_start=seg_start, w=w, row_in=row_in, row_out=row_out, seg_slot=seg_slot, scale=scale, gu=gu,
-                  out=out)
+    dev = _one_gpu(who, "dy seg_start w row_in row_out seg_slot scale gu out", dy, seg_start, w, row_in, row_out, seg_slot, scale, gu, out)
     dt = _half(who, dy)
     n_seg = _segments(who, seg_start, seg_slot)
     w_stride = _mats(who, "w", w, dy.dtype, (None, None, None))
@@ -467,7 +473,7 @@ def grouped_mm_dw(dy, x, seg_start, row_dy=None, row_x=None, scale=None, dtype=N
     grouped_mm took row_in and row_out, this takes row_x=row_in and row_dy=row_out.
     """
     who = "grouped_mm_dw"
-    dev = _one_gpu(who, dy=dy, x=x, seg_start=seg_start, row_dy=row_dy, row_x=row_x, scale=scale, out=out)
+    dev = _one_gpu(who, "dy x seg_start row_dy row_x scale out", dy, x, seg_start, row_dy, row_x, scale, out)
     dt = _half(who, dy)
     n_seg = _segments(who, seg_start, None)
     lddy, ldx = _rows(who, "dy", dy, dy.dtype, None, None), _rows(who, "x", x, dy.dtype, None, None)
@@ -515,7 +521,7 @@ def lora_add(base, x, a, b, ids, scale=None, out=None, workspace=None):
     moe_lora_workspace_bytes, for callers that keep one per call in flight.
     """
     who = "lora_add"
-    dev = _one_gpu(who, base=base, x=x, a=a, b=b, ids=ids, scale=scale, out=out, workspace=workspace)
+    dev = _one_gpu(who, "base x a b ids scale out workspace", base, x, a, b, ids, scale, out, workspace)
     dt, n_ad, rank, n_in, n_out, a_stride, b_stride = _lora_args(who, x, a, b, ids, scale)
     n_tok = x.shape[0]
     ldx = _rows(who, "x", x, x.dtype, n_tok, n_in)
@@ -538,7 +544,7 @@ def lora_grad(dy, x, a, b, ids, scale=None, workspace=None):
     scratch of moe_lora_grad_workspace_bytes.
     """
     who = "lora_grad"
-    dev = _one_gpu(who, dy=dy, x=x, a=a, b=b, ids=ids, scale=scale, workspace=workspace)
+    dev = _one_gpu(who, "dy x a b ids scale workspace", dy, x, a, b, ids, scale, workspace)
     dt, n_ad, rank, n_in, n_out, a_stride, b_stride = _lora_args(who, x, a, b, ids, scale)
     n_tok = x.shape[0]
     ldx = _rows(who, "x", x, x.dtype, n_tok, n_in)
