@@ -279,8 +279,8 @@ int moe_pair_combine(const void* y, const void* scores, const void* residual, in
  * for fp16 or bf16 weights (dtype 0 or 1, inputs, weights and outputs alike), with their gradients, the
  * row plan they take, and low-rank adapters.  Pointers are device memory, 16-byte aligned; ld* are
  * elements from row to row and *_stride elements from matrix to matrix, both multiples of 8, as all row
- * lengths are; within a matrix rows follow each other.  Row numbers and sizes are 32-bit, offsets
- * 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).  Nothing is allocated,
+ * lengths are; within a matrix rows follow each other.  Row numbers are 32-bit, sizes up to
+ * 2^30, offsets 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).  Nothing is allocated,
  * kept between calls or synchronised.  Sums are fp32, rounded once. */
 
 /* The rows of a batch sorted by expert, as prefill.resident_plan (loader.py:583-591) makes them on the
@@ -295,7 +295,8 @@ int moe_expert_plan(const int32_t* ids, int n_ids, int k, int n_exp, void* works
 /* y[row_out[r]] = scale[u] W_u x[row_in[r]] for the rows r of segment u: seg_start[u] .. seg_start[u + 1]
  * - 1, W_u [n][k] = w + seg_slot[u] * w_stride (seg_slot null: u), scale fp32 per slot or null; row_in /
  * row_out null: row r.  n_seg in 0..1024.  A row_in outside x gives a row of zeros; a row_out outside y
- * is not written.  Rows of no segment, and of one whose slot is outside 0 .. n_slots - 1, are written as
+ * is not written; two rows with one row_out leave either's result.  seg_start does not decrease (of
+ * one that does, some rows are missed).  Rows of no segment, and of one whose slot is outside 0 .. n_slots - 1, are written as
  * zeros if fill != 0 and left as they are if not. */
 int moe_grouped_mm(const void* x, int64_t ldx, int n_x, const int32_t* row_in, const int32_t* seg_start,
                    const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots, int n,
@@ -303,7 +304,7 @@ int moe_grouped_mm(const void* x, int64_t ldx, int n_x, const int32_t* row_in, c
                    void* stream);
 /* h[r] = silu(g) * u with (g, u) = W x[row_in[r]], W [2 * inter][hidden]: inter gate rows, then inter up
  * rows.  gu (or null): receives (g, u), [n_rows][2 * inter], for moe_grouped_mm_dx.  Other arguments as
- * moe_grouped_mm; h and gu have row r at r. */
+ * moe_grouped_mm; h and gu have row r at r, and fill is for both. */
 int moe_grouped_gate_up(const void* x, int64_t ldx, int n_x, const int32_t* row_in, const int32_t* seg_start,
                         const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots,
                         int inter, int hidden, void* h, int64_t ldh, void* gu, int64_t ldgu, int dtype, int fill,
@@ -325,7 +326,7 @@ int moe_grouped_mm_dw(const void* dy, int64_t lddy, int n_dy, const int32_t* row
 /* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scale[i] B_i (A_i x[t]),
  * i = ids[t]; A_i [rank][n_in] = a + i * a_stride, B_i [n_out][rank] = b + i * b_stride, scale fp32 per
  * adapter or null.  An id outside 0 .. n_ad - 1 gives out[t] = base[t].  out may be base.  rank: a
- * multiple of 8 up to 256.  workspace: moe_lora_workspace_bytes bytes, any contents, one per call in
+ * multiple of 8 up to 256; n_out < 2^23.  workspace: moe_lora_workspace_bytes bytes, any contents, one per call in
  * flight. */
 uint64_t moe_lora_workspace_bytes(int n_tok, int rank);
 int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, const void* a, int64_t a_stride,

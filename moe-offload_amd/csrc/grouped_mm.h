@@ -6,6 +6,7 @@
 namespace gmm {
 
 constexpr int kMaxSeg = 1024;
+constexpr int kMaxSide = 1 << 30;     // rows, columns and contractions: sums of two of them and a tile stay below 2^31
 
 // Rows r of segment s: seg_start[s] .. seg_start[s + 1] - 1, weights of slot seg_slot[s] (s where null).
 struct Segs {
@@ -55,7 +56,8 @@ struct Tile {
 // The row tile (bm rows of one segment at most) and column tile of this block; false: none is left for it.
 // scratch: THREADS / 64 + 3 words of LDS, free again once every thread is back.
 // Every thread sums the tiles of its own few segments, a scan over the block turns the sums into first
-// tiles, and the thread whose segments hold the block's item publishes it.
+// tiles, and the thread whose segments hold the block's item publishes it.  (No thread does where seg_start is not in
+// order and the sums wrap: the block then has no rows.)
 template <int THREADS>
 __device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, uint32_t* scratch, Tile& out) {
     uint32_t* wave_sum = scratch;
@@ -76,6 +78,7 @@ __device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, uint
         if (lane >= d) inc += o;
     }
     if (lane == 63) wave_sum[wv] = inc;
+    if (t == 0) found[0] = found[1] = 0;
     __syncthreads();
     uint32_t first = inc - sum, total = 0;
 #pragma unroll
@@ -105,7 +108,7 @@ __device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, uint
     out.r1 = __builtin_amdgcn_readfirstlane(found[1]);
     out.slot = __builtin_amdgcn_readfirstlane(found[2]);
     out.col = (int)(item % (uint32_t)n_col);
-    return true;
+    return out.r0 < out.r1;
 }
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

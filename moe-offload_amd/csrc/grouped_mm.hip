@@ -653,7 +653,7 @@ bool bad(const char* who, const char* what) {
 }
 
 // Whether a matrix of `rows` rows may be read or written in 16-byte pieces of `width` elements.
-bool bad_matrix(const char* who, const char* name, const void* p, int64_t ld, int64_t width, int64_t rows, int dtype_bytes) {
+bool bad_matrix(const char* who, const char* name, const void* p, int64_t ld, int64_t width, int64_t rows) {
     if (rows < 0 || width <= 0 || width % 8 || ld % 8 || (rows > 1 && ld < width) || ld < 0) {
         moe_set_error("%s: %s: %lld rows of %lld elements at a step of %lld (multiples of 8 wanted)", who, name,
                       (long long)rows, (long long)width, (long long)ld);
@@ -663,14 +663,15 @@ bool bad_matrix(const char* who, const char* name, const void* p, int64_t ld, in
         moe_set_error("%s: %s: null or not 16-byte aligned", who, name);
         return true;
     }
-    (void)dtype_bytes;
     return false;
 }
 
-bool bad_segs(const char* who, const Segs& S, int dtype, const void* w) {
+bool bad_segs(const char* who, const Segs& S, int n, int k, int dtype, const void* w) {
     if (dtype != 0 && dtype != 1) return bad(who, "dtype is 0 (fp16) or 1 (bf16)");
-    if (S.n_seg < 0 || S.n_seg > gmm::kMaxSeg || S.n_rows < 0 || S.n_slots < 0) {
-        moe_set_error("%s: n_seg=%d (0..%d) n_rows=%d n_slots=%d", who, S.n_seg, gmm::kMaxSeg, S.n_rows, S.n_slots);
+    if (S.n_seg < 0 || S.n_seg > kMaxSeg || S.n_rows < 0 || S.n_rows > kMaxSide || S.n_slots < 0 || n < 0 || n > kMaxSide ||
+        k < 0 || k > kMaxSide) {
+        moe_set_error("%s: n_seg=%d (0..%d) n_rows=%d n_slots=%d matrices of %d x %d (up to %d)", who, S.n_seg, kMaxSeg, S.n_rows,
+                      S.n_slots, n, k, kMaxSide);
         return true;
     }
     if (!S.start) return bad(who, "seg_start is null");
@@ -689,8 +690,8 @@ int moe_grouped_mm(const void* x, int64_t ldx, int n_x, const int32_t* row_in, c
     const char* who = "grouped_mm";
     Args a = {};
     a.S = Segs{seg_start, seg_slot, n_seg, n_rows, n_slots, fill};
-    if (bad_segs(who, a.S, dtype, w) || bad_matrix(who, "x", x, ldx, k, n_x, 2) ||
-        bad_matrix(who, "w", w, w_stride, k, n_slots, 2) || bad_matrix(who, "y", y, ldy, n, n_y, 2))
+    if (bad_segs(who, a.S, n, k, dtype, w) || bad_matrix(who, "x", x, ldx, k, n_x) ||
+        bad_matrix(who, "w", w, w_stride, k, n_slots) || bad_matrix(who, "y", y, ldy, n, n_y))
         return -1;
     if (n_slots > 1 && w_stride < (int64_t)n * k) return bad(who, "w_stride is less than a matrix"), -1;
     if ((!row_in && n_rows > n_x) || (!row_out && n_rows > n_y)) return bad(who, "more rows than x or y has"), -1;
@@ -707,11 +708,10 @@ int moe_grouped_gate_up(const void* x, int64_t ldx, int n_x, const int32_t* row_
     const char* who = "grouped_gate_up";
     Args a = {};
     a.S = Segs{seg_start, seg_slot, n_seg, n_rows, n_slots, fill};
-    if (bad_segs(who, a.S, dtype, w) || bad_matrix(who, "x", x, ldx, hidden, n_x, 2) ||
-        bad_matrix(who, "w", w, w_stride, hidden, n_slots, 2) || bad_matrix(who, "h", h, ldh, inter, n_rows, 2) ||
-        (gu && bad_matrix(who, "gu", gu, ldgu, 2 * (int64_t)inter, n_rows, 2)))
+    if (bad_segs(who, a.S, inter, hidden, dtype, w) || bad_matrix(who, "x", x, ldx, hidden, n_x) ||
+        bad_matrix(who, "w", w, w_stride, hidden, n_slots) || bad_matrix(who, "h", h, ldh, inter, n_rows) ||
+        (gu && bad_matrix(who, "gu", gu, ldgu, 2 * (int64_t)inter, n_rows)))
         return -1;
-    if (inter > 0x3FFFFFFF) return bad(who, "inter is too large"), -1;
     if (n_slots > 1 && w_stride < 2 * (int64_t)inter * hidden) return bad(who, "w_stride is less than a matrix"), -1;
     if (!row_in && n_rows > n_x) return bad(who, "more rows than x has"), -1;
     if (n_rows == 0) return 0;
@@ -727,10 +727,10 @@ int moe_grouped_mm_dx(const void* dy, int64_t lddy, int n_dy, const int32_t* row
     const char* who = "grouped_mm_dx";
     Args a = {};
     a.S = Segs{seg_start, seg_slot, n_seg, n_rows, n_slots, fill};
-    if (bad_segs(who, a.S, dtype, w) || bad_matrix(who, "dy", dy, lddy, n, n_dy, 2) ||
-        bad_matrix(who, "w", w, w_stride, k, n_slots, 2) ||
-        bad_matrix(who, "dx", dx, lddx, (gu ? 2 : 1) * (int64_t)k, n_dx, 2) ||
-        (gu && bad_matrix(who, "gu", gu, ldgu, 2 * (int64_t)k, n_rows, 2)))
+    if (bad_segs(who, a.S, n, k, dtype, w) || bad_matrix(who, "dy", dy, lddy, n, n_dy) ||
+        bad_matrix(who, "w", w, w_stride, k, n_slots) ||
+        bad_matrix(who, "dx", dx, lddx, (gu ? 2 : 1) * (int64_t)k, n_dx) ||
+        (gu && bad_matrix(who, "gu", gu, ldgu, 2 * (int64_t)k, n_rows)))
         return -1;
     if (n_slots > 1 && w_stride < (int64_t)n * k) return bad(who, "w_stride is less than a matrix"), -1;
     if ((!row_in && n_rows > n_dy) || (!row_out && n_rows > n_dx)) return bad(who, "more rows than dy or dx has"), -1;
@@ -746,8 +746,8 @@ int moe_grouped_mm_dw(const void* dy, int64_t lddy, int n_dy, const int32_t* row
     const char* who = "grouped_mm_dw";
     Args a = {};
     a.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 0};
-    if (bad_segs(who, a.S, dtype, dw) || bad_matrix(who, "dy", dy, lddy, n, n_dy, 2) ||
-        bad_matrix(who, "x", x, ldx, k, n_x, 2) || bad_matrix(who, "dw", dw, dw_stride, k, n_seg, out_f32 ? 4 : 2))
+    if (bad_segs(who, a.S, n, k, dtype, dw) || bad_matrix(who, "dy", dy, lddy, n, n_dy) ||
+        bad_matrix(who, "x", x, ldx, k, n_x) || bad_matrix(who, "dw", dw, dw_stride, k, n_seg))
         return -1;
     if (n_seg > 1 && dw_stride < (int64_t)n * k) return bad(who, "dw_stride is less than a matrix"), -1;
     if ((!row_dy && n_rows > n_dy) || (!row_x && n_rows > n_x)) return bad(who, "more rows than dy or x has"), -1;

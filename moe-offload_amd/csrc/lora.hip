@@ -5,12 +5,16 @@
 // shared projection's output (a grouped product, the 2-bit experts' rows, a router's logits) and may be
 // out itself.  v = A_i x stays in fp32 between the two products, and out is rounded once.
 //
-// Two launches.  k_lora_v: 16 tokens and up to 32 ranks per block, the contraction split over its waves, both
-// operands from global memory straight in the matrix unit's layout (each byte of x is used for 16 ranks at a
-// TODO  The tokens of a tile may have different adapters: the
-// tile is multiplied by each adapter that occurs in it and every token keeps its own adapter's result.  In a
-// batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks of
-// their own.
+// Two launches.  k_lora_v multiplies 16 or 32 tokens by up to 32 ranks per block, the contraction dealt to its waves.
+// k_lora_out multiplies v by B's rows and adds base; v keeps its fp32 bits on the 16-bit matrix unit as a sum of
+// 16-bit parts.  Both take their operands through LDS in loads of whole lines.  The tokens of a tile may have
+// different adapters: the tile is multiplied by each adapter that occurs in it and every token keeps its own adapter's
+// result.  In a batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks
+// of their own.
+//
+// The gradients: dv[t] = s_i B_i^T dy[t] beside v in one launch, both rounded to 16 bits as an activation between two
+// layers is, then the grouped products over the tokens sorted by adapter, dx = A_i^T dv, dA_i = sum dv x^T,
+// dB_i = s_i sum dy v^T.
 #include <hip/hip_bf16.h>
 
 #include <algorithm>
@@ -219,10 +223,11 @@ int lora_v_dv_typed(const void* x, int64_t ldx, const void* A, int64_t a_stride,
              rank, (T*)v, (T*)dv, s);
 }
 
-// fp32 values as sums of values of T that keep their bits: bf16 has fp32's range, three of its 8 bits each are 24 bits;
-// fp16 values are first scaled by a power of two per token, so that the largest is just below 2^15, and two of 11 bits
-// each are 22 bits, or 2^-40 of the token's largest value.  (The fp32 matrix unit takes 8 times as long and wants B
-// widened.)  An infinity or NaN stays in the first part.
+// fp32 values as sums of values of T that keep their bits.  bf16 has fp32's range: three parts, each the upper half of
+// what the ones before it leave, are the value itself (rounded parts would overflow near the largest values).  fp16 values
+// are first scaled by a power of two per token, so that the largest is just below 2^15, and two parts of 11 bits each are
+// 22 bits, or 2^-40 of the token's largest value.  (The fp32 matrix unit takes 8 times as long and wants B widened.)  An
+// infinity or NaN stays in the first part.
 template <typename T>
 constexpr int kParts = __is_same(T, _Float16) ? 2 : 3;
 
@@ -236,7 +241,8 @@ __device__ __forceinline__ void split8(const float* v, uint4 (&part)[kParts<T>])
         const bool fine = __builtin_fabsf(rest) < __builtin_inff();
 #pragma unroll
         for (int k = 0; k < kParts<T>; ++k) {
-            p[k][e] = (T)rest;
+            if (kParts<T> == 3 && fine) p[k][e] = __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16));
+            else p[k][e] = (T)rest;
             rest = fine ? rest - (float)p[k][e] : 0.f;
         }
     }
@@ -244,9 +250,6 @@ __device__ __forceinline__ void split8(const float* v, uint4 (&part)[kParts<T>])
     for (int k = 0; k < kParts<T>; ++k) part[k] = __builtin_bit_cast(uint4, p[k]);
 }
 
-// out = base + B_i v for 16 tokens (blockIdx.x) and 128 columns per wave.  The wave's eight subtiles of 16 columns are
-// dealt out so that lane n has the columns 8 n .. 8 n + 7, one of each: 16 bytes per token, and 16 lanes' are one row's
-// 256.
 // out = base + B_i v for 16 ST tokens (blockIdx.x) and 128 columns per wave, W waves.  The wave's eight subtiles of 16
 // columns are dealt out so that lane n has the columns 8 n .. 8 n + 7, one of each: 16 bytes per token, and 16 lanes' are
 // one row's 256.  B's rows and v go through LDS, 64 ranks at a time, in loads of whole lines: loaded straight into the
@@ -443,12 +446,15 @@ int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, co
              n_out, rank, v, (T*)out, ldo, s);
 }
 
+constexpr int kMaxOut = 65535 * 128;                          // the second grid dimension, 128 columns each
+
 // The shapes and strides that both entry points take; base or dy is [n_tok][n_out].
 bool bad_shapes(const char* who, int dtype, int n_tok, int n_ad, int n_in, int n_out, int rank, int64_t ldx, int64_t ldy,
                 int64_t a_stride, int64_t b_stride) {
     if ((dtype != 0 && dtype != 1) || n_tok < 0 || n_ad < 0 || n_in <= 0 || n_out <= 0 || rank <= 0 || n_in % 8 ||
-        n_out % 8 || rank % 8 || rank > 256 || (n_out + 127) / 128 > 65535) {
-        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^23)",
+        n_out % 8 || rank % 8 || rank > 256 || n_out > kMaxOut || n_in > kMaxSide || n_tok > kMaxSide) {
+        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^23, n_in and "
+                      "n_tok <= 2^30)",
                       who, dtype, n_tok, n_ad, n_in, n_out, rank);
         return true;
     }

@@ -370,7 +370,7 @@ def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_
     x: fp16 or bf16 [*, K]; w: same type [n_slots, N, K]; segment u is rows seg_start[u]:seg_start[u + 1]
     with slot seg_slot[u] (u when None).  row_in / row_out None: row r.  The number of sorted rows is
     row_in's or row_out's, else x's.  A new output has n_out_rows rows, or as many as there are sorted rows
-    (row_out is then one place for each, as expert_plan's); rows of no segment, or of one whose slot is
+    (row_out must then name each of its rows once, as expert_plan's does); rows of no segment, or of one whose slot is
     outside w, are zeros in it and left as they are in a given `out`.  A row_in outside x gives a row of
     zeros, a row_out outside the output is dropped.
     """
@@ -401,8 +401,8 @@ def grouped_gate_up(x, row_token, seg_start, w, seg_slot=None, h_out=None, gu_ou
 
     x: fp16 or bf16 [n_tok, hidden]; w: same type [n_slots, 2 * inter, hidden], a slot's inter gate rows
     before its inter up rows; seg_start, seg_slot as grouped_mm.  gu_out ([M, 2 * inter], optional)
-    receives (g, u) for grouped_mm_dx.  Returns [M, inter]; rows of no valid segment are zeros in a new
-    output and left as they are in a given one.
+    receives (g, u) for grouped_mm_dx.  Returns [M, inter]; rows of no valid segment are zeros, in gu_out
+    too, if h_out is None, and left as they are in both if it is given.
     """
     who = "grouped_gate_up"
     dev = _one_gpu(who, "x row_token seg_start w seg_slot h_out gu_out", x, row_token, seg_start, w, seg_slot, h_out, gu_out)

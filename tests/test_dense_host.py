@@ -132,3 +132,20 @@ def test_nothing_to_do_launches_nothing():
     assert lib.moe_lora_grad_workspace_bytes(0, 3, 8) == 16
     assert lib.moe_lora_workspace_bytes(5, 16) == 320 and lib.moe_lora_workspace_bytes(0, 16) == 0
     assert ctypes.sizeof(ctypes.c_int64) == 8
+
+
+BIG = 2 ** 30 + 8
+
+
+@pytest.mark.parametrize("name,good,bad", [
+    ("moe_grouped_mm", MM, [dict(n=BIG, ldy=BIG, w_stride=64 * BIG), dict(k=BIG, ldx=BIG, w_stride=64 * BIG), dict(n_rows=BIG, n_x=BIG, n_y=BIG)]),
+    ("moe_grouped_gate_up", UP, [dict(hidden=BIG, ldx=BIG, w_stride=64 * BIG), dict(n_rows=BIG, n_x=BIG)]),
+    ("moe_grouped_mm_dx", DX, [dict(n=BIG, lddy=BIG, w_stride=64 * BIG), dict(k=BIG, lddx=BIG, w_stride=64 * BIG), dict(n_rows=BIG, n_dy=BIG, n_dx=BIG)]),
+    ("moe_grouped_mm_dw", DW, [dict(n=BIG, lddy=BIG, dw_stride=64 * BIG), dict(k=BIG, ldx=BIG, dw_stride=64 * BIG), dict(n_rows=BIG, n_dy=BIG, n_x=BIG)]),
+    ("moe_lora_add", LORA, [dict(n_in=BIG, ldx=BIG, a_stride=8 * BIG), dict(n_tok=BIG)]),
+    ("moe_lora_grad", GRAD, [dict(n_in=BIG, ldx=BIG, lddx=BIG, a_stride=8 * BIG), dict(n_tok=BIG)]),
+])
+def test_sizes_whose_sums_would_pass_31_bits_are_refused(name, good, bad):
+    for change in bad:
+        assert set(change) <= set(good)
+        refused(name, *{**good, **change}.values())

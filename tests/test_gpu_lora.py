@@ -224,3 +224,19 @@ def test_beside_the_2bit_experts():
     ref.check(out, *ref.lora(base, x, a, b, ad, scale))
     dx, da, db = ops.lora_grad(out, x, a, b, ad, scale=scale)
     assert da.shape == a.shape and db.shape == b.shape and bool(dx.isfinite().all())
+
+
+def test_v_past_the_largest_rounded_value():
+    # v = 2^127 (1 + 255/256) is finite in fp32 and rounds to infinity in bf16; times 2^-120 it is 255.5
+    from moe_offload import ops
+    x = torch.zeros((3, 8), dtype=torch.bfloat16, device=DEV)
+    x[:, 0], x[:, 1] = 2.0 ** 63, 2.0 ** 62
+    x[1] = -x[1]
+    a = torch.zeros((1, 8, 8), dtype=torch.bfloat16, device=DEV)
+    a[0, 0, 0], a[0, 0, 1] = 2.0 ** 64, 2.0 ** 65 * (255 / 256)
+    b = torch.zeros((1, 16, 8), dtype=torch.bfloat16, device=DEV)
+    b[0, :, 0] = 2.0 ** -120
+    base = torch.full((3, 16), -128.0, dtype=torch.bfloat16, device=DEV)
+    out = ops.lora_add(base, x, a, b, torch.zeros(3, dtype=torch.int32, device=DEV))
+    # 127.5 and -383.5, exact in the sum, rounded once (127.5 is a value of the type; -383.5 lies between -382 and -384)
+    assert out[0].tolist() == [127.5] * 16 and out[2].tolist() == [127.5] * 16 and out[1].tolist() == [-384.0] * 16
