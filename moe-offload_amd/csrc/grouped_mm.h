@@ -15,6 +15,20 @@ struct Segs {
     int n_seg, n_rows, n_slots, fill;
 };
 
+// Two weights' gradients over the same rows, dw [n_seg][n][k] contiguous, as moe_grouped_mm_dw computes them (the caller
+// has checked the arguments): in one launch where both are narrow.
+struct Dw {
+    const void* dy;
+    int64_t lddy;
+    const void* x;
+    int64_t ldx;
+    int n, k;
+    const float* scale;
+    void* dw;
+};
+int dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, int dtype,
+            hipStream_t s);
+
 // Block index -> work item, keeping consecutive items on one XCD (blocks are dealt to the 8 XCDs round
 // robin), so that the blocks of one row tile find its rows in that XCD's L2.
 __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t nb) {

@@ -57,10 +57,10 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
 
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
-// next tile's first step during the last of this one: two images, one barrier per step.  Narrow weights' gradients have
-// S = 4 images, three steps under way: their tiles are too few to hide a step's way behind each other's.
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, int S = 2, bool NT = false>
-__global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
+// next tile's first step during the last of this one: two images, one barrier per step.  (Four images, three steps under
+// way, let half as many blocks live on a CU: adapters' gradients of 4096 tokens, rank 64, 36 us, and 26 with two.)
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, bool NT>
+__device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, uint32_t blocks) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
     constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
     constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;        // 1 KiB each
@@ -68,10 +68,10 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
     constexpr bool kThroughLds = OP == kDw && BP == 128;
-    static_assert(!kThroughLds || (S == 2 && SP == 4 && SQ == 4 && kStage / kWaves == 8192), "");
+    static_assert(!kThroughLds || (SP == 4 && SQ == 4 && kStage / kWaves == 8192), "");
     static_assert(!NT || kThroughLds, "");
     constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     __shared__ int2 idx[OP == kDw ? kIdx : 1];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     int r0, r1, slot, tile, p0 = 0, nc = a.nc, seg = 0;
     if constexpr (OP == kDw) {
         const int tp = (a.np + BP - 1) / BP;
-        const uint32_t item = xcd_order(blockIdx.x, gridDim.x);
+        const uint32_t item = xcd_order(block, blocks);
         seg = item / (groups * tp);
         p0 = (int)(item / groups % tp) * BP;
         tile = (int)(item % groups) * a.span;
@@ -229,14 +229,9 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
         load_tile = tile;
         load_c = c0;
         place();
-        uint32_t to = stage;
 #pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-#pragma unroll
-            for (int d = 0; d < kLoads; ++d) load(d, to);
-            to = to == (S - 1) * kStage ? 0 : to + kStage;
-            advance();
-        }
+        for (int d = 0; d < kLoads; ++d) load(d, stage);
+        advance();
     };
     if (nc > 0 && !parts) {
         if constexpr (OP == kDw) {
@@ -260,14 +255,14 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
                 __syncthreads();
                 start(part0);
             }
-            // this wave's loads of the step have landed (they return in order; later steps' may be under way) and its
-            // reads of the step before are done; past the barrier, so are everyone's
+            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
+            // everyone's
             if (landed) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             landed = false;
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const uint32_t fill = stage == 0 ? (S - 1) * kStage : stage - kStage;
+            const uint32_t fill = kStage - stage;
             // The step's second half is read from LDS, and the next step's loads are issued, between the first half's
             // products, row by row (past the last step they fetch zeros that nobody reads)
             uint4 vp[2][SP], vq[2][SQ];
@@ -299,10 +294,10 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
             for (int i = 0; i < SP; ++i)
 #pragma unroll
                 for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
-            stage = stage == (S - 1) * kStage ? 0 : stage + kStage;
+            stage = fill;
         }
         // The next tile's first step is waited for before the stores: in the loop the wait would take them in.
-        if (S == 2 && BP < 256 && nc > 0 && tile + 1 < end) {
+        if (BP < 256 && nc > 0 && tile + 1 < end) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             landed = !parts;
         }
@@ -471,6 +466,19 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, bool NT = false>
+__global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
+    tiles_of_block<T, OP, BP, BQ, WP, WQ, NT>(a, blockIdx.x, gridDim.x);
+}
+
+// Two narrow weights' gradients (an adapter's A and B) in one launch: n_a blocks are the first one's.
+template <typename T>
+__global__ __launch_bounds__(256, 4) void k_grouped_dw_pair(Args a, Args b, uint32_t n_a) {
+    const bool first = blockIdx.x < n_a;
+    const Args c = first ? a : b;
+    tiles_of_block<T, kDw, 64, 64, 2, 2, false>(c, first ? blockIdx.x : blockIdx.x - n_a, first ? n_a : gridDim.x - n_a);
+}
+
 // A few rows per segment (decoding): one wave per 16 rows of a segment and 16 weight rows (mm: 16 columns; gate_up: 8
 // gate rows and the 8 up rows of the same outputs), which it streams through an LDS ring of its own, kFewRing steps of
 // 64 ahead, without a barrier.  Loads that put the weights straight into the matrix unit's layout would take 16 bytes
@@ -567,8 +575,9 @@ __global__ __launch_bounds__(64) void k_grouped_few(Args a) {
 // Row tiles of a call as far as the host knows it: a segment's last tile is half full on average.
 int64_t row_tiles(const Args& a, int bp) { return (a.S.n_rows + (int64_t)(a.S.n_seg - 1) * (bp / 2) + bp - 1) / bp; }
 
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, int S = 2, bool NT = false>
-int launch_tiles(Args a, hipStream_t s) {
+// Sets the column tiles per block and returns the blocks, or -1.
+template <int OP, int BP, int BQ>
+int64_t blocks_of(Args& a) {
     const int qstep = OP == kGateUp ? BQ / 2 : BQ, tiles = (a.nq + qstep - 1) / qstep;
     int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
     if constexpr (OP == kDw) {
@@ -592,7 +601,14 @@ int launch_tiles(Args a, hipStream_t s) {
         moe_set_error("grouped product: %lld x %lld tiles are more than one launch takes", (long long)most, (long long)groups);
         return -1;
     }
-    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS, S, NT>), dim3((uint32_t)(most * groups)), dim3(64 * WP * WQ), 0, s, a);
+    return most * groups;
+}
+
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, bool NT = false>
+int launch_tiles(Args a, hipStream_t s) {
+    const int64_t blocks = blocks_of<OP, BP, BQ>(a);
+    if (blocks < 0) return -1;
+    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS, NT>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -616,30 +632,66 @@ int launch_few(const Args& a, hipStream_t s) {
     return 0;
 }
 
+// The tiles of a weights' gradient.
+enum { kDw256, kDw128, kDw128Past, kDw64 };
+
+int dw_tiles(const Args& a) {
+    const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
+    auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * ((a.nq + b - 1) / b); };
+    // with few rows the output's bytes bound it, and smaller tiles have more of them under way (512 x 40 rows, 1024 x
+    // 2048: 592 us, and 737 with the large tiles)
+    if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return kDw256;
+    // an output larger than the 256 MB of Infinity Cache only pushes the inputs out of it, and its lines are written
+    // back under the next kernel (512 x 40 rows, 1024 x 2048, 2 GB: 520 us, and 591 with ordinary stores)
+    if (per_seg < 512 && (int64_t)a.S.n_seg * a.np * a.nq * (a.out_f32 ? 4 : 2) > 256 << 20) return kDw128Past;
+    // an adapter's: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 30 us with them, 21 with 64's)
+    if (a.np <= 64 || a.nq <= 64) return kDw64;
+    return kDw128;
+}
+
 template <typename T, int OP>
 int launch(const Args& a, hipStream_t s) {
-    const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
-    auto cols = [&](int bq) { return (a.nq + (OP == kGateUp ? bq / 2 : bq) - 1) / (OP == kGateUp ? bq / 2 : bq); };
     if constexpr (OP == kDw) {
-        // with few rows the output's bytes bound it, and smaller tiles have more of them under way (512 x 40 rows, 1024 x
-        // 2048: 592 us, and 737 with the large tiles)
-        auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * cols(b); };
-        if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
-        // an output larger than the 256 MB of Infinity Cache only pushes the inputs out of it, and its lines are written
-        // back under the next kernel
-        if (per_seg < 512 && (int64_t)a.S.n_seg * a.np * a.nq * (a.out_f32 ? 4 : 2) > 256 << 20)
-            return launch_tiles<T, OP, 128, 128, 2, 2, 2, 2, true>(a, s);
-        if (a.np <= 64 || a.nq <= 64) return launch_tiles<T, OP, 64, 64, 2, 2, 2, 4>(a, s);
-        return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
+        switch (dw_tiles(a)) {
+            case kDw256: return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
+            case kDw128: return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
+            case kDw128Past: return launch_tiles<T, OP, 128, 128, 2, 2, 2, true>(a, s);
+            default: return launch_tiles<T, OP, 64, 64, 2, 2, 4>(a, s);
+        }
     } else {
+        const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
+        auto cols = [&](int bq) { return (a.nq + (OP == kGateUp ? bq / 2 : bq) - 1) / (OP == kGateUp ? bq / 2 : bq); };
+        // Few rows: a wave per tile of 16 columns, while there are too few tiles of 64 rows and 128 columns to fill the card
+        // (gate_up of 512 x 2048 for 32 rows over 32 segments: 14 us, and 26 with tiles; past kFewTiles the tiles' fewer
+        // loads of x win)
         if constexpr (OP == kMM || OP == kGateUp) {
             if (per_seg <= 16 && std::min(a.S.n_seg, a.S.n_rows) * (int64_t)cols(128) < kFewTiles) return launch_few<T, OP>(a, s);
         }
+        // Tiles of 64 rows waste less of short segments, tiles of 128 read the weights half as often: us of either, mm of
+        // 512 segments, 1024 x 2048, 48 rows each 406 and 411, 64 rows 425 and 427, 80 rows 515 and 438; 64 segments, 2048 x
+        // 1024, 64 rows 54 and 51, 96 rows 74 and 58; 512 segments of 1 to 80 rows, mm_dx 521 and 534
         if (per_seg <= 48) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
         if (big_tiles(row_tiles(a, 128) * cols(128), row_tiles(a, 256) * cols(256)))
             return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
         return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
     }
+}
+
+template <typename T>
+int launch_dw_pair(Args a, Args b, hipStream_t s) {
+    if (dw_tiles(a) != kDw64 || dw_tiles(b) != kDw64) {
+        const int rc = launch<T, kDw>(a, s);
+        return rc ? rc : launch<T, kDw>(b, s);
+    }
+    const int64_t n_a = blocks_of<kDw, 64, 64>(a), n_b = blocks_of<kDw, 64, 64>(b);
+    if (n_a < 0 || n_b < 0) return -1;
+    if (n_a + n_b > 0x7FFFFFFF) {
+        moe_set_error("grouped product: %lld tiles are more than one launch takes", (long long)(n_a + n_b));
+        return -1;
+    }
+    hipLaunchKernelGGL((k_grouped_dw_pair<T>), dim3((uint32_t)(n_a + n_b)), dim3(256), 0, s, a, b, (uint32_t)n_a);
+    HIP_TRY(hipGetLastError());
+    return 0;
 }
 
 template <int OP>
@@ -680,6 +732,18 @@ bool bad_segs(const char* who, const Segs& S, int n, int k, int dtype, const voi
 }
 
 }  // namespace
+
+int gmm::dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, int dtype,
+                 hipStream_t s) {
+    auto args = [&](const Dw& d) {
+        Args r = {};
+        r.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 0};
+        r.p = d.dy, r.q = d.x, r.out = d.dw, r.row_p = r.row_q = rows, r.scale = d.scale;
+        r.ldp = d.lddy, r.ldq = d.ldx, r.ldo = (int64_t)d.n * d.k, r.n_p = r.n_q = n_rows, r.np = d.n, r.nq = d.k;
+        return r;
+    };
+    return dtype ? launch_dw_pair<__bf16>(args(a), args(b), s) : launch_dw_pair<_Float16>(args(a), args(b), s);
+}
 
 extern "C" {
 

@@ -531,7 +531,6 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
         p += up16(bytes);
         return q;
     };
-    const int64_t mat = (int64_t)rank * n_in;
     void* v = take((uint64_t)n_tok * rank * 2);
     void* dv = take((uint64_t)n_tok * rank * 2);
     int32_t* order = (int32_t*)take((uint64_t)n_tok * 4);
@@ -545,10 +544,8 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
                            (hipStream_t)stream)) ||
         moe_grouped_mm_dx(dv, rank, n_tok, order, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, nullptr, 0,
                           dx, lddx, n_tok, order, dtype, 1, stream) ||
-        moe_grouped_mm_dw(dv, rank, n_tok, order, x, ldx, n_tok, order, seg, n_ad, n_tok, rank, n_in, nullptr, da, mat, 0,
-                          dtype, stream) ||
-        moe_grouped_mm_dw(dy, lddy, n_tok, order, v, rank, n_tok, order, seg, n_ad, n_tok, n_out, rank, scale, db,
-                          (int64_t)rank * n_out, 0, dtype, stream))
+        gmm::dw_pair(gmm::Dw{dv, rank, x, ldx, rank, n_in, nullptr, da}, gmm::Dw{dy, lddy, v, rank, n_out, rank, scale, db}, order,
+                     n_tok, seg, n_ad, dtype, (hipStream_t)stream))
         return -1;
     return 0;
 }
