@@ -55,6 +55,14 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
     return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
+// 16 bytes out, past the caches where PAST.
+template <bool PAST>
+__device__ __forceinline__ void store16(void* to, uint4 v) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
+    else *(u32x4*)to = __builtin_bit_cast(u32x4, v);
+}
+
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
 // next tile's first step during the last of this one: two images, one barrier per step.  (Four images, three steps under
@@ -67,9 +75,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
-    constexpr bool kThroughLds = OP == kDw && BP == 128;
-    static_assert(!kThroughLds || (SP == 4 && SQ == 4 && kStage / kWaves == 8192), "");
-    static_assert(!NT || kThroughLds, "");
+    constexpr bool kThroughLds = OP == kDw ? BP >= 128 : OP == kDxGlu || (BP == 256 && OP != kGateUp);
+    constexpr bool kPast = NT || BP == 256;
+    static_assert(!kThroughLds || (SQ == 4 && kStage / kWaves >= 4096), "");
     constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     __shared__ int2 idx[OP == kDw ? kIdx : 1];
@@ -185,7 +193,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
         if (load_c >= part1) {
             load_c = 0;
             load_tile = parts ? end : load_tile + 1;
-            if (kThroughLds && nc <= kBC && load_tile < end && (load_tile + 1) * BQ <= a.nq) {
+            if (OP == kDw && BP == 128 && nc <= kBC && load_tile < end && (load_tile + 1) * BQ <= a.nq) {
                 // the same rows again, further right: no row numbers, no multiplications (lanes without a row stay at zero)
 #pragma unroll
                 for (int j = 0; j < kLoadsQ; ++j) qp[j] += qp[j] == zero ? 0 : BQ;
@@ -310,50 +318,104 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                                      // everyone has read the image
             asm volatile("" ::: "memory");
+            int l = lane;
+            asm volatile("" : "+v"(l));                                        // no addresses are kept over the products
+            const int n = l & 15, kq = l >> 4;
             const uint32_t area = lds0 + (kStage - stage) + wv * (kStage / kWaves);
             typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) u32x4* lds16;
-            const int64_t top = (int64_t)seg * a.ldo;
-            const int first = p0 + wp * SP * 16;                               // output row of the wave's row 0
-            // subtile rows [i0, i0 + kPass) of the wave's 16 SQ columns; unit u of row r is at u ^ (r & 7) in its low bits
-            auto pass = [&](auto bytes_c, int i0, auto put, auto* dst) {
-                constexpr int kBytes = decltype(bytes_c)::value, UNITS = SQ * kBytes, kRowsPer = 64 / UNITS;
-                constexpr int kPass = kStage / kWaves / (UNITS * 256);
-                auto at = [&](int row, int u) { return area + (uint32_t)(row * UNITS + (u ^ (row & 7))) * 16; };
-                put(at);
-#pragma unroll
-                for (int it = 0; it < kPass * 16 / kRowsPer; ++it) {
-                    const int row = it * kRowsPer + lane / UNITS, u = lane % UNITS;
-                    const u32x4 v = *(lds16)(uintptr_t)at(row, u);
-                    const int o = first + i0 * 16 + row, c = q0 + wq * SQ * 16 + u * (16 / kBytes);
-                    if (o < a.np && c < a.nq) {
-                        auto* to = (u32x4*)(dst + top + (int64_t)o * a.nq + c);
-                        if constexpr (NT) __builtin_nontemporal_store(v, to);
-                        else *to = v;
-                    }
+            const int col = q0 + wq * SQ * 16;
+            // row m % 16 of the wave's subtile row i: where its results go in out's elements, -1 if nowhere
+            auto row_at = [&](int i, int m) -> int64_t {
+                if constexpr (OP == kDw) {
+                    const int o = p0 + wp * SP * 16 + i * 16 + m;
+                    return o < a.np ? (int64_t)seg * a.ldo + (int64_t)o * a.nq : -1;
+                } else {
+                    const int o = __shfl(orow[i], m, 64);
+                    return o < 0 ? -1 : (int64_t)o * a.ldo;
                 }
-                __builtin_amdgcn_sched_barrier(0);
             };
-            if (a.out_f32) {
+            // kPass subtile rows at a time, rows of UNITS 16-byte units; unit u of row r is at u ^ (r & 7) in its low bits
+            auto result = [&](int i, int j) { return (dead_rows >> i & 1) ? f32x4{} : acc[i][j] * s; };
+            auto pass = [&](auto bytes_c, auto* dst) {
+                constexpr int kBytes = decltype(bytes_c)::value, UNITS = SQ * kBytes, kRowsPer = 64 / UNITS;
+                constexpr int kFit = kStage / kWaves / (UNITS * 256), kPass = kFit < SP ? kFit : SP;
+                static_assert(SP % kPass == 0, "");
+                auto at = [&](int row, int u) { return area + (uint32_t)(row * UNITS + (u ^ (row & 7))) * 16; };
 #pragma unroll
-                for (int i0 = 0; i0 < SP; i0 += 2)
-                    pass(std::integral_constant<int, 4>(), i0, [&](auto at) {
+                for (int i0 = 0; i0 < SP; i0 += kPass) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < kPass; ++i)
+                        if constexpr (kBytes == 4) {
 #pragma unroll
                             for (int j = 0; j < SQ; ++j)
-                                *(lds16)(uintptr_t)at(i * 16 + n, 4 * j + kq) = __builtin_bit_cast(u32x4, acc[i0 + i][j] * s);
-                    }, (float*)a.out);
-            } else {
-                pass(std::integral_constant<int, 2>(), 0, [&](auto at) {
+                                *(lds16)(uintptr_t)at(i * 16 + n, 4 * j + kq) = __builtin_bit_cast(u32x4, result(i0 + i, j));
+                        } else {
 #pragma unroll
-                    for (int i = 0; i < SP; ++i)
-#pragma unroll
-                        for (int j = 0; j < SQ; j += 2) {
-                            const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
-                            *(lds16)(uintptr_t)at(i * 16 + n, 2 * j + (kq & 1) * 2 + (kq >> 1)) = (u32x4){v.x, v.y, v.z, v.w};
+                            for (int j = 0; j < SQ; j += 2)
+                                *(lds16)(uintptr_t)at(i * 16 + n, 2 * j + (kq & 1) * 2 + (kq >> 1)) = __builtin_bit_cast(
+                                    u32x4, pair8(round4<T>(result(i0 + i, j)), round4<T>(result(i0 + i, j + 1))));
                         }
-                }, (T*)a.out);
+#pragma unroll
+                    for (int it = 0; it < kPass * 16 / kRowsPer; ++it) {
+                        const int row = it * kRowsPer + l / UNITS, u = l % UNITS, c = col + u * (16 / kBytes);
+                        const u32x4 v = *(lds16)(uintptr_t)at(row, u);
+                        const int64_t o = row_at(i0 + it * kRowsPer / 16, row & 15);
+                        if (o >= 0 && c < a.nq) store16<kPast>(dst + o + c, __builtin_bit_cast(uint4, v));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            if constexpr (OP == kDxGlu) {
+                // dh in fp32, one subtile row at a time; a lane then has 8 adjacent columns of a row, of dh and of (g, u)
+                auto at = [&](int row, int u) { return area + (uint32_t)(row * 16 + (u ^ (row & 7))) * 16; };
+                const int u8 = l & 7, c = col + u8 * 8;
+#pragma unroll
+                for (int i = 0; i < SP; ++i) {
+                    uint4 gv[2], uv[2];
+                    int64_t o[2];
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) {
+                        const int m = it * 8 + (l >> 3), r = r0 + wp * SP * 16 + i * 16 + m;
+                        o[it] = row_at(i, m);
+                        const uint32_t dead = __shfl(dead_rows, m, 64);                 // (by every lane, before any condition)
+                        const bool ok = o[it] >= 0 && c < inter && !(dead >> i & 1);
+                        const T* gr = ok ? (const T*)a.gu + (int64_t)r * a.ldgu + c : zero;
+                        gv[it] = *(const uint4*)gr;
+                        uv[it] = *(const uint4*)(ok ? gr + inter : zero);
+                    }
+#pragma unroll
+                    for (int j = 0; j < SQ; ++j) *(lds16)(uintptr_t)at(n, 4 * j + kq) = __builtin_bit_cast(u32x4, result(i, j));
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) {
+                        const int m = it * 8 + (l >> 3);
+                        uint2 dg[2], du[2];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const f32x4 dh = __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + b));
+                            const f32x4 g = widen4<T>(b ? make_uint2(gv[it].z, gv[it].w) : make_uint2(gv[it].x, gv[it].y));
+                            const f32x4 u = widen4<T>(b ? make_uint2(uv[it].z, uv[it].w) : make_uint2(uv[it].x, uv[it].y));
+                            f32x4 vg, vu;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float sg = 1.0f / (1.0f + __expf(-g[e]));
+                                vg[e] = dh[e] * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
+                                vu[e] = dh[e] * g[e] * sg;
+                            }
+                            dg[b] = round4<T>(vg);
+                            du[b] = round4<T>(vu);
+                        }
+                        if (o[it] >= 0 && c < inter) {
+                            T* d = (T*)a.out + o[it] + c;
+                            store16<kPast>(d, make_uint4(dg[0].x, dg[0].y, dg[1].x, dg[1].y));
+                            store16<kPast>(d + inter, make_uint4(du[0].x, du[0].y, du[1].x, du[1].y));
+                        }
+                    }
+                }
+            } else if (OP == kDw && a.out_f32) {
+                pass(std::integral_constant<int, 4>(), (float*)a.out);
+            } else {
+                pass(std::integral_constant<int, 2>(), (T*)a.out);
             }
             continue;
         }
@@ -368,14 +430,14 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     for (int j = 0; j < SQ; ++j) {
                         const int q = q0 + wq * SQ * 16 + j * 16 + kq * 4;
                         if (live && q < a.nq)
-                            *(float4*)((float*)a.out + row + q) = make_float4(acc[i][j][0] * s, acc[i][j][1] * s, acc[i][j][2] * s, acc[i][j][3] * s);
+                            store16<kPast>((float*)a.out + row + q, __builtin_bit_cast(uint4, acc[i][j] * s));
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < SQ; j += 2) {
                         const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
                         const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                        if (live && q < a.nq) *(uint4*)((T*)a.out + row + q) = v;
+                        if (live && q < a.nq) store16<kPast>((T*)a.out + row + q, v);
                     }
                 }
                 continue;
@@ -411,44 +473,14 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     for (int j = 0; j < SQ / 2; j += 2) {
                         const int c = q0 + wq * SQ * 8 + j * 16 + pair_col;
                         const uint4 vh = pair8(h[j], h[j + 1]);
-                        if (live && c < inter) *(uint4*)((T*)a.out + (int64_t)r * a.ldo + c) = vh;
+                        if (live && c < inter) store16<kPast>((T*)a.out + (int64_t)r * a.ldo + c, vh);
                         if (a.gu_out) {
                             const uint4 vg = pair8(g2[j], g2[j + 1]), vu = pair8(u2[j], u2[j + 1]);
                             if (live && c < inter) {
-                                *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + c) = vg;
-                                *(uint4*)((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c) = vu;
+                                store16<kPast>((T*)a.gu_out + (int64_t)r * a.ldgu + c, vg);
+                                store16<kPast>((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c, vu);
                             }
                         }
-                    }
-                }
-            } else if constexpr (OP == kDxGlu) {
-#pragma unroll
-                for (int j = 0; j < SQ; j += 2) {
-                    uint2 dg[2], du[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const int q = q0 + wq * SQ * 16 + (j + b) * 16 + kq * 4;
-                        f32x4 g = {}, u = {}, vg, vu;
-                        if (live && !dead && q < inter) {
-                            const T* gr = (const T*)a.gu + (int64_t)r * a.ldgu + q;
-                            g = widen4<T>(*(const uint2*)gr);
-                            u = widen4<T>(*(const uint2*)(gr + inter));
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float dh = dead ? 0.f : acc[i][j + b][e] * s, sg = 1.0f / (1.0f + __expf(-g[e]));
-                            vg[e] = dh * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
-                            vu[e] = dh * g[e] * sg;
-                        }
-                        dg[b] = round4<T>(vg);
-                        du[b] = round4<T>(vu);
-                    }
-                    const uint4 vg = pair8(dg[0], dg[1]), vu = pair8(du[0], du[1]);
-                    const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                    if (live && q < inter) {
-                        T* d = (T*)a.out + (int64_t)o * a.ldo + q;
-                        *(uint4*)d = vg;
-                        *(uint4*)(d + inter) = vu;
                     }
                 }
             } else {
@@ -457,7 +489,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     const f32x4 zero = {};
                     const uint4 v = pair8(round4<T>(dead ? zero : acc[i][j] * s), round4<T>(dead ? zero : acc[i][j + 1] * s));
                     const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                    if (live && q < a.nq) *(uint4*)((T*)a.out + (int64_t)o * a.ldo + q) = v;
+                    if (live && q < a.nq) store16<kPast>((T*)a.out + (int64_t)o * a.ldo + q, v);
                 }
             }
         }
