@@ -55,7 +55,10 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
     return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
-// 16 bytes out, past the caches where PAST.
+// 16 bytes out, past the caches where PAST.  Results are read again by the next launch at the earliest, and their lines
+// wait in L2 for a write that then meets the next tile's loads: us with and without, mm 8192 x 8192 x 8192 852 and 908,
+// weights' gradient 4096 x 1024 of 16 x 1024 rows 148 and 160, mm 1024 x 4096 of 16 x 1024 rows 131 and 161, mm_dx 1024 x
+// 2048 of 512 x 40 rows 429 and 439; the whole layer, 2048 tokens over 512 experts of 512 x 2048, 638 and 643.
 template <bool PAST>
 __device__ __forceinline__ void store16(void* to, uint4 v) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -75,8 +78,8 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
-    constexpr bool kThroughLds = OP == kDw ? BP >= 128 : OP == kDxGlu || (BP == 256 && OP != kGateUp);
-    constexpr bool kPast = NT || BP == 256;
+    constexpr bool kThroughLds = OP == kDxGlu || (OP != kGateUp && BP >= 128);
+    constexpr bool kPast = NT || OP != kDw || BP == 256;
     static_assert(!kThroughLds || (SQ == 4 && kStage / kWaves >= 4096), "");
     constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
@@ -312,9 +315,10 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
         if constexpr (kThroughLds) {
             // The results go through the image just multiplied, a part of it for each wave, and out in whole lines: a lane
             // of the matrix unit's result has 8 or 16 bytes of a row and its neighbour another row's, each a cache access
-            // of its own.  That pays where the output is most of the bytes (weights' gradient over 512 x 40 rows, 1024 x
-            // 2048: 640 us, like this 591, with stores past the caches 520) and costs a barrier where it is not (mm of 777
-            // x 6 rows over 100 segments, 1152 x 320: 20.6 us, like this 24.4).
+            // of its own, and a store past the caches wants whole lines (mm 1024 x 4096, 16 x 2048 rows to places in no
+            // order: 304 us, and 327 straight from the registers; weights' gradient over 512 x 40 rows, 1024 x 2048, 591 and
+            // 640 with ordinary stores).  Tiles of 64 rows have too few steps to pay for the barrier (mm of 100 x 47 rows,
+            // 1152 x 320: 21.0 us, and 19.0 without), but silu's gradient reads (g, u) in whole lines too this way.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                                      // everyone has read the image
             asm volatile("" ::: "memory");
