@@ -521,10 +521,11 @@ __global__ __launch_bounds__(256, 4) void k_grouped_dw_pair(Args a, Args b, uint
 // per lane from 16 rows at a time, four times the cache accesses.  The steps are k_grouped's, in its order, so a row's
 // result has the same bits whichever of the two a call's size selects.
 constexpr int kFewRing = 8;
+constexpr int few_step(int op) { return op == kGateUp ? 8 : 16; }             // output columns of a wave of k_grouped_few
 
 template <typename T, int OP>
 __global__ __launch_bounds__(64) void k_grouped_few(Args a) {
-    constexpr int kQStep = OP == kGateUp ? 8 : 16;
+    constexpr int kQStep = few_step(OP);
     constexpr uint32_t kStage = 4096;                                          // 16 weight rows, 16 rows of x
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kFewRing * kStage];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
@@ -608,8 +609,12 @@ __global__ __launch_bounds__(64) void k_grouped_few(Args a) {
     }
 }
 
-// Row tiles of a call as far as the host knows it: a segment's last tile is half full on average.
-int64_t row_tiles(const Args& a, int bp) { return (a.S.n_rows + (int64_t)(a.S.n_seg - 1) * (bp / 2) + bp - 1) / bp; }
+// Row tiles of a call as far as the host knows it: as many segments as can have rows have a tile, and but for one of them
+// a last tile that is half full.
+int64_t row_tiles(const Args& a, int bp) {
+    const int64_t segs = std::min(a.S.n_seg, a.S.n_rows);
+    return std::max((a.S.n_rows + (segs - 1) * (bp / 2) + bp - 1) / bp, segs);
+}
 
 // Sets the column tiles per block and returns the blocks, or -1.
 template <int OP, int BP, int BQ>
@@ -650,18 +655,23 @@ int launch_tiles(Args a, hipStream_t s) {
 }
 
 // Tiles of 256 x 256 (one block per CU) multiply 1.3 times as fast as tiles of 128 x 128 (two per CU) once every CU has
-// one, but there are a quarter of them: TFLOP/s of 128 and 256, bf16, 16 segments: mm 4096 x 1024 of 2048 rows each 744
-// and 853, of 1024 rows 681 and 951; 1024 x 4096 of 2048 rows 916 and 1179; mm_dx 4096 x 1024 of 1024 rows 892 and 1196;
-// one segment of 2048 rows, 4096 x 2048, (512 and 128 tiles) 920 and 655.
+// one, but there are a quarter of them: TFLOP/s of 128 and 256, bf16, 16 segments: mm 4096 x 1024 of 2048 rows each 778
+// and 955, of 1024 rows 893 and 1020; 1024 x 4096 of 2048 rows 912 and 1158; weights' gradient 4096 x 1024 of 1024 rows
+// 648 and 926; one segment, 8192 x 8192 x 8192, 952 and 1385 (the library's product: 1370); 2048 rows of 4096 x 2048
+// (512 and 128 tiles) 920 and 655.  Rows per tile are what the host can expect of ragged segments.
 bool big_tiles(int64_t tiles128, int64_t tiles256) {
     return (tiles256 + 255) / 256 * 256 * 4 * 10 < (tiles128 + 511) / 512 * 512 * 13;
 }
 
-constexpr int64_t kFewTiles = 1024;
+// Tiles of 64 x 64 (1024 blocks at a time, half the work each) or 64 x 128 (768): both wait for memory, so the rounds of
+// blocks count.  us of mm with 64 x 64 and 64 x 128: 100 x 10 rows, 1152 x 1024, (900 tiles of 128) 38 and 42; 64 x 1 rows,
+// 2048 x 2048, (1024) 125 and 133; 500 rows, 2048 x 4096, (128) 37 and 42; 40 x 12 rows, 2048 x 1024, (640) 32 and 28; 100
+// x 1 rows, 2048 x 512, (1600) 42 and 39; mm_dx of 512 x 40 rows, 1024 x 2048, (8192) 485 and 442.
+bool narrow_tiles(int64_t tiles) { return (2 * tiles + 1023) / 1024 * 512 * 115 < (tiles + 767) / 768 * 768 * 100; }
 
 template <typename T, int OP>
 int launch_few(const Args& a, hipStream_t s) {
-    const int qstep = OP == kGateUp ? 8 : 16;
+    const int qstep = few_step(OP);
     const int64_t rows = (int64_t)a.S.n_rows / 16 + std::min(a.S.n_seg + 2, a.S.n_rows), tiles = (a.nq + qstep - 1) / qstep;
     hipLaunchKernelGGL((k_grouped_few<T, OP>), dim3((uint32_t)(rows * tiles)), dim3(64), 0, s, a);
     HIP_TRY(hipGetLastError());
@@ -680,8 +690,10 @@ int dw_tiles(const Args& a) {
     // an output larger than the 256 MB of Infinity Cache only pushes the inputs out of it, and its lines are written
     // back under the next kernel (512 x 40 rows, 1024 x 2048, 2 GB: 520 us, and 591 with ordinary stores)
     if (per_seg < 512 && (int64_t)a.S.n_seg * a.np * a.nq * (a.out_f32 ? 4 : 2) > 256 << 20) return kDw128Past;
-    // an adapter's: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 30 us with them, 21 with 64's)
-    if (a.np <= 64 || a.nq <= 64) return kDw64;
+    // an adapter's: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 30 us with them, 21 with 64's).
+    // Where not every CU gets one of 128, more and shorter steps of 64 are done sooner too: 2 x 4000 rows, 512 x 1024, 67 and
+    // 39 us, 1113 rows, 2272 x 96, 22.9 and 12.9, 8 x 300 rows, 1024 x 512, 12.1 and 11.1
+    if (a.np <= 64 || a.nq <= 64 || tiles(128) <= 256) return kDw64;
     return kDw128;
 }
 
@@ -697,16 +709,22 @@ int launch(const Args& a, hipStream_t s) {
     } else {
         const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
         auto cols = [&](int bq) { return (a.nq + (OP == kGateUp ? bq / 2 : bq) - 1) / (OP == kGateUp ? bq / 2 : bq); };
-        // Few rows: a wave per tile of 16 columns, while there are too few tiles of 64 rows and 128 columns to fill the card
-        // (gate_up of 512 x 2048 for 32 rows over 32 segments: 14 us, and 26 with tiles; past kFewTiles the tiles' fewer
-        // loads of x win)
+        // A wave per 16 rows and 16 columns where that leaves no SIMD with more than one: us, and with tiles, gate_up of 512 x
+        // 2048 for 10 rows of 10 segments 14 and 26, mm of 100 rows, 2048 x 4096, (896 waves) 24 and 35, 1000 rows, 256 x
+        // 4096, (1008) 15.5 and 21.5; 100 rows, 4096 x 1024, (1792) 16.5 and 10.9, 100 x 6 rows, 1152 x 320, (7200) 35 and 18
         if constexpr (OP == kMM || OP == kGateUp) {
-            if (per_seg <= 16 && std::min(a.S.n_seg, a.S.n_rows) * (int64_t)cols(128) < kFewTiles) return launch_few<T, OP>(a, s);
+            if (row_tiles(a, 16) * ((a.nq + few_step(OP) - 1) / few_step(OP)) <= 1024) return launch_few<T, OP>(a, s);
         }
         // Tiles of 64 rows waste less of short segments, tiles of 128 read the weights half as often: us of either, mm of
         // 512 segments, 1024 x 2048, 48 rows each 406 and 411, 64 rows 425 and 427, 80 rows 515 and 438; 64 segments, 2048 x
-        // 1024, 64 rows 54 and 51, 96 rows 74 and 58; 512 segments of 1 to 80 rows, mm_dx 521 and 534
-        if (per_seg <= 48) return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
+        // 1024, 64 rows 54 and 51, 96 rows 74 and 58; 512 segments of 1 to 80 rows, mm_dx 521 and 534; and where not every
+        // CU gets one of 128, mm of 4 x 300 rows, 1024 x 2048, 23 and 27
+        if (per_seg <= 48 || row_tiles(a, 128) * cols(128) <= 256) {
+            if constexpr (OP != kDxGlu) {
+                if (narrow_tiles(row_tiles(a, 64) * cols(128))) return launch_tiles<T, OP, 64, 64, 2, 2, 4>(a, s);
+            }
+            return launch_tiles<T, OP, 64, 128, 2, 2, 3>(a, s);
+        }
         if (big_tiles(row_tiles(a, 128) * cols(128), row_tiles(a, 256) * cols(256)))
             return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
         return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
