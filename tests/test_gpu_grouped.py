@@ -326,8 +326,69 @@ def test_large_products(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_middle_products(dtype):
+    """Segments of a few hundred rows, wide outputs: tiles of 128 rows, ends inside them."""
+    from moe_offload import ops
+    seg = np.array([0, 300, 300, 633, 890], np.int32)
+    m, e, n, k = 890, 4, 3728, 72
+    x, w, wu = rnd((m, k), dtype, 1), rnd((e, n, k), dtype, 2, k ** -0.5), rnd((e, n, k), dtype, 3, k ** -0.5)
+    order = i32(np.random.default_rng(0).permutation(m))
+    at, xr = order.long(), x[order.long()].double()
+    want, slack, _ = ref.product(xr, seg, w)
+    ref.check(ops.grouped_mm(x, i32(seg), w, row_in=order, row_out=order)[at], want, slack, "mm")
+    gu = torch.empty((m, n), dtype=dtype, device=DEV)
+    h = ops.grouped_gate_up(x, order, i32(seg), wu, gu_out=gu)
+    want, slack, _ = ref.product(xr, seg, wu)
+    ref.check(gu, want, slack, "gu")
+    ref.check(h, *ref.glu(*want.chunk(2, 1), *slack.chunk(2, 1)), "h")
+    wd = rnd((e, k, n), dtype, 5, k ** -0.5)
+    want, slack, _ = ref.product(xr, seg, wd, transposed=True)
+    ref.check(ops.grouped_mm_dx(x, i32(seg), wd, row_in=order, row_out=order)[at], want, slack, "dx")
+    g2 = rnd((m, 2 * n), dtype, 6)
+    ref.check(ops.grouped_mm_dx(x, i32(seg), wd, row_in=order, gu=g2), *ref.glu_grad(want, slack, g2), "dgu")
+
+
+@pytest.mark.parametrize("lens", [[16400], [90] * 40, [40] * 40], ids=["long", "middle", "short"])
+def test_several_tiles_of_a_block(lens):
+    """More columns than blocks: each has several tiles of columns.  Rows have the bits that they have in a call of their own."""
+    from moe_offload import ops
+    dtype, n, k, e = torch.bfloat16, 8208, 72, len(lens)
+    seg = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    m = int(seg[-1])
+    x, w, wd = rnd((m, k), dtype, 1), rnd((e, n, k), dtype, 2, k ** -0.5), rnd((e, k, n), dtype, 3, k ** -0.5)
+    gu = torch.empty((m, n), dtype=dtype, device=DEV)
+    g2 = rnd((m, 16), dtype, 4).repeat(1, n // 8)
+    y, h = ops.grouped_mm(x, i32(seg), w), ops.grouped_gate_up(x, None, i32(seg), w, gu_out=gu)
+    dx, dgu = ops.grouped_mm_dx(x, i32(seg), wd), ops.grouped_mm_dx(x, i32(seg), wd, gu=g2)
+    for u, r0 in ((0, 0), (0, lens[0] // 2), (e - 1, m - min(lens[-1], 150))):
+        r1 = min(r0 + 150, int(seg[u + 1]))
+        s, part = i32([0, r1 - r0]), slice(r0, r1)
+        assert torch.equal(y[part], ops.grouped_mm(x[part], s, w[u:u + 1])), (u, "mm")
+        g1 = torch.empty((r1 - r0, n), dtype=dtype, device=DEV)
+        assert torch.equal(h[part], ops.grouped_gate_up(x[part], None, s, w[u:u + 1], gu_out=g1)) and torch.equal(gu[part], g1), (u, "gate_up")
+        assert torch.equal(dx[part], ops.grouped_mm_dx(x[part], s, wd[u:u + 1])), (u, "dx")
+        assert torch.equal(dgu[part], ops.grouped_mm_dx(x[part], s, wd[u:u + 1], gu=g2[part])), (u, "dgu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_most_segments(dtype):
+    """1024 segments, most of them empty or of one row."""
+    from moe_offload import ops
+    lens = np.random.default_rng(5).integers(0, 3, 1024)
+    lens[700] = 130
+    seg = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    m, n, k = int(seg[-1]), 24, 72
+    x, w = rnd((m, k), dtype, 1), rnd((1024, n, k), dtype, 2, k ** -0.5)
+    ref.check(ops.grouped_mm(x, i32(seg), w), *ref.product(x.double().cpu(), seg, w)[:2], "mm")
+    dy = rnd((m, n), dtype, 3)
+    ref.check(ops.grouped_mm_dx(dy, i32(seg), w), *ref.product(dy.double().cpu(), seg, w, transposed=True)[:2], "dx")
+    ref.check(ops.grouped_mm_dw(dy, x, i32(seg)), *ref.weight_grad(dy.double().cpu(), x.double().cpu(), seg, 1024), "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,k,lens", [(64, 264, [1024, 0, 1025, 2500]), (200, 40, [3000, 1]), (264, 392, [1100, 2049, 64]),
-                                      (1032, 1000, [512] * 10 + [0, 1030, 2600, 511, 700, 3])])
+                                      (1032, 1000, [512] * 10 + [0, 1030, 2600, 511, 700, 3]),
+                                      (2056, 2088, [600, 0, 1500])])
 def test_dw_of_long_segments(dtype, n, k, lens):
     """More rows than a block holds the numbers of, in each of the tile sizes, some rows missing."""
     from moe_offload import ops

@@ -32,7 +32,8 @@ def make(dtype, tokens, n_ad, rank, n_in, n_out, seed=0, runs=True):
 @pytest.mark.parametrize("runs", [True, False])
 @pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [
     (1, 1, 8, 8, 8), (1, 5, 16, 2048, 2048), (7, 3, 24, 264, 136), (16, 16, 64, 512, 520), (17, 40, 8, 1000, 72),
-    (64, 4, 128, 128, 256), (65, 2, 40, 72, 1032), (333, 5, 8, 640, 2560), (500, 9, 256, 72, 264), (1500, 3, 48, 320, 200)])
+    (64, 4, 128, 128, 256), (65, 2, 40, 72, 1032), (333, 5, 8, 640, 2560), (500, 9, 256, 72, 264), (1500, 3, 48, 320, 200),
+    (1100, 5, 16, 136, 264), (300, 1024, 8, 72, 40)])
 def test_add(dtype, runs, tokens, n_ad, rank, n_in, n_out):
     from moe_offload import ops
     base, x, a, b, ids, scale = make(dtype, tokens, n_ad, rank, n_in, n_out, runs=runs)
@@ -143,7 +144,8 @@ def test_replayed_graphs_and_streams(tokens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [(1, 3, 8, 64, 72), (50, 4, 24, 136, 264), (333, 5, 8, 640, 256)])
+@pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [(1, 3, 8, 64, 72), (50, 4, 24, 136, 264), (333, 5, 8, 640, 256), (100, 2, 96, 136, 72),
+                                                         (1100, 3, 16, 136, 264), (1500, 2, 40, 264, 136), (40, 1024, 8, 24, 16)])
 def test_gradients(dtype, tokens, n_ad, rank, n_in, n_out):
     """(dx, da, db) against the formula in 64 bits.  v and dv are rounded once before the second product, which
     moves each of its terms by at most half a step: eps / 2 of the sum of their magnitudes."""
