@@ -194,7 +194,9 @@ __global__ __launch_bounds__(64 * kVWaves) void k_lora_v_dv(const T* x, int64_t 
         ranks_of<T, SR, ST, D, false, T>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
 }
 
-// Blocks of a tile's adapters: up to 256 tokens each gets its own (16 tokens have 16 at most).
+// Blocks of a tile's adapters: up to 256 tokens each gets its own (16 tokens have 16 at most).  One after another and side
+// by side, us of lora_add, 2048 x 2048: 8 tokens of 8 adapters, rank 16, 34 and 9.6, 200 tokens, 4 to an adapter, 22 and
+// 10.6; but 1000 tokens, 100 to an adapter, 2560 x 2560, rank 64, 20.8 and 32.9: most of the blocks find none left.
 template <int ST>
 uint32_t split_of(int n_tok) {
     return ST == 1 && n_tok <= 256 ? (uint32_t)(n_tok < 16 ? n_tok : 16) : 1;
@@ -204,6 +206,7 @@ template <typename T, int ST>
 int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy, int64_t lddy, const T* B, int64_t b_stride,
               const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, T* v, T* dv, hipStream_t s) {
     const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST)), split = 2 * split_of<ST>(n_tok);
+    // (a tile of 32 ranks for 16: lora_add of 4096 tokens, rank 16, 28.1 us, and 26.8 with a tile of 16)
     if (rank <= 16)
         hipLaunchKernelGGL((k_lora_v_dv<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                            a_stride, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv);
@@ -214,11 +217,16 @@ int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy
     return 0;
 }
 
+// Tokens of a tile: 32 use each load of an adapter twice, 16 are more blocks.  us of lora_add with 32 and 16, rank 64, 2560 x
+// 2560: 4096 tokens 33 and 36 with inputs from memory, 34 and 29 with all in cache; 1000 tokens 24 and 21; lora_grad of
+// 4096 tokens, 2560 x 2048, 60.6 and 64.5.
+constexpr int kFewTokens = 1024;
+
 template <typename T>
 int lora_v_dv_typed(const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* dy, int64_t lddy, const void* B,
                     int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
                     void* v, void* dv, hipStream_t s) {
-    auto f = n_tok <= 1024 ? lora_v_dv<T, 1> : lora_v_dv<T, 2>;
+    auto f = n_tok <= kFewTokens ? lora_v_dv<T, 1> : lora_v_dv<T, 2>;
     return f((const T*)x, ldx, (const T*)A, a_stride, (const T*)dy, lddy, (const T*)B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out,
              rank, (T*)v, (T*)dv, s);
 }
@@ -250,17 +258,17 @@ __device__ __forceinline__ void split8(const float* v, uint4 (&part)[kParts<T>])
     for (int k = 0; k < kParts<T>; ++k) part[k] = __builtin_bit_cast(uint4, p[k]);
 }
 
-// out = base + B_i v for 16 ST tokens (blockIdx.x) and 128 columns per wave, W waves.  The wave's eight subtiles of 16
+// out = base + B_i v for 16 ST tokens (blockIdx.x) and 128 columns per wave.  The wave's eight subtiles of 16
 // columns are dealt out so that lane n has the columns 8 n .. 8 n + 7, one of each: 16 bytes per token, and 16 lanes' are
 // one row's 256.  B's rows and v go through LDS, 64 ranks at a time, in loads of whole lines: loaded straight into the
 // matrix unit's layout every lane's 16 bytes are a cache access of their own, and those set the pace.
-template <typename T, int ST, int W>
-__global__ __launch_bounds__(64 * W, 2) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
+template <typename T, int ST>
+__global__ __launch_bounds__(256, 2) void k_lora_out(const T* base, int64_t ldb, const float* __restrict__ v,
                                                         const T* __restrict__ B, int64_t b_stride, const int32_t* __restrict__ ids,
                                                         int n_tok, int n_ad, int n_out, int rank, T* out, int64_t ldo) {
-    constexpr int SC = 8, kVLoads = (4 * ST + W - 1) / W;
+    constexpr int W = 4, SC = 8, kVLoads = ST;
     constexpr uint32_t kB = 128 * 128;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kB + kVLoads * W * 1024];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * kB + 4 * ST * 1024];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
     const uint32_t lds_b = (uint32_t)(uintptr_t)(lds_u8*)lds + wv * kB, lds_v = (uint32_t)(uintptr_t)(lds_u8*)lds + W * kB;
     const int first = ((int)blockIdx.y * W + wv) * 128, q = first + n * 8;
@@ -429,10 +437,8 @@ int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, in
                                a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
         HIP_TRY(hipGetLastError());
     }
-    // few tokens: a wave per block, to reach more of the card
-    constexpr int W = ST == 1 ? 1 : 4;
-    hipLaunchKernelGGL((k_lora_out<T, ST, W>), dim3(tiles, (n_out + 128 * W - 1) / (128 * W), split), dim3(64 * W), 0, s, base, ldb,
-                       v, B, b_stride, ids, n_tok, n_ad, n_out, rank, out, ldo);
+    hipLaunchKernelGGL((k_lora_out<T, ST>), dim3(tiles, (n_out + 511) / 512, split), dim3(256), 0, s, base, ldb, v, B, b_stride, ids,
+                       n_tok, n_ad, n_out, rank, out, ldo);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -441,7 +447,7 @@ template <typename T>
 int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* B,
                    int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
                    float* v, void* out, int64_t ldo, hipStream_t s) {
-    auto f = n_tok <= 1024 ? lora_add<T, 1> : lora_add<T, 2>;
+    auto f = n_tok <= kFewTokens ? lora_add<T, 1> : lora_add<T, 2>;
     return f((const T*)base, ldb, (const T*)x, ldx, (const T*)A, a_stride, (const T*)B, b_stride, ids, scale, n_tok, n_ad, n_in,
              n_out, rank, v, (T*)out, ldo, s);
 }
