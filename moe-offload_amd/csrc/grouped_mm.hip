@@ -66,6 +66,17 @@ __device__ __forceinline__ void store16(void* to, uint4 v) {
     else *(u32x4*)to = __builtin_bit_cast(u32x4, v);
 }
 
+// Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
+// runs of `run` items; more of them even out over whole shares of one XCD each, which read a row once.  us of gradients,
+// dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 435 (of 1024 rows each, dw
+// alone, 173 and 163), 8 adapters of 4096 tokens 57.9 and 60.6; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
+constexpr int kManySegs = 128;
+
+__device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run) {
+    const uint32_t i = b / 8;
+    return b < nb / (8 * run) * (8 * run) ? (i / run * 8 + b % 8) * run + i % run : b;
+}
+
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
 // next tile's first step during the last of this one: two images, one barrier per step.  (Four images, three steps under
@@ -91,7 +102,8 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     int r0, r1, slot, tile, p0 = 0, nc = a.nc, seg = 0;
     if constexpr (OP == kDw) {
         const int tp = (a.np + BP - 1) / BP;
-        const uint32_t item = xcd_order(block, blocks);
+        const uint32_t run = ((uint32_t)groups * tp + 7) / 8;
+        const uint32_t item = a.S.n_seg < kManySegs ? dealt(block, blocks, run) : xcd_order(block, blocks);
         seg = item / (groups * tp);
         p0 = (int)(item / groups % tp) * BP;
         tile = (int)(item % groups) * a.span;
