@@ -229,6 +229,10 @@ def _one_gpu(who: str, names: str, *tensors) -> int:
     return dev
 
 
+# sizes go to the library as 32-bit integers, which ctypes would cut without a word
+_MAX_SIDE = 2 ** 30
+
+
 def _rows(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, width: int | None) -> int:
     """Checks a matrix with contiguous rows; returns the elements from row to row."""
     shape = t.shape
@@ -238,6 +242,8 @@ def _rows(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | 
         raise ValueError(f"{who}: {name} has shape {tuple(shape)}, not ({'*' if rows is None else rows}, "
                          f"{'*' if width is None else width})")
     n, w = shape
+    if n > _MAX_SIDE or w > _MAX_SIDE:
+        raise ValueError(f"{who}: {name}: {n} rows of {w} elements (up to 2^30)")
     step, inner = t.stride()
     if w % 8 or w == 0:
         raise ValueError(f"{who}: {name}: rows of {w} elements (a multiple of 8 wanted)")
@@ -256,6 +262,8 @@ def _mats(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple
     if len(have) != 3 or any(s is not None and s != d for s, d in zip(shape, have)):
         raise ValueError(f"{who}: {name} has shape {tuple(have)}, not {tuple('*' if s is None else s for s in shape)}")
     m, n, k = have
+    if m > _MAX_SIDE or n > _MAX_SIDE or k > _MAX_SIDE:
+        raise ValueError(f"{who}: {name}: {m} matrices of {n} x {k} (up to 2^30)")
     if n % 8 or n == 0 or k % 8 or k == 0:
         raise ValueError(f"{who}: {name}: matrices of {n} x {k} (multiples of 8 wanted)")
     if m == 0:
@@ -271,6 +279,8 @@ def _index(who: str, name: str, t: torch.Tensor | None, n: int | None = None) ->
         return
     if t.dtype != torch.int32:
         raise TypeError(f"{who}: {name} is {t.dtype}, not torch.int32")
+    if t.numel() > _MAX_SIDE:
+        raise ValueError(f"{who}: {name} has {t.numel()} entries (up to 2^30)")
     if not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{who}: {name} must be contiguous" + ("" if n is None else f" with {n} entries, not {t.numel()}"))
 
@@ -372,7 +382,7 @@ def grouped_mm(x, seg_start, w, row_in=None, row_out=None, n_out_rows=None, seg_
     row_in's or row_out's, else x's.  A new output has n_out_rows rows, or as many as there are sorted rows
     (row_out must then name each of its rows once, as expert_plan's does); rows of no segment, or of one whose slot is
     outside w, are zeros in it and left as they are in a given `out`.  A row_in outside x gives a row of
-    zeros, a row_out outside the output is dropped.
+    zeros, a row_out outside the output is dropped.  Outputs, here and below, must not overlap inputs.
     """
     who = "grouped_mm"
     dev = _one_gpu(who, "x seg_start w row_in row_out seg_slot scale out", x, seg_start, w, row_in, row_out, seg_slot, scale, out)

@@ -149,3 +149,14 @@ def test_sizes_whose_sums_would_pass_31_bits_are_refused(name, good, bad):
     for change in bad:
         assert set(change) <= set(good)
         refused(name, *{**good, **change}.values())
+
+
+def test_sizes_past_the_library_s_integers_are_refused():
+    big, bf = 2 ** 31 + 8, torch.bfloat16
+    for check, t in ((lambda t: ops._rows("op", "x", t, bf, None, None), torch.empty((big, 8), dtype=bf, device="meta")),
+                     (lambda t: ops._rows("op", "x", t, bf, None, None), torch.empty((1, big), dtype=bf, device="meta")),
+                     (lambda t: ops._mats("op", "w", t, bf, (None, None, None)), torch.empty((big, 8, 8), dtype=bf, device="meta")),
+                     (lambda t: ops._mats("op", "w", t, bf, (None, None, None)), torch.empty((1, 8, big), dtype=bf, device="meta")),
+                     (lambda t: ops._index("op", "ids", t), torch.empty(big, dtype=torch.int32, device="meta"))):
+        with pytest.raises(ValueError, match="2\\^30"):
+            check(t)
