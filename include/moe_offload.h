@@ -277,11 +277,11 @@ int moe_pair_combine(const void* y, const void* scores, const void* residual, in
 /* ---- Part 2b: unquantised experts and adapters (no counterpart in the reference) ------------ */
 /* The reference multiplies 2-bit experts only (prefill_qproj.py:18-40); these are its sorted products
  * for fp16 or bf16 weights (dtype 0 or 1, inputs, weights and outputs alike), with their gradients, the
- * row plan they take, and low-rank adapters.  Pointers are device memory, 16-byte aligned; ld* are
- * elements from row to row and *_stride elements from matrix to matrix, both multiples of 8, as all row
- * lengths are; within a matrix rows follow each other.  Row numbers are 32-bit, sizes up to
- * 2^30, offsets 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).  Nothing is allocated,
- * kept between calls or synchronised.  Sums are fp32, rounded once. */
+ * row plan they take, and low-rank adapters.  Pointers are device memory, matrices and workspaces 16-byte
+ * aligned; ld* are elements from row to row and *_stride elements from matrix to matrix, both multiples
+ * of 8, as all row lengths are; within a matrix rows follow each other.  Row numbers are 32-bit, sizes
+ * up to 2^30, offsets 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).
+ * Nothing is allocated, kept between calls or synchronised.  Sums are fp32, rounded once. */
 
 /* The rows of a batch sorted by expert, as prefill.resident_plan (loader.py:583-591) makes them on the
  * host: ids i32 [n_ids], pair p = token * k + j.  Sorted row r is pair row_out[r] of token row_token[r];
@@ -296,8 +296,8 @@ int moe_expert_plan(const int32_t* ids, int n_ids, int k, int n_exp, void* works
  * - 1, W_u [n][k] = w + seg_slot[u] * w_stride (seg_slot null: u), scale fp32 per slot or null; row_in /
  * row_out null: row r.  n_seg in 0..1024.  A row_in outside x gives a row of zeros; a row_out outside y
  * is not written; two rows with one row_out leave either's result.  seg_start does not decrease (of
- * one that does, some rows are missed).  Rows of no segment, and of one whose slot is outside 0 .. n_slots - 1, are written as
- * zeros if fill != 0 and left as they are if not. */
+ * one that does, some rows are missed).  Rows of no segment, and of one whose slot is outside
+ * 0 .. n_slots - 1, are written as zeros if fill != 0 and left as they are if not. */
 int moe_grouped_mm(const void* x, int64_t ldx, int n_x, const int32_t* row_in, const int32_t* seg_start,
                    const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots, int n,
                    int k, const float* scale, void* y, int64_t ldy, int n_y, const int32_t* row_out, int dtype, int fill,

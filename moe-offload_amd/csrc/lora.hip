@@ -454,7 +454,7 @@ int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, co
              n_out, rank, v, (T*)out, ldo, s);
 }
 
-constexpr int kMaxOut = 65535 * 128;                          // the second grid dimension, 128 columns each
+constexpr int kMaxOut = (1 << 23) - 8;                        // the second grid dimension, 512 columns each, and its loads
 
 // The shapes and strides that both entry points take; base or dy is [n_tok][n_out].
 bool bad_shapes(const char* who, int dtype, int n_tok, int n_ad, int n_in, int n_out, int rank, int64_t ldx, int64_t ldy,
