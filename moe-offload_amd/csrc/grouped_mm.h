@@ -16,7 +16,8 @@ struct Segs {
 };
 
 // Two weights' gradients over the same rows, dw [n_seg][n][k] contiguous, as moe_grouped_mm_dw computes them (the caller
-// has checked the arguments): in one launch where both are narrow.
+// has checked the arguments): in one launch where both are narrow.  split: 1 dy's rows, 2 x's rows are two rows each, 2 r
+// and 2 r + 1, whose sum they are.
 struct Dw {
     const void* dy;
     int64_t lddy;
@@ -25,9 +26,14 @@ struct Dw {
     int n, k;
     const float* scale;
     void* dw;
+    int split;
 };
 int dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, int dtype,
             hipStream_t s);
+
+// dx[rows[r]] = W_u^T (dv[2 rows[r]] + dv[2 rows[r] + 1]), W_u [n][k]; zeros for rows of no segment.
+int dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
+                int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s);
 
 // Block index -> work item, keeping consecutive items on one XCD (blocks are dealt to the 8 XCDs round
 // robin), so that the blocks of one row tile find its rows in that XCD's L2.

@@ -45,6 +45,8 @@ struct Args {
     int np, nq, nc;              // extents: output columns in p (mm_dw) and q, and the contraction
     int out_f32;
     int span;                    // column tiles per block
+    int fold;                    // mm_dx: contraction indexes from here on use the weights' rows from 0 on again (0: none do)
+    int split;                   // mm_dw: 1 dy, 2 x: each row is two, whose sum it is
 };
 
 // Two subtiles' 4 adjacent 16-bit results per lane -> 8 adjacent: lanes 16-31 and 48-63 take the second
@@ -111,7 +113,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
         p0 = (int)(item / groups % tp) * BP;
         tile = (int)(item % groups) * a.span;
         seg_rows(a.S, seg + 1, r0, r1, slot);
-        nc = r1 - r0;
+        nc = (r1 - r0) << (a.split ? 1 : 0);
     } else {
         Tile at;
         __shared__ uint32_t scratch[kWaves + 3];
@@ -143,9 +145,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     auto hold_rows = [&](int c0, int c1) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
         for (int c = c0 + t; c < c1; c += 64 * kWaves) {
-            const int v = a.row_p ? a.row_p[r0 + c] : r0 + c, x = a.row_q ? a.row_q[r0 + c] : r0 + c;
+            const int r = r0 + (a.split ? c >> 1 : c), v = a.row_p ? a.row_p[r] : r, x = a.row_q ? a.row_q[r] : r;
             const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
-            idx[c - c0] = make_int2(both ? v : -1, both ? x : -1);
+            idx[c - c0] = make_int2(both ? a.split & 1 ? 2 * v + (c & 1) : v : -1, both ? a.split & 2 ? 2 * x + (c & 1) : x : -1);
         }
     };
     if constexpr (OP != kDw) {
@@ -181,7 +183,8 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             for (int j = 0; j < kLoadsQ; ++j) {
                 if constexpr (kAlongQ) {
                     const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + (lane % kUnitsQ ^ 2 * turn<BQ>(row)) * 8;
-                    qp[j] = any && load_c + row < nc ? Q + (int64_t)(load_c + row) * a.nq + (q < a.nq ? q : 0) : zero;
+                    const int c = load_c + row, w = OP == kDx && a.fold && c >= a.fold ? c - a.fold : c;
+                    qp[j] = any && c < nc ? Q + (int64_t)w * a.nq + (q < a.nq ? q : 0) : zero;
                 } else {
                     const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
                     int64_t q;
@@ -201,7 +204,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     };
     auto advance = [&]() {
         load_c += kBC;
-        if (OP != kDw && load_tile < end && load_c + kBC <= nc) {                // wave-uniform; past the end all stay at zero
+        if (OP != kDw && !(OP == kDx && a.fold) && load_tile < end && load_c + kBC <= nc) {    // wave-uniform; past the end all stay at zero
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) pp[j] += kBC;
 #pragma unroll
@@ -641,7 +644,7 @@ int64_t blocks_of(Args& a) {
     int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
     if constexpr (OP == kDw) {
         rows = most = (int64_t)a.S.n_seg * ((a.np + BP - 1) / BP);
-        steps = a.S.n_rows / a.S.n_seg / kBC + 1;
+        steps = ((int64_t)a.S.n_rows << (a.split ? 1 : 0)) / a.S.n_seg / kBC + 1;
     } else {
         rows = row_tiles(a, BP);
         most = (int64_t)a.S.n_rows / BP + (a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
@@ -811,10 +814,19 @@ int gmm::dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, cons
         Args r = {};
         r.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 0};
         r.p = d.dy, r.q = d.x, r.out = d.dw, r.row_p = r.row_q = rows, r.scale = d.scale;
-        r.ldp = d.lddy, r.ldq = d.ldx, r.ldo = (int64_t)d.n * d.k, r.n_p = r.n_q = n_rows, r.np = d.n, r.nq = d.k;
+        r.ldp = d.lddy, r.ldq = d.ldx, r.ldo = (int64_t)d.n * d.k, r.n_p = r.n_q = n_rows, r.np = d.n, r.nq = d.k, r.split = d.split;
         return r;
     };
     return dtype ? launch_dw_pair<__bf16>(args(a), args(b), s) : launch_dw_pair<_Float16>(args(a), args(b), s);
+}
+
+int gmm::dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
+                     int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s) {
+    Args a = {};
+    a.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 1};
+    a.p = dv, a.q = w, a.out = dx, a.row_p = a.row_out = rows;
+    a.ldp = 2 * (int64_t)n, a.ldq = w_stride, a.ldo = lddx, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = 2 * n, a.fold = n;
+    return launch_typed<kDx>(a, dtype, s);
 }
 
 extern "C" {

@@ -12,9 +12,10 @@
 // result.  In a batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks
 // of their own.
 //
-// The gradients: dv[t] = s_i B_i^T dy[t] beside v in one launch, both rounded to 16 bits as an activation between two
-// layers is, then the grouped products over the tokens sorted by adapter, dx = A_i^T dv, dA_i = sum dv x^T,
-// dB_i = s_i sum dy v^T.
+// The gradients: dv[t] = s_i B_i^T dy[t] beside v in one launch, then the grouped products over the tokens sorted by
+// adapter, dx = A_i^T dv, dA_i = sum dv x^T, dB_i = s_i sum dy v^T.  v and dv are two 16-bit parts each there, along the
+// contraction: rounded to 16 bits they alone would put the gradients 1.4 times as far from the exact ones as their own
+// rounding does.
 #include <hip/hip_bf16.h>
 
 #include <algorithm>
@@ -62,7 +63,8 @@ constexpr int kVWaves = 8;
 // v[t][j] = s_i W_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), where W_i[j] is row j of A_i, or
 // (ALONG) column j of B_i [nc][rank].  Each wave multiplies every eighth step of 64 along the contraction, through an LDS
 // ring of its own (D steps of the tokens' and the ranks' operands); the waves' sums are added in their order.  O: fp32, or
-// T where v is an operand of a product next.  4096 tokens, rank 64, 2560: 14 us for 24 MB, one block of 8 waves per 32
+// T where v is an operand of a product next: then row 2 t is v[t] rounded and row 2 t + 1 what that leaves, together 16
+// (bf16) or 22 bits.  4096 tokens, rank 64, 2560: 14 us for 24 MB, one block of 8 waves per 32
 // tokens and 32 ranks, whose few steps each (5) are mostly the first loads' way.
 template <typename T, int SR, int ST, int D, bool ALONG, typename O>
 __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* __restrict__ x, int64_t ldx,
@@ -164,7 +166,15 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
             for (int m = 0; m < ST; ++m)
                 if (wv % ST == m && mine[m] && j < rank) {
                     if constexpr (sizeof(O) == 4) *(f32x4*)(v + t[m] * rank + j) = sum;
-                    else *(uint2*)(v + t[m] * rank + j) = round4<T>(sum);
+                    else {
+                        const uint2 hi = round4<T>(sum);
+                        const f32x4 rest = sum - widen4<T>(hi);
+                        f32x4 lo;                                              // an infinity or NaN stays in the first part
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) lo[e] = __builtin_fabsf(rest[e]) < __builtin_inff() ? rest[e] : 0.f;
+                        *(uint2*)(v + 2 * t[m] * rank + j) = hi;
+                        *(uint2*)(v + (2 * t[m] + 1) * rank + j) = round4<T>(lo);
+                    }
                 }
         }
         __syncthreads();
@@ -514,7 +524,7 @@ extern "C" int moe_lora_add(const void* base, int64_t ld_base, const void* x, in
 
 extern "C" uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank) {
     if (n_tok < 0 || n_ad < 1 || rank <= 0) return 0;
-    return 2 * up16((uint64_t)n_tok * rank * 2) + 2 * up16((uint64_t)n_tok * 4) + up16((uint64_t)(n_ad + 1) * 4) +
+    return 2 * up16((uint64_t)n_tok * rank * 4) + 2 * up16((uint64_t)n_tok * 4) + up16((uint64_t)(n_ad + 1) * 4) +
            moe_expert_plan_workspace_bytes(n_tok, n_ad);
 }
 
@@ -524,8 +534,8 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
                              void* db, void* stream) {
     const char* who = "lora_grad";
     if (bad_shapes(who, dtype, n_tok, n_ad, n_in, n_out, rank, ldx, lddy, a_stride, b_stride)) return -1;
-    if (n_ad < 1 || n_ad > gmm::kMaxSeg || lddx % 8 || (n_tok > 1 && lddx < n_in)) {
-        moe_set_error("%s: n_ad=%d (1..%d) lddx=%lld", who, n_ad, gmm::kMaxSeg, (long long)lddx);
+    if (n_ad < 1 || n_ad > gmm::kMaxSeg || n_tok > gmm::kMaxSide / 2 || lddx % 8 || (n_tok > 1 && lddx < n_in)) {
+        moe_set_error("%s: n_ad=%d (1..%d) n_tok=%d (up to 2^29) lddx=%lld", who, n_ad, gmm::kMaxSeg, n_tok, (long long)lddx);
         return -1;
     }
     if (n_tok > 0 && !ids) {
@@ -539,8 +549,8 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
         p += up16(bytes);
         return q;
     };
-    void* v = take((uint64_t)n_tok * rank * 2);
-    void* dv = take((uint64_t)n_tok * rank * 2);
+    void* v = take((uint64_t)n_tok * rank * 4);
+    void* dv = take((uint64_t)n_tok * rank * 4);
     int32_t* order = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* same = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* seg = (int32_t*)take((uint64_t)(n_ad + 1) * 4);
@@ -550,9 +560,8 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
     if (moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
         (n_tok > 0 && v_dv(x, ldx, a, a_stride, dy, lddy, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv,
                            (hipStream_t)stream)) ||
-        moe_grouped_mm_dx(dv, rank, n_tok, order, seg, nullptr, n_ad, n_tok, a, a_stride, n_ad, rank, n_in, nullptr, nullptr, 0,
-                          dx, lddx, n_tok, order, dtype, 1, stream) ||
-        gmm::dw_pair(gmm::Dw{dv, rank, x, ldx, rank, n_in, nullptr, da}, gmm::Dw{dy, lddy, v, rank, n_out, rank, scale, db}, order,
+        (n_tok > 0 && gmm::dx_of_parts(dv, order, n_tok, seg, n_ad, a, a_stride, rank, n_in, dx, lddx, dtype, (hipStream_t)stream)) ||
+        gmm::dw_pair(gmm::Dw{dv, rank, x, ldx, rank, n_in, nullptr, da, 1}, gmm::Dw{dy, lddy, v, rank, n_out, rank, scale, db, 2}, order,
                      n_tok, seg, n_ad, dtype, (hipStream_t)stream))
         return -1;
     return 0;

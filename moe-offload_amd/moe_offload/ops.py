@@ -549,7 +549,7 @@ def lora_grad(dy, x, a, b, ids, scale=None, workspace=None):
     """The gradients of lora_add in x (the adapter's part; base's is dy itself), a and b: (dx, da, db).
 
     With the tokens sorted by adapter: v = a x, dv = scale b^T dy, dx = a^T dv, da = sum dv x^T, db = scale
-    sum dy v^T.  v and dv are rounded to the inputs' type, as activations between two layers are.  Tokens
+    sum dy v^T.  v and dv are kept as sums of two values of the inputs' type.  Tokens
     without an adapter get dx = 0, adapters without tokens da = db = 0.  At most 1024 adapters.  workspace:
     scratch of moe_lora_grad_workspace_bytes.
     """

@@ -147,12 +147,12 @@ def test_replayed_graphs_and_streams(tokens):
 @pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [(1, 3, 8, 64, 72), (50, 4, 24, 136, 264), (333, 5, 8, 640, 256), (100, 2, 96, 136, 72),
                                                          (1100, 3, 16, 136, 264), (1500, 2, 40, 264, 136), (40, 1024, 8, 24, 16)])
 def test_gradients(dtype, tokens, n_ad, rank, n_in, n_out):
-    """(dx, da, db) against the formula in 64 bits.  v and dv are rounded once before the second product, which
-    moves each of its terms by at most half a step: eps / 2 of the sum of their magnitudes."""
+    """(dx, da, db) against the formula in 64 bits.  v and dv are sums of two values of the type before the second product:
+    the first is off by at most half a step, eps / 2 of the value, and the second by as much of that."""
     from moe_offload import dense, ops
     base, x, a, b, ids, scale = make(dtype, tokens, n_ad, rank, n_in, n_out, runs=False)
     dy = rnd((tokens, n_out), dtype, 40)
-    half, tiny = torch.finfo(dtype).eps / 2, {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}[dtype]
+    half, tiny = (torch.finfo(dtype).eps / 2) ** 2, {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}[dtype]
     dx, da, db = ops.lora_grad(dy, x, a, b, ids, scale=scale)
     wx, sx = torch.zeros(x.shape, dtype=torch.float64), torch.zeros(x.shape, dtype=torch.float64)
     for j in range(n_ad):
