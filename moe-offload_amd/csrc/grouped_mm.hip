@@ -71,7 +71,7 @@ __device__ __forceinline__ void store16(void* to, uint4 v) {
 // Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
 // runs of `run` items; more of them even out over whole shares of one XCD each, which read a row once.  us of gradients,
 // dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 435 (of 1024 rows each, dw
-// alone, 173 and 163), 8 adapters of 4096 tokens 57.9 and 60.6; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
+// alone, 173 and 163), 8 adapters of 4096 tokens (in one part) 57.9 and 60.6; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
 constexpr int kManySegs = 128;
 
 __device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run) {
@@ -142,12 +142,13 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     // The rows of x or dy, the same in every step.  mm_dw: numbers of the rows [c0, c1) of dy and x, -1 for one that is
     // missing on either side: zeros on the one would still meet an infinity on the other.
     int rp[kLoadsP];
+    const int halves = OP == kDw && a.split ? 1 : 0;                           // two contraction indexes per row
     auto hold_rows = [&](int c0, int c1) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
-        for (int c = c0 + t; c < c1; c += 64 * kWaves) {
-            const int r = r0 + (a.split ? c >> 1 : c), v = a.row_p ? a.row_p[r] : r, x = a.row_q ? a.row_q[r] : r;
+        for (int c = (c0 >> halves) + t; c < (c1 + halves) >> halves; c += 64 * kWaves) {
+            const int v = a.row_p ? a.row_p[r0 + c] : r0 + c, x = a.row_q ? a.row_q[r0 + c] : r0 + c;
             const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
-            idx[c - c0] = make_int2(both ? a.split & 1 ? 2 * v + (c & 1) : v : -1, both ? a.split & 2 ? 2 * x + (c & 1) : x : -1);
+            idx[c - (c0 >> halves)] = make_int2(both ? v : -1, both ? x : -1);
         }
     };
     if constexpr (OP != kDw) {
@@ -159,8 +160,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             rp[j] = v >= 0 && v < a.n_p ? v : 0;
         }
     }
-    // mm_dw of more rows than are held: tile by tile, kIdx rows [part0, part1) at a time
-    const bool parts = OP == kDw && nc > kIdx;
+    // mm_dw of more rows than are held: tile by tile, what `held` indexes [part0, part1) need at a time
+    const int held = kIdx << halves;
+    const bool parts = OP == kDw && nc > held;
     int part0 = 0, part1 = nc;
     int load_tile = tile, load_c = 0;                                          // the step that is loaded next
     auto place = [&]() {
@@ -170,8 +172,11 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) {
                 const int row = along_row(j, kLoadsP, kUnitsP), col = (lane % kUnitsP ^ 2 * turn<BP>(row)) * 8;
-                const int2 v = idx[any && load_c + row < part1 ? load_c + row - part0 : 0];
-                const bool ok = any && load_c + row < part1 && v.x >= 0;
+                const int c = load_c + row, odd = c & halves;
+                int2 v = idx[any && c < part1 ? (c - part0) >> halves : 0];
+                const bool ok = any && c < part1 && v.x >= 0;
+                if (a.split & 1) v.x = 2 * v.x + odd;
+                if (a.split & 2) v.y = 2 * v.y + odd;
                 pp[j] = ok ? P + v.x * a.ldp + (p0 + col < a.np ? p0 + col : 0) : zero;
                 qp[j] = ok ? Q + v.y * a.ldq + (q0 + col < a.nq ? q0 + col : 0) : zero;
             }
@@ -275,9 +280,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
         f32x4 acc[SP][SQ] = {};
 #pragma unroll 1
         for (int c0 = 0; c0 < nc; c0 += kBC) {
-            if (OP == kDw && parts && c0 % kIdx == 0) {
+            if (OP == kDw && parts && c0 % held == 0) {
                 part0 = c0;
-                part1 = c0 + kIdx < nc ? c0 + kIdx : nc;
+                part1 = c0 + held < nc ? c0 + held : nc;
                 __syncthreads();                                               // the rows held so far are all placed
                 hold_rows(part0, part1);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the part before's loads past its end
@@ -526,8 +531,8 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
 }
 
 // Two narrow weights' gradients (an adapter's A and B) in one launch: n_a blocks are the first one's.  4096 tokens of 8
-// adapters, rank 64, 2560 and 2048 wide: 21 us (as two launches 22 + 18 with four images, 26 together with two and whole
-// segments per XCD); waits for memory half of the time.
+// adapters, rank 64, 2560 and 2048 wide: 37 us for rows in two parts, 21 for single ones (those as two launches 22 + 18 with
+// four images, 26 together with two and whole segments per XCD); waits for memory half of the time.
 template <typename T>
 __global__ __launch_bounds__(256, 4) void k_grouped_dw_pair(Args a, Args b, uint32_t n_a) {
     const bool first = blockIdx.x < n_a;
