@@ -167,6 +167,8 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
                 if (wv % ST == m && mine[m] && j < rank) {
                     if constexpr (sizeof(O) == 4) *(f32x4*)(v + t[m] * rank + j) = sum;
                     else {
+                        // (opaque: the product above, rounded to fp32 or straight to fp16, must be one value for both parts)
+                        asm volatile("" : "+v"(sum));
                         const uint2 hi = round4<T>(sum);
                         const f32x4 rest = sum - widen4<T>(hi);
                         f32x4 lo;                                              // an infinity or NaN stays in the first part

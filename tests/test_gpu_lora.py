@@ -145,7 +145,8 @@ def test_replayed_graphs_and_streams(tokens):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [(1, 3, 8, 64, 72), (50, 4, 24, 136, 264), (333, 5, 8, 640, 256), (100, 2, 96, 136, 72),
-                                                         (1100, 3, 16, 136, 264), (1500, 2, 40, 264, 136), (40, 1024, 8, 24, 16)])
+                                                         (1100, 3, 16, 136, 264), (1500, 2, 40, 264, 136), (40, 1024, 8, 24, 16),
+                                                         (5000, 1, 8, 64, 72), (4500, 1, 136, 264, 136)])
 def test_gradients(dtype, tokens, n_ad, rank, n_in, n_out):
     """(dx, da, db) against the formula in 64 bits.  v and dv are sums of two values of the type before the second product:
     the first is off by at most half a step, eps / 2 of the value, and the second by as much of that."""
