@@ -58,23 +58,26 @@ __device__ __forceinline__ void each_adapter(const int (&id)[ST], const bool (&h
     }
 }
 
-constexpr int kVWaves = 8;
+constexpr int kVWaves = 4;      // (8, one block per CU: lora_add of 64 tokens 11.2 us, with 4 10.4; lora_grad of 4096 72.9 and 70.1)
+constexpr int kVRing = 2;
 
 // v[t][j] = s_i W_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), where W_i[j] is row j of A_i, or
-// (ALONG) column j of B_i [nc][rank].  Each wave multiplies every eighth step of 64 along the contraction, through an LDS
-// ring of its own (D steps of the tokens' and the ranks' operands); the waves' sums are added in their order.  O: fp32, or
+// (ALONG) column j of B_i [nc][rank].  Each wave multiplies every fourth step of 64 along the contraction, through an LDS
+// ring of its own (two steps of the tokens' and the ranks' operands); the waves' sums are added in their order.  O: fp32, or
 // T where v is an operand of a product next: then row 2 t is v[t] rounded and row 2 t + 1 what that leaves, together 16
-// (bf16) or 22 bits.  4096 tokens, rank 64, 2560: 14 us for 24 MB, one block of 8 waves per 32
-// tokens and 32 ranks, whose few steps each (5) are mostly the first loads' way.
-template <typename T, int SR, int ST, int D, bool ALONG, typename O>
+// (bf16) or 22 bits.  4096 tokens, rank 64, 2560: 13 us for
+// 24 MB, a block per 32 tokens and 32 ranks, whose waves' few steps (10) are mostly the loads' way; v and dv for the
+// gradients, 2560 and 2048, 20 us for 40 MB.
+template <typename T, int SR, int ST, bool ALONG, typename O>
 __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* __restrict__ x, int64_t ldx,
                                          const T* __restrict__ W, int64_t w_stride, const int32_t* __restrict__ ids,
                                          const float* __restrict__ scale, int n_tok, int n_ad, int nc, int rank,
                                          O* __restrict__ v) {
     constexpr int kLoads = 2 * (ST + SR);
     constexpr uint32_t kStage = kLoads * 1024;
+    static_assert(SR * ST <= kVWaves, "a wave per subtile of the sums");
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
-    const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)lds + wv * D * kStage;
+    const uint32_t ring = (uint32_t)(uintptr_t)(lds_u8*)lds + wv * kVRing * kStage;
     const int j0 = blockIdx.y * (16 * SR), cu = ((lane & 7) ^ (lane >> 3)) * 8;
     const T* zero = (const T*)&g_zero16;
     asm("" : "+s"(zero));
@@ -97,7 +100,7 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
     Frags<ALONG, 16 * SR, SR> fw;
     fx.init(ring, 0, lane);
     fw.init(ring + ST * 2048, 0, lane);
-    const int steps = ((nc + 63) / 64 - wv + kVWaves - 1) / kVWaves;           // wv, wv + 8, ...
+    const int steps = ((nc + 63) / 64 - wv + kVWaves - 1) / kVWaves;           // wv, wv + 4, ...
     each_adapter<ST>(id, has, z, n_z, [&](int i, const bool (&mine)[ST]) {
         const float si = scale ? scale[i] : 1.0f;
         const T* wp[2 * SR];
@@ -116,7 +119,7 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
         }
         auto issue = [&](int s) {
             const int c = (s * kVWaves + wv) * 64;                             // (also past the last step)
-            const uint32_t to = ring + (uint32_t)(s % D) * kStage;
+            const uint32_t to = ring + (uint32_t)(s % kVRing) * kStage;
 #pragma unroll
             for (int j = 0; j < 2 * ST; ++j) load_to_lds(c + cu < nc ? xp[j] + c : zero, to + j * 1024);
 #pragma unroll
@@ -125,11 +128,11 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
         };
         f32x4 acc[SR][ST] = {};
 #pragma unroll
-        for (int s = 0; s < D; ++s) issue(s);
+        for (int s = 0; s < kVRing; ++s) issue(s);
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) {
-            const uint32_t stage = (uint32_t)(s % D) * kStage;
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");   // loads return in order
+            const uint32_t stage = (uint32_t)(s % kVRing) * kStage;
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kVRing - 1) * kLoads) : "memory");   // loads return in order
             uint4 xv[2][ST], wr[2][SR];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -139,7 +142,7 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
                 for (int r = 0; r < SR; ++r) wr[ks][r] = fw.read(stage, r, ks);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                        // read before the next load overwrites it
-            issue(s + D);
+            issue(s + kVRing);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -183,28 +186,28 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
     });
 }
 
-template <int SR, int ST, int D>
-constexpr uint32_t kRings = kVWaves * D * 2 * (ST + SR) * 1024;
+template <int SR, int ST>
+constexpr uint32_t kRings = kVWaves * kVRing * 2 * (ST + SR) * 1024;
 
-template <typename T, int SR, int ST, int D>
+template <typename T, int SR, int ST>
 __global__ __launch_bounds__(64 * kVWaves) void k_lora_v(const T* x, int64_t ldx, const T* A, int64_t a_stride, const int32_t* ids,
                                                          const float* scale, int n_tok, int n_ad, int n_in, int rank, float* v) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST, D>];
-    ranks_of<T, SR, ST, D, false, float>(lds, blockIdx.z, gridDim.z, x, ldx, A, a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST>];
+    ranks_of<T, SR, ST, false, float>(lds, blockIdx.z, gridDim.z, x, ldx, A, a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
 }
 
 // The gradients' v = A_i x[t] and dv = s_i B_i^T dy[t], one in the even blocks of the third dimension, one in the odd.
-template <typename T, int SR, int ST, int D>
+template <typename T, int SR, int ST>
 __global__ __launch_bounds__(64 * kVWaves) void k_lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy,
                                                             int64_t lddy, const T* B, int64_t b_stride, const int32_t* ids,
                                                             const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
                                                             T* v, T* dv) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST, D>];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST>];
     const int z = blockIdx.z >> 1, n_z = gridDim.z >> 1;
     if (blockIdx.z & 1)
-        ranks_of<T, SR, ST, D, true, T>(lds, z, n_z, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_out, rank, dv);
+        ranks_of<T, SR, ST, true, T>(lds, z, n_z, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_out, rank, dv);
     else
-        ranks_of<T, SR, ST, D, false, T>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
+        ranks_of<T, SR, ST, false, T>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
 }
 
 // Blocks of a tile's adapters: up to 256 tokens each gets its own (16 tokens have 16 at most).  One after another and side
@@ -221,10 +224,10 @@ int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy
     const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST)), split = 2 * split_of<ST>(n_tok);
     // (a tile of 32 ranks for 16: lora_add of 4096 tokens, rank 16, 28.1 us, and 26.8 with a tile of 16)
     if (rank <= 16)
-        hipLaunchKernelGGL((k_lora_v_dv<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+        hipLaunchKernelGGL((k_lora_v_dv<T, 1, ST>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                            a_stride, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv);
     else
-        hipLaunchKernelGGL((k_lora_v_dv<T, 2, ST, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+        hipLaunchKernelGGL((k_lora_v_dv<T, 2, ST>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                            a_stride, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv);
     HIP_TRY(hipGetLastError());
     return 0;
@@ -444,10 +447,10 @@ int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, in
     const uint32_t split = split_of<ST>(n_tok);
     if (n_ad > 0) {
         if (rank <= 16)
-            hipLaunchKernelGGL((k_lora_v<T, 1, ST, ST == 1 ? 4 : 2>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+            hipLaunchKernelGGL((k_lora_v<T, 1, ST>), dim3(tiles, 1, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                                a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
         else
-            hipLaunchKernelGGL((k_lora_v<T, 2, ST, 2>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
+            hipLaunchKernelGGL((k_lora_v<T, 2, ST>), dim3(tiles, (rank + 31) / 32, split), dim3(64 * kVWaves), 0, s, x, ldx, A,
                                a_stride, ids, scale, n_tok, n_ad, n_in, rank, v);
         HIP_TRY(hipGetLastError());
     }
