@@ -57,15 +57,13 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
     return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
-// 16 bytes out, past the caches where PAST.  Results are read again by the next launch at the earliest, and their lines
+// 16 bytes out, past the caches.  Results are read again by the next launch at the earliest, and their lines
 // wait in L2 for a write that then meets the next tile's loads: us with and without, mm 8192 x 8192 x 8192 852 and 908,
 // weights' gradient 4096 x 1024 of 16 x 1024 rows 148 and 160, mm 1024 x 4096 of 16 x 1024 rows 131 and 161, mm_dx 1024 x
 // 2048 of 512 x 40 rows 429 and 439; the whole layer, 2048 tokens over 512 experts of 512 x 2048, 638 and 643.
-template <bool PAST>
 __device__ __forceinline__ void store16(void* to, uint4 v) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
-    else *(u32x4*)to = __builtin_bit_cast(u32x4, v);
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
 }
 
 // Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
@@ -86,7 +84,7 @@ __device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run)
 // Few rows per segment: memory bounds it (gate_up of 512 x 10 rows, 1280 x 2560, 570 us, 5.9 TB/s, matrix unit 17% busy;
 // weights' gradient over 512 x 40 rows, 1024 x 2048, 457 us, 4.6 TB/s written).  Many: the matrix unit and, with short
 // contractions, a tile's results (8192 x 8192 x 8192 795 us, 1385 TFLOP/s; 16 x 2048 rows, 4096 x 1024, 289 us, 950).
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, bool NT>
+template <typename T, int OP, int BP, int BQ, int WP, int WQ>
 __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, uint32_t blocks) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
     constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
@@ -95,7 +93,6 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
     constexpr bool kThroughLds = OP == kDxGlu || (OP != kGateUp && BP >= 128);
-    constexpr bool kPast = NT || OP != kDw || BP == 256;
     static_assert(!kThroughLds || (SQ == 4 && kStage / kWaves >= 4096), "");
     constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
@@ -340,7 +337,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             // of the matrix unit's result has 8 or 16 bytes of a row and its neighbour another row's, each a cache access
             // of its own, and a store past the caches wants whole lines (mm 1024 x 4096, 16 x 2048 rows to places in no
             // order: 304 us, and 327 straight from the registers; weights' gradient over 512 x 40 rows, 1024 x 2048, 591 and
-            // 640 with ordinary stores).  Tiles of 64 rows have too few steps to pay for the barrier (mm of 100 x 47 rows,
+            // 640 with ordinary stores, 520 like this).  Tiles of 64 rows have too few steps to pay for the barrier (mm of 100 x 47 rows,
             // 1152 x 320: 21.0 us, and 19.0 without), but silu's gradient reads (g, u) in whole lines too this way.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                                      // everyone has read the image
@@ -388,7 +385,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                         const int row = it * kRowsPer + l / UNITS, u = l % UNITS, c = col + u * (16 / kBytes);
                         const u32x4 v = *(lds16)(uintptr_t)at(row, u);
                         const int64_t o = row_at(i0 + it * kRowsPer / 16, row & 15);
-                        if (o >= 0 && c < a.nq) store16<kPast>(dst + o + c, __builtin_bit_cast(uint4, v));
+                        if (o >= 0 && c < a.nq) store16(dst + o + c, __builtin_bit_cast(uint4, v));
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -434,8 +431,8 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                         }
                         if (o[it] >= 0 && c < inter) {
                             T* d = (T*)a.out + o[it] + c;
-                            store16<kPast>(d, make_uint4(dg[0].x, dg[0].y, dg[1].x, dg[1].y));
-                            store16<kPast>(d + inter, make_uint4(du[0].x, du[0].y, du[1].x, du[1].y));
+                            store16(d, make_uint4(dg[0].x, dg[0].y, dg[1].x, dg[1].y));
+                            store16(d + inter, make_uint4(du[0].x, du[0].y, du[1].x, du[1].y));
                         }
                     }
                 }
@@ -457,14 +454,14 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     for (int j = 0; j < SQ; ++j) {
                         const int q = q0 + wq * SQ * 16 + j * 16 + kq * 4;
                         if (live && q < a.nq)
-                            store16<kPast>((float*)a.out + row + q, __builtin_bit_cast(uint4, acc[i][j] * s));
+                            store16((float*)a.out + row + q, __builtin_bit_cast(uint4, acc[i][j] * s));
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < SQ; j += 2) {
                         const uint4 v = pair8(round4<T>(acc[i][j] * s), round4<T>(acc[i][j + 1] * s));
                         const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                        if (live && q < a.nq) store16<kPast>((T*)a.out + row + q, v);
+                        if (live && q < a.nq) store16((T*)a.out + row + q, v);
                     }
                 }
                 continue;
@@ -500,12 +497,12 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     for (int j = 0; j < SQ / 2; j += 2) {
                         const int c = q0 + wq * SQ * 8 + j * 16 + pair_col;
                         const uint4 vh = pair8(h[j], h[j + 1]);
-                        if (live && c < inter) store16<kPast>((T*)a.out + (int64_t)r * a.ldo + c, vh);
+                        if (live && c < inter) store16((T*)a.out + (int64_t)r * a.ldo + c, vh);
                         if (a.gu_out) {
                             const uint4 vg = pair8(g2[j], g2[j + 1]), vu = pair8(u2[j], u2[j + 1]);
                             if (live && c < inter) {
-                                store16<kPast>((T*)a.gu_out + (int64_t)r * a.ldgu + c, vg);
-                                store16<kPast>((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c, vu);
+                                store16((T*)a.gu_out + (int64_t)r * a.ldgu + c, vg);
+                                store16((T*)a.gu_out + (int64_t)r * a.ldgu + inter + c, vu);
                             }
                         }
                     }
@@ -516,7 +513,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     const f32x4 zero = {};
                     const uint4 v = pair8(round4<T>(dead ? zero : acc[i][j] * s), round4<T>(dead ? zero : acc[i][j + 1] * s));
                     const int q = q0 + wq * SQ * 16 + j * 16 + pair_col;
-                    if (live && q < a.nq) store16<kPast>((T*)a.out + (int64_t)o * a.ldo + q, v);
+                    if (live && q < a.nq) store16((T*)a.out + (int64_t)o * a.ldo + q, v);
                 }
             }
         }
@@ -525,9 +522,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, bool NT = false>
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
-    tiles_of_block<T, OP, BP, BQ, WP, WQ, NT>(a, blockIdx.x, gridDim.x);
+    tiles_of_block<T, OP, BP, BQ, WP, WQ>(a, blockIdx.x, gridDim.x);
 }
 
 // Two narrow weights' gradients (an adapter's A and B) in one launch: n_a blocks are the first one's.  4096 tokens of 8
@@ -537,7 +534,7 @@ template <typename T>
 __global__ __launch_bounds__(256, 4) void k_grouped_dw_pair(Args a, Args b, uint32_t n_a) {
     const bool first = blockIdx.x < n_a;
     const Args c = first ? a : b;
-    tiles_of_block<T, kDw, 64, 64, 2, 2, false>(c, first ? blockIdx.x : blockIdx.x - n_a, first ? n_a : gridDim.x - n_a);
+    tiles_of_block<T, kDw, 64, 64, 2, 2>(c, first ? blockIdx.x : blockIdx.x - n_a, first ? n_a : gridDim.x - n_a);
 }
 
 // A few rows per segment (decoding): one wave per 16 rows of a segment and 16 weight rows (mm: 16 columns; gate_up: 8
@@ -671,11 +668,11 @@ int64_t blocks_of(Args& a) {
     return most * groups;
 }
 
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS, bool NT = false>
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 int launch_tiles(Args a, hipStream_t s) {
     const int64_t blocks = blocks_of<OP, BP, BQ>(a);
     if (blocks < 0) return -1;
-    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS, NT>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
+    hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -705,7 +702,7 @@ int launch_few(const Args& a, hipStream_t s) {
 }
 
 // The tiles of a weights' gradient.
-enum { kDw256, kDw128, kDw128Past, kDw64 };
+enum { kDw256, kDw128, kDw64 };
 
 int dw_tiles(const Args& a) {
     const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
@@ -713,9 +710,6 @@ int dw_tiles(const Args& a) {
     // with few rows the output's bytes bound it, and smaller tiles have more of them under way (512 x 40 rows, 1024 x
     // 2048: 592 us, and 737 with the large tiles)
     if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return kDw256;
-    // an output larger than the 256 MB of Infinity Cache only pushes the inputs out of it, and its lines are written
-    // back under the next kernel (512 x 40 rows, 1024 x 2048, 2 GB: 520 us, and 591 with ordinary stores)
-    if (per_seg < 512 && (int64_t)a.S.n_seg * a.np * a.nq * (a.out_f32 ? 4 : 2) > 256 << 20) return kDw128Past;
     // an adapter's: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 30 us with them, 21 with 64's).
     // Where not every CU gets one of 128, more and shorter steps of 64 are done sooner too: 2 x 4000 rows, 512 x 1024, 67 and
     // 39 us, 1113 rows, 2272 x 96, 22.9 and 12.9, 8 x 300 rows, 1024 x 512, 12.1 and 11.1
@@ -729,7 +723,6 @@ int launch(const Args& a, hipStream_t s) {
         switch (dw_tiles(a)) {
             case kDw256: return launch_tiles<T, OP, 256, 256, 2, 4, 2>(a, s);
             case kDw128: return launch_tiles<T, OP, 128, 128, 2, 2, 2>(a, s);
-            case kDw128Past: return launch_tiles<T, OP, 128, 128, 2, 2, 2, true>(a, s);
             default: return launch_tiles<T, OP, 64, 64, 2, 2, 4>(a, s);
         }
     } else {
