@@ -15,23 +15,8 @@ struct Segs {
     int n_seg, n_rows, n_slots, fill;
 };
 
-// Two weights' gradients over the same rows, dw [n_seg][n][k] contiguous, as moe_grouped_mm_dw computes them (the caller
-// has checked the arguments): in one launch where both are narrow.  split: 1 dy's rows, 2 x's rows are two rows each, 2 r
-// and 2 r + 1, whose sum they are.
-struct Dw {
-    const void* dy;
-    int64_t lddy;
-    const void* x;
-    int64_t ldx;
-    int n, k;
-    const float* scale;
-    void* dw;
-    int split;
-};
-int dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, int dtype,
-            hipStream_t s);
-
-// dx[rows[r]] = W_u^T (dv[2 rows[r]] + dv[2 rows[r] + 1]), W_u [n][k]; zeros for rows of no segment.
+// dx[rows[r]] = W_u^T (dv[3 rows[r]] + dv[3 rows[r] + 1] + dv[3 rows[r] + 2]), W_u [n][k] of dtype, dv three bf16 parts
+// of a value each (bf16_parts); zeros for rows of no segment.
 int dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
                 int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s);
 
@@ -40,6 +25,17 @@ int dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* 
 __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t nb) {
     const uint32_t per = nb / 8, rem = nb % 8, x = b % 8, i = b / 8;
     return x < rem ? x * (per + 1) + i : rem * (per + 1) + (x - rem) * per + i;
+}
+
+// Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
+// runs of `run` items; more of them even out over whole shares of one XCD each, which read a row once.  us of gradients,
+// dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 435 (of 1024 rows each, dw
+// alone, 173 and 163), 8 adapters of 4096 tokens, all of lora_grad, 62.5 and 76.1; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
+constexpr int kManySegs = 128;
+
+__device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run) {
+    const uint32_t i = b / 8;
+    return b < nb / (8 * run) * (8 * run) ? (i / run * 8 + b % 8) * run + i % run : b;
 }
 
 // Rows and slot of virtual segment v: 0 the rows before the first segment, 1 .. n_seg the segments, and
@@ -143,6 +139,43 @@ __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// An fp32 value as the sum of three bf16 values, each the upper half of what the ones before it leave: all of its 24 bits,
+// over fp32's range (rounded parts would overflow near the largest values).  An infinity or NaN stays in the first part.
+__device__ __forceinline__ void bf16_parts(float v, __bf16 (&p)[3]) {
+    const bool fine = __builtin_fabsf(v) < __builtin_inff();
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        p[k] = fine ? __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16)) : (__bf16)v;
+        v = fine ? v - (float)p[k] : 0.f;
+    }
+}
+
+// c + a b, or (FIRST false) c + b a, where b is a part of such a value.  bf16: as it is.  fp16: a's 11 bits are two bf16
+// values, the upper 8 and the other 3, so no value needs a scale.  (The fp32 matrix unit takes 16 times as long as one
+// 16-bit product, two parts times three 6 times.)
+template <typename T, bool FIRST = true>
+__device__ __forceinline__ f32x4 mfma_parts(uint4 a, uint4 b, f32x4 c) {
+    auto add = [&](uint4 part) { c = FIRST ? mfma<__bf16>(part, b, c) : mfma<__bf16>(b, part, c); };
+    if constexpr (__is_same(T, _Float16)) {
+        typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+        const f16x8 w = __builtin_bit_cast(f16x8, a);
+        u16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = (float)w[e];
+            const uint32_t top = __builtin_bit_cast(uint32_t, f) & 0xFFFF0000u;
+            const float rest = f - __builtin_bit_cast(float, top);
+            hi[e] = (uint16_t)(top >> 16);                                     // (a NaN's quiet bit is among them)
+            lo[e] = (uint16_t)(__builtin_bit_cast(uint32_t, __builtin_fmaxf(rest, -256.f)) >> 16);
+        }
+        add(__builtin_bit_cast(uint4, hi));
+        add(__builtin_bit_cast(uint4, lo));
+    } else {
+        add(a);
+    }
+    return c;
+}
+
 template <typename T>
 __device__ __forceinline__ uint2 round4(f32x4 v) {
     typedef T t4 __attribute__((ext_vector_type(4)));
@@ -155,6 +188,23 @@ __device__ __forceinline__ f32x4 widen4(uint2 w) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const t4 r = __builtin_bit_cast(t4, w);
     return (f32x4){(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
+}
+
+// Two subtiles' 4 adjacent 16-bit results per lane -> 8 adjacent: lanes 16-31 and 48-63 take the second
+// subtile.  Returns the 16 bytes and which subtile (0, 1) and half (0, 1) of its 16 columns they are.
+__device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+    return make_uint4(x[0], y[0], x[1], y[1]);
+}
+
+// 16 bytes out, past the caches.  Results are read again by the next launch at the earliest, and their lines
+// wait in L2 for a write that then meets the next tile's loads: us with and without, mm 8192 x 8192 x 8192 852 and 908,
+// weights' gradient 4096 x 1024 of 16 x 1024 rows 148 and 160, mm 1024 x 4096 of 16 x 1024 rows 131 and 161, mm_dx 1024 x
+// 2048 of 512 x 40 rows 429 and 439; the whole layer, 2048 tokens over 512 experts of 512 x 2048, 638 and 643.
+__device__ __forceinline__ void store16(void* to, uint4 v) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
 }
 
 // What an operand's lanes read where it has nothing: contraction indexes past the end.

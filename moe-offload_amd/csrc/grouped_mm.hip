@@ -27,7 +27,7 @@ namespace {
 
 using namespace gmm;
 
-enum { kMM = 0, kGateUp = 1, kDx = 2, kDxGlu = 3, kDw = 4 };
+enum { kMM = 0, kGateUp = 1, kDx = 2, kDxGlu = 3, kDw = 4, kDxParts = 5 };
 
 struct Args {
     Segs S;
@@ -45,47 +45,17 @@ struct Args {
     int np, nq, nc;              // extents: output columns in p (mm_dw) and q, and the contraction
     int out_f32;
     int span;                    // column tiles per block
-    int fold;                    // mm_dx: contraction indexes from here on use the weights' rows from 0 on again (0: none do)
-    int split;                   // mm_dw: 1 dy, 2 x: each row is two, whose sum it is
+    int fold;                    // kDxParts: the weights' rows, which the contraction goes through three times
 };
-
-// Two subtiles' 4 adjacent 16-bit results per lane -> 8 adjacent: lanes 16-31 and 48-63 take the second
-// subtile.  Returns the 16 bytes and which subtile (0, 1) and half (0, 1) of its 16 columns they are.
-__device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
-    const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
-    const auto y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
-    return make_uint4(x[0], y[0], x[1], y[1]);
-}
-
-// 16 bytes out, past the caches.  Results are read again by the next launch at the earliest, and their lines
-// wait in L2 for a write that then meets the next tile's loads: us with and without, mm 8192 x 8192 x 8192 852 and 908,
-// weights' gradient 4096 x 1024 of 16 x 1024 rows 148 and 160, mm 1024 x 4096 of 16 x 1024 rows 131 and 161, mm_dx 1024 x
-// 2048 of 512 x 40 rows 429 and 439; the whole layer, 2048 tokens over 512 experts of 512 x 2048, 638 and 643.
-__device__ __forceinline__ void store16(void* to, uint4 v) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
-}
-
-// Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
-// runs of `run` items; more of them even out over whole shares of one XCD each, which read a row once.  us of gradients,
-// dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 435 (of 1024 rows each, dw
-// alone, 173 and 163), 8 adapters of 4096 tokens (in one part) 57.9 and 60.6; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
-constexpr int kManySegs = 128;
-
-__device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run) {
-    const uint32_t i = b / 8;
-    return b < nb / (8 * run) * (8 * run) ? (i / run * 8 + b % 8) * run + i % run : b;
-}
 
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers while the step before it is multiplied, the
-// next tile's first step during the last of this one: two images, one barrier per step.  (Four images, three steps under
-// way, let half as many blocks live on a CU: adapters' gradients of 4096 tokens, rank 64, 36 us, and 26 with two.)
+// next tile's first step during the last of this one: two images, one barrier per step.
 // Few rows per segment: memory bounds it (gate_up of 512 x 10 rows, 1280 x 2560, 570 us, 5.9 TB/s, matrix unit 17% busy;
 // weights' gradient over 512 x 40 rows, 1024 x 2048, 457 us, 4.6 TB/s written).  Many: the matrix unit and, with short
 // contractions, a tile's results (8192 x 8192 x 8192 795 us, 1385 TFLOP/s; 16 x 2048 rows, 4096 x 1024, 289 us, 950).
-template <typename T, int OP, int BP, int BQ, int WP, int WQ>
-__device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, uint32_t blocks) {
+template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
+__global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
     constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
     constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;        // 1 KiB each
@@ -105,12 +75,12 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     if constexpr (OP == kDw) {
         const int tp = (a.np + BP - 1) / BP;
         const uint32_t run = ((uint32_t)groups * tp + 7) / 8;
-        const uint32_t item = a.S.n_seg < kManySegs ? dealt(block, blocks, run) : xcd_order(block, blocks);
+        const uint32_t item = a.S.n_seg < kManySegs ? dealt(blockIdx.x, gridDim.x, run) : xcd_order(blockIdx.x, gridDim.x);
         seg = item / (groups * tp);
         p0 = (int)(item / groups % tp) * BP;
         tile = (int)(item % groups) * a.span;
         seg_rows(a.S, seg + 1, r0, r1, slot);
-        nc = (r1 - r0) << (a.split ? 1 : 0);
+        nc = r1 - r0;
     } else {
         Tile at;
         __shared__ uint32_t scratch[kWaves + 3];
@@ -139,13 +109,12 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     // The rows of x or dy, the same in every step.  mm_dw: numbers of the rows [c0, c1) of dy and x, -1 for one that is
     // missing on either side: zeros on the one would still meet an infinity on the other.
     int rp[kLoadsP];
-    const int halves = OP == kDw && a.split ? 1 : 0;                           // two contraction indexes per row
     auto hold_rows = [&](int c0, int c1) {
         static_assert(OP != kDw || BP == BQ, "both operands' loads of a step have the same rows");
-        for (int c = (c0 >> halves) + t; c < (c1 + halves) >> halves; c += 64 * kWaves) {
+        for (int c = c0 + t; c < c1; c += 64 * kWaves) {
             const int v = a.row_p ? a.row_p[r0 + c] : r0 + c, x = a.row_q ? a.row_q[r0 + c] : r0 + c;
             const bool both = v >= 0 && v < a.n_p && x >= 0 && x < a.n_q;
-            idx[c - (c0 >> halves)] = make_int2(both ? v : -1, both ? x : -1);
+            idx[c - c0] = make_int2(both ? v : -1, both ? x : -1);
         }
     };
     if constexpr (OP != kDw) {
@@ -157,9 +126,8 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             rp[j] = v >= 0 && v < a.n_p ? v : 0;
         }
     }
-    // mm_dw of more rows than are held: tile by tile, what `held` indexes [part0, part1) need at a time
-    const int held = kIdx << halves;
-    const bool parts = OP == kDw && nc > held;
+    // mm_dw of more rows than are held: tile by tile, kIdx of them [part0, part1) at a time
+    const bool parts = OP == kDw && nc > kIdx;
     int part0 = 0, part1 = nc;
     int load_tile = tile, load_c = 0;                                          // the step that is loaded next
     auto place = [&]() {
@@ -169,11 +137,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) {
                 const int row = along_row(j, kLoadsP, kUnitsP), col = (lane % kUnitsP ^ 2 * turn<BP>(row)) * 8;
-                const int c = load_c + row, odd = c & halves;
-                int2 v = idx[any && c < part1 ? (c - part0) >> halves : 0];
+                const int c = load_c + row;
+                const int2 v = idx[any && c < part1 ? c - part0 : 0];
                 const bool ok = any && c < part1 && v.x >= 0;
-                if (a.split & 1) v.x = 2 * v.x + odd;
-                if (a.split & 2) v.y = 2 * v.y + odd;
                 pp[j] = ok ? P + v.x * a.ldp + (p0 + col < a.np ? p0 + col : 0) : zero;
                 qp[j] = ok ? Q + v.y * a.ldq + (q0 + col < a.nq ? q0 + col : 0) : zero;
             }
@@ -185,7 +151,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             for (int j = 0; j < kLoadsQ; ++j) {
                 if constexpr (kAlongQ) {
                     const int row = along_row(j, kLoadsQ, kUnitsQ), q = q0 + (lane % kUnitsQ ^ 2 * turn<BQ>(row)) * 8;
-                    const int c = load_c + row, w = OP == kDx && a.fold && c >= a.fold ? c - a.fold : c;
+                    const int c = load_c + row, w = OP != kDxParts || c < a.fold ? c : c < 2 * a.fold ? c - a.fold : c - 2 * a.fold;
                     qp[j] = any && c < nc ? Q + (int64_t)w * a.nq + (q < a.nq ? q : 0) : zero;
                 } else {
                     const int row = (wv * kLoadsQ + j) * 8 + (lane >> 3);
@@ -206,7 +172,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     };
     auto advance = [&]() {
         load_c += kBC;
-        if (OP != kDw && !(OP == kDx && a.fold) && load_tile < end && load_c + kBC <= nc) {    // wave-uniform; past the end all stay at zero
+        if (OP != kDw && OP != kDxParts && load_tile < end && load_c + kBC <= nc) {    // wave-uniform; past the end all stay at zero
 #pragma unroll
             for (int j = 0; j < kLoadsP; ++j) pp[j] += kBC;
 #pragma unroll
@@ -254,6 +220,10 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
             }
         }
     }
+    auto multiply = [](uint4 q, uint4 p, f32x4 c) {
+        if constexpr (OP == kDxParts) return mfma_parts<T>(q, p, c);
+        else return mfma<T>(q, p, c);
+    };
     uint32_t stage = 0;
     bool landed = false;                                                       // the next step's loads have been waited for
     auto start = [&](int c0) {
@@ -277,9 +247,9 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
         f32x4 acc[SP][SQ] = {};
 #pragma unroll 1
         for (int c0 = 0; c0 < nc; c0 += kBC) {
-            if (OP == kDw && parts && c0 % held == 0) {
+            if (OP == kDw && parts && c0 % kIdx == 0) {
                 part0 = c0;
-                part1 = c0 + held < nc ? c0 + held : nc;
+                part1 = c0 + kIdx < nc ? c0 + kIdx : nc;
                 __syncthreads();                                               // the rows held so far are all placed
                 hold_rows(part0, part1);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the part before's loads past its end
@@ -315,7 +285,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
                     for (int e = (i - kFrom) * kEach; e < (i - kFrom + 1) * kEach; ++e) vp[1][e] = fp.read(stage, e, 1);
                 }
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply(vq[0][j], vp[0][i], acc[i][j]);
 #pragma unroll
                 for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
                 __builtin_amdgcn_sched_barrier(0);
@@ -324,7 +294,7 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
 #pragma unroll
             for (int i = 0; i < SP; ++i)
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply(vq[1][j], vp[1][i], acc[i][j]);
             stage = fill;
         }
         // The next tile's first step is waited for before the stores: in the loop the wait would take them in.
@@ -522,21 +492,6 @@ __device__ __forceinline__ void tiles_of_block(const Args& a, uint32_t block, ui
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
-__global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
-    tiles_of_block<T, OP, BP, BQ, WP, WQ>(a, blockIdx.x, gridDim.x);
-}
-
-// Two narrow weights' gradients (an adapter's A and B) in one launch: n_a blocks are the first one's.  4096 tokens of 8
-// adapters, rank 64, 2560 and 2048 wide: 37 us for rows in two parts, 21 for single ones (those as two launches 22 + 18 with
-// four images, 26 together with two and whole segments per XCD); waits for memory half of the time.
-template <typename T>
-__global__ __launch_bounds__(256, 4) void k_grouped_dw_pair(Args a, Args b, uint32_t n_a) {
-    const bool first = blockIdx.x < n_a;
-    const Args c = first ? a : b;
-    tiles_of_block<T, kDw, 64, 64, 2, 2>(c, first ? blockIdx.x : blockIdx.x - n_a, first ? n_a : gridDim.x - n_a);
-}
-
 // A few rows per segment (decoding): one wave per 16 rows of a segment and 16 weight rows (mm: 16 columns; gate_up: 8
 // gate rows and the 8 up rows of the same outputs), which it streams through an LDS ring of its own, kFewRing steps of
 // 64 ahead, without a barrier.  Loads that put the weights straight into the matrix unit's layout would take 16 bytes
@@ -646,7 +601,7 @@ int64_t blocks_of(Args& a) {
     int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
     if constexpr (OP == kDw) {
         rows = most = (int64_t)a.S.n_seg * ((a.np + BP - 1) / BP);
-        steps = ((int64_t)a.S.n_rows << (a.split ? 1 : 0)) / a.S.n_seg / kBC + 1;
+        steps = (int64_t)a.S.n_rows / a.S.n_seg / kBC + 1;
     } else {
         rows = row_tiles(a, BP);
         most = (int64_t)a.S.n_rows / BP + (a.S.n_seg + 2 < a.S.n_rows ? a.S.n_seg + 2 : a.S.n_rows);
@@ -750,23 +705,6 @@ int launch(const Args& a, hipStream_t s) {
     }
 }
 
-template <typename T>
-int launch_dw_pair(Args a, Args b, hipStream_t s) {
-    if (dw_tiles(a) != kDw64 || dw_tiles(b) != kDw64) {
-        const int rc = launch<T, kDw>(a, s);
-        return rc ? rc : launch<T, kDw>(b, s);
-    }
-    const int64_t n_a = blocks_of<kDw, 64, 64>(a), n_b = blocks_of<kDw, 64, 64>(b);
-    if (n_a < 0 || n_b < 0) return -1;
-    if (n_a + n_b > 0x7FFFFFFF) {
-        moe_set_error("grouped product: %lld tiles are more than one launch takes", (long long)(n_a + n_b));
-        return -1;
-    }
-    hipLaunchKernelGGL((k_grouped_dw_pair<T>), dim3((uint32_t)(n_a + n_b)), dim3(256), 0, s, a, b, (uint32_t)n_a);
-    HIP_TRY(hipGetLastError());
-    return 0;
-}
-
 template <int OP>
 int launch_typed(const Args& a, int dtype, hipStream_t s) {
     return dtype ? launch<__bf16, OP>(a, s) : launch<_Float16, OP>(a, s);
@@ -806,25 +744,13 @@ bool bad_segs(const char* who, const Segs& S, int n, int k, int dtype, const voi
 
 }  // namespace
 
-int gmm::dw_pair(const Dw& a, const Dw& b, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, int dtype,
-                 hipStream_t s) {
-    auto args = [&](const Dw& d) {
-        Args r = {};
-        r.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 0};
-        r.p = d.dy, r.q = d.x, r.out = d.dw, r.row_p = r.row_q = rows, r.scale = d.scale;
-        r.ldp = d.lddy, r.ldq = d.ldx, r.ldo = (int64_t)d.n * d.k, r.n_p = r.n_q = n_rows, r.np = d.n, r.nq = d.k, r.split = d.split;
-        return r;
-    };
-    return dtype ? launch_dw_pair<__bf16>(args(a), args(b), s) : launch_dw_pair<_Float16>(args(a), args(b), s);
-}
-
 int gmm::dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
                      int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s) {
     Args a = {};
     a.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 1};
     a.p = dv, a.q = w, a.out = dx, a.row_p = a.row_out = rows;
-    a.ldp = 2 * (int64_t)n, a.ldq = w_stride, a.ldo = lddx, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = 2 * n, a.fold = n;
-    return launch_typed<kDx>(a, dtype, s);
+    a.ldp = 3 * (int64_t)n, a.ldq = w_stride, a.ldo = lddx, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = 3 * n, a.fold = n;
+    return launch_typed<kDxParts>(a, dtype, s);
 }
 
 extern "C" {

@@ -3,19 +3,19 @@
 // Token t belongs to a request with adapter i = ids[t]:   out[t] = base[t] + s_i B_i (A_i x[t]),
 // A_i [rank][n_in], B_i [n_out][rank]; an id outside the adapters leaves out[t] = base[t].  base is the
 // shared projection's output (a grouped product, the 2-bit experts' rows, a router's logits) and may be
-// out itself.  v = A_i x stays in fp32 between the two products, and out is rounded once.
+// out itself.  v = A_i x is written and read in fp32 between the two products, and out is rounded once.
 //
 // Two launches.  k_lora_v multiplies 16 or 32 tokens by up to 32 ranks per block, the contraction dealt to its waves.
-// k_lora_out multiplies v by B's rows and adds base; v keeps its fp32 bits on the 16-bit matrix unit as a sum of
-// 16-bit parts.  Both take their operands through LDS in loads of whole lines.  The tokens of a tile may have
-// different adapters: the tile is multiplied by each adapter that occurs in it and every token keeps its own adapter's
-// result.  In a batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to blocks
-// of their own.
+// k_lora_out multiplies v by B's rows and adds base; on the 16-bit matrix unit v is a sum of 16-bit parts: all of its bits
+// for bf16, 22 of them for fp16 (split8).  Both take their operands through LDS in loads of whole lines.  The tokens of a
+// tile may have different adapters: the tile is multiplied by each adapter that occurs in it and every token keeps its own
+// adapter's result.  In a batch of prompts that is one adapter nearly always; for few tokens the adapters of a tile go to
+// blocks of their own.
 //
-// The gradients: dv[t] = s_i B_i^T dy[t] beside v in one launch, then the grouped products over the tokens sorted by
-// adapter, dx = A_i^T dv, dA_i = sum dv x^T, dB_i = s_i sum dy v^T.  v and dv are two 16-bit parts each there, along the
-// contraction: rounded to 16 bits they alone would put the gradients 1.4 times as far from the exact ones as their own
-// rounding does.
+// The gradients: dv[t] = s_i B_i^T dy[t] beside v in one launch, then over the tokens sorted by adapter dx = A_i^T dv (a
+// grouped product), and dA_i = sum dv x^T, dB_i = s_i sum dy v^T in one launch.  v and dv are three bf16 parts each there,
+// which are all of their fp32 bits whatever their magnitude: two rounded parts would lose bits, and two fp16 parts also the
+// values past 65504 and, step by step, those below 2^-14, where a gradient's are.
 #include <hip/hip_bf16.h>
 
 #include <algorithm>
@@ -58,14 +58,13 @@ __device__ __forceinline__ void each_adapter(const int (&id)[ST], const bool (&h
     }
 }
 
-constexpr int kVWaves = 4;      // (8, one block per CU: lora_add of 64 tokens 11.2 us, with 4 10.4; lora_grad of 4096 72.9 and 70.1)
+constexpr int kVWaves = 4;      // (8, one block per CU: lora_add of 64 tokens 8.9 us, with 4 8.7; lora_grad of 4096 64.7 and 62.5)
 constexpr int kVRing = 2;
 
 // v[t][j] = s_i W_i[j] x[t] for 16 ST tokens (blockIdx.x) and 16 SR ranks (blockIdx.y), where W_i[j] is row j of A_i, or
 // (ALONG) column j of B_i [nc][rank].  Each wave multiplies every fourth step of 64 along the contraction, through an LDS
 // ring of its own (two steps of the tokens' and the ranks' operands); the waves' sums are added in their order.  O: fp32, or
-// T where v is an operand of a product next: then row 2 t is v[t] rounded and row 2 t + 1 what that leaves, together 16
-// (bf16) or 22 bits.  4096 tokens, rank 64, 2560: 13 us for
+// bf16 where v is an operand of a product next: rows 3 t .. 3 t + 2 are the parts of v[t].  4096 tokens, rank 64, 2560: 13 us for
 // 24 MB, a block per 32 tokens and 32 ranks, whose waves' few steps (10) are mostly the loads' way; v and dv for the
 // gradients, 2560 and 2048, 20 us for 40 MB.
 template <typename T, int SR, int ST, bool ALONG, typename O>
@@ -170,15 +169,17 @@ __device__ __forceinline__ void ranks_of(uint8_t* lds, int z, int n_z, const T* 
                 if (wv % ST == m && mine[m] && j < rank) {
                     if constexpr (sizeof(O) == 4) *(f32x4*)(v + t[m] * rank + j) = sum;
                     else {
-                        // (opaque: the product above, rounded to fp32 or straight to fp16, must be one value for both parts)
-                        asm volatile("" : "+v"(sum));
-                        const uint2 hi = round4<T>(sum);
-                        const f32x4 rest = sum - widen4<T>(hi);
-                        f32x4 lo;                                              // an infinity or NaN stays in the first part
+                        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                        bf16x4 part[3];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) lo[e] = __builtin_fabsf(rest[e]) < __builtin_inff() ? rest[e] : 0.f;
-                        *(uint2*)(v + 2 * t[m] * rank + j) = hi;
-                        *(uint2*)(v + (2 * t[m] + 1) * rank + j) = round4<T>(lo);
+                        for (int e = 0; e < 4; ++e) {
+                            __bf16 p[3];
+                            bf16_parts(sum[e], p);
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) part[k][e] = p[k];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) *(bf16x4*)(v + (3 * t[m] + k) * rank + j) = part[k];
                     }
                 }
         }
@@ -201,13 +202,13 @@ template <typename T, int SR, int ST>
 __global__ __launch_bounds__(64 * kVWaves) void k_lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy,
                                                             int64_t lddy, const T* B, int64_t b_stride, const int32_t* ids,
                                                             const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
-                                                            T* v, T* dv) {
+                                                            __bf16* v, __bf16* dv) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kRings<SR, ST>];
     const int z = blockIdx.z >> 1, n_z = gridDim.z >> 1;
     if (blockIdx.z & 1)
-        ranks_of<T, SR, ST, true, T>(lds, z, n_z, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_out, rank, dv);
+        ranks_of<T, SR, ST, true, __bf16>(lds, z, n_z, dy, lddy, B, b_stride, ids, scale, n_tok, n_ad, n_out, rank, dv);
     else
-        ranks_of<T, SR, ST, false, T>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
+        ranks_of<T, SR, ST, false, __bf16>(lds, z, n_z, x, ldx, A, a_stride, ids, nullptr, n_tok, n_ad, n_in, rank, v);
 }
 
 // Blocks of a tile's adapters: up to 256 tokens each gets its own (16 tokens have 16 at most).  One after another and side
@@ -220,7 +221,8 @@ uint32_t split_of(int n_tok) {
 
 template <typename T, int ST>
 int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy, int64_t lddy, const T* B, int64_t b_stride,
-              const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, T* v, T* dv, hipStream_t s) {
+              const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, __bf16* v,
+              __bf16* dv, hipStream_t s) {
     const uint32_t tiles = (uint32_t)(((int64_t)n_tok + 16 * ST - 1) / (16 * ST)), split = 2 * split_of<ST>(n_tok);
     // (a tile of 32 ranks for 16: lora_add of 4096 tokens, rank 16, 28.1 us, and 26.8 with a tile of 16)
     if (rank <= 16)
@@ -235,23 +237,22 @@ int lora_v_dv(const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* dy
 
 // Tokens of a tile: 32 use each load of an adapter twice, 16 are more blocks.  us of lora_add with 32 and 16, rank 64, 2560 x
 // 2560: 4096 tokens 33 and 36 with inputs from memory, 34 and 29 with all in cache; 1000 tokens 24 and 21; lora_grad of
-// 4096 tokens, 2560 x 2048, v and dv in 16 bits, 60.6 and 64.5.
+// 4096 tokens, 2560 x 2048, 62.5 and 64.1.
 constexpr int kFewTokens = 1024;
 
 template <typename T>
 int lora_v_dv_typed(const void* x, int64_t ldx, const void* A, int64_t a_stride, const void* dy, int64_t lddy, const void* B,
                     int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank,
-                    void* v, void* dv, hipStream_t s) {
+                    __bf16* v, __bf16* dv, hipStream_t s) {
     auto f = n_tok <= kFewTokens ? lora_v_dv<T, 1> : lora_v_dv<T, 2>;
     return f((const T*)x, ldx, (const T*)A, a_stride, (const T*)dy, lddy, (const T*)B, b_stride, ids, scale, n_tok, n_ad, n_in, n_out,
-             rank, (T*)v, (T*)dv, s);
+             rank, v, dv, s);
 }
 
-// fp32 values as sums of values of T that keep their bits.  bf16 has fp32's range: three parts, each the upper half of
-// what the ones before it leave, are the value itself (rounded parts would overflow near the largest values).  fp16 values
-// are first scaled by a power of two per token, so that the largest is just below 2^15, and two parts of 11 bits each are
-// 22 bits, or 2^-40 of the token's largest value.  (The fp32 matrix unit takes 8 times as long and wants B widened.)  An
-// infinity or NaN stays in the first part.
+// fp32 values as sums of values of T.  bf16: three parts, which are the value itself.  fp16 values are first scaled by a
+// power of two per token, so that the largest is just below 2^15, and two parts of 11 bits each are 22 bits, or 2^-40 of the
+// token's largest value: what is lost is a tenth of a percent of half a step of out's type.  An infinity or NaN stays in the
+// first part.
 template <typename T>
 constexpr int kParts = __is_same(T, _Float16) ? 2 : 3;
 
@@ -261,13 +262,14 @@ __device__ __forceinline__ void split8(const float* v, uint4 (&part)[kParts<T>])
     t8 p[kParts<T>];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        float rest = v[e];
-        const bool fine = __builtin_fabsf(rest) < __builtin_inff();
+        if constexpr (kParts<T> == 3) {
+            __bf16 q[3];
+            bf16_parts(v[e], q);
 #pragma unroll
-        for (int k = 0; k < kParts<T>; ++k) {
-            if (kParts<T> == 3 && fine) p[k][e] = __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16));
-            else p[k][e] = (T)rest;
-            rest = fine ? rest - (float)p[k][e] : 0.f;
+            for (int k = 0; k < 3; ++k) p[k][e] = q[k];
+        } else {
+            p[0][e] = (T)v[e];
+            p[1][e] = (T)(__builtin_fabsf(v[e]) < __builtin_inff() ? v[e] - (float)p[0][e] : 0.f);
         }
     }
 #pragma unroll
@@ -439,6 +441,170 @@ __global__ __launch_bounds__(256, 2) void k_lora_out(const T* base, int64_t ldb,
     });
 }
 
+// da_i = sum over adapter i's tokens of dv x^T, or (DA false) db_i = s_i sum of dy v^T; order[r] is the r-th token in the
+// order of the adapters, `parts` holds dv or v.
+struct DwArgs {
+    const void* wide;                 // x or dy
+    int64_t ld;
+    const __bf16* parts;
+    int n_wide;
+    int span;                         // tiles per block, side by side along the wide operand
+    const float* scale;
+    void* out;
+};
+
+// A block computes `span` tiles of 64 x 64 results of one adapter.  A step of 64 tokens is one image of the wide operand and
+// one of each part, straight from memory to LDS while the step before it is multiplied (the next tile's first during the
+// last of this one): a wide row is loaded once and multiplied by all three parts.  Four waves, 32 x 32 results each, multiply
+// the step's first 32 tokens and four its others, and their sums are added at the end: the longest segment's steps one after
+// another are what bounds it (4096 tokens of 8 adapters, rank 64, 2560 and 2048 wide: 21 us in bf16, 32 in fp16, whose two
+// parts are made in registers; four waves and steps of 32 tokens 25 and 38; without the loads or without the products hardly
+// less).
+constexpr int kDwTile = 64, kDwWaves = 8, kDwStep = 8 * kDwWaves, kDwHeld = 1024;     // kDwHeld: tokens whose numbers are in LDS
+constexpr uint32_t kDwImage = kDwStep * kDwTile * 2, kDwStage = 4 * kDwImage;
+
+template <typename T, bool DA>
+__device__ __forceinline__ void dw_tiles(uint8_t* lds, const DwArgs& a, const int32_t* __restrict__ order,
+                                         const int32_t* __restrict__ seg_start, int n_tok, int n_ad, int rank, uint32_t block,
+                                         uint32_t blocks) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)lds;
+    const int tiles = (a.n_wide + kDwTile - 1) / kDwTile, groups = (tiles + a.span - 1) / a.span, rt = (rank + kDwTile - 1) / kDwTile;
+    const uint32_t run = ((uint32_t)groups * rt + 7) / 8;
+    const uint32_t item = n_ad < kManySegs ? dealt(block, blocks, run) : xcd_order(block, blocks);
+    const int seg = item / (groups * rt), j0 = (int)(item / groups % rt) * kDwTile, tile0 = (int)(item % groups) * a.span;
+    const int end = tile0 + a.span < tiles ? tile0 + a.span : tiles;
+    const Segs S{seg_start, nullptr, n_ad, n_tok, n_ad, 0};
+    int r0, r1, slot;
+    seg_rows(S, seg + 1, r0, r1, slot);
+    const int steps = (r1 - r0 + kDwStep - 1) / kDwStep;
+
+    // A wave loads 8 tokens of each image, a lane 16 bytes of its token's row; tokens past the end read zeros.
+    const int row = wv * 8 + (lane >> 3), col = ((lane & 7) ^ 2 * turn<kDwTile>(row)) * 8;
+    const T* zero = (const T*)&g_zero16;
+    asm("" : "+s"(zero));
+    const int64_t part_col = j0 + col < rank ? j0 + col : 0;                   // (columns past the end are not stored)
+    int* held = (int*)(lds + 2 * kDwStage);
+    auto load = [&](int t, int tile, uint32_t stage) {
+        const int c = tile * kDwTile + col;
+        const uint32_t to = lds0 + stage + wv * 1024;
+        load_to_lds(t >= 0 ? (const T*)a.wide + t * a.ld + (c < a.n_wide ? c : 0) : zero, to);
+        const __bf16* p = a.parts + (int64_t)t * 3 * rank + part_col;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) load_to_lds(t >= 0 ? (const void*)(p + k * rank) : zero, to + (k + 1) * kDwImage);
+    };
+    const int w0 = (wv & 1) * 32, p0 = (wv >> 1 & 1) * 32, half = wv >> 2;     // this wave's results in the tile, and tokens
+    Frags<true, kDwTile, 2> fw, fp;
+    fw.init(lds0, w0, lane);
+    fp.init(lds0 + kDwImage, p0, lane);
+    const float s = a.scale ? a.scale[seg] : 1.0f;
+    const int np = DA ? rank : a.n_wide, nq = DA ? a.n_wide : rank;
+    int next = 0, next_tile = tile0, chunk = -1;                               // the step that is loaded next; tokens held
+    uint32_t stage = 0;
+    auto advance = [&]() {
+        const int c = next * kDwStep;
+        if (c / kDwHeld != chunk) {
+            chunk = c / kDwHeld;
+            __syncthreads();                                                   // everyone has read the numbers held so far
+            for (int i = threadIdx.x; i < kDwHeld; i += 64 * kDwWaves) held[i] = r0 + c + i < r1 ? order[r0 + c + i] : -1;
+            __syncthreads();
+        }
+        load(held[c % kDwHeld + row], next_tile, stage);
+        if (++next == steps) next = 0, ++next_tile;
+    };
+    if (steps > 0) advance();
+#pragma unroll 1
+    for (int tile = tile0; tile < end; ++tile) {
+        f32x4 acc[2][2] = {};                                                  // [rows of out][along them]
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
+            // everyone's
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const uint32_t at = stage;
+            stage = kDwStage - stage;
+            if (next_tile < end) advance();
+            uint4 w[2], p[3][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i] = fw.read(at, i, half);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) p[k][i] = fp.read(at + k * kDwImage, i, half);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (DA) acc[i][j] = mfma_parts<T>(w[j], p[k][i], acc[i][j]);
+                        else acc[i][j] = mfma_parts<T, false>(w[i], p[k][j], acc[i][j]);
+                    }
+        }
+        if (r1 - r0 > kDwStep / 2) {
+            // through the image just multiplied
+            typedef __attribute__((address_space(3))) f32x4* ptr;
+            const uint32_t mine = lds0 + (kDwStage - stage) + ((wv & 3) * 256 + lane) * 16;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                                      // everyone has read it
+            asm volatile("" ::: "memory");
+            if (half) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *(ptr)(uintptr_t)(mine + i * 1024) = acc[i >> 1][i & 1];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (!half) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] += *(ptr)(uintptr_t)(mine + i * 1024);
+            }
+        }
+        if (half) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = (DA ? j0 + p0 : tile * kDwTile + w0) + i * 16 + n;
+            const int c = (DA ? tile * kDwTile + w0 : j0 + p0) + (kq & 1) * 16 + (kq >> 1) * 8;
+            const uint4 v = pair8(round4<T>(acc[i][0] * s), round4<T>(acc[i][1] * s));
+            if (r < np && c < nq) store16((T*)a.out + ((int64_t)seg * np + r) * nq + c, v);
+        }
+    }
+}
+
+// Both in one launch, the first n_a blocks da's.
+template <typename T>
+__global__ __launch_bounds__(64 * kDwWaves, 4) void k_lora_dw(DwArgs a, DwArgs b, const int32_t* order, const int32_t* seg_start, int n_tok,
+                                                    int n_ad, int rank, uint32_t n_a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kDwStage + kDwHeld * 4];
+    if (blockIdx.x < n_a) dw_tiles<T, true>(lds, a, order, seg_start, n_tok, n_ad, rank, blockIdx.x, n_a);
+    else dw_tiles<T, false>(lds, b, order, seg_start, n_tok, n_ad, rank, blockIdx.x - n_a, gridDim.x - n_a);
+}
+
+// Sets the tiles per block and returns the blocks.  Tiles of short segments share a block's start while that leaves 1024
+// blocks.  us of the gradients of 4096 tokens at 1, 2, 4, 8 and 16 tiles: 512 adapters, rank 16, 2048 x 2048 (one step) 413,
+// -, 344, 332, 325; 64 adapters, rank 128, 2560 x 2560 (two steps expected) 143, 137, 147, 153, -.
+int64_t dw_blocks(DwArgs& a, int n_tok, int n_ad, int rank) {
+    const int64_t tiles = (a.n_wide + kDwTile - 1) / kDwTile, rows = (int64_t)n_ad * ((rank + kDwTile - 1) / kDwTile);
+    const int64_t steps = (int64_t)n_tok / n_ad / kDwStep + 1;
+    a.span = (int)std::max<int64_t>(1, std::min<int64_t>({steps == 1 ? 16 : 4 / steps, rows * tiles / 1024, tiles}));
+    return rows * ((tiles + a.span - 1) / a.span);
+}
+
+template <typename T>
+int lora_dw(DwArgs a, DwArgs b, const int32_t* order, const int32_t* seg_start, int n_tok, int n_ad, int rank, hipStream_t s) {
+    const int64_t n_a = dw_blocks(a, n_tok, n_ad, rank), n_b = dw_blocks(b, n_tok, n_ad, rank);
+    if (n_a + n_b > 0x7FFFFFFF) {
+        moe_set_error("lora_grad: %lld tiles are more than one launch takes", (long long)(n_a + n_b));
+        return -1;
+    }
+    hipLaunchKernelGGL((k_lora_dw<T>), dim3((uint32_t)(n_a + n_b)), dim3(64 * kDwWaves), 0, s, a, b, order, seg_start, n_tok, n_ad, rank,
+                       (uint32_t)n_a);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
 template <typename T, int ST>
 int lora_add(const T* base, int64_t ldb, const T* x, int64_t ldx, const T* A, int64_t a_stride, const T* B, int64_t b_stride,
              const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out, int rank, float* v, T* out,
@@ -529,7 +695,7 @@ extern "C" int moe_lora_add(const void* base, int64_t ld_base, const void* x, in
 
 extern "C" uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank) {
     if (n_tok < 0 || n_ad < 1 || rank <= 0) return 0;
-    return 2 * up16((uint64_t)n_tok * rank * 4) + 2 * up16((uint64_t)n_tok * 4) + up16((uint64_t)(n_ad + 1) * 4) +
+    return 2 * up16((uint64_t)n_tok * rank * 6) + 2 * up16((uint64_t)n_tok * 4) + up16((uint64_t)(n_ad + 1) * 4) +
            moe_expert_plan_workspace_bytes(n_tok, n_ad);
 }
 
@@ -554,20 +720,21 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
         p += up16(bytes);
         return q;
     };
-    void* v = take((uint64_t)n_tok * rank * 4);
-    void* dv = take((uint64_t)n_tok * rank * 4);
+    __bf16* v = (__bf16*)take((uint64_t)n_tok * rank * 6);
+    __bf16* dv = (__bf16*)take((uint64_t)n_tok * rank * 6);
     int32_t* order = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* same = (int32_t*)take((uint64_t)n_tok * 4);
     int32_t* seg = (int32_t*)take((uint64_t)(n_ad + 1) * 4);
     auto v_dv = dtype ? lora_v_dv_typed<__bf16> : lora_v_dv_typed<_Float16>;
+    auto dw = dtype ? lora_dw<__bf16> : lora_dw<_Float16>;
     // the tokens sorted by adapter: a token's row number everywhere but in seg is its own.  Without tokens da and db are the
     // products over empty segments.
     if (moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
         (n_tok > 0 && v_dv(x, ldx, a, a_stride, dy, lddy, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv,
                            (hipStream_t)stream)) ||
         (n_tok > 0 && gmm::dx_of_parts(dv, order, n_tok, seg, n_ad, a, a_stride, rank, n_in, dx, lddx, dtype, (hipStream_t)stream)) ||
-        gmm::dw_pair(gmm::Dw{dv, rank, x, ldx, rank, n_in, nullptr, da, 1}, gmm::Dw{dy, lddy, v, rank, n_out, rank, scale, db, 2}, order,
-                     n_tok, seg, n_ad, dtype, (hipStream_t)stream))
+        dw(DwArgs{x, ldx, dv, n_in, 1, nullptr, da}, DwArgs{dy, lddy, v, n_out, 1, scale, db}, order, seg, n_tok, n_ad, rank,
+           (hipStream_t)stream))
         return -1;
     return 0;
 }

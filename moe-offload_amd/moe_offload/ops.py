@@ -549,9 +549,8 @@ def lora_grad(dy, x, a, b, ids, scale=None, workspace=None):
     """The gradients of lora_add in x (the adapter's part; base's is dy itself), a and b: (dx, da, db).
 
     With the tokens sorted by adapter: v = a x, dv = scale b^T dy, dx = a^T dv, da = sum dv x^T, db = scale
-    sum dy v^T.  v and dv are kept as sums of two values of the inputs' type.  Tokens
-    without an adapter get dx = 0, adapters without tokens da = db = 0.  At most 1024 adapters.  workspace:
-    scratch of moe_lora_grad_workspace_bytes.
+    sum dy v^T.  v and dv are fp32 between the products.  Tokens without an adapter get dx = 0, adapters
+    without tokens da = db = 0.  At most 1024 adapters.  workspace: scratch of moe_lora_grad_workspace_bytes.
     """
     who = "lora_grad"
     dev = _one_gpu(who, "dy x a b ids scale workspace", dy, x, a, b, ids, scale, workspace)
