@@ -202,7 +202,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     Frags<kAlongQ, BQ, SQ> fq;
     fp.init(lds0, wp * SP * 16, lane);
     fq.init(lds0 + kStageP, wq * SQ * 16, lane);
-    const float s = a.scale && slot >= 0 ? a.scale[slot] : 1.0f;
+    const float s = a.scale && slot >= 0 && (OP != kDw || nc > 0) ? a.scale[slot] : 1.0f;   // (dw of no rows: zeros, whatever the scale)
     // 16-byte stores: lane (n, kq) of a pair of subtiles holds columns 8 (kq / 2) .. + 7 of subtile kq % 2
     const int pair_col = (kq & 1) * 16 + (kq >> 1) * 8;
     // the output row of this lane's row in each subtile (-1: none); bit i of dead: its results are zeros

@@ -497,7 +497,7 @@ __device__ __forceinline__ void dw_tiles(uint8_t* lds, const DwArgs& a, const in
     Frags<true, kDwTile, 2> fw, fp;
     fw.init(lds0, w0, lane);
     fp.init(lds0 + kDwImage, p0, lane);
-    const float s = a.scale ? a.scale[seg] : 1.0f;
+    const float s = a.scale && steps > 0 ? a.scale[seg] : 1.0f;               // (no tokens: zeros, whatever the scale)
     const int np = DA ? rank : a.n_wide, nq = DA ? a.n_wide : rank;
     int next = 0, next_tile = tile0, chunk = -1;                               // the step that is loaded next; tokens held
     uint32_t stage = 0;

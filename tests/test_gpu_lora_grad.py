@@ -123,3 +123,16 @@ def test_several_tiles_of_a_block(dtype):
     for tokens, n_ad in ((600, 200), (4000, 100)):
         args = make(dtype, tokens, n_ad, 16, 1608, 904)
         check(ops.lora_grad(*args[:-1], scale=args[-1]), *args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_an_idle_adapter_s_scale_is_not_used(dtype, bad):
+    from moe_offload import ops
+    dy, x, a, b, ids, scale = make(dtype, 70, 4, 16, 72, 136)
+    ids[ids == 2] = 1
+    scale[2] = bad
+    dx, da, db = ops.lora_grad(dy, x, a, b, ids, scale=scale)
+    assert not bool(da[2].any()) and not bool(db[2].any())
+    scale[2] = 1.0
+    check((dx, da, db), dy, x, a, b, ids, scale)
