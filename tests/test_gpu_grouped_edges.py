@@ -29,3 +29,34 @@ def test_weights_gradient_of_no_rows_is_zero_whatever_the_scale(dtype, bad, n, k
         dw = ops.grouped_mm_dw(dy, x, seg, scale=scale, dtype=out)
         assert not bool(dw[0].any()) and not bool(dw[2].any())
         assert torch.equal(dw, ops.grouped_mm_dw(dy, x, seg, scale=good, dtype=out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,k", [(0, 2), (0, 1), (5, 0)])
+def test_layer_without_tokens(dtype, tokens, k):
+    """A step whose batch routes nothing here runs back too: no rows of dx (or zeros without experts), zero weights' gradients."""
+    from moe_offload import dense
+    x, ids = rnd((tokens, 64), dtype, 1).requires_grad_(), torch.zeros((tokens, k), dtype=torch.int32, device=DEV)
+    wgu, wd = rnd((3, 48, 64), dtype, 2).requires_grad_(), rnd((3, 64, 24), dtype, 3).requires_grad_()
+    y = dense.switch_glu(x, ids, wgu, wd)
+    assert y.shape == (tokens, k, 64) and y.dtype == dtype
+    y.sum().backward()
+    assert x.grad.shape == (tokens, 64) and not bool(x.grad.any())
+    assert wgu.grad.shape == wgu.shape and not bool(wgu.grad.any()) and wd.grad.shape == wd.shape and not bool(wd.grad.any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wanted", range(1, 8))
+def test_each_subset_of_the_layer_s_gradients(dtype, wanted):
+    from moe_offload import dense
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(-1, 4, (37, 3), generator=g, dtype=torch.int32).to(DEV)
+    data = rnd((37, 72), dtype, 1), rnd((4, 80, 72), dtype, 2, 0.1), rnd((4, 72, 40), dtype, 3, 0.1)
+    dy = rnd((37, 3, 72), dtype, 4)
+
+    def grads(mask):
+        leaves = [t.clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate(data)]
+        dense.switch_glu(leaves[0], ids, leaves[1], leaves[2]).backward(dy)
+        return [t.grad for t in leaves]
+    for i, (got, full) in enumerate(zip(grads(wanted), grads(7))):
+        assert (got is None) if not wanted >> i & 1 else torch.equal(got, full)
