@@ -79,15 +79,20 @@ class _LoraAdd(torch.autograd.Function):
         _refuse_capture("lora_add")
         x, a, b, ids, scale = ctx.saved_tensors
         dx = da = db = None
-        if any(ctx.needs_input_grad[1:4]):
+        if a.shape[0] == 0:
+            dx, da, db = torch.zeros_like(x), torch.empty_like(a), torch.empty_like(b)
+        elif any(ctx.needs_input_grad[1:4]):
             dx, da, db = ops.lora_grad(dy.contiguous(), x, a, b, ids, scale=scale)
         return dy, dx, da, db, None, None
 
 
 def lora_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
              scale: torch.Tensor | None = None) -> torch.Tensor:
-    """ops.lora_add, differentiable in base, x, a and b (the scale is a constant); at most 1024 adapters."""
+    """ops.lora_add, differentiable in base, x, a and b (the scale is a constant); at most 1024 adapters where a gradient
+    in x, a or b is wanted."""
     if scale is not None and scale.requires_grad:
         raise ValueError("lora_add: scale has no gradient here")
+    if a.dim() == 3 and a.shape[0] > 1024 and torch.is_grad_enabled() and any(t.requires_grad for t in (x, a, b)):
+        raise ValueError(f"lora_add: {a.shape[0]} adapters (gradients for up to 1024)")
     _refuse_capture("lora_add")
     return _LoraAdd.apply(base, x, a, b, ids, scale)

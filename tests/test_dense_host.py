@@ -160,3 +160,16 @@ def test_sizes_past_the_library_s_integers_are_refused():
                      (lambda t: ops._index("op", "ids", t), torch.empty(big, dtype=torch.int32, device="meta"))):
         with pytest.raises(ValueError, match="2\\^30"):
             check(t)
+
+
+def test_adapters_past_the_gradients_limit_are_refused_where_the_call_is_made():
+    base, x, ids = torch.zeros((2, 8)), torch.zeros((2, 8)), torch.zeros(2, dtype=torch.int32)
+    a, b = torch.zeros((1025, 8, 8)), torch.zeros((1025, 8, 8))
+    for i in range(3):
+        args = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, a, b))]
+        with pytest.raises(ValueError, match="1024"):
+            dense.lora_add(base, *args, ids)
+        with torch.no_grad(), pytest.raises(ValueError, match="not on a GPU"):       # forward alone has no such limit
+            dense.lora_add(base, *args, ids)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        dense.lora_add(base.requires_grad_(), x, a, b, ids)

@@ -136,3 +136,19 @@ def test_an_idle_adapter_s_scale_is_not_used(dtype, bad):
     assert not bool(da[2].any()) and not bool(db[2].any())
     scale[2] = 1.0
     check((dx, da, db), dy, x, a, b, ids, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_autograd_without_adapters_and_with_many(dtype):
+    from moe_offload import dense
+    base, x = rnd((5, 24), dtype, 1).requires_grad_(), rnd((5, 16), dtype, 2).requires_grad_()
+    a, b = rnd((0, 8, 16), dtype, 3).requires_grad_(), rnd((0, 24, 8), dtype, 4).requires_grad_()
+    ids = torch.zeros(5, dtype=torch.int32, device=DEV)
+    out = dense.lora_add(base, x, a, b, ids)
+    dy = rnd((5, 24), dtype, 5)
+    out.backward(dy)
+    assert torch.equal(out, base) and torch.equal(base.grad, dy) and not bool(x.grad.any()) and a.grad.shape == a.shape and b.grad.shape == b.shape
+    a, b = rnd((1025, 8, 16), dtype, 3), rnd((1025, 24, 8), dtype, 4)
+    base.grad = None
+    dense.lora_add(base, x.detach(), a, b, ids + 1024).backward(dy)               # base's own gradient has no such limit
+    assert torch.equal(base.grad, dy)
