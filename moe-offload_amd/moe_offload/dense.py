@@ -21,6 +21,12 @@ def _refuse_capture(who: str) -> None:
         raise RuntimeError(f"{who}: autograd is not captured into a graph; call the operators in moe_offload.ops")
 
 
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """A gradient as the operators take it: autograd may hand down a view that starts anywhere."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _SwitchGlu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, w_gate_up, w_down):
@@ -38,7 +44,7 @@ class _SwitchGlu(torch.autograd.Function):
         _refuse_capture("switch_glu")
         x, w_gate_up, w_down, row_token, row_out, seg_start, gu, h = ctx.saved_tensors
         n_tok, k, hidden = dy.shape
-        dy = dy.reshape(n_tok * k, hidden).contiguous()
+        dy = _operand(dy.reshape(n_tok * k, hidden))
         dx = dw_gate_up = dw_down = None
         if ctx.needs_input_grad[3]:
             dw_down = ops.grouped_mm_dw(dy, h, seg_start, row_dy=row_out)
@@ -82,7 +88,7 @@ class _LoraAdd(torch.autograd.Function):
         if a.shape[0] == 0:
             dx, da, db = torch.zeros_like(x), torch.empty_like(a), torch.empty_like(b)
         elif any(ctx.needs_input_grad[1:4]):
-            dx, da, db = ops.lora_grad(dy.contiguous(), x, a, b, ids, scale=scale)
+            dx, da, db = ops.lora_grad(_operand(dy), x, a, b, ids, scale=scale)
         return dy, dx, da, db, None, None
 
 

@@ -60,3 +60,25 @@ def test_each_subset_of_the_layer_s_gradients(dtype, wanted):
         return [t.grad for t in leaves]
     for i, (got, full) in enumerate(zip(grads(wanted), grads(7))):
         assert (got is None) if not wanted >> i & 1 else torch.equal(got, full)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ahead", [3, 8])
+def test_incoming_gradients_that_start_anywhere(dtype, ahead):
+    """Behind a concatenation autograd hands down a view of the whole gradient, contiguous and aligned to an element only."""
+    from moe_offload import dense
+    ids = i32([[0, 2], [1, 0], [2, 2], [-1, 1], [0, 1]])
+    leaves = [t.requires_grad_() for t in (rnd((5, 72), dtype, 1), rnd((3, 48, 72), dtype, 2), rnd((3, 72, 24), dtype, 3), rnd((5, 40), dtype, 4),
+                                           rnd((2, 8, 72), dtype, 5), rnd((2, 40, 8), dtype, 6))]
+    x, wgu, wd, base, a, b = leaves
+    w = rnd((ahead + 5 * 2 * 72 + 5 * 40,), dtype, 7)
+
+    def grads(shift):
+        y, z = dense.switch_glu(x, ids, wgu, wd), dense.lora_add(base, x, a, b, ids[:, 0].contiguous())
+        if shift:
+            out = torch.cat([torch.zeros(ahead, dtype=dtype, device=DEV), y.reshape(-1), z.reshape(-1)])
+            return torch.autograd.grad((out * w).sum(), leaves)
+        n = ahead + y.numel()
+        return torch.autograd.grad([y, z], leaves, [w[ahead:n].view(y.shape).clone(), w[n:].view(z.shape).clone()])
+    for got, want in zip(grads(True), grads(False)):
+        assert torch.equal(got, want)
