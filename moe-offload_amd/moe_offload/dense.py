@@ -3,8 +3,8 @@
     plan rows by expert -> gate and up projections, silu(g) * u -> down projections, one row per (token, k)
 
 and back, each product and each gradient one launch of libmoe_offload.so.  What the forward pass keeps is the
-row plan, (g, u) and h.  The score-weighted sum over a token's experts is the caller's (torch operations or
-ops.pair_combine), so the scores' gradient is too.
+row plan, (g, u) and h.  The score-weighted sum over a token's experts is the caller's, in torch operations, and
+so is the scores' gradient (ops.pair_combine has none, and takes fp16 rows only).
 
 A graph capture of a forward or backward pass through autograd is refused: an eager graph of the same leaves
 that is still alive would end the process.  Programs that capture call ops.grouped_* and ops.lora_* themselves.

@@ -161,9 +161,20 @@ def q2_grouped_switch_glu(x, row_token, seg_start, pool, hidden, inter, group=64
 
 
 def pair_combine(y, scores, residual=None, out=None):
-    """out fp32 [n_tok, hidden] = residual + sum_j scores[t, j] * y[t*k + j]."""
+    """out fp32 [n_tok, hidden] = residual + sum_j scores[t, j] * y[t*k + j].
+
+    y (a row per (token, k)), scores [n_tok, k] and residual [n_tok, hidden] are fp16 and contiguous; no gradient.
+    """
     n_tok, k = scores.shape
     hidden = y.shape[-1]
+    for name, t, dtype, n in (("y", y, torch.float16, n_tok * k * hidden), ("scores", scores, torch.float16, n_tok * k),
+                              ("residual", residual, torch.float16, n_tok * hidden), ("out", out, torch.float32, n_tok * hidden)):
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"pair_combine: {name} is {t.dtype}, not {dtype}")
+        if not t.is_contiguous() or t.numel() < n:
+            raise ValueError(f"pair_combine: {name} of shape {tuple(t.shape)} must be contiguous with {n} values for {n_tok} tokens")
     out = out if out is not None else torch.empty((n_tok, hidden), dtype=torch.float32, device=y.device)
     rc = _lib.lib().moe_pair_combine(_p(y), _p(scores), _p(residual), n_tok, k, hidden, _p(out), _stream())
     _lib.check(rc, "moe_pair_combine")

@@ -173,3 +173,17 @@ def test_adapters_past_the_gradients_limit_are_refused_where_the_call_is_made():
             dense.lora_add(base, *args, ids)
     with pytest.raises(ValueError, match="not on a GPU"):
         dense.lora_add(base.requires_grad_(), x, a, b, ids)
+
+
+def test_pair_combine_takes_contiguous_fp16():
+    """Other types, and rows that do not follow each other, would be read as if they were."""
+    y, scores, res, out = (torch.zeros((6, 16), dtype=torch.float16), torch.zeros((3, 2), dtype=torch.float16),
+                           torch.zeros((3, 16), dtype=torch.float16), torch.zeros((3, 16)))
+    for args in ((y.bfloat16(), scores), (y, scores.float()), (y, scores.bfloat16(), res), (y, scores, res.float()),
+                 (y, scores, res, out.half())):
+        with pytest.raises(TypeError, match="pair_combine"):
+            ops.pair_combine(*args)
+    for args in ((torch.zeros((6, 32), dtype=torch.float16)[:, :16], scores), (y[:5], scores), (y, torch.zeros((2, 3), dtype=torch.float16).T),
+                 (y, scores, res[:2]), (y, scores, res, out[:2])):
+        with pytest.raises(ValueError, match="pair_combine"):
+            ops.pair_combine(*args)
