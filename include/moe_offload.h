@@ -280,7 +280,8 @@ int moe_pair_combine(const void* y, const void* scores, const void* residual, in
  * row plan they take, and low-rank adapters.  Pointers are device memory, matrices and workspaces 16-byte
  * aligned; ld* are elements from row to row and *_stride elements from matrix to matrix, both multiples
  * of 8, as all row lengths are; within a matrix rows follow each other.  Row numbers are 32-bit, sizes
- * up to 2^30, offsets 64-bit.  Outputs must not overlap inputs (but for moe_lora_add's out == base).
+ * up to 2^30, offsets 64-bit; a call whose tiles are more than one launch of 2^32 threads takes (from about
+ * 2^35 results on) is refused before anything is queued.  Outputs must not overlap inputs (but for moe_lora_add's out == base).
  * Nothing is allocated, kept between calls or synchronised.  Sums are fp32, rounded once. */
 
 /* The rows of a batch sorted by expert, as prefill.resident_plan (loader.py:583-591) makes them on the
@@ -326,7 +327,7 @@ int moe_grouped_mm_dw(const void* dy, int64_t lddy, int n_dy, const int32_t* row
 /* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scale[i] B_i (A_i x[t]),
  * i = ids[t]; A_i [rank][n_in] = a + i * a_stride, B_i [n_out][rank] = b + i * b_stride, scale fp32 per
  * adapter or null.  An id outside 0 .. n_ad - 1 gives out[t] = base[t].  out may be base.  rank: a
- * multiple of 8 up to 256; n_out < 2^23.  workspace: moe_lora_workspace_bytes bytes, any contents, one per call in
+ * multiple of 8 up to 256; n_out < 2^23; n_tok up to 2^29 - 32.  workspace: moe_lora_workspace_bytes bytes, any contents, one per call in
  * flight. */
 uint64_t moe_lora_workspace_bytes(int n_tok, int rank);
 int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, const void* a, int64_t a_stride,
@@ -335,7 +336,7 @@ int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, 
 /* The gradients of moe_lora_add, given dy [n_tok][n_out] (base's own is dy):  dx[t] = A_i^T dv[t] (zeros without
  * an adapter), da_i [rank][n_in] = sum of dv[t] x[t]^T and db_i [n_out][rank] = scale[i] * sum of dy[t] v[t]^T over
  * adapter i's tokens (zeros without any), v = A_i x[t], dv = scale[i] * B_i^T dy[t], both in fp32 between the
- * products.  n_tok up to 2^29.  da and
+ * products.  da and
  * db are contiguous; n_ad in 1..1024.  workspace: moe_lora_grad_workspace_bytes bytes, 16-byte aligned, any
  * contents, one per call in flight. */
 uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank);

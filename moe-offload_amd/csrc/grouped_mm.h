@@ -7,6 +7,7 @@ namespace gmm {
 
 constexpr int kMaxSeg = 1024;
 constexpr int kMaxSide = 1 << 30;     // rows, columns and contractions: sums of two of them and a tile stay below 2^31
+constexpr int64_t kMaxThreads = 0xFFFFFFFF;                   // of a launch, in a dimension
 
 // Rows r of segment s: seg_start[s] .. seg_start[s + 1] - 1, weights of slot seg_slot[s] (s where null).
 struct Segs {
@@ -16,9 +17,9 @@ struct Segs {
 };
 
 // dx[rows[r]] = W_u^T (dv[3 rows[r]] + dv[3 rows[r] + 1] + dv[3 rows[r] + 2]), W_u [n][k] of dtype, dv three bf16 parts
-// of a value each (bf16_parts); zeros for rows of no segment.
+// of a value each (bf16_parts); zeros for rows of no segment.  dry: launches nothing, -1 if one launch does not take it.
 int dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
-                int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s);
+                int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, bool dry, hipStream_t s);
 
 // Block index -> work item, keeping consecutive items on one XCD (blocks are dealt to the 8 XCDs round
 // robin), so that the blocks of one row tile find its rows in that XCD's L2.

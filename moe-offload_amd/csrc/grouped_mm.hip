@@ -46,6 +46,7 @@ struct Args {
     int out_f32;
     int span;                    // column tiles per block
     int fold;                    // kDxParts: the weights' rows, which the contraction goes through three times
+    int dry;                     // only whether one launch takes the call
 };
 
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
@@ -595,7 +596,7 @@ int64_t row_tiles(const Args& a, int bp) {
 }
 
 // Sets the column tiles per block and returns the blocks, or -1.
-template <int OP, int BP, int BQ>
+template <int OP, int BP, int BQ, int THREADS>
 int64_t blocks_of(Args& a) {
     const int qstep = OP == kGateUp ? BQ / 2 : BQ, tiles = (a.nq + qstep - 1) / qstep;
     int64_t rows, most, steps;                                // row tiles expected and at most, steps per tile
@@ -616,7 +617,7 @@ int64_t blocks_of(Args& a) {
     const int64_t span = std::min(target / steps, rows * tiles / 1024);
     a.span = (int)std::max<int64_t>(1, std::min<int64_t>(span, tiles));
     const int64_t groups = (tiles + a.span - 1) / a.span;
-    if (most > 0x7FFFFFFF / groups) {
+    if (most > kMaxThreads / THREADS / groups) {
         moe_set_error("grouped product: %lld x %lld tiles are more than one launch takes", (long long)most, (long long)groups);
         return -1;
     }
@@ -625,8 +626,9 @@ int64_t blocks_of(Args& a) {
 
 template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 int launch_tiles(Args a, hipStream_t s) {
-    const int64_t blocks = blocks_of<OP, BP, BQ>(a);
+    const int64_t blocks = blocks_of<OP, BP, BQ, 64 * WP * WQ>(a);
     if (blocks < 0) return -1;
+    if (a.dry) return 0;
     hipLaunchKernelGGL((k_grouped<T, OP, BP, BQ, WP, WQ, BLOCKS>), dim3((uint32_t)blocks), dim3(64 * WP * WQ), 0, s, a);
     HIP_TRY(hipGetLastError());
     return 0;
@@ -745,8 +747,9 @@ bool bad_segs(const char* who, const Segs& S, int n, int k, int dtype, const voi
 }  // namespace
 
 int gmm::dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int32_t* seg_start, int n_seg, const void* w,
-                     int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, hipStream_t s) {
+                     int64_t w_stride, int n, int k, void* dx, int64_t lddx, int dtype, bool dry, hipStream_t s) {
     Args a = {};
+    a.dry = dry;
     a.S = Segs{seg_start, nullptr, n_seg, n_rows, n_seg, 1};
     a.p = dv, a.q = w, a.out = dx, a.row_p = a.row_out = rows;
     a.ldp = 3 * (int64_t)n, a.ldq = w_stride, a.ldo = lddx, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = 3 * n, a.fold = n;

@@ -593,12 +593,13 @@ int64_t dw_blocks(DwArgs& a, int n_tok, int n_ad, int rank) {
 }
 
 template <typename T>
-int lora_dw(DwArgs a, DwArgs b, const int32_t* order, const int32_t* seg_start, int n_tok, int n_ad, int rank, hipStream_t s) {
+int lora_dw(DwArgs a, DwArgs b, const int32_t* order, const int32_t* seg_start, int n_tok, int n_ad, int rank, bool dry, hipStream_t s) {
     const int64_t n_a = dw_blocks(a, n_tok, n_ad, rank), n_b = dw_blocks(b, n_tok, n_ad, rank);
-    if (n_a + n_b > 0x7FFFFFFF) {
+    if (n_a + n_b > kMaxThreads / (64 * kDwWaves)) {
         moe_set_error("lora_grad: %lld tiles are more than one launch takes", (long long)(n_a + n_b));
         return -1;
     }
+    if (dry) return 0;
     hipLaunchKernelGGL((k_lora_dw<T>), dim3((uint32_t)(n_a + n_b)), dim3(64 * kDwWaves), 0, s, a, b, order, seg_start, n_tok, n_ad, rank,
                        (uint32_t)n_a);
     HIP_TRY(hipGetLastError());
@@ -636,15 +637,16 @@ int lora_add_typed(const void* base, int64_t ldb, const void* x, int64_t ldx, co
 }
 
 constexpr int kMaxOut = (1 << 23) - 8;                        // the second grid dimension, 512 columns each, and its loads
+constexpr int kMaxTok = (int)(kMaxThreads / 256) * 32;        // blocks of 256 threads for 32 tokens each
 
 // The shapes and strides that both entry points take; base or dy is [n_tok][n_out].
 bool bad_shapes(const char* who, int dtype, int n_tok, int n_ad, int n_in, int n_out, int rank, int64_t ldx, int64_t ldy,
                 int64_t a_stride, int64_t b_stride) {
     if ((dtype != 0 && dtype != 1) || n_tok < 0 || n_ad < 0 || n_in <= 0 || n_out <= 0 || rank <= 0 || n_in % 8 ||
-        n_out % 8 || rank % 8 || rank > 256 || n_out > kMaxOut || n_in > kMaxSide || n_tok > kMaxSide) {
-        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^23, n_in and "
-                      "n_tok <= 2^30)",
-                      who, dtype, n_tok, n_ad, n_in, n_out, rank);
+        n_out % 8 || rank % 8 || rank > 256 || n_out > kMaxOut || n_in > kMaxSide || n_tok > kMaxTok) {
+        moe_set_error("%s: dtype=%d n_tok=%d n_ad=%d n_in=%d n_out=%d rank=%d (multiples of 8, rank <= 256, n_out < 2^23, n_in <= "
+                      "2^30, n_tok <= %d)",
+                      who, dtype, n_tok, n_ad, n_in, n_out, rank, kMaxTok);
         return true;
     }
     if (ldx % 8 || ldy % 8 || a_stride % 8 || b_stride % 8 || (n_tok > 1 && (ldx < n_in || ldy < n_out)) ||
@@ -705,8 +707,8 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
                              void* db, void* stream) {
     const char* who = "lora_grad";
     if (bad_shapes(who, dtype, n_tok, n_ad, n_in, n_out, rank, ldx, lddy, a_stride, b_stride)) return -1;
-    if (n_ad < 1 || n_ad > gmm::kMaxSeg || n_tok > gmm::kMaxSide / 2 || lddx % 8 || (n_tok > 1 && lddx < n_in)) {
-        moe_set_error("%s: n_ad=%d (1..%d) n_tok=%d (up to 2^29) lddx=%lld", who, n_ad, gmm::kMaxSeg, n_tok, (long long)lddx);
+    if (n_ad < 1 || n_ad > gmm::kMaxSeg || lddx % 8 || (n_tok > 1 && lddx < n_in)) {
+        moe_set_error("%s: n_ad=%d (1..%d) lddx=%lld", who, n_ad, gmm::kMaxSeg, (long long)lddx);
         return -1;
     }
     if (n_tok > 0 && !ids) {
@@ -727,14 +729,18 @@ extern "C" int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_
     int32_t* seg = (int32_t*)take((uint64_t)(n_ad + 1) * 4);
     auto v_dv = dtype ? lora_v_dv_typed<__bf16> : lora_v_dv_typed<_Float16>;
     auto dw = dtype ? lora_dw<__bf16> : lora_dw<_Float16>;
+    const auto dx_dw = [&](bool dry) {
+        return (n_tok > 0 && gmm::dx_of_parts(dv, order, n_tok, seg, n_ad, a, a_stride, rank, n_in, dx, lddx, dtype, dry,
+                                              (hipStream_t)stream)) ||
+               dw(DwArgs{x, ldx, dv, n_in, 1, nullptr, da}, DwArgs{dy, lddy, v, n_out, 1, scale, db}, order, seg, n_tok, n_ad, rank,
+                  dry, (hipStream_t)stream);
+    };
     // the tokens sorted by adapter: a token's row number everywhere but in seg is its own.  Without tokens da and db are the
     // products over empty segments.
-    if (moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
+    if (dx_dw(true) || moe_expert_plan(ids, n_tok, 1, n_ad, p, same, order, seg, stream) ||
         (n_tok > 0 && v_dv(x, ldx, a, a_stride, dy, lddy, b, b_stride, ids, scale, n_tok, n_ad, n_in, n_out, rank, v, dv,
                            (hipStream_t)stream)) ||
-        (n_tok > 0 && gmm::dx_of_parts(dv, order, n_tok, seg, n_ad, a, a_stride, rank, n_in, dx, lddx, dtype, (hipStream_t)stream)) ||
-        dw(DwArgs{x, ldx, dv, n_in, 1, nullptr, da}, DwArgs{dy, lddy, v, n_out, 1, scale, db}, order, seg, n_tok, n_ad, rank,
-           (hipStream_t)stream))
+        dx_dw(false))
         return -1;
     return 0;
 }

@@ -187,3 +187,23 @@ def test_pair_combine_takes_contiguous_fp16():
                  (y, scores, res[:2]), (y, scores, res, out[:2])):
         with pytest.raises(ValueError, match="pair_combine"):
             ops.pair_combine(*args)
+
+
+TOKENS = 32 * (2 ** 24 - 1)                                    # 2^24 - 1 blocks of 256 threads
+
+
+@pytest.mark.parametrize("name,good,change", [
+    ("moe_grouped_mm", MM, dict(n_rows=2 ** 30, n_x=2 ** 30, n_y=2 ** 30, n=8192, ldy=8192, k=4096, ldx=4096, w_stride=8192 * 4096)),
+    ("moe_grouped_gate_up", UP, dict(n_rows=2 ** 30, n_x=2 ** 30, inter=4096, ldh=4096, hidden=4096, ldx=4096, w_stride=8192 * 4096)),
+    ("moe_grouped_mm_dx", DX, dict(n_rows=2 ** 30, n_dy=2 ** 30, n_dx=2 ** 30, n=4096, lddy=4096, k=8192, lddx=8192, w_stride=8192 * 4096)),
+    ("moe_grouped_mm_dw", DW, dict(n_seg=1024, n=2 ** 16, lddy=2 ** 16, k=2 ** 16, ldx=2 ** 16, dw_stride=2 ** 32)),
+    ("moe_lora_add", LORA, dict(n_tok=TOKENS + 1)),
+    ("moe_lora_grad", GRAD, dict(n_tok=TOKENS + 1)),
+    ("moe_lora_grad", GRAD, dict(n_tok=2 ** 28, n_in=8192, ldx=8192, lddx=8192, rank=256, a_stride=2 ** 21, b_stride=2 ** 14)),
+    ("moe_lora_grad", GRAD, dict(n_ad=1024, n_in=2 ** 30, ldx=2 ** 30, lddx=2 ** 30, a_stride=2 ** 33)),
+])
+def test_calls_that_one_launch_does_not_take_are_refused_before_any(name, good, change):
+    """gridDim.x * blockDim.x stays below 2^32; without a GPU, a call that gets as far as a launch says something else."""
+    assert set(change) <= set(good)
+    msg = refused(name, *{**good, **change}.values())
+    assert "more than one launch takes" in msg or "n_tok" in msg and str(TOKENS) in msg, msg
