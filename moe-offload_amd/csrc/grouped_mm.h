@@ -212,9 +212,10 @@ __device__ __forceinline__ void store16(void* to, uint4 v) {
 static __device__ uint4 g_zero16;
 
 // 16 bytes per lane from global memory straight into LDS: lane l's land at lds + 16 l (lds wave-uniform).
-// The issuing code waits for them itself (vmcnt), and no register receives data.
+// The issuing code waits for them itself (vmcnt), and no register receives data.  m0, where the instruction finds the LDS
+// address, is an operand, so that the compiler knows what it holds.
 __device__ __forceinline__ void load_to_lds(const void* g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(g) : "memory");
 }
 
 constexpr int kBC = 64;                                       // contraction indexes per step
