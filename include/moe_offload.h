@@ -313,7 +313,8 @@ int moe_grouped_gate_up(const void* x, int64_t ldx, int n_x, const int32_t* row_
 /* dx[row_out[r]] = scale[u] W_u^T dy[row_in[r]], W_u [n][k]: the gradient of moe_grouped_mm in x, with
  * row_in and row_out in each other's place (a row of x that several rows read gets their sum from the
  * caller).  gu != null: W_u's input was moe_grouped_gate_up's h (k = inter) and dx [..][2 * k] receives
- * the gradient of (g, u) instead; gu has sorted row r at r. */
+ * the gradient of (g, u) instead; gu has sorted row r at r.  A g that is infinite there (past the type's
+ * range) has its limit's gradient, an infinite u an infinite or NaN one. */
 int moe_grouped_mm_dx(const void* dy, int64_t lddy, int n_dy, const int32_t* row_in, const int32_t* seg_start,
                       const int32_t* seg_slot, int n_seg, int n_rows, const void* w, int64_t w_stride, int n_slots, int n,
                       int k, const float* scale, const void* gu, int64_t ldgu, void* dx, int64_t lddx, int n_dx,

@@ -393,9 +393,11 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
                             f32x4 vg, vu;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float sg = 1.0f / (1.0f + __expf(-g[e]));
-                                vg[e] = dh[e] * u[e] * sg * (1.0f + g[e] * (1.0f - sg));
-                                vu[e] = dh[e] * g[e] * sg;
+                                // sig is 0 or 1 from -200 and 200 on; an infinity (g past fp16's range) would meet a zero
+                                const float low = g[e] < -200.f ? -200.f : g[e], both = low > 200.f ? 200.f : low;
+                                const float sg = 1.0f / (1.0f + __expf(-low));
+                                vg[e] = dh[e] * u[e] * sg * (1.0f + both * (1.0f - sg));
+                                vu[e] = dh[e] * low * sg;
                             }
                             dg[b] = round4<T>(vg);
                             du[b] = round4<T>(vu);

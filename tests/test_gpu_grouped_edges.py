@@ -82,3 +82,29 @@ def test_incoming_gradients_that_start_anywhere(dtype, ahead):
         return torch.autograd.grad([y, z], leaves, [w[ahead:n].view(y.shape).clone(), w[n:].view(z.shape).clone()])
     for got, want in zip(grads(True), grads(False)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [3, 200, 700])
+def test_gradient_of_gates_past_fp16(rows):
+    """g = -70000 or 70000 is finite in the forward pass' fp32 and infinite in the (g, u) it keeps: silu' is 0 or 1 there."""
+    from moe_offload import ops
+    dt = torch.float16
+    x = torch.zeros((rows, 8), dtype=dt, device=DEV)
+    x[:, 0], x[:, 1] = 700.0, 1.0
+    x[1::3, 0] = -700.0
+    x[2::3, 0] = 0.5
+    w = torch.zeros((1, 128, 8), dtype=dt, device=DEV)
+    w[0, :64, 0], w[0, 64:, 1] = 100.0, 2.0 ** -7
+    seg = i32([0, rows])
+    gu = torch.empty((rows, 128), dtype=dt, device=DEV)
+    h = ops.grouped_gate_up(x, None, seg, w, gu_out=gu)
+    assert bool(h.isfinite().all()) and bool(gu[0::3, :64].isposinf().all()) and bool(gu[1::3, :64].isneginf().all())
+    wd = torch.zeros((1, 8, 64), dtype=dt, device=DEV)
+    wd[0, 0] = 1.0
+    dy = torch.zeros((rows, 8), dtype=dt, device=DEV)
+    dy[:, 0] = 0.25
+    d = ops.grouped_mm_dx(dy, seg, wd, gu=gu).float()
+    assert bool((d[0::3, :64] == 2.0 ** -9).all()) and bool(d[0::3, 64:].isposinf().all())          # dh u, dh g
+    assert not bool(d[1::3].any())
+    sg = torch.sigmoid(torch.tensor(50.0))
+    assert torch.equal(d[2::3, :64], torch.full_like(d[2::3, :64], 2.0 ** -9)) and bool((d[2::3, 64:] == 12.5).all()) and float(sg) == 1.0
