@@ -96,7 +96,7 @@ def test_one_large_token_beside_small_ones():
 # dx's tiles are chosen by the call's sizes: few tokens 64 x 64 and 64 x 128, then 128 x 128, then 256 x 256
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens,n_ad,rank,n_in,n_out", [
-    (900, 20, 40, 2568, 136), (4096, 8, 64, 2560, 520), (4096, 32, 136, 2568, 264), (6000, 3, 256, 1288, 72), (5000, 300, 24, 328, 2056)])
+    (900, 20, 40, 2568, 136), (1200, 30, 24, 2568, 72), (4096, 8, 64, 2560, 520), (4096, 32, 136, 2568, 264), (6000, 3, 256, 1288, 72), (5000, 300, 24, 328, 2056)])
 def test_larger_batches(dtype, tokens, n_ad, rank, n_in, n_out):
     from moe_offload import ops
     args = make(dtype, tokens, n_ad, rank, n_in, n_out)
