@@ -152,3 +152,40 @@ def test_autograd_without_adapters_and_with_many(dtype):
     base.grad = None
     dense.lora_add(base, x.detach(), a, b, ids + 1024).backward(dy)               # base's own gradient has no such limit
     assert torch.equal(base.grad, dy)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_long_adapter_among_many(dtype):
+    """The sizes promise short segments, so a block has many tiles; one segment is longer than the row numbers it holds."""
+    from moe_offload import ops
+    dy, x, a, b, ids, scale = make(dtype, 3000, 500, 16, 1608, 904)
+    ids[torch.arange(3000, device=DEV) % 5 != 0] = 123
+    check(ops.lora_grad(dy, x, a, b, ids, scale=scale), dy, x, a, b, ids, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [40, 1500])
+def test_infinities_and_nan_stay_in_their_token_and_adapter(dtype, tokens):
+    from moe_offload import ops
+    dy, x, a, b, ids, scale = make(dtype, tokens, 4, 16, 136, 72)
+    clean = ops.lora_grad(dy, x, a, b, ids, scale=scale)
+    t = int((ids == 1).nonzero()[0])
+    for bad in (float("nan"), float("inf")):
+        x2, dy2 = x.clone(), dy.clone()
+        x2[(ids < 0) | (ids >= 4)] = bad                                       # not read: these tokens have no adapter
+        dy2[(ids < 0) | (ids >= 4)] = bad
+        assert all(torch.equal(p, q) for p, q in zip(ops.lora_grad(dy2, x2, a, b, ids, scale=scale), clean))
+        x2[t, 5] = bad                                                         # v, so db; and da's column 5
+        dx, da, db = ops.lora_grad(dy2, x2, a, b, ids, scale=scale)
+        keep = [0, 2, 3]
+        assert torch.equal(dx, clean[0]) and torch.equal(da[keep], clean[1][keep]) and torch.equal(db[keep], clean[2][keep])
+        assert not bool(da[1, :, 5].isfinite().any()) and not bool(db[1].isfinite().any())
+        cols = torch.arange(136, device=DEV) != 5
+        assert torch.equal(da[1][:, cols], clean[1][1][:, cols])
+        dy2[t, 3] = bad                                                        # dv, so dx of the token and da of its adapter
+        dx, da, db = ops.lora_grad(dy2, x, a, b, ids, scale=scale)
+        others = torch.arange(tokens, device=DEV) != t
+        assert torch.equal(dx[others], clean[0][others]) and not bool(dx[t].isfinite().any())
+        assert torch.equal(da[keep], clean[1][keep]) and not bool(da[1].isfinite().any())
+        rows = torch.arange(72, device=DEV) != 3
+        assert torch.equal(db[keep], clean[2][keep]) and torch.equal(db[1][rows], clean[2][1][rows]) and not bool(db[1, 3].isfinite().any())
