@@ -30,8 +30,8 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t nb) {
 
 // Weights' gradients: blocks of one segment are as long as it is.  Up to kManySegs segments each is dealt to all 8 XCDs in
 // runs of `run` items; more of them even out over whole shares of one XCD each, which read a row once.  us of gradients,
-// dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 435 (of 1024 rows each, dw
-// alone, 173 and 163), 8 adapters of 4096 tokens, all of lora_grad, 62.5 and 76.1; 512 experts of 1024 x 2048, 40 rows, 998 and 911.
+// dealt and in whole shares: 16 experts of 4096 x 1024, 1024 rows on average, with mm_dx 396 and 437 (of 1024 rows each, dw
+// alone, 145 both ways), 8 adapters of 4096 tokens, all of lora_grad, 62.5 and 76.1; 512 experts of 1024 x 2048, 40 rows, 999 and 914.
 constexpr int kManySegs = 128;
 
 __device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run) {
@@ -200,9 +200,9 @@ __device__ __forceinline__ uint4 pair8(uint2 a, uint2 b) {
 }
 
 // 16 bytes out, past the caches.  Results are read again by the next launch at the earliest, and their lines
-// wait in L2 for a write that then meets the next tile's loads: us with and without, mm 8192 x 8192 x 8192 852 and 908,
-// weights' gradient 4096 x 1024 of 16 x 1024 rows 148 and 160, mm 1024 x 4096 of 16 x 1024 rows 131 and 161, mm_dx 1024 x
-// 2048 of 512 x 40 rows 429 and 439; the whole layer, 2048 tokens over 512 experts of 512 x 2048, 638 and 643.
+// wait in L2 for a write that then meets the next tile's loads: us with and without, weights' gradient 1024 x 2048 of 512 x
+// 40 rows 377 and 607, 4096 x 1024 of 16 x 256 rows 63 and 74, mm 4096 x 1024 of 16 x 2048 rows 258 and 276, mm_dx 1024 x
+// 2048 of 512 x 40 rows 431 and 441, gate_up 1024 x 4096 of 16 x 2048 rows 478 and 485.
 __device__ __forceinline__ void store16(void* to, uint4 v) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);

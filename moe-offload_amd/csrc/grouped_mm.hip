@@ -306,10 +306,10 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
         if constexpr (kThroughLds) {
             // The results go through the image just multiplied, a part of it for each wave, and out in whole lines: a lane
             // of the matrix unit's result has 8 or 16 bytes of a row and its neighbour another row's, each a cache access
-            // of its own, and a store past the caches wants whole lines (mm 1024 x 4096, 16 x 2048 rows to places in no
-            // order: 304 us, and 327 straight from the registers; weights' gradient over 512 x 40 rows, 1024 x 2048, 591 and
-            // 640 with ordinary stores, 520 like this).  Tiles of 64 rows have too few steps to pay for the barrier (mm of 100 x 47 rows,
-            // 1152 x 320: 21.0 us, and 19.0 without), but silu's gradient reads (g, u) in whole lines too this way.
+            // of its own, and a store past the caches wants whole lines (mm 4096 x 1024, 16 x 2048 rows to places in no
+            // order: 258 us, and 276 straight from the registers; weights' gradient over 512 x 40 rows, 1024 x 2048, 377 and
+            // 687).  Tiles of 64 rows have too few steps to pay for the barrier (mm of 100 x 47 rows, 1152 x 320: 20.3 us, and
+            // 19.5 without), but silu's gradient reads (g, u) in whole lines too this way.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                                      // everyone has read the image
             asm volatile("" ::: "memory");
@@ -612,9 +612,9 @@ int64_t blocks_of(Args& a) {
     }
     // Column tiles per block: short tiles share one block's start (the search for its rows, the first load's way) while
     // that leaves 1024 blocks.  us per launch at 1, 2, 4 and 16 tiles: weights' gradient 4096 x 1024 of 16 x 256 rows (4
-    // steps) 75, 68, 65, -, 1024 x 2048 of 512 x 40 rows (1 step) 871, -, 632, 606; mm 4096 x 1024 of 16 x 512 rows (16
-    // steps) 85, 80, -, -.  Tiles of 64 rows wait for memory and have three blocks per CU to do so: mm_dx 1024 x 2048 of
-    // 512 x 40 rows (16 steps) 514 and, at 3 tiles, 540.
+    // steps) 68, 61, 57, 77, 1024 x 2048 of 512 x 40 rows (1 step) 594, 449, 402, 381; mm 4096 x 1024 of 16 x 512 rows (16
+    // steps) 77, 69, 122, 422.  Tiles of 64 rows wait for memory and have three blocks per CU to do so: mm_dx 1024 x 2048 of
+    // 512 x 40 rows (16 steps) 431, 436, 456, 469.
     const int64_t target = OP == kDw ? 16 : BP == 64 ? 8 : 32;
     const int64_t span = std::min(target / steps, rows * tiles / 1024);
     a.span = (int)std::max<int64_t>(1, std::min<int64_t>(span, tiles));
@@ -666,12 +666,13 @@ enum { kDw256, kDw128, kDw64 };
 int dw_tiles(const Args& a) {
     const int64_t per_seg = a.S.n_rows / std::max(a.S.n_seg, 1);
     auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * ((a.nq + b - 1) / b); };
-    // with few rows the output's bytes bound it, and smaller tiles have more of them under way (512 x 40 rows, 1024 x
-    // 2048: 592 us, and 737 with the large tiles)
+    // with few rows the output's bytes bound it, and either size wins somewhere: us with tiles of 128 and of 256, 512 x 80
+    // rows, 1280 x 2560, 1101 and 1177, 128 x 64 rows, 4096 x 1024, 204 and 210, 64 x 100 rows, 2048 x 1024, 76 and 78, 512 x
+    // 40 rows, 1024 x 2048, 377 and 380 (ragged, with mm_dx, 914 and 851); from 512 rows on the large ones lose nowhere
     if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return kDw256;
-    // an adapter's: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 30 us with them, 21 with 64's).
-    // Where not every CU gets one of 128, more and shorter steps of 64 are done sooner too: 2 x 4000 rows, 512 x 1024, 67 and
-    // 39 us, 1113 rows, 2272 x 96, 22.9 and 12.9, 8 x 300 rows, 1024 x 512, 12.1 and 11.1
+    // narrow ones: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 13.9 us with them, 9.4 with 64's).
+    // Where not every CU gets one of 128, more and shorter steps of 64 are done sooner too: 2 x 4000 rows, 512 x 1024, 66 and
+    // 41 us, 1113 rows, 2272 x 96, 22.7 and 12.9, 8 x 300 rows, 1024 x 512, 11.4 and 10.7
     if (a.np <= 64 || a.nq <= 64 || tiles(128) <= 256) return kDw64;
     return kDw128;
 }

@@ -53,6 +53,7 @@ class _SwitchGlu(torch.autograd.Function):
             if ctx.needs_input_grad[2]:
                 dw_gate_up = ops.grouped_mm_dw(dgu, x, seg_start, row_x=row_token)
             if ctx.needs_input_grad[0]:
+                # a row per (token, k), rounded to the inputs' type as every operator's result is; their sum is fp32
                 rows = ops.grouped_mm_dx(dgu, seg_start, w_gate_up, row_out=row_out)
                 dx = rows.view(n_tok, k, x.shape[1]).sum(1, dtype=torch.float32).to(x.dtype)
         return dx, None, dw_gate_up, dw_down
