@@ -337,7 +337,8 @@ int moe_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, 
 /* The gradients of moe_lora_add, given dy [n_tok][n_out] (base's own is dy):  dx[t] = A_i^T dv[t] (zeros without
  * an adapter), da_i [rank][n_in] = sum of dv[t] x[t]^T and db_i [n_out][rank] = scale[i] * sum of dy[t] v[t]^T over
  * adapter i's tokens (zeros without any), v = A_i x[t], dv = scale[i] * B_i^T dy[t], both in fp32 between the
- * products.  da and
+ * products (here and in moe_lora_add as sums of 16-bit parts: an infinity in x, dy, a or b gives infinities or NaN where
+ * it enters).  da and
  * db are contiguous; n_ad in 1..1024.  workspace: moe_lora_grad_workspace_bytes bytes, 16-byte aligned, any
  * contents, one per call in flight. */
 uint64_t moe_lora_grad_workspace_bytes(int n_tok, int n_ad, int rank);

@@ -460,7 +460,8 @@ def grouped_mm_dx(dy, seg_start, w, row_in=None, row_out=None, n_out_rows=None, 
     Where grouped_mm read x[a[r]] and wrote y[b[r]], this takes row_in=b and writes one row per sorted
     row; rows of x read several times get the sum of theirs from the caller (row_out = the pairs' order,
     then a sum over k).  gu: w's input was grouped_gate_up's h, and gu the (g, u) it kept, [M, 2 * K] in
-    sorted order; the result is then the gradient of (g, u), [*, 2 * K].  Other arguments as grouped_mm.
+    sorted order; the result is then the gradient of (g, u), [*, 2 * K] (an infinite g, past the type's range,
+    has its limit's).  Other arguments as grouped_mm.
     """
     who = "grouped_mm_dx"
     dev = _one_gpu(who, "dy seg_start w row_in row_out seg_slot scale gu out", dy, seg_start, w, row_in, row_out, seg_slot, scale, gu, out)
