@@ -668,7 +668,7 @@ int dw_tiles(const Args& a) {
     auto tiles = [&](int b) { return (int64_t)a.S.n_seg * ((a.np + b - 1) / b) * ((a.nq + b - 1) / b); };
     // with few rows the output's bytes bound it, and either size wins somewhere: us with tiles of 128 and of 256, 512 x 80
     // rows, 1280 x 2560, 1101 and 1177, 128 x 64 rows, 4096 x 1024, 204 and 210, 64 x 100 rows, 2048 x 1024, 76 and 78, 512 x
-    // 40 rows, 1024 x 2048, 377 and 380 (ragged, with mm_dx, 914 and 851); from 512 rows on the large ones lose nowhere
+    // 40 rows, 1024 x 2048, 377 and 380 (ragged, with mm_dx, 914 and 851); from 512 rows on the rounds of blocks decide
     if (per_seg >= 512 && big_tiles(tiles(128), tiles(256))) return kDw256;
     // narrow ones: tiles of 128 would be half empty, and few (8 x 512 rows, 64 x 2048: 13.9 us with them, 9.4 with 64's).
     // Where not every CU gets one of 128, more and shorter steps of 64 are done sooner too: 2 x 4000 rows, 512 x 1024, 66 and
