@@ -346,6 +346,61 @@ int moe_lora_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, cons
                   int64_t b_stride, const int32_t* ids, const float* scale, int n_tok, int n_ad, int n_in, int n_out,
                   int rank, int dtype, void* workspace, void* dx, int64_t lddx, void* da, void* db, void* stream);
 
+/* ---- Part 2c: around the unquantised experts (no counterpart in the reference) --------------- */
+/* A batch's routing, the weighted sum behind the experts, projections that all tokens share, and the gradients' norm: with
+ * Part 2b a layer in training and in serving.  Device pointers throughout but for moe_clip_grads' lists; nothing is
+ * allocated on the device, kept between calls or synchronised.  Outputs must not overlap inputs but where it is said. */
+
+/* Each token's experts and their weights from its logits (fp16, bf16 or fp32: dtype 0, 1, 2; ld elements from row to row):
+ *   s = softmax(l) (score 0) or sigmoid(l) (score 1);  c = s + bias[e], or l itself where bias (fp32 [n_exp]) is null
+ *   n_group groups of n_exp / n_group adjacent experts; a group's value is the sum of its group_best (1 or 2) largest c --
+ *   of s, where bias is null and group_best is 2 --, or of those it has; the topk_group groups of the largest values stay
+ *   ids [n_tok][k]: the k largest c among the experts that stay, in descending order, equals to the lowest index (groups too)
+ *   weights fp32 [n_tok][k] = scale * s[id], with renorm != 0 divided by the sum of the k s[id] first
+ * c and the groups' values are exact where bias is null and group_best 1, else 64-bit sums.  An expert whose logit, or bias, is
+ * -inf or NaN is never chosen; places left over get id -1, weight 0.  A NaN among a token's logits makes its k weights NaN.
+ * Infinite logits have the weights' limits: several of +inf share a softmax evenly.  n_exp in 1..1024, k in 1..32 and at
+ * most n_exp, n_group in 1..64 and a divisor of n_exp. */
+int moe_route(const void* logits, int64_t ld, int n_tok, int n_exp, int k, int score, int renorm, const float* bias, int n_group,
+              int topk_group, int group_best, float scale, int dtype, int32_t* ids, float* weights, void* stream);
+/* The gradient of moe_route's weights in the logits, with ids as it gave them (the choice, and with it the bias, has none):
+ * dlogits [n_tok][n_exp] of the logits' type, ldd elements from row to row, all written.  Places whose id is outside
+ * 0 .. n_exp - 1 add nothing; an id that comes twice adds both. */
+int moe_route_grad(const float* dweights, const void* logits, int64_t ld, const int32_t* ids, int n_tok, int n_exp, int k, int score,
+                   int renorm, float scale, int dtype, void* dlogits, int64_t ldd, void* stream);
+/* out[t] = residual[t] + sum over j of weights[t][j] * y[t * k + j]: rows of hidden elements (a multiple of 8) of fp16 or bf16
+ * (dtype 0, 1), residual may be null, weights fp32 [n_tok][k], out of that type or fp32 (out_f32 != 0).  A weight of 0 adds
+ * nothing, whatever its row holds.  out may be residual (of its type and step).  Matrices 16-byte aligned, steps
+ * multiples of 8; n_tok * k up to 2^30. */
+int moe_combine(const void* y, int64_t ldy, const float* weights, const void* residual, int64_t ldr, int n_tok, int k, int hidden,
+                int dtype, int out_f32, void* out, int64_t ldo, void* stream);
+/* Its gradients: dy[t * k + j] = weights[t][j] * dout[t], dweights[t][j] = <dout[t], y[t * k + j]> (the residual's is dout). */
+int moe_combine_grad(const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* weights, int n_tok, int k, int hidden,
+                     int dtype, void* dy, int64_t lddy, float* dweights, void* stream);
+/* y = act(z) + residual, z = x W^T + bias: x [n_tok][n_in], W [n_out][n_in] contiguous, bias [n_out], residual [n_tok][n_out]
+ * (either may be null) of fp16 or bf16 (dtype 0, 1), y of that type or fp32 (out_f32 != 0).  act: 0 none, 1 silu, 2 gelu (z
+ * times the normal distribution's integral), 3 the squared relu.  z, where it is not null, receives the pre-activations in
+ * the inputs' type.  y may be residual (of its type and step).  Matrices 16-byte aligned; n_in, n_out and steps multiples of 8. */
+int moe_linear(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual, int64_t ldr, int n_tok, int n_in,
+               int n_out, int act, int dtype, int out_f32, void* z, int64_t ldz, void* y, int64_t ldy, void* stream);
+/* Its gradients from dy (of the inputs' type, or fp32: dy_f32 != 0) and the z it kept (act != 0): dz = dy act'(z), rounded to
+ * the inputs' type, dx [n_tok][n_in] = dz W, dw [n_out][n_in] = dz^T x (fp32 if dw_f32 != 0), db [n_out] = the sum of dz over
+ * the tokens; the residual's is dy.  Those that are null are not computed; outputs are contiguous.  n_tok up to 2^22 - 64.
+ * workspace: moe_linear_grad_workspace_bytes bytes, 16-byte aligned, any contents, one per call in flight. */
+uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_out, int act, int dy_f32, int want_db);
+int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const void* x, int64_t ldx, const void* w, const void* z, int64_t ldz,
+                    int n_tok, int n_in, int n_out, int act, int dtype, void* workspace, void* dx, void* dw, int dw_f32, void* db,
+                    void* stream);
+/* The norm of n tensors together, sqrt of the sum of all squares, into *norm (device memory); and, unless outs is null, each
+ * tensor times min(1, max_norm / (norm + 1e-6)) into outs[i], which may be grads[i].  grads, outs, sizes (elements) and types
+ * (0 fp16, 1 bf16, 2 fp32) are host arrays, read before the call returns; the addresses in them are device memory, aligned to
+ * their elements.  A tensor of no elements may be null.  Nothing that is written may overlap another tensor.  An infinite norm
+ * makes every value 0 or NaN, a NaN every value NaN.  workspace: moe_clip_workspace_bytes bytes for n tensors of n_elements
+ * together, 16-byte aligned, any contents, one per call in flight. */
+uint64_t moe_clip_workspace_bytes(int n, int64_t n_elements);
+int moe_clip_grads(int n, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* types, double max_norm,
+                   void* workspace, float* norm, void* stream);
+
 /* 2-bit codebook experts: the Nemotron model of README.md:37 (IQ2_XXS GGUF, 240 experts, top-9),
  * run by the reference only inside llama.cpp's Metal backend (llama-moe-cache.patch:1-12 adds the
  * mul_mm_id map for 9 experts per token; format in csrc/moe_common.h CbLayout): non-gated up ->

@@ -124,6 +124,20 @@ SIGNATURES: dict[str, tuple] = {
     "moe_lora_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int]),
     "moe_lora_grad": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_int,
                                _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp]),
+    # around the unquantised experts
+    "moe_route": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_int, _c_int, _c_f, _c_int,
+                           _c_vp, _c_vp, _c_vp]),
+    "moe_route_grad": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_int, _c_vp, _c_i64,
+                                _c_vp]),
+    "moe_combine": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_vp]),
+    "moe_combine_grad": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_vp, _c_vp]),
+    "moe_linear": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp,
+                            _c_i64, _c_vp, _c_i64, _c_vp]),
+    "moe_linear_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "moe_linear_grad": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                 _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp]),
+    "moe_clip_workspace_bytes": (_c_u64, [_c_int, _c_i64]),
+    "moe_clip_grads": (_c_int, [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_double, _c_vp, _c_vp, _c_vp]),
     # no reference counterpart
     "c_last_error": (ctypes.c_char_p, []),
     "c_clear_error": (None, []),

@@ -1,10 +1,10 @@
-"""Unquantised experts and adapters in training: the operators of `ops` with their gradients under autograd.
+"""Layers of unquantised experts and adapters in training: the operators of `ops` with their gradients under autograd.
 
-    plan rows by expert -> gate and up projections, silu(g) * u -> down projections, one row per (token, k)
+    logits (linear) -> ids and weights (route) -> rows by expert, gate and up, silu(g) * u, down (switch_glu)
+    -> weighted sum onto the residual (combine);   moe_layer is all of them
 
-and back, each product and each gradient one launch of libmoe_offload.so.  What the forward pass keeps is the
-row plan, (g, u) and h.  The score-weighted sum over a token's experts is the caller's, in torch operations, and
-so is the scores' gradient (ops.pair_combine has none, and takes fp16 rows only).
+and back, each product and each gradient one launch of libmoe_offload.so, or a few.  What switch_glu's forward pass keeps
+is the row plan, (g, u) and h.  clip_grad_norm limits the gradients' norm before the optimizer's step.
 
 A graph capture of a forward or backward pass through autograd is refused: an eager graph of the same leaves
 that is still alive would end the process.  Programs that capture call ops.grouped_* and ops.lora_* themselves.
@@ -103,3 +103,103 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         raise ValueError(f"lora_add: {a.shape[0]} adapters (gradients for up to 1024)")
     _refuse_capture("lora_add")
     return _LoraAdd.apply(base, x, a, b, ids, scale)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, score, bias, n_group, topk_group, group_best, renorm, scale):
+        ids, weights = ops.route(logits, k, score=score, bias=bias, n_group=n_group, topk_group=topk_group, group_best=group_best,
+                                 renorm=renorm, scale=scale)
+        ctx.save_for_backward(logits, ids)
+        ctx.rule = {"score": score, "renorm": renorm, "scale": scale}
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dweights):
+        _refuse_capture("route")
+        logits, ids = ctx.saved_tensors
+        return (ops.route_grad(dweights.contiguous(), logits, ids, **ctx.rule),) + (None,) * 8
+
+
+def route(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_best=1, renorm=True, scale=1.0):
+    """ops.route, its weights differentiable in the logits.  The bias, which only the choice sees, has no gradient."""
+    if bias is not None and bias.requires_grad:
+        raise ValueError("route: the bias has no gradient here")
+    _refuse_capture("route")
+    return _Route.apply(logits, k, score, bias, n_group, topk_group, group_best, renorm, scale)
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, residual):
+        ctx.save_for_backward(y, weights)
+        return ops.combine(y, weights, residual=residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        _refuse_capture("combine")
+        y, weights = ctx.saved_tensors
+        dy = dweights = None
+        if any(ctx.needs_input_grad[:2]):
+            dy, dweights = ops.combine_grad(_operand(dout), y, weights)
+        return dy, dweights, dout if ctx.needs_input_grad[2] else None
+
+
+def combine(y, weights, residual=None):
+    """ops.combine, differentiable in y, weights and residual."""
+    _refuse_capture("combine")
+    return _Combine.apply(y, weights, residual)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual, dtype):
+        z = None
+        if act is not None and any(ctx.needs_input_grad[:3]):
+            z = torch.empty((x.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
+        ctx.save_for_backward(x, w, z)
+        ctx.act = act
+        return ops.linear(x, w, bias=bias, act=act, residual=residual, z_out=z, dtype=dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _refuse_capture("linear")
+        x, w, z = ctx.saved_tensors
+        want_dx, want_dw, want_db, _, want_dr, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if want_dx or want_dw or want_db:
+            dx, dw, db = ops.linear_grad(_operand(dy), x, w, z=z, act=ctx.act, bias=want_db, want_dx=want_dx, want_dw=want_dw)
+        return dx, dw, db, None, dy.to(x.dtype) if want_dr else None, None
+
+
+def linear(x, w, bias=None, act=None, residual=None, dtype=None):
+    """ops.linear, differentiable in x, w, bias and residual; with an activation the pre-activations are kept in the
+    inputs' type for the backward pass."""
+    _refuse_capture("linear")
+    return _Linear.apply(x, w, bias, act, residual, dtype)
+
+
+def moe_layer(x, w_router, w_gate_up, w_down, k, score="softmax", bias=None, n_group=1, topk_group=1, group_best=1, renorm=True,
+              scale=1.0, residual=None):
+    """A layer of unquantised experts from its tokens to its output, [n_tok, hidden], differentiable in x, the three weights
+    and the residual: the router's logits in fp32, each token's k experts (the arguments of ops.route), their SwitchGLU, the
+    weighted sum plus the residual.
+
+    x: fp16 or bf16 [n_tok, hidden]; w_router: same type [n_exp, hidden], n_exp a multiple of 8; w_gate_up, w_down as
+    switch_glu.
+    """
+    if w_router.dim() != 2 or w_gate_up.dim() != 3 or w_router.shape[0] != w_gate_up.shape[0]:
+        raise ValueError(f"moe_layer: w_router {tuple(w_router.shape)} and w_gate_up {tuple(w_gate_up.shape)} do not fit")
+    logits = linear(x, w_router, dtype=torch.float32)
+    ids, weights = route(logits, k, score, bias, n_group, topk_group, group_best, renorm, scale)
+    return combine(switch_glu(x, ids, w_gate_up, w_down), weights, residual)
+
+
+def clip_grad_norm(parameters, max_norm):
+    """ops.clip_grad_norm of the parameters' gradients, in place (those without one are left out); returns the norm before."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    return ops.clip_grad_norm([p.grad for p in parameters if p.grad is not None], max_norm)

@@ -5,6 +5,8 @@ no PyTorch fallback for any of them.
 """
 from __future__ import annotations
 
+from array import array
+
 import torch
 
 from . import _lib
@@ -579,3 +581,305 @@ def lora_grad(dy, x, a, b, ids, scale=None, workspace=None):
     _call("moe_lora_grad", dev, _p(dy), lddy, _p(x), ldx, _p(a), a_stride, _p(b), b_stride, _p(ids), _p(scale), n_tok, n_ad,
           n_in, n_out, rank, dt, _p(workspace), _p(dx), n_in, _p(da), _p(db))
     return dx, da, db
+
+
+# ---- around the unquantised experts: routing, the weighted sum, shared projections, the gradients' norm ----------
+
+_REAL = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_ACTS = {None: 0, "silu": 1, "gelu": 2, "relu2": 3}
+
+
+def _choice(who: str, name: str, value, of: dict) -> int:
+    if value not in of:
+        raise ValueError(f"{who}: {name}={value!r} (one of {', '.join(repr(v) for v in of)})")
+    return of[value]
+
+
+def _scored_rows(who: str, name: str, t: torch.Tensor, shape: tuple | None = None) -> int:
+    """Checks logits or their gradient (any real type, rows contiguous at any step); returns the step."""
+    if t.dtype not in _REAL:
+        raise TypeError(f"{who}: {name} is {t.dtype} (torch.float16, torch.bfloat16 and torch.float32 are supported)")
+    if t.dim() != 2 or (shape is not None and t.shape != shape):
+        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}" + ("" if shape is None else f", not {tuple(shape)}"))
+    n, w = t.shape
+    if n > _MAX_SIDE or not 1 <= w <= 1024:
+        raise ValueError(f"{who}: {name}: {n} tokens (up to 2^30), {w} experts (1..1024)")
+    step, inner = t.stride()
+    if (w > 1 and inner != 1) or (n > 1 and step < w):
+        raise ValueError(f"{who}: {name}: rows must be contiguous and apart, not {t.stride()}")
+    return step if n > 1 else w
+
+
+def _per_place(who: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{who}: {name} is {t.dtype}, not {dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous of shape {tuple(shape)}, not {tuple(t.shape)}")
+
+
+def _route_k(who: str, k: int, n_exp: int) -> None:
+    if not 1 <= k <= min(32, n_exp):
+        raise ValueError(f"{who}: k={k} of {n_exp} experts (1..32)")
+
+
+def route(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_best=1, renorm=True, scale=1.0, ids=None,
+          weights=None):
+    """Each token's k experts and their weights: int32 ids [n_tok, k] and fp32 weights [n_tok, k], the best first.
+
+    logits: fp16, bf16 or fp32 [n_tok, n_exp], up to 1024 experts.  s = softmax(logits) or sigmoid(logits); experts compare by
+    c = s + bias (fp32 [n_exp]), without a bias by their logits.  n_group > 1: of the n_group groups of adjacent experts only
+    the topk_group stay whose group_best (1 or 2) largest c have the largest sum (without a bias, and for 2, of s).  Equals go
+    to the lowest index.  weights = scale * s[ids], renorm: divided by the sum of the chosen s first.
+
+    An expert whose logit or bias is -inf or NaN is never chosen (mask with -inf: any other value may be chosen where
+    there is too little else); places left over get id -1 and weight 0, which expert_plan, the grouped products and combine take.
+    A NaN among a token's logits makes all its weights NaN.  Several logits of +inf share a softmax evenly.
+    """
+    who = "route"
+    dev = _one_gpu(who, "logits bias ids weights", logits, bias, ids, weights)
+    score = _choice(who, "score", score, _SCORES)
+    ld = _scored_rows(who, "logits", logits)
+    n_tok, n_exp = logits.shape
+    _route_k(who, k, n_exp)
+    if bias is not None:
+        _per_place(who, "bias", bias, (n_exp,), torch.float32)
+    if not 1 <= n_group <= 64 or n_exp % n_group or not 1 <= topk_group <= n_group or group_best not in (1, 2):
+        raise ValueError(f"{who}: n_group={n_group} (1..64, a divisor of {n_exp}), topk_group={topk_group} (1..n_group), "
+                         f"group_best={group_best} (1 or 2)")
+    if ids is None:
+        ids = torch.empty((n_tok, k), dtype=torch.int32, device=logits.device)
+    if weights is None:
+        weights = torch.empty((n_tok, k), dtype=torch.float32, device=logits.device)
+    _per_place(who, "ids", ids, (n_tok, k), torch.int32)
+    _per_place(who, "weights", weights, (n_tok, k), torch.float32)
+    _call("moe_route", dev, _p(logits), ld, n_tok, n_exp, k, score, int(bool(renorm)), _p(bias), n_group, topk_group, group_best,
+          scale, _REAL[logits.dtype], _p(ids), _p(weights))
+    return ids, weights
+
+
+def route_grad(dweights, logits, ids, score="softmax", renorm=True, scale=1.0, out=None):
+    """The gradient in the logits, [n_tok, n_exp] of their type, of the weights that route gave with these ids.
+
+    dweights: fp32 [n_tok, k].  The choice has no gradient, so neither has the bias.  Places whose id is outside the experts
+    add nothing.
+    """
+    who = "route_grad"
+    dev = _one_gpu(who, "dweights logits ids out", dweights, logits, ids, out)
+    score = _choice(who, "score", score, _SCORES)
+    ld = _scored_rows(who, "logits", logits)
+    n_tok, n_exp = logits.shape
+    if ids.dim() != 2:
+        raise ValueError(f"{who}: ids has shape {tuple(ids.shape)}, not (n_tok, k)")
+    k = ids.shape[1]
+    _route_k(who, k, n_exp)
+    _per_place(who, "ids", ids, (n_tok, k), torch.int32)
+    _per_place(who, "dweights", dweights, (n_tok, k), torch.float32)
+    if out is None:
+        out = torch.empty((n_tok, n_exp), dtype=logits.dtype, device=logits.device)
+    if out.dtype != logits.dtype:
+        raise TypeError(f"{who}: out is {out.dtype}, not {logits.dtype}")
+    ldd = _scored_rows(who, "out", out, logits.shape)
+    _call("moe_route_grad", dev, _p(dweights), _p(logits), ld, _p(ids), n_tok, n_exp, k, score, int(bool(renorm)), scale,
+          _REAL[logits.dtype], _p(out), ldd)
+    return out
+
+
+def _pair_rows(who: str, name: str, t: torch.Tensor, n_tok: int, k: int, like: torch.Tensor) -> torch.Tensor:
+    """A row per (token, place), given as [n_tok, k, hidden] or [n_tok * k, hidden], in the second form."""
+    if t.dim() == 3 and t.shape[:2] == (n_tok, k):
+        if n_tok > 1 and k > 1 and t.stride(0) != k * t.stride(1):
+            raise ValueError(f"{who}: {name}: a token's rows must follow the token's before it, not {t.stride()}")
+        return t.view(n_tok * k, t.shape[2]) if t.numel() else t.reshape(n_tok * k, t.shape[2])
+    if t.dim() != 2 or t.shape[0] != n_tok * k:
+        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, not ({n_tok}, {k}, *) or ({n_tok * k}, *)")
+    return t
+
+
+def _any_rows(who: str, name: str, t: torch.Tensor, dtypes: tuple, rows: int, width: int) -> int:
+    """_rows for outputs of one of two types."""
+    if t.dtype not in dtypes:
+        raise TypeError(f"{who}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
+    return _rows(who, name, t, t.dtype, rows, width)
+
+
+def combine(y, weights, residual=None, dtype=None, out=None):
+    """out[t] = residual[t] + sum over j of weights[t, j] * y[t * k + j]: a layer's output from its experts' rows.
+
+    y: fp16 or bf16 [n_tok, k, hidden] (or [n_tok * k, hidden]), as grouped_mm and dense.switch_glu give them; weights: fp32
+    [n_tok, k]; residual: of y's type or None; out: of y's type, or fp32 with dtype=torch.float32.  A weight of 0 adds
+    nothing, whatever its row holds.  out=residual adds in place.
+    """
+    who = "combine"
+    dev = _one_gpu(who, "y weights residual out", y, weights, residual, out)
+    dt = _half(who, y)
+    if weights.dim() != 2 or weights.shape[1] < 1:
+        raise ValueError(f"{who}: weights has shape {tuple(weights.shape)}, not (n_tok, k)")
+    n_tok, k = weights.shape
+    _per_place(who, "weights", weights, (n_tok, k), torch.float32)
+    y = _pair_rows(who, "y", y, n_tok, k, weights)
+    hidden = y.shape[1]
+    ldy = _rows(who, "y", y, y.dtype, n_tok * k, None)
+    ldr = _rows(who, "residual", residual, y.dtype, n_tok, hidden) if residual is not None else 0
+    if out is None:
+        out = torch.empty((n_tok, hidden), dtype=dtype or y.dtype, device=y.device)
+    elif dtype not in (None, out.dtype):
+        raise TypeError(f"{who}: out is {out.dtype}, not {dtype}")
+    ldo = _any_rows(who, "out", out, (y.dtype, torch.float32), n_tok, hidden)
+    _call("moe_combine", dev, _p(y), ldy, _p(weights), _p(residual), ldr, n_tok, k, hidden, dt, int(out.dtype == torch.float32),
+          _p(out), ldo)
+    return out
+
+
+def combine_grad(dout, y, weights):
+    """combine's gradients: dy, of y's shape and type, and fp32 dweights [n_tok, k] (the residual's is dout, of y's type)."""
+    who = "combine_grad"
+    dev = _one_gpu(who, "dout y weights", dout, y, weights)
+    dt = _half(who, y)
+    if weights.dim() != 2 or weights.shape[1] < 1:
+        raise ValueError(f"{who}: weights has shape {tuple(weights.shape)}, not (n_tok, k)")
+    n_tok, k = weights.shape
+    _per_place(who, "weights", weights, (n_tok, k), torch.float32)
+    rows = _pair_rows(who, "y", y, n_tok, k, weights)
+    hidden = rows.shape[1]
+    ldy = _rows(who, "y", rows, y.dtype, n_tok * k, None)
+    ldd = _rows(who, "dout", dout, y.dtype, n_tok, hidden)
+    dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    dw = torch.empty((n_tok, k), dtype=torch.float32, device=y.device)
+    _call("moe_combine_grad", dev, _p(dout), ldd, _p(rows), ldy, _p(weights), n_tok, k, hidden, dt, _p(dy), hidden, _p(dw))
+    return dy, dw
+
+
+def _shared_weight(who: str, w: torch.Tensor, dtype: torch.dtype, n_in: int) -> None:
+    if _rows(who, "w", w, dtype, None, n_in) != n_in or w.shape[0] % 8 or w.shape[0] == 0:
+        raise ValueError(f"{who}: w must be contiguous with a multiple of 8 rows, not {tuple(w.shape)} at {w.stride()}")
+
+
+def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out=None):
+    """act(x @ w.T + bias) + residual: a projection that all tokens share (the router, a shared expert), in one launch.
+
+    x: fp16 or bf16 [n_tok, n_in]; w: same type [n_out, n_in], contiguous; bias: same type [n_out] or None; act: None, "silu",
+    "gelu" (exact, by the normal distribution's integral) or "relu2" (the squared relu); residual: same type [n_tok, n_out] or None.
+    The result has the inputs' type, or fp32 with dtype=torch.float32 (router logits).  z_out, [n_tok, n_out] of the inputs'
+    type, receives x @ w.T + bias for linear_grad.  out=residual adds in place.
+    """
+    who = "linear"
+    dev = _one_gpu(who, "x w bias residual z_out out", x, w, bias, residual, z_out, out)
+    dt = _half(who, x)
+    act = _choice(who, "act", act, _ACTS)
+    ldx = _rows(who, "x", x, x.dtype, None, None)
+    n_tok, n_in = x.shape
+    _shared_weight(who, w, x.dtype, n_in)
+    n_out = w.shape[0]
+    if bias is not None:
+        _per_place(who, "bias", bias, (n_out,), x.dtype)
+    ldr = _rows(who, "residual", residual, x.dtype, n_tok, n_out) if residual is not None else 0
+    ldz = _rows(who, "z_out", z_out, x.dtype, n_tok, n_out) if z_out is not None else 0
+    if out is None:
+        out = torch.empty((n_tok, n_out), dtype=dtype or x.dtype, device=x.device)
+    elif dtype not in (None, out.dtype):
+        raise TypeError(f"{who}: out is {out.dtype}, not {dtype}")
+    ldy = _any_rows(who, "out", out, (x.dtype, torch.float32), n_tok, n_out)
+    _call("moe_linear", dev, _p(x), ldx, _p(w), _p(bias), _p(residual), ldr, n_tok, n_in, n_out, act, dt,
+          int(out.dtype == torch.float32), _p(z_out), ldz, _p(out), ldy)
+    return out
+
+
+def linear_grad(dy, x, w, z=None, act=None, bias=False, want_dx=True, want_dw=True, dw_dtype=None, workspace=None):
+    """linear's gradients (dx, dw, dbias), None for those that are not wanted; the residual's is dy.
+
+    dy: x's type, or fp32, [n_tok, n_out]; z: what linear wrote to z_out, where act is not None; bias: whether the bias's
+    gradient is wanted.  dw in x's type, or fp32 with dw_dtype=torch.float32.  dz = dy act'(z) is rounded to x's type before
+    the products (dy alone too, where it is fp32).  workspace: scratch of moe_linear_grad_workspace_bytes.
+    """
+    who = "linear_grad"
+    dev = _one_gpu(who, "dy x w z workspace", dy, x, w, z, workspace)
+    dt = _half(who, x)
+    act_id = _choice(who, "act", act, _ACTS)
+    ldx = _rows(who, "x", x, x.dtype, None, None)
+    n_tok, n_in = x.shape
+    _shared_weight(who, w, x.dtype, n_in)
+    n_out = w.shape[0]
+    lddy = _any_rows(who, "dy", dy, (x.dtype, torch.float32), n_tok, n_out)
+    if (z is None) != (act is None):
+        raise ValueError(f"{who}: z goes with an activation (act={act!r})")
+    ldz = _rows(who, "z", z, x.dtype, n_tok, n_out) if z is not None else 0
+    dw_dtype = dw_dtype or x.dtype
+    if dw_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{who}: gradients of {x.dtype} come as {x.dtype} or torch.float32, not {dw_dtype}")
+    dx = torch.empty((n_tok, n_in), dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty((n_out, n_in), dtype=dw_dtype, device=x.device) if want_dw else None
+    db = torch.empty(n_out, dtype=x.dtype, device=x.device) if bias else None
+    dy_f32 = int(dy.dtype == torch.float32)
+    nb = _lib.lib().moe_linear_grad_workspace_bytes(n_tok, n_out, act_id, dy_f32, int(bool(bias)))
+    ws = _scratch(nb, x, workspace, who) if nb else None
+    _call("moe_linear_grad", dev, _p(dy), lddy, dy_f32, _p(x), ldx, _p(w), _p(z), ldz, n_tok, n_in, n_out, act_id, dt, _p(ws), _p(dx),
+          _p(dw), int(dw_dtype == torch.float32), _p(db))
+    return dx, dw, db
+
+
+def _dense_layout(t: torch.Tensor) -> bool:
+    """Whether a tensor's elements fill one piece of memory, in whatever order of its dimensions."""
+    if t.is_contiguous() or t.numel() == 0:
+        return True
+    want = 1
+    for step, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if step != want:
+            return False
+        want *= n
+    return True
+
+
+def _tensor_list(who: str, name: str, tensors) -> list:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{who}: {name} must be tensors, not {type(t).__name__}")
+        if t.dtype not in _REAL:
+            raise TypeError(f"{who}: {name}: {t.dtype} (torch.float16, torch.bfloat16 and torch.float32 are supported)")
+        if t.layout != torch.strided or not _dense_layout(t):
+            raise ValueError(f"{who}: {name}: a tensor of shape {tuple(t.shape)} does not fill its memory")
+    return tensors
+
+
+def _clip(who, grads, outs, max_norm):
+    gpus = {t.get_device() for t in grads}
+    if outs is not None:
+        gpus |= {t.get_device() for t in outs}
+    if len(gpus) != 1 or min(gpus) < 0:
+        raise ValueError(f"{who}: the tensors must be on one GPU" + (" (there are none)" if not gpus else f", not {sorted(gpus)}"))
+    dev, n = gpus.pop(), len(grads)
+    sizes = [t.numel() for t in grads]
+    ptrs, types = array("Q", [t.data_ptr() for t in grads]), array("i", [_REAL[t.dtype] for t in grads])
+    out_ptrs = None if outs is None else ptrs if outs is grads else array("Q", [t.data_ptr() for t in outs])
+    lens = array("q", sizes)
+    ws = torch.empty(_lib.lib().moe_clip_workspace_bytes(n, sum(sizes)), dtype=torch.uint8, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _call("moe_clip_grads", dev, n, ptrs.buffer_info()[0], None if out_ptrs is None else out_ptrs.buffer_info()[0],
+          lens.buffer_info()[0], types.buffer_info()[0], max_norm, _p(ws), _p(norm))
+    return norm
+
+
+def grad_norm(grads):
+    """The norm of all tensors together, sqrt(sum of squares), fp32 on their GPU.  Any mixture of fp16, bf16 and fp32 tensors of
+    any shape whose elements fill their memory; the squares are summed in 64 bits."""
+    return _clip("grad_norm", _tensor_list("grad_norm", "grads", grads), None, 0.0)
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """grad_norm, and every tensor times min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_: in place, or into
+    the tensors of `out` (their shapes, types and strides).  Returns the norm before.  Nothing that is written may overlap
+    another tensor (the same one twice in the list, say).  An infinite norm leaves zeros and NaN, a NaN leaves NaN."""
+    who = "clip_grad_norm"
+    grads = _tensor_list(who, "grads", grads)
+    if not max_norm >= 0:
+        raise ValueError(f"{who}: max_norm={max_norm}")
+    outs = grads
+    if out is not None:
+        outs = _tensor_list(who, "out", out)
+        if len(outs) != len(grads):
+            raise ValueError(f"{who}: {len(outs)} tensors in out for {len(grads)}")
+        for g, o in zip(grads, outs):
+            if o.shape != g.shape or o.dtype != g.dtype or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                raise ValueError(f"{who}: out has {o.dtype} {tuple(o.shape)} at {o.stride()} for {g.dtype} {tuple(g.shape)} at {g.stride()}")
+    return _clip(who, grads, outs, float(max_norm))

@@ -1,0 +1,156 @@
+"""Refusals of routing, the weighted sum, shared projections and the gradients' norm, without a GPU: the tensor checks of
+moe_offload.ops and the argument checks of the C entry points, none of which launches anything."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from moe_offload import _lib, dense, ops  # noqa: E402
+
+P = 64                                             # stands for some aligned device address, which is never read here
+BF = torch.bfloat16
+
+
+def refused(name, *args):
+    lib = _lib.lib()
+    lib.c_clear_error()
+    rc = getattr(lib, name)(*args)
+    msg = _lib.last_error()
+    lib.c_clear_error()
+    assert rc == -1 and msg, (name, args)
+    return msg
+
+
+def taken(name, *args):
+    lib = _lib.lib()
+    lib.c_clear_error()
+    assert getattr(lib, name)(*args) == 0 and not _lib.last_error(), (name, args)
+
+
+def swapped(good, i, value):
+    return good[:i] + (value,) + good[i + 1:]
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x, w, l = torch.zeros((4, 16), dtype=BF), torch.zeros((8, 16), dtype=BF), torch.zeros((4, 8))
+    ids, s = torch.zeros((4, 2), dtype=torch.int32), torch.zeros((4, 2))
+    y = torch.zeros((4, 2, 16), dtype=BF)
+    for call in (lambda: ops.route(l, 2), lambda: ops.route_grad(s, l, ids), lambda: ops.combine(y, s), lambda: ops.combine_grad(x, y, s),
+                 lambda: ops.linear(x, w), lambda: ops.linear_grad(x[:, :8], x, w), lambda: dense.route(l, 2), lambda: dense.combine(y, s),
+                 lambda: dense.linear(x, w), lambda: dense.moe_layer(x, w, torch.zeros((8, 16, 16), dtype=BF), torch.zeros((8, 16, 8), dtype=BF), 2)):
+        with pytest.raises(ValueError, match="not on a GPU"):
+            call()
+    for call in (lambda: ops.grad_norm([x]), lambda: ops.clip_grad_norm([x], 1.0)):
+        with pytest.raises(ValueError, match="on one GPU"):
+            call()
+    with pytest.raises(TypeError, match="must be a tensor"):
+        ops.route([1.0], 1)
+    with pytest.raises(TypeError, match="must be tensors"):
+        ops.grad_norm([1.0])
+
+
+def test_row_checks():
+    rows = lambda t, *a: ops._scored_rows("op", "logits", t, *a)  # noqa: E731
+    assert rows(torch.zeros((4, 7))) == 7
+    assert rows(torch.zeros((4, 9), dtype=BF)[:, 2:]) == 9
+    assert rows(torch.zeros((1, 9))[:, :5]) == 5
+    assert rows(torch.zeros((0, 9))) == 9
+    for bad in (torch.zeros(4), torch.zeros((4, 0)), torch.zeros((4, 1025)), torch.zeros((7, 4)).T, torch.zeros((1, 5)).expand(4, 5),
+                torch.zeros(64).as_strided((4, 8), (4, 1))):
+        with pytest.raises(ValueError):
+            rows(bad)
+    with pytest.raises(TypeError):
+        rows(torch.zeros((4, 4), dtype=torch.float64))
+    with pytest.raises(ValueError):
+        rows(torch.zeros((4, 4)), (4, 5))
+    y = torch.zeros((6, 2, 16), dtype=BF)
+    assert ops._pair_rows("op", "y", y, 6, 2, y).shape == (12, 16)
+    assert ops._pair_rows("op", "y", y.reshape(12, 16), 6, 2, y).shape == (12, 16)
+    assert ops._pair_rows("op", "y", torch.zeros((6, 1, 32), dtype=BF)[:, :, :16], 6, 1, y).stride() == (32, 1)
+    for bad in (y[:5], y.reshape(12, 16)[:11], torch.zeros((6, 4, 16), dtype=BF)[:, :2], torch.zeros((2, 6, 16), dtype=BF).transpose(0, 1)):
+        with pytest.raises(ValueError):
+            ops._pair_rows("op", "y", bad, 6, 2, y)
+    for bad in (torch.zeros((16, 12), dtype=BF), torch.zeros((12, 16), dtype=BF), torch.zeros((8, 32), dtype=BF)[:, :16], torch.zeros((0, 16), dtype=BF),
+                torch.zeros((16, 8), dtype=BF).T):
+        with pytest.raises(ValueError):
+            ops._shared_weight("op", bad, BF, 16)
+    ops._shared_weight("op", torch.zeros((8, 16), dtype=BF), BF, 16)
+    for good in (torch.zeros((3, 4)), torch.zeros((3, 4)).T, torch.zeros(0), torch.zeros((2, 3, 4)).permute(2, 0, 1), torch.zeros(())):
+        assert ops._dense_layout(good)
+    for bad in (torch.zeros(8)[::2], torch.zeros(1).expand(4), torch.zeros((4, 8))[:, :4]):
+        assert not ops._dense_layout(bad)
+
+
+def test_layer_shapes_and_constants_are_checked():
+    x, wr = torch.zeros((4, 16), dtype=BF), torch.zeros((8, 16), dtype=BF)
+    with pytest.raises(ValueError, match="do not fit"):
+        dense.moe_layer(x, wr, torch.zeros((9, 16, 16), dtype=BF), torch.zeros((9, 16, 8), dtype=BF), 2)
+    with pytest.raises(ValueError, match="bias has no gradient"):
+        dense.route(torch.zeros((4, 8)), 2, bias=torch.zeros(8, requires_grad=True))
+
+
+def test_route_arguments():
+    good = (P, 512, 4, 512, 10, 0, 1, None, 8, 4, 2, 1.0, 2, P, P, None)
+    for i, bad in ((0, None), (1, 511), (2, -1), (3, 0), (3, 1025), (4, 0), (4, 33), (5, 2), (5, -1), (6, 2), (8, 0), (8, 65), (8, 3), (9, 0),
+                   (9, 9), (10, 0), (10, 3), (12, 3), (12, -1), (13, None), (14, None)):
+        refused("moe_route", *swapped(good, i, bad))
+    refused("moe_route", P, 4, 4, 4, 5, 0, 1, None, 1, 1, 1, 1.0, 2, P, P, None)          # more places than experts
+    taken("moe_route", None, 512, 0, 512, 10, 0, 1, None, 8, 4, 2, 1.0, 2, None, None, None)
+    good = (P, P, 512, P, 4, 512, 10, 0, 1, 1.0, 2, P, 512, None)
+    for i, bad in ((0, None), (1, None), (2, 511), (3, None), (4, -1), (5, 0), (6, 0), (7, 2), (8, 2), (10, 3), (11, None), (12, 511)):
+        refused("moe_route_grad", *swapped(good, i, bad))
+    taken("moe_route_grad", *swapped(good, 4, 0))
+
+
+def test_combine_arguments():
+    good = (P, 64, P, P, 64, 4, 2, 64, 1, 0, P, 64, None)
+    for i, bad in ((0, None), (0, P + 8), (1, 60), (1, 56), (2, None), (3, P + 8), (4, 8), (5, -1), (6, 0), (7, 0), (7, 12), (8, 2), (10, None),
+                   (10, P + 2), (11, 12)):
+        refused("moe_combine", *swapped(good, i, bad))
+    refused("moe_combine", P, 64, P, None, 0, 1 << 20, 1 << 11, 64, 1, 0, P, 64, None)
+    taken("moe_combine", *swapped(good, 5, 0))
+    good = (P, 64, P, 64, P, 4, 2, 64, 1, P, 64, P, None)
+    for i, bad in ((0, None), (1, 12), (2, P + 8), (3, 8), (4, None), (5, -1), (6, 0), (7, 12), (8, -1), (9, None), (10, 60), (11, None)):
+        refused("moe_combine_grad", *swapped(good, i, bad))
+    taken("moe_combine_grad", *swapped(good, 5, 0))
+
+
+def test_linear_arguments():
+    good = (P, 64, P, P, P, 128, 4, 64, 128, 1, 1, 0, P, 128, P, 128, None)
+    for i, bad in ((0, None), (0, P + 8), (1, 56), (1, 68), (2, None), (2, P + 2), (3, P + 8), (4, P + 8), (5, 64), (6, -1), (7, 0), (7, 12), (8, 0),
+                   (8, 12), (9, 4), (9, -1), (10, 2), (12, P + 8), (13, 64), (14, None), (14, P + 8), (15, 64)):
+        refused("moe_linear", *swapped(good, i, bad))
+    refused("moe_linear", P, 64, P, None, None, 0, (1 << 30) + 8, 64, 128, 0, 1, 0, None, 0, P, 128, None)
+    assert "more than one launch" in refused("moe_linear", P, 8, P, None, None, 0, 1 << 30, 8, 1 << 30, 0, 1, 0, None, 0, P, 1 << 30, None)
+    taken("moe_linear", *swapped(good, 6, 0))
+    good = (P, 128, 0, P, 64, P, P, 128, 4, 64, 128, 1, 1, P, P, P, 0, P, None)
+    for i, bad in ((0, None), (1, 64), (3, None), (4, 60), (5, None), (6, None), (7, 64), (8, -1), (8, 1 << 22), (9, 12), (10, 12), (11, 4), (12, 2),
+                   (13, None), (13, P + 8), (14, P + 8), (15, P + 8)):
+        refused("moe_linear_grad", *swapped(good, i, bad))
+    ws = _lib.lib().moe_linear_grad_workspace_bytes
+    assert ws(0, 128, 0, 0, 0) == 0 and ws(100, 128, 0, 0, 0) == 0 and ws(100, 128, 1, 0, 0) >= 2 * 100 * 128 and ws(100, 128, 0, 1, 0) >= 2 * 100 * 128
+    assert ws(100, 128, 0, 0, 1) >= 4 * 128 and ws(1 << 20, 4096, 1, 0, 0) >= 1 << 33
+
+
+def clip(grads, outs, sizes, types, limit=1.0, ws=P, norm=P):
+    n = len(sizes)
+    u64, i64, i32 = ctypes.c_uint64 * max(n, 1), ctypes.c_int64 * max(n, 1), ctypes.c_int32 * max(n, 1)
+    return n, u64(*grads), None if outs is None else u64(*outs), i64(*sizes), i32(*types), limit, ws, norm, None
+
+
+def test_clip_arguments():
+    a = 1 << 20
+    for bad in (clip([a], [a], [4], [3]), clip([a], [a], [-1], [0]), clip([a], [a], [(1 << 40) + 1], [0]), clip([0], [a], [4], [0]), clip([a], [0], [4], [0]),
+                clip([a + 1], [a + 1], [4], [0]), clip([a + 2], [a], [4], [2]), clip([a], [a + 2], [4], [2]), clip([a], [a], [4], [0], -1.0),
+                clip([a], [a], [4], [0], float("nan")), clip([a], [a], [4], [0], ws=None), clip([a], [a], [4], [0], ws=P + 8),
+                clip([a], [a], [4], [0], norm=None)):
+        refused("moe_clip_grads", *bad)
+    refused("moe_clip_grads", -1, None, None, None, None, 1.0, P, P, None)
+    refused("moe_clip_grads", 1, None, None, None, None, 1.0, P, P, None)
+    for bad in (clip([a, a], [a, a], [4, 4], [0, 0]), clip([a, a + 6], [a, a + 6], [4, 4], [0, 0]), clip([a], [a + 2], [4], [0]),
+                clip([a, a + 8], [a + 8, a], [4, 4], [0, 0]), clip([a, a + 100], [a + 200, a + 206], [4, 4], [0, 0]),
+                clip([a, a + 64, a + 2], [a, a + 64, a + 256], [32, 4, 4], [0, 0, 0])):
+        assert "overlaps" in refused("moe_clip_grads", *bad)
+    ws = _lib.lib().moe_clip_workspace_bytes
+    assert ws(0, 0) >= 16 and ws(3, 1 << 20) >= 16 + 8 * 66
