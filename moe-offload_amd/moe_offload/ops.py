@@ -648,11 +648,13 @@ def route(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_
         raise ValueError(f"{who}: n_group={n_group} (1..64, a divisor of {n_exp}), topk_group={topk_group} (1..n_group), "
                          f"group_best={group_best} (1 or 2)")
     if ids is None:
-        ids = torch.empty((n_tok, k), dtype=torch.int32, device=logits.device)
+        ids = logits.new_empty((n_tok, k), dtype=torch.int32)
+    else:
+        _per_place(who, "ids", ids, (n_tok, k), torch.int32)
     if weights is None:
-        weights = torch.empty((n_tok, k), dtype=torch.float32, device=logits.device)
-    _per_place(who, "ids", ids, (n_tok, k), torch.int32)
-    _per_place(who, "weights", weights, (n_tok, k), torch.float32)
+        weights = logits.new_empty((n_tok, k), dtype=torch.float32)
+    else:
+        _per_place(who, "weights", weights, (n_tok, k), torch.float32)
     _call("moe_route", dev, _p(logits), ld, n_tok, n_exp, k, score, int(bool(renorm)), _p(bias), n_group, topk_group, group_best,
           scale, _REAL[logits.dtype], _p(ids), _p(weights))
     return ids, weights
@@ -676,24 +678,29 @@ def route_grad(dweights, logits, ids, score="softmax", renorm=True, scale=1.0, o
     _per_place(who, "ids", ids, (n_tok, k), torch.int32)
     _per_place(who, "dweights", dweights, (n_tok, k), torch.float32)
     if out is None:
-        out = torch.empty((n_tok, n_exp), dtype=logits.dtype, device=logits.device)
-    if out.dtype != logits.dtype:
+        out, ldd = logits.new_empty((n_tok, n_exp)), n_exp
+    elif out.dtype != logits.dtype:
         raise TypeError(f"{who}: out is {out.dtype}, not {logits.dtype}")
-    ldd = _scored_rows(who, "out", out, logits.shape)
+    else:
+        ldd = _scored_rows(who, "out", out, logits.shape)
     _call("moe_route_grad", dev, _p(dweights), _p(logits), ld, _p(ids), n_tok, n_exp, k, score, int(bool(renorm)), scale,
           _REAL[logits.dtype], _p(out), ldd)
     return out
 
 
-def _pair_rows(who: str, name: str, t: torch.Tensor, n_tok: int, k: int, like: torch.Tensor) -> torch.Tensor:
-    """A row per (token, place), given as [n_tok, k, hidden] or [n_tok * k, hidden], in the second form."""
-    if t.dim() == 3 and t.shape[:2] == (n_tok, k):
-        if n_tok > 1 and k > 1 and t.stride(0) != k * t.stride(1):
+def _pair_rows(who: str, name: str, t: torch.Tensor, n_tok: int, k: int) -> tuple[int, int]:
+    """Checks a row per (token, place), given as [n_tok, k, hidden] or [n_tok * k, hidden]; returns hidden and the step."""
+    if t.dim() == 3:
+        if t.shape[0] != n_tok or t.shape[1] != k:
+            raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, not ({n_tok}, {k}, *)")
+        far, near, inner = t.stride()
+        if n_tok > 1 and k > 1 and far != k * near:
             raise ValueError(f"{who}: {name}: a token's rows must follow the token's before it, not {t.stride()}")
-        return t.view(n_tok * k, t.shape[2]) if t.numel() else t.reshape(n_tok * k, t.shape[2])
-    if t.dim() != 2 or t.shape[0] != n_tok * k:
-        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, not ({n_tok}, {k}, *) or ({n_tok * k}, *)")
-    return t
+        hidden, step = t.shape[2], near if k > 1 else far
+        if inner != 1 or hidden % 8 or hidden == 0 or (n_tok * k > 1 and (step < hidden or step % 8)):
+            raise ValueError(f"{who}: {name}: rows of {hidden} elements at {t.stride()} (contiguous, multiples of 8 wanted)")
+        return hidden, step if n_tok * k > 1 else hidden
+    return t.shape[-1], _rows(who, name, t, t.dtype, n_tok * k, None)
 
 
 def _any_rows(who: str, name: str, t: torch.Tensor, dtypes: tuple, rows: int, width: int) -> int:
@@ -701,6 +708,17 @@ def _any_rows(who: str, name: str, t: torch.Tensor, dtypes: tuple, rows: int, wi
     if t.dtype not in dtypes:
         raise TypeError(f"{who}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
     return _rows(who, name, t, t.dtype, rows, width)
+
+
+def _result(who: str, like: torch.Tensor, out: torch.Tensor | None, dtype: torch.dtype | None, rows: int, width: int):
+    """The output and its step: new, of like's type or fp32 as dtype says, or checked."""
+    if out is not None:
+        if dtype not in (None, out.dtype):
+            raise TypeError(f"{who}: out is {out.dtype}, not {dtype}")
+        return out, _any_rows(who, "out", out, (like.dtype, torch.float32), rows, width)
+    if dtype not in (None, like.dtype, torch.float32):
+        raise TypeError(f"{who}: results of {like.dtype} come as {like.dtype} or torch.float32, not {dtype}")
+    return like.new_empty((rows, width), dtype=dtype), width
 
 
 def combine(y, weights, residual=None, dtype=None, out=None):
@@ -717,15 +735,9 @@ def combine(y, weights, residual=None, dtype=None, out=None):
         raise ValueError(f"{who}: weights has shape {tuple(weights.shape)}, not (n_tok, k)")
     n_tok, k = weights.shape
     _per_place(who, "weights", weights, (n_tok, k), torch.float32)
-    y = _pair_rows(who, "y", y, n_tok, k, weights)
-    hidden = y.shape[1]
-    ldy = _rows(who, "y", y, y.dtype, n_tok * k, None)
+    hidden, ldy = _pair_rows(who, "y", y, n_tok, k)
     ldr = _rows(who, "residual", residual, y.dtype, n_tok, hidden) if residual is not None else 0
-    if out is None:
-        out = torch.empty((n_tok, hidden), dtype=dtype or y.dtype, device=y.device)
-    elif dtype not in (None, out.dtype):
-        raise TypeError(f"{who}: out is {out.dtype}, not {dtype}")
-    ldo = _any_rows(who, "out", out, (y.dtype, torch.float32), n_tok, hidden)
+    out, ldo = _result(who, y, out, dtype, n_tok, hidden)
     _call("moe_combine", dev, _p(y), ldy, _p(weights), _p(residual), ldr, n_tok, k, hidden, dt, int(out.dtype == torch.float32),
           _p(out), ldo)
     return out
@@ -740,13 +752,11 @@ def combine_grad(dout, y, weights):
         raise ValueError(f"{who}: weights has shape {tuple(weights.shape)}, not (n_tok, k)")
     n_tok, k = weights.shape
     _per_place(who, "weights", weights, (n_tok, k), torch.float32)
-    rows = _pair_rows(who, "y", y, n_tok, k, weights)
-    hidden = rows.shape[1]
-    ldy = _rows(who, "y", rows, y.dtype, n_tok * k, None)
+    hidden, ldy = _pair_rows(who, "y", y, n_tok, k)
     ldd = _rows(who, "dout", dout, y.dtype, n_tok, hidden)
     dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     dw = torch.empty((n_tok, k), dtype=torch.float32, device=y.device)
-    _call("moe_combine_grad", dev, _p(dout), ldd, _p(rows), ldy, _p(weights), n_tok, k, hidden, dt, _p(dy), hidden, _p(dw))
+    _call("moe_combine_grad", dev, _p(dout), ldd, _p(y), ldy, _p(weights), n_tok, k, hidden, dt, _p(dy), hidden, _p(dw))
     return dy, dw
 
 
@@ -775,11 +785,7 @@ def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out
         _per_place(who, "bias", bias, (n_out,), x.dtype)
     ldr = _rows(who, "residual", residual, x.dtype, n_tok, n_out) if residual is not None else 0
     ldz = _rows(who, "z_out", z_out, x.dtype, n_tok, n_out) if z_out is not None else 0
-    if out is None:
-        out = torch.empty((n_tok, n_out), dtype=dtype or x.dtype, device=x.device)
-    elif dtype not in (None, out.dtype):
-        raise TypeError(f"{who}: out is {out.dtype}, not {dtype}")
-    ldy = _any_rows(who, "out", out, (x.dtype, torch.float32), n_tok, n_out)
+    out, ldy = _result(who, x, out, dtype, n_tok, n_out)
     _call("moe_linear", dev, _p(x), ldx, _p(w), _p(bias), _p(residual), ldr, n_tok, n_in, n_out, act, dt,
           int(out.dtype == torch.float32), _p(z_out), ldz, _p(out), ldy)
     return out

@@ -65,12 +65,16 @@ def test_row_checks():
     with pytest.raises(ValueError):
         rows(torch.zeros((4, 4)), (4, 5))
     y = torch.zeros((6, 2, 16), dtype=BF)
-    assert ops._pair_rows("op", "y", y, 6, 2, y).shape == (12, 16)
-    assert ops._pair_rows("op", "y", y.reshape(12, 16), 6, 2, y).shape == (12, 16)
-    assert ops._pair_rows("op", "y", torch.zeros((6, 1, 32), dtype=BF)[:, :, :16], 6, 1, y).stride() == (32, 1)
-    for bad in (y[:5], y.reshape(12, 16)[:11], torch.zeros((6, 4, 16), dtype=BF)[:, :2], torch.zeros((2, 6, 16), dtype=BF).transpose(0, 1)):
+    pairs = lambda t: ops._pair_rows("op", "y", t, 6, 2)  # noqa: E731
+    assert pairs(y) == (16, 16) and pairs(y.reshape(12, 16)) == (16, 16) and pairs(torch.zeros((6, 2, 32), dtype=BF)[:, :, 8:24]) == (16, 32)
+    assert ops._pair_rows("op", "y", torch.zeros((6, 1, 32), dtype=BF)[:, :, :16], 6, 1) == (16, 32)
+    assert ops._pair_rows("op", "y", torch.zeros((1, 4, 16), dtype=BF)[:, 1:2], 1, 1) == (16, 16)
+    assert ops._pair_rows("op", "y", torch.zeros((0, 2, 16), dtype=BF), 0, 2) == (16, 16)
+    for bad in (y[:5], y.reshape(12, 16)[:11], torch.zeros((6, 4, 16), dtype=BF)[:, :2], torch.zeros((2, 6, 16), dtype=BF).transpose(0, 1),
+                torch.zeros((6, 2, 12), dtype=BF), torch.zeros((6, 2, 0), dtype=BF), torch.zeros((6, 16, 2), dtype=BF).transpose(1, 2),
+                torch.zeros((6, 2, 20), dtype=BF)[:, :, :16], torch.zeros((1, 1, 16), dtype=BF).expand(6, 2, 16), torch.zeros(192, dtype=BF)):
         with pytest.raises(ValueError):
-            ops._pair_rows("op", "y", bad, 6, 2, y)
+            pairs(bad)
     for bad in (torch.zeros((16, 12), dtype=BF), torch.zeros((12, 16), dtype=BF), torch.zeros((8, 32), dtype=BF)[:, :16], torch.zeros((0, 16), dtype=BF),
                 torch.zeros((16, 8), dtype=BF).T):
         with pytest.raises(ValueError):
