@@ -19,6 +19,8 @@ namespace {
 constexpr int kTable = 96;                 // ranges of a launch: the table stays below the 4 KiB that a launch's arguments have
 constexpr int kClipThreads = 256;
 constexpr int kChunk = 16384;              // elements of a block
+constexpr uint32_t kMostChunks = 1u << 23; // of a launch (2^31 threads)
+constexpr uint32_t kSquareBlocks = 2048;   // of a launch: eight per CU, each with a sum
 constexpr int kHead = 16;                  // bytes of the workspace before the blocks' sums: the factor
 
 struct Range {
@@ -49,34 +51,48 @@ __device__ __forceinline__ int range_of(const Table& t, uint32_t chunk) {
 template <typename T>
 constexpr int kPer = 16 / (int)sizeof(T);
 
-// Calls f(i, whole) for this thread's groups of kPer elements of a chunk: elements i .. i + kPer - 1 of the range, of which
-// some lie outside 0 .. n - 1 where whole is false.
+// Calls f(values, i, from, to) for this thread's groups of kPer elements i .. i + kPer - 1 of a chunk, of which from .. to - 1
+// (counted from i) are the range's.  A chunk that is the range's as a whole is loaded at once.
 template <typename T, typename F>
 __device__ __forceinline__ void for_chunk(const Range& r, uint32_t chunk, const F& f) {
-    const int64_t skew = ((uintptr_t)r.p % 16) / sizeof(T);
-    const int64_t from = (int64_t)chunk * kChunk - skew;
-#pragma unroll 4
-    for (int j = 0; j < kChunk / (kPer<T> * kClipThreads); ++j) {
-        const int64_t i = from + (int64_t)(j * kClipThreads + threadIdx.x) * kPer<T>;
-        if (i >= r.n || i <= -kPer<T>) continue;
-        f(i, i >= 0 && i + kPer<T> <= r.n);
+    typedef T tv __attribute__((ext_vector_type(kPer<T>)));
+    constexpr int kGroups = kChunk / (kPer<T> * kClipThreads), kAtOnce = 8;
+    const int64_t skew = ((uintptr_t)r.p % 16) / sizeof(T), first = (int64_t)chunk * kChunk - skew;
+    const int64_t i0 = first + (int64_t)threadIdx.x * kPer<T>;
+    if (first >= 0 && first + kChunk <= r.n) {
+        const tv* p = (const tv*)((const T*)r.p + i0);
+#pragma unroll
+        for (int j0 = 0; j0 < kGroups; j0 += kAtOnce) {
+            tv v[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) v[j] = p[(j0 + j) * kClipThreads];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) f(v[j], i0 + (int64_t)(j0 + j) * kClipThreads * kPer<T>, 0, kPer<T>);
+        }
+        return;
+    }
+    for (int j = 0; j < kGroups; ++j) {
+        const int64_t i = i0 + (int64_t)j * kClipThreads * kPer<T>;
+        const int from = i < 0 ? (int)(i > -kPer<T> ? -i : kPer<T>) : 0, to = i + kPer<T> <= r.n ? kPer<T> : i < r.n ? (int)(r.n - i) : 0;
+        if (from >= to) continue;
+        tv v = {};
+        if (from == 0 && to == kPer<T>) {
+            v = *(const tv*)((const T*)r.p + i);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer<T>; ++e)
+                if (e >= from && e < to) v[e] = ((const T*)r.p)[i + e];
+        }
+        f(v, i, from, to);
     }
 }
 
 template <typename T>
 __device__ __forceinline__ double squares(const Range& r, uint32_t chunk) {
-    typedef T tv __attribute__((ext_vector_type(kPer<T>)));
     double sum = 0;
-    for_chunk<T>(r, chunk, [&](int64_t i, bool whole) {
-        const T* p = (const T*)r.p + i;
-        if (whole) {
-            const tv v = *(const tv*)p;
+    for_chunk<T>(r, chunk, [&](auto v, int64_t, int, int) {                    // (zeros where the range has none)
 #pragma unroll
-            for (int e = 0; e < kPer<T>; ++e) sum += (double)(float)v[e] * (double)(float)v[e];
-        } else {
-            for (int e = 0; e < kPer<T>; ++e)
-                if (i + e >= 0 && i + e < r.n) sum += (double)(float)p[e] * (double)(float)p[e];
-        }
+        for (int e = 0; e < kPer<T>; ++e) sum += (double)(float)v[e] * (double)(float)v[e];
     });
     return sum;
 }
@@ -90,13 +106,16 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
     return v;
 }
 
-__global__ __launch_bounds__(kClipThreads) void k_clip_squares(Table t, double* __restrict__ sums) {
+__global__ __launch_bounds__(kClipThreads) void k_clip_squares(Table t, uint32_t chunks, double* __restrict__ sums) {
     __shared__ double scratch[kClipThreads / 64];
-    const int i = range_of(t, blockIdx.x);
-    const uint32_t chunk = blockIdx.x - t.first[i];
-    const int type = t.type[i];
-    const double v = type == 0 ? squares<_Float16>(t.range[i], chunk)
-                     : type == 1 ? squares<__bf16>(t.range[i], chunk) : squares<float>(t.range[i], chunk);
+    double v = 0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int i = range_of(t, c);
+        const uint32_t chunk = c - t.first[i];
+        const int type = t.type[i];
+        v += type == 0 ? squares<_Float16>(t.range[i], chunk)
+             : type == 1 ? squares<__bf16>(t.range[i], chunk) : squares<float>(t.range[i], chunk);
+    }
     const double sum = block_sum(v, scratch);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
@@ -116,29 +135,30 @@ __global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ s
 
 template <typename T>
 __device__ __forceinline__ void scale(const Range& r, uint32_t chunk, float f) {
-    typedef T tv __attribute__((ext_vector_type(kPer<T>)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const bool aligned = ((uintptr_t)r.p - (uintptr_t)r.out) % 16 == 0;
-    for_chunk<T>(r, chunk, [&](int64_t i, bool whole) {
-        const T* p = (const T*)r.p + i;
+    for_chunk<T>(r, chunk, [&](auto v, int64_t i, int from, int to) {
         T* o = (T*)r.out + i;
-        if (whole && aligned) {
-            tv v = *(const tv*)p;
 #pragma unroll
-            for (int e = 0; e < kPer<T>; ++e) v[e] = (T)((float)v[e] * f);
-            *(tv*)o = v;
+        for (int e = 0; e < kPer<T>; ++e) v[e] = (T)((float)v[e] * f);
+        if (aligned && from == 0 && to == kPer<T>) {
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)o);
         } else {
+#pragma unroll
             for (int e = 0; e < kPer<T>; ++e)
-                if (i + e >= 0 && i + e < r.n) o[e] = (T)((float)p[e] * f);
+                if (e >= from && e < to) o[e] = v[e];
         }
     });
 }
 
-__global__ __launch_bounds__(kClipThreads) void k_clip_scale(Table t, const float* __restrict__ factor) {
+// Chunks from the last to the first: what the squares' pass read last may still be in the caches.
+__global__ __launch_bounds__(kClipThreads) void k_clip_scale(Table t, uint32_t chunks, const float* __restrict__ factor) {
     const float f = *factor;
-    const int i = range_of(t, blockIdx.x);
+    const uint32_t c = chunks - 1 - blockIdx.x;
+    const int i = range_of(t, c);
     const Range r = t.range[i];
     if (f == 1.f && r.p == r.out) return;
-    const uint32_t chunk = blockIdx.x - t.first[i];
+    const uint32_t chunk = c - t.first[i];
     const int type = t.type[i];
     if (type == 0) scale<_Float16>(r, chunk, f);
     else if (type == 1) scale<__bf16>(r, chunk, f);
@@ -152,14 +172,18 @@ uint64_t chunks_of(const void* p, int64_t n, int type) {
     return n > 0 ? (skew + (uint64_t)n + kChunk - 1) / kChunk : 0;
 }
 
+struct Item {
+    Range r;
+    int type;
+};
+
 // Whether something is written where something else is read or written.
-bool overlap(int n, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* types) {
+bool overlap(const std::vector<Item>& items) {
     struct Span { uintptr_t a, b; bool out; };
     std::vector<Span> spans;
-    spans.reserve(2 * (size_t)n);
-    for (int i = 0; i < n; ++i) {
-        if (sizes[i] == 0) continue;
-        const uintptr_t bytes = (uintptr_t)sizes[i] * size_of(types[i]), g = (uintptr_t)grads[i], o = (uintptr_t)outs[i];
+    spans.reserve(2 * items.size());
+    for (const Item& it : items) {
+        const uintptr_t bytes = (uintptr_t)it.r.n * size_of(it.type), g = (uintptr_t)it.r.p, o = (uintptr_t)it.r.out;
         if (g != o) spans.push_back({g, g + bytes, false});
         spans.push_back({o, o + bytes, true});
     }
@@ -175,8 +199,8 @@ bool overlap(int n, const void* const* grads, void* const* outs, const int64_t* 
 
 int clip(int n, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* types, double max_norm,
          void* workspace, float* norm, hipStream_t s) {
-    // ranges of neighbours in memory are one
-    struct Item { Range r; int type; };
+    // Ranges of neighbours in memory are one: gradients that are views of a flat buffer, in its order, need one launch
+    // however many they are (384 of them 0.13 ms on the host as ranges of their own, 0.01 as one).
     std::vector<Item> items;
     for (int i = 0; i < n; ++i) {
         if (sizes[i] == 0) continue;
@@ -191,27 +215,29 @@ int clip(int n, const void* const* grads, void* const* outs, const int64_t* size
         }
         items.push_back({{grads[i], out, sizes[i]}, types[i]});
     }
+    if (outs && overlap(items)) {
+        moe_set_error("clip_grads: what is written overlaps another tensor");
+        return -1;
+    }
     double* sums = (double*)((char*)workspace + kHead);
     float* factor = (float*)workspace;
+    // Calls launch(table, chunks) for as many ranges as one takes at a time.
     auto launches = [&](auto&& launch) {
         Table t;
         t.n = 0;
         t.first[0] = 0;
-        uint64_t before = 0;
         auto flush = [&]() {
             if (t.n == 0) return hipSuccess;
-            launch(t, before);
-            before += t.first[t.n];
+            launch(t, t.first[t.n]);
             t.n = 0;
             return hipGetLastError();
         };
-        constexpr uint64_t kMost = 1u << 23;                                   // blocks of a launch (2^31 threads)
         for (const Item& it : items) {
             // a range of more chunks than a launch takes is cut at a chunk's end, where its address is aligned
             Range r = it.r;
             while (r.n > 0) {
                 const int64_t skew = ((uintptr_t)r.p % 16) / size_of(it.type);
-                const uint64_t room = kMost - t.first[t.n], want = chunks_of(r.p, r.n, it.type), have = std::min(room, want);
+                const uint64_t room = kMostChunks - t.first[t.n], want = chunks_of(r.p, r.n, it.type), have = std::min(room, want);
                 const int64_t take = have == want ? r.n : (int64_t)have * kChunk - skew;
                 t.range[t.n] = {r.p, r.out, take};
                 t.type[t.n] = (uint8_t)it.type;
@@ -220,22 +246,23 @@ int clip(int n, const void* const* grads, void* const* outs, const int64_t* size
                 r.p = (const char*)r.p + take * size_of(it.type);
                 if (r.out) r.out = (char*)r.out + take * size_of(it.type);
                 r.n -= take;
-                if (t.n == kTable || t.first[t.n] == kMost)
+                if (t.n == kTable || t.first[t.n] == kMostChunks)
                     if (const hipError_t e = flush()) return e;
             }
         }
         return flush();
     };
-    uint64_t chunks = 0;
-    HIP_TRY(launches([&](const Table& t, uint64_t before) {
-        hipLaunchKernelGGL(k_clip_squares, dim3(t.first[t.n]), dim3(kClipThreads), 0, s, t, sums + before);
-        chunks = before + t.first[t.n];
+    int64_t blocks = 0;
+    HIP_TRY(launches([&](const Table& t, uint32_t chunks) {
+        const uint32_t grid = chunks < kSquareBlocks ? chunks : kSquareBlocks;
+        hipLaunchKernelGGL(k_clip_squares, dim3(grid), dim3(kClipThreads), 0, s, t, chunks, sums + blocks);
+        blocks += grid;
     }));
-    hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(1024), 0, s, sums, (int64_t)chunks, max_norm, factor, norm);
+    hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(1024), 0, s, sums, blocks, max_norm, factor, norm);
     HIP_TRY(hipGetLastError());
     if (!outs) return 0;
-    HIP_TRY(launches([&](const Table& t, uint64_t) {
-        hipLaunchKernelGGL(k_clip_scale, dim3(t.first[t.n]), dim3(kClipThreads), 0, s, t, factor);
+    HIP_TRY(launches([&](const Table& t, uint32_t chunks) {
+        hipLaunchKernelGGL(k_clip_scale, dim3(chunks), dim3(kClipThreads), 0, s, t, chunks, factor);
     }));
     return 0;
 }
@@ -271,10 +298,6 @@ extern "C" int moe_clip_grads(int n, const void* const* grads, void* const* outs
         }
     }
     try {
-        if (outs && overlap(n, grads, outs, sizes, types)) {
-            moe_set_error("clip_grads: what is written overlaps another tensor");
-            return -1;
-        }
         return clip(n, grads, outs, sizes, types, max_norm, workspace, norm, (hipStream_t)stream);
     } catch (const std::exception& e) {
         moe_set_error("clip_grads: %s", e.what());

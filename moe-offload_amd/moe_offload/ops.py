@@ -6,6 +6,7 @@ no PyTorch fallback for any of them.
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -826,6 +827,8 @@ def linear_grad(dy, x, w, z=None, act=None, bias=False, want_dx=True, want_dw=Tr
 
 def _dense_layout(t: torch.Tensor) -> bool:
     """Whether a tensor's elements fill one piece of memory, in whatever order of its dimensions."""
+    if t.layout != torch.strided:
+        return False
     if t.is_contiguous() or t.numel() == 0:
         return True
     want = 1
@@ -836,40 +839,47 @@ def _dense_layout(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensor_list(who: str, name: str, tensors) -> list:
+_dtype_of = attrgetter("dtype")
+_Tensor = torch.Tensor
+
+
+def _tensor_list(who: str, name: str, tensors) -> tuple[list, array]:
+    """The tensors of a list and their types' numbers.  (Lists are long: whole passes in C, no code per tensor.)"""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{who}: {name} must be tensors, not {type(t).__name__}")
-        if t.dtype not in _REAL:
-            raise TypeError(f"{who}: {name}: {t.dtype} (torch.float16, torch.bfloat16 and torch.float32 are supported)")
-        if t.layout != torch.strided or not _dense_layout(t):
-            raise ValueError(f"{who}: {name}: a tensor of shape {tuple(t.shape)} does not fill its memory")
-    return tensors
+    for kind in set(map(type, tensors)):
+        if not issubclass(kind, torch.Tensor):
+            raise TypeError(f"{who}: {name} must be tensors, not {kind.__name__}")
+    types = list(map(_REAL.get, map(_dtype_of, tensors)))
+    if None in types:
+        raise TypeError(f"{who}: {name}: {tensors[types.index(None)].dtype} (torch.float16, torch.bfloat16 and torch.float32 are supported)")
+    if not all(map(_Tensor.is_contiguous, tensors)):
+        for t in tensors:
+            if not _dense_layout(t):
+                raise ValueError(f"{who}: {name}: a tensor of shape {tuple(t.shape)} does not fill its memory")
+    return tensors, array("i", types)
 
 
-def _clip(who, grads, outs, max_norm):
-    gpus = {t.get_device() for t in grads}
-    if outs is not None:
-        gpus |= {t.get_device() for t in outs}
+def _clip(who, grads, types, outs, max_norm):
+    gpus = set(map(_Tensor.get_device, grads))
+    if outs is not None and outs is not grads:
+        gpus.update(map(_Tensor.get_device, outs))
     if len(gpus) != 1 or min(gpus) < 0:
         raise ValueError(f"{who}: the tensors must be on one GPU" + (" (there are none)" if not gpus else f", not {sorted(gpus)}"))
-    dev, n = gpus.pop(), len(grads)
-    sizes = [t.numel() for t in grads]
-    ptrs, types = array("Q", [t.data_ptr() for t in grads]), array("i", [_REAL[t.dtype] for t in grads])
-    out_ptrs = None if outs is None else ptrs if outs is grads else array("Q", [t.data_ptr() for t in outs])
-    lens = array("q", sizes)
-    ws = torch.empty(_lib.lib().moe_clip_workspace_bytes(n, sum(sizes)), dtype=torch.uint8, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _call("moe_clip_grads", dev, n, ptrs.buffer_info()[0], None if out_ptrs is None else out_ptrs.buffer_info()[0],
-          lens.buffer_info()[0], types.buffer_info()[0], max_norm, _p(ws), _p(norm))
+    dev = gpus.pop()
+    # (an array takes a list faster than a map)
+    sizes, ptrs = array("q", list(map(_Tensor.numel, grads))), array("Q", list(map(_Tensor.data_ptr, grads)))
+    out_ptrs = None if outs is None else ptrs if outs is grads else array("Q", list(map(_Tensor.data_ptr, outs)))
+    ws = grads[0].new_empty(_lib.lib().moe_clip_workspace_bytes(len(grads), sum(sizes)), dtype=torch.uint8)
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    _call("moe_clip_grads", dev, len(grads), ptrs.buffer_info()[0], None if out_ptrs is None else out_ptrs.buffer_info()[0],
+          sizes.buffer_info()[0], types.buffer_info()[0], max_norm, _p(ws), _p(norm))
     return norm
 
 
 def grad_norm(grads):
     """The norm of all tensors together, sqrt(sum of squares), fp32 on their GPU.  Any mixture of fp16, bf16 and fp32 tensors of
     any shape whose elements fill their memory; the squares are summed in 64 bits."""
-    return _clip("grad_norm", _tensor_list("grad_norm", "grads", grads), None, 0.0)
+    return _clip("grad_norm", *_tensor_list("grad_norm", "grads", grads), None, 0.0)
 
 
 def clip_grad_norm(grads, max_norm, out=None):
@@ -877,15 +887,15 @@ def clip_grad_norm(grads, max_norm, out=None):
     the tensors of `out` (their shapes, types and strides).  Returns the norm before.  Nothing that is written may overlap
     another tensor (the same one twice in the list, say).  An infinite norm leaves zeros and NaN, a NaN leaves NaN."""
     who = "clip_grad_norm"
-    grads = _tensor_list(who, "grads", grads)
+    grads, types = _tensor_list(who, "grads", grads)
     if not max_norm >= 0:
         raise ValueError(f"{who}: max_norm={max_norm}")
     outs = grads
     if out is not None:
-        outs = _tensor_list(who, "out", out)
+        outs, _ = _tensor_list(who, "out", out)
         if len(outs) != len(grads):
             raise ValueError(f"{who}: {len(outs)} tensors in out for {len(grads)}")
         for g, o in zip(grads, outs):
             if o.shape != g.shape or o.dtype != g.dtype or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
                 raise ValueError(f"{who}: out has {o.dtype} {tuple(o.shape)} at {o.stride()} for {g.dtype} {tuple(g.shape)} at {g.stride()}")
-    return _clip(who, grads, outs, float(max_norm))
+    return _clip(who, grads, types, outs, float(max_norm))

@@ -48,6 +48,9 @@ def test_tensors_off_the_gpu_are_refused():
         ops.route([1.0], 1)
     with pytest.raises(TypeError, match="must be tensors"):
         ops.grad_norm([1.0])
+    for sparse in (torch.eye(4).to_sparse(), torch.eye(4).to_sparse_csr()):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.grad_norm([sparse])
 
 
 def test_row_checks():
