@@ -385,9 +385,9 @@ int moe_linear(const void* x, int64_t ldx, const void* w, const void* bias, cons
                int n_out, int act, int dtype, int out_f32, void* z, int64_t ldz, void* y, int64_t ldy, void* stream);
 /* Its gradients from dy (of the inputs' type, or fp32: dy_f32 != 0) and the z it kept (act != 0): dz = dy act'(z), rounded to
  * the inputs' type, dx [n_tok][n_in] = dz W, dw [n_out][n_in] = dz^T x (fp32 if dw_f32 != 0), db [n_out] = the sum of dz over
- * the tokens; the residual's is dy.  Those that are null are not computed; outputs are contiguous.  n_tok up to 2^22 - 64.
+ * the tokens; the residual's is dy.  Those that are null are not computed; outputs are contiguous.
  * workspace: moe_linear_grad_workspace_bytes bytes, 16-byte aligned, any contents, one per call in flight. */
-uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_out, int act, int dy_f32, int want_db);
+uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_in, int n_out, int act, int dy_f32, int want_dw, int want_db);
 int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const void* x, int64_t ldx, const void* w, const void* z, int64_t ldz,
                     int n_tok, int n_in, int n_out, int act, int dtype, void* workspace, void* dx, void* dw, int dw_f32, void* db,
                     void* stream);

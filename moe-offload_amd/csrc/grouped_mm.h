@@ -9,26 +9,12 @@ constexpr int kMaxSeg = 1024;
 constexpr int kMaxSide = 1 << 30;     // rows, columns and contractions: sums of two of them and a tile stay below 2^31
 constexpr int64_t kMaxThreads = 0xFFFFFFFF;                   // of a launch, in a dimension
 
-// Rows r of segment s: seg_start[s] .. seg_start[s + 1] - 1, weights of slot seg_slot[s] (s where null).  start null: one
-// segment of all rows.
+// Rows r of segment s: seg_start[s] .. seg_start[s + 1] - 1, weights of slot seg_slot[s] (s where null).
 struct Segs {
     const int32_t* start;
     const int32_t* slot;
     int n_seg, n_rows, n_slots, fill;
 };
-
-// A projection that all rows share, y = act(x w^T + bias) + res with z = x w^T + bias kept where z is not null, and its
-// gradients: dx = dz w, dw = dz^T x.  Arguments as moe_linear's and checked there; act: linear.h's.
-struct Linear {
-    const void *x, *w, *bias, *res;
-    void *y, *z;
-    int64_t ldx, ldr, ldy, ldz;
-    int n_rows, n, k, act, out_f32;
-};
-int linear(const Linear& l, int dtype, hipStream_t s);
-int linear_dx(const void* dz, int64_t lddz, const void* w, void* dx, int n_rows, int n, int k, int dtype, bool dry, hipStream_t s);
-int linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int n_rows, int n, int k, int out_f32, int dtype,
-              bool dry, hipStream_t s);
 
 // dx[rows[r]] = W_u^T (dv[3 rows[r]] + dv[3 rows[r] + 1] + dv[3 rows[r] + 2]), W_u [n][k] of dtype, dv three bf16 parts
 // of a value each (bf16_parts); zeros for rows of no segment.  dry: launches nothing, -1 if one launch does not take it.
@@ -58,7 +44,7 @@ __device__ __forceinline__ uint32_t dealt(uint32_t b, uint32_t nb, uint32_t run)
 // unless they are to be filled with zeros.
 __device__ __forceinline__ void seg_rows(const Segs& S, int v, int& r0, int& r1, int& slot) {
     auto at = [&](int i) {
-        const int r = S.start ? S.start[i] : i ? S.n_rows : 0;
+        const int r = S.start[i];
         return r < 0 ? 0 : r > S.n_rows ? S.n_rows : r;
     };
     slot = -1;
@@ -91,16 +77,6 @@ struct Tile {
 // order and the sums wrap: the block then has no rows.)
 template <int THREADS>
 __device__ __forceinline__ bool find_tile(const Segs& S, int bm, int n_col, uint32_t* scratch, Tile& out) {
-    if (!S.start) {
-        const uint32_t total = tiles_of(S.n_rows, bm);
-        if (blockIdx.x >= (uint64_t)total * n_col) return false;
-        const uint32_t item = xcd_order(blockIdx.x, total * (uint32_t)n_col);
-        out.r0 = (int)(item / (uint32_t)n_col) * bm;
-        out.r1 = out.r0 + bm < S.n_rows ? out.r0 + bm : S.n_rows;
-        out.slot = 0;
-        out.col = (int)(item % (uint32_t)n_col);
-        return true;
-    }
     uint32_t* wave_sum = scratch;
     int* found = (int*)(scratch + THREADS / 64);
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
@@ -199,29 +175,6 @@ __device__ __forceinline__ f32x4 mfma_parts(uint4 a, uint4 b, f32x4 c) {
         add(a);
     }
     return c;
-}
-
-// The activations, and their slopes.  Arguments past -200 are taken there, where both are their limits (0): an infinity
-// would meet a zero.  A NaN stays one.
-enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu2 = 3 };
-
-__device__ __forceinline__ float activation(int act, float z) {
-    if (act == kActNone) return z;
-    if (act == kActRelu2) return z < 0.f ? 0.f : z * z;
-    const float low = z < -200.f ? -200.f : z;
-    if (act == kActSilu) return low / (1.0f + __expf(-low));
-    return 0.5f * low * erfcf(low * -0.70710678f);
-}
-
-__device__ __forceinline__ float slope(int act, float z) {
-    if (act == kActNone) return 1.f;
-    if (act == kActRelu2) return z < 0.f ? 0.f : 2.f * z;
-    const float low = z < -200.f ? -200.f : z, both = low > 200.f ? 200.f : low;
-    if (act == kActSilu) {
-        const float sg = 1.0f / (1.0f + __expf(-low));
-        return sg * (1.0f + both * (1.0f - sg));
-    }
-    return 0.5f * erfcf(both * -0.70710678f) + both * 0.39894228f * __expf(-0.5f * both * both);
 }
 
 template <typename T>

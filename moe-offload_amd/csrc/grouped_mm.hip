@@ -12,9 +12,7 @@
 // rows by 2-bit experts only (mlx-qwen38/prefill_qproj.py:18-40); these are the same products for the
 // weights before quantisation.
 //
-//     linear   y[r]           = act(z) + residual[r],  z = W x[r] + bias: one segment of all rows (moe_linear)
-//
-// All are one tile product  out[p][q] = sum over c of P[p][c] Q[q][c]  with q the direction in which
+// All four are one tile product  out[p][q] = sum over c of P[p][c] Q[q][c]  with q the direction in which
 // the output is contiguous; an operand is either contiguous in c (x, dy; W for mm) or has its c along the
 // rows of memory (W for mm_dx, both operands for mm_dw).  The matrix unit takes Q as its first operand,
 // so a lane of the result holds four adjacent q of one p.
@@ -29,7 +27,7 @@ namespace {
 
 using namespace gmm;
 
-enum { kMM = 0, kGateUp = 1, kDx = 2, kDxGlu = 3, kDw = 4, kDxParts = 5, kLinear = 6 };
+enum { kMM = 0, kGateUp = 1, kDx = 2, kDxGlu = 3, kDw = 4, kDxParts = 5 };
 
 struct Args {
     Segs S;
@@ -49,10 +47,6 @@ struct Args {
     int span;                    // column tiles per block
     int fold;                    // kDxParts: the weights' rows, which the contraction goes through three times
     int dry;                     // only whether one launch takes the call
-    const void* bias;            // linear: of the output columns (may be null)
-    const void* res;             // and a residual (may be null), ldgu and gu_out: where z goes (may be null)
-    int64_t ldres;
-    int act;
 };
 
 // A block of WP x WQ waves computes `span` tiles of BP x BQ results side by side in q.  A step of 64 contraction
@@ -64,13 +58,13 @@ struct Args {
 template <typename T, int OP, int BP, int BQ, int WP, int WQ, int BLOCKS>
 __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
-    constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx && OP != kLinear;
+    constexpr bool kAlongP = OP == kDw, kAlongQ = OP >= kDx;
     constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves;        // 1 KiB each
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
     constexpr int kQStep = OP == kGateUp ? BQ / 2 : BQ;                        // output columns of a tile
     static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1, "");
-    constexpr bool kThroughLds = OP == kDxGlu || OP == kLinear || (OP != kGateUp && BP >= 128);
-    static_assert(!kThroughLds || ((SQ == 4 || OP == kLinear) && kStage / kWaves >= SQ * 1024), "");
+    constexpr bool kThroughLds = OP == kDxGlu || (OP != kGateUp && BP >= 128);
+    static_assert(!kThroughLds || (SQ == 4 && kStage / kWaves >= 4096), "");
     constexpr int kIdx = 1024;                                                 // mm_dw: rows whose numbers are held
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     __shared__ int2 idx[OP == kDw ? kIdx : 1];
@@ -367,59 +361,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BLOCKS) void k_grouped(Args a) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            if constexpr (OP == kLinear) {
-                // z in fp32, one subtile row at a time; a lane then has 8 adjacent columns of a row
-                constexpr int kUnits = SQ * 2, kRowsPer = 64 / kUnits;
-                auto at = [&](int row, int u) { return area + (uint32_t)(row * SQ * 4 + (u ^ (row & 7))) * 16; };
-                const int u8 = l % kUnits, c = col + u8 * 8;
-                const bool in = c < a.nq;
-                f32x4 b[2] = {};
-                if (a.bias && in) {
-                    const uint4 v = *(const uint4*)((const T*)a.bias + c);
-                    b[0] = widen4<T>(make_uint2(v.x, v.y));
-                    b[1] = widen4<T>(make_uint2(v.z, v.w));
-                }
-#pragma unroll
-                for (int i = 0; i < SP; ++i) {
-                    constexpr int kIts = 16 / kRowsPer;
-                    uint4 rv[kIts];
-                    int64_t o[kIts];
-#pragma unroll
-                    for (int it = 0; it < kIts; ++it) {
-                        const int r = r0 + wp * SP * 16 + i * 16 + it * kRowsPer + l / kUnits;
-                        o[it] = r < r1 && in ? r : -1;
-                        rv[it] = a.res && o[it] >= 0 ? *(const uint4*)((const T*)a.res + o[it] * a.ldres + c) : make_uint4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < SQ; ++j) *(lds16)(uintptr_t)at(n, 4 * j + kq) = __builtin_bit_cast(u32x4, acc[i][j]);
-#pragma unroll
-                    for (int it = 0; it < kIts; ++it) {
-                        const int m = it * kRowsPer + l / kUnits;
-                        f32x4 z[2], y[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            z[h] = __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + h)) + b[h];
-                            const f32x4 rs = widen4<T>(h ? make_uint2(rv[it].z, rv[it].w) : make_uint2(rv[it].x, rv[it].y));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) y[h][e] = activation(a.act, z[h][e]) + rs[e];
-                        }
-                        if (o[it] < 0) continue;
-                        auto both = [](const f32x4 (&v)[2]) {
-                            const uint2 lo = round4<T>(v[0]), hi = round4<T>(v[1]);
-                            return make_uint4(lo.x, lo.y, hi.x, hi.y);
-                        };
-                        if (a.gu_out) store16((T*)a.gu_out + o[it] * a.ldgu + c, both(z));
-                        if (a.out_f32) {
-                            float* d = (float*)a.out + o[it] * a.ldo + c;
-                            store16(d, __builtin_bit_cast(uint4, y[0]));
-                            store16(d + 4, __builtin_bit_cast(uint4, y[1]));
-                        } else {
-                            store16((T*)a.out + o[it] * a.ldo + c, both(y));
-                        }
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            } else if constexpr (OP == kDxGlu) {
+            if constexpr (OP == kDxGlu) {
                 // dh in fp32, one subtile row at a time; a lane then has 8 adjacent columns of a row, of dh and of (g, u)
                 auto at = [&](int row, int u) { return area + (uint32_t)(row * 16 + (u ^ (row & 7))) * 16; };
                 const int u8 = l & 7, c = col + u8 * 8;
@@ -815,32 +757,6 @@ int gmm::dx_of_parts(const void* dv, const int32_t* rows, int n_rows, const int3
     a.p = dv, a.q = w, a.out = dx, a.row_p = a.row_out = rows;
     a.ldp = 3 * (int64_t)n, a.ldq = w_stride, a.ldo = lddx, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = 3 * n, a.fold = n;
     return launch_typed<kDxParts>(a, dtype, s);
-}
-
-int gmm::linear(const Linear& l, int dtype, hipStream_t s) {
-    Args a = {};
-    a.S = Segs{nullptr, nullptr, 1, l.n_rows, 1, 0};
-    a.p = l.x, a.q = l.w, a.out = l.y, a.bias = l.bias, a.res = l.res, a.gu_out = l.z;
-    a.ldp = l.ldx, a.ldo = l.ldy, a.ldres = l.ldr, a.ldgu = l.ldz;
-    a.n_p = a.n_out = l.n_rows, a.nq = l.n, a.nc = l.k, a.act = l.act, a.out_f32 = l.out_f32;
-    return launch_typed<kLinear>(a, dtype, s);
-}
-
-int gmm::linear_dx(const void* dz, int64_t lddz, const void* w, void* dx, int n_rows, int n, int k, int dtype, bool dry, hipStream_t s) {
-    Args a = {};
-    a.dry = dry;
-    a.S = Segs{nullptr, nullptr, 1, n_rows, 1, 0};
-    a.p = dz, a.q = w, a.out = dx, a.ldp = lddz, a.ldo = k, a.n_p = a.n_out = n_rows, a.nq = k, a.nc = n;
-    return launch_typed<kDx>(a, dtype, s);
-}
-
-int gmm::linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, void* dw, int n_rows, int n, int k, int out_f32, int dtype,
-                   bool dry, hipStream_t s) {
-    Args a = {};
-    a.dry = dry;
-    a.S = Segs{nullptr, nullptr, 1, n_rows, 1, 0};
-    a.p = dz, a.q = x, a.out = dw, a.ldp = lddz, a.ldq = ldx, a.n_p = n_rows, a.n_q = n_rows, a.np = n, a.nq = k, a.out_f32 = out_f32;
-    return launch_typed<kDw>(a, dtype, s);
 }
 
 extern "C" {

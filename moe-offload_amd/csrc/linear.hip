@@ -3,11 +3,17 @@
 //     z = x W^T + bias,   y = act(z) + residual        (bias and residual may be absent; z is kept where it is asked for)
 //     dz = dy act'(z),    dx = dz W,   dW = dz^T x,   dbias = the sum of dz over the tokens
 // act: none, silu, gelu (z times the normal distribution's integral) or the squared relu.  x, W, bias, residual and z are
-// fp16 or bf16, y too or fp32, sums and everything between a load and a store fp32.  The products are the grouped
-// products' kernels (grouped_mm.hip) over one segment of all tokens; this file has the entry points and dz.
+// fp16 or bf16, y too or fp32, sums and everything between a load and a store fp32.
+//
+// All three products are one tile product  out[p][q] = sum over c of P[p][c] Q[q][c]  as the grouped products' are
+// (grouped_mm.h: loads straight into LDS, operands along or across a row of memory), without rows to look up: x and W have c
+// along a row, W for dx has it along the column, dz and x for dW both.
 //
 // dz is rounded to the inputs' type before the matrix unit takes it, unless it is dy as it came: half a step of each
 // value, the same as that of the products' own results, and independent from value to value.
+#include <algorithm>
+#include <type_traits>
+
 #include "grouped_mm.h"
 #include "lane_reduce.h"
 
@@ -15,8 +21,431 @@ namespace {
 
 using namespace gmm;
 
+enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu2 = 3 };
+
+// The normal distribution's integral up to -|z|, by Abramowitz and Stegun's 7.1.26 (Handbook of Mathematical Functions):
+// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most.
+__device__ __forceinline__ float normal_tail(float z) {
+    const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return 0.5f * poly * __expf(-x * x);
+}
+
+// The activations, and their slopes.  Arguments past -200 are taken there, where both are their limits (0): an infinity
+// would meet a zero.  A NaN stays one.
+__device__ __forceinline__ float activation(int act, float z) {
+    if (act == kActNone) return z;
+    if (act == kActRelu2) return z < 0.f ? 0.f : z * z;
+    const float low = z < -200.f ? -200.f : z;
+    if (act == kActSilu) return low / (1.0f + __expf(-low));
+    const float tail = normal_tail(low);
+    return low < 0.f ? low * tail : low * (1.f - tail);
+}
+
+__device__ __forceinline__ float slope(int act, float z) {
+    if (act == kActNone) return 1.f;
+    if (act == kActRelu2) return z < 0.f ? 0.f : 2.f * z;
+    const float low = z < -200.f ? -200.f : z, both = low > 200.f ? 200.f : low;
+    if (act == kActSilu) {
+        const float sg = 1.0f / (1.0f + __expf(-low));
+        return sg * (1.0f + both * (1.0f - sg));
+    }
+    const float tail = normal_tail(both);
+    return (both < 0.f ? tail : 1.f - tail) + both * 0.39894228f * __expf(-0.5f * both * both);
+}
+
+// What a product does with its results: z = sum + bias, out = act(z) + res.
+struct Epilogue {
+    const void* bias;
+    const void* res;
+    void* z;
+    int64_t ldr, ldz;
+    int act, out_f32;
+};
+
+struct Product {
+    const void* p;
+    const void* q;
+    void* out;
+    int64_t ldp, ldq, ldo;       // elements from row to row of memory
+    int np, nq, nc;              // extents: rows and columns of out, and the contraction
+    int parts, part_c;           // dW: the contraction in parts of part_c, each with results of its own (fp32, [parts][np][nq])
+};
+
+enum { kForward = 0, kDx = 1, kDw = 2 };
+
+template <typename T>
+__device__ __forceinline__ uint4 round8(const f32x4 (&v)[2]) {
+    const uint2 lo = round4<T>(v[0]), hi = round4<T>(v[1]);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+template <typename T>
+__device__ __forceinline__ void widen8(uint4 v, f32x4 (&f)[2]) {
+    f[0] = widen4<T>(make_uint2(v.x, v.y));
+    f[1] = widen4<T>(make_uint2(v.z, v.w));
+}
+
+// 8 adjacent columns of a row out: act(sum + bias) + res, and z.
+template <typename T>
+__device__ __forceinline__ void finish8(const Product& a, const Epilogue& e, int64_t r, int c, const f32x4 (&sum)[2], const f32x4 (&bias)[2],
+                                        uint4 res) {
+    f32x4 z[2], y[2], rs[2];
+    widen8<T>(res, rs);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        z[h] = sum[h] + bias[h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[h][i] = activation(e.act, z[h][i]) + rs[h][i];
+    }
+    if (e.z) store16((T*)e.z + r * e.ldz + c, round8<T>(z));
+    if (e.out_f32) {
+        float* d = (float*)a.out + r * a.ldo + c;
+        store16(d, __builtin_bit_cast(uint4, y[0]));
+        store16(d + 4, __builtin_bit_cast(uint4, y[1]));
+    } else {
+        store16((T*)a.out + r * a.ldo + c, round8<T>(y));
+    }
+}
+
+template <int BP, int BQ>
+__host__ __device__ inline int64_t tiles_in(const Product& a) {
+    return ((int64_t)a.np + BP - 1) / BP * (((int64_t)a.nq + BQ - 1) / BQ);
+}
+
+// Item -> tile: panels of PANEL columns of tiles, row by row in each, so that the tiles that an XCD works on at a time (its items
+// follow each other) are a square rather than a line, and share their rows of both operands in its L2.
+template <int BP, int BQ, int PANEL>
+__device__ __forceinline__ void tile_at(const Product& a, uint32_t item, int& p0, int& q0) {
+    const uint32_t tp = (a.np + BP - 1) / BP, tq = (a.nq + BQ - 1) / BQ, full = tp * PANEL;
+    const uint32_t panel = item / full, left = tq - panel * PANEL, width = left < PANEL ? left : PANEL, i = item - panel * full;
+    p0 = (int)(i / width) * BP;
+    q0 = (int)(panel * PANEL + i % width) * BQ;
+}
+
+// One tile of BP x BQ results by WP x WQ waves, or SPLIT = 2 times as many that take turns at the steps.  A step of 64 contraction
+// indexes goes from global memory to LDS without passing registers, RING - 1 steps ahead of the one that is multiplied: with one
+// tile per block nothing else hides the way through memory.  One barrier per step (and two steps, of SPLIT = 2).
+template <typename T, int KIND, typename C>
+__device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e, uint32_t item, uint8_t* lds) {
+    constexpr int BP = C::BP, BQ = C::BQ, WP = C::WP, WQ = C::WQ, RING = C::RING, SPLIT = C::SPLIT;
+    constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
+    constexpr bool kAlongP = KIND == kDw, kAlongQ = KIND != kForward;
+    constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves, kLoads = kLoadsP + kLoadsQ;   // 1 KiB each
+    constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
+    static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1 && RING * kStage / kWaves >= SQ * 1024, "");
+    const int t = threadIdx.x, lane = t & 63, all = __builtin_amdgcn_readfirstlane(t >> 6), turn_of = all / kWaves, wv = all % kWaves;
+    const uint32_t lds_all = (uint32_t)(uintptr_t)(lds_u8*)lds, lds0 = lds_all + turn_of * RING * kStage;
+    const T* P = (const T*)a.p;
+    const T* Q = (const T*)a.q;
+    int nc = a.nc;
+    int64_t part = 0;
+    if constexpr (KIND == kDw) {
+        const uint32_t tiles = (uint32_t)tiles_in<BP, BQ>(a);
+        part = item / tiles;
+        item -= (uint32_t)part * tiles;
+        P += part * a.part_c * a.ldp;
+        Q += part * a.part_c * a.ldq;
+        nc = nc - part * a.part_c < a.part_c ? (int)(nc - part * a.part_c) : a.part_c;
+    }
+    int p0, q0;
+    tile_at<BP, BQ, C::PANEL>(a, item, p0, q0);
+    const T* zero = (const T*)&g_zero16;
+    asm("" : "+s"(zero));                                                      // kept in registers
+    // Where this lane's 16 bytes of each of its wave's next loads are.  Rows and columns past the end read some that exist:
+    // their results are not stored.  Contraction indexes past the end read zeros.
+    const T* pp[kLoadsP];
+    const T* qp[kLoadsQ];
+    const int cu = ((lane & 7) ^ (lane >> 3)) * 8;                             // not ALONG: first c of the 16 bytes
+    int load_c = turn_of * kBC;
+    auto place_one = [&](auto along, auto width, const T* base, int64_t ld, int first, int n, int wave_loads, int j) -> const T* {
+        constexpr int W = decltype(width)::value, kUnits = W / 8;
+        if constexpr (decltype(along)::value) {
+            const int row = (wv * wave_loads + j) * (64 / kUnits) + lane / kUnits, col = first + (lane % kUnits ^ 2 * turn<W>(row)) * 8;
+            const int c = load_c + row;
+            return c < nc ? base + c * ld + (col < n ? col : 0) : zero;
+        } else {
+            const int r = first + (wv * wave_loads + j) * 8 + (lane >> 3);
+            return load_c + cu < nc ? base + (r < n ? r : n - 1) * ld + load_c + cu : zero;
+        }
+    };
+    auto place = [&]() {
+#pragma unroll
+        for (int j = 0; j < kLoadsP; ++j)
+            pp[j] = place_one(std::integral_constant<bool, kAlongP>(), std::integral_constant<int, BP>(), P, a.ldp, p0, a.np, kLoadsP, j);
+#pragma unroll
+        for (int j = 0; j < kLoadsQ; ++j)
+            qp[j] = place_one(std::integral_constant<bool, kAlongQ>(), std::integral_constant<int, BQ>(), Q, a.ldq, q0, a.nq, kLoadsQ, j);
+    };
+    auto advance = [&]() {
+        load_c += SPLIT * kBC;
+        if (load_c + kBC <= nc) {
+#pragma unroll
+            for (int j = 0; j < kLoadsP; ++j) pp[j] += kAlongP ? SPLIT * kBC * a.ldp : SPLIT * kBC;
+#pragma unroll
+            for (int j = 0; j < kLoadsQ; ++j) qp[j] += kAlongQ ? SPLIT * kBC * a.ldq : SPLIT * kBC;
+        } else {
+            place();
+        }
+    };
+    auto load = [&](int d, uint32_t stage) {
+        if (d < kLoadsP) load_to_lds(pp[d], lds0 + stage + (wv * kLoadsP + d) * 1024);
+        else load_to_lds(qp[d - kLoadsP], lds0 + stage + kStageP + (wv * kLoadsQ + d - kLoadsP) * 1024);
+    };
+    const int wp = wv / WQ, wq = wv % WQ;
+    Frags<kAlongP, BP, SP> fp;
+    Frags<kAlongQ, BQ, SQ> fq;
+    fp.init(lds0, wp * SP * 16, lane);
+    fq.init(lds0 + kStageP, wq * SQ * 16, lane);
+    f32x4 acc[SP][SQ] = {};
+    place();
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s) {
+#pragma unroll
+        for (int d = 0; d < kLoads; ++d) load(d, s * kStage);
+        advance();
+    }
+    uint32_t stage = 0, fill = (RING - 1) * kStage;
+#pragma unroll 1
+    for (int c0 = 0; c0 < nc; c0 += SPLIT * kBC) {
+        // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
+        // everyone's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * kLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        uint4 vp[2][SP], vq[2][SQ];
+#pragma unroll
+        for (int j = 0; j < SQ; ++j) vq[0][j] = fq.read(stage, j, 0);
+#pragma unroll
+        for (int i = 0; i < SP; ++i) vp[0][i] = fp.read(stage, i, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // the step's second half is read from LDS, and the loads ahead are issued, between the first half's products
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+            constexpr int kFrom = SP > 4 ? SP / 2 : 0, kEach = SP > 4 ? 2 : 1;
+            if (i == kFrom) {
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) vq[1][j] = fq.read(stage, j, 1);
+            }
+            if (i >= kFrom) {
+#pragma unroll
+                for (int x = (i - kFrom) * kEach; x < (i - kFrom + 1) * kEach; ++x) vp[1][x] = fp.read(stage, x, 1);
+            }
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+#pragma unroll
+            for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
+#pragma unroll
+        for (int i = 0; i < SP; ++i)
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+        stage = stage + kStage == RING * kStage ? 0 : stage + kStage;
+        fill = fill + kStage == RING * kStage ? 0 : fill + kStage;
+    }
+    // The results go through LDS, one of a wave's subtile rows at a time: a lane of the matrix unit's result has 4 columns of
+    // a row and its neighbour another row's; out of LDS 8 columns, and whole lines side by side.  (The loads past the last
+    // step write there too, so they are waited for.)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) u32x4* lds16;
+    constexpr int kUnits = SQ * 2, kRowsPer = 64 / kUnits, kIts = 16 / kRowsPer;
+    constexpr int kOwn = SP / SPLIT;                                           // subtile rows that a wave finishes
+    if constexpr (SPLIT == 2) {
+        // the waves of a turn hand the other's half of the rows over and add what they get
+        static_assert(2 * kWaves * kOwn * SQ * 1024 <= SPLIT * RING * kStage, "");
+        auto box = [&](int turn, int i, int j) { return lds_all + (uint32_t)((((turn * kWaves + wv) * kOwn + i) * SQ + j) * 1024 + lane * 16); };
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+            for (int j = 0; j < SQ; ++j)
+                *(lds16)(uintptr_t)box(turn_of, i, j) = __builtin_bit_cast(u32x4, turn_of ? acc[i][j] : acc[kOwn + i][j]);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+            for (int j = 0; j < SQ; ++j)
+                acc[i][j] = (turn_of ? acc[kOwn + i][j] : acc[i][j]) + __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)box(1 - turn_of, i, j));
+        __syncthreads();
+    }
+    int l = lane;
+    asm volatile("" : "+v"(l));                                                // no addresses are kept over the products
+    const int l16 = l & 15, lq = l >> 4, u8 = l % kUnits, c = q0 + wq * SQ * 16 + u8 * 8;
+    const uint32_t area = lds_all + all * (SQ * 1024);
+    auto at = [&](int row, int u) { return area + (uint32_t)(row * SQ * 4 + (u ^ (row & 7))) * 16; };
+    const bool in = c < a.nq;
+    f32x4 bias[2] = {};
+    if (KIND == kForward && e.bias && in) widen8<T>(*(const uint4*)((const T*)e.bias + c), bias);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        uint4 rv[kIts];
+        int row[kIts];
+#pragma unroll
+        for (int it = 0; it < kIts; ++it) {
+            const int r = p0 + wp * SP * 16 + (turn_of * kOwn + i) * 16 + it * kRowsPer + l / kUnits;
+            row[it] = r < a.np && in ? r : -1;
+            rv[it] = KIND == kForward && e.res && row[it] >= 0 ? *(const uint4*)((const T*)e.res + row[it] * e.ldr + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < SQ; ++j) *(lds16)(uintptr_t)at(l16, 4 * j + lq) = __builtin_bit_cast(u32x4, acc[i][j]);
+#pragma unroll
+        for (int it = 0; it < kIts; ++it) {
+            const int m = it * kRowsPer + l / kUnits;
+            const f32x4 sum[2] = {__builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8)), __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + 1))};
+            if (row[it] < 0) continue;
+            if constexpr (KIND == kForward) {
+                finish8<T>(a, e, row[it], c, sum, bias, rv[it]);
+            } else if (KIND == kDw && e.out_f32) {
+                float* d = (float*)a.out + (part * a.np + row[it]) * a.ldo + c;
+                store16(d, __builtin_bit_cast(uint4, sum[0]));
+                store16(d + 4, __builtin_bit_cast(uint4, sum[1]));
+            } else {
+                store16((T*)a.out + row[it] * a.ldo + c, round8<T>(sum));
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// A tile's sides, its waves, how many share the steps, its ring, the blocks per CU that registers are kept for, the panel.
+template <int BP_, int BQ_, int WP_, int WQ_, int SPLIT_, int RING_, int BLOCKS_, int PANEL_>
+struct Tiles {
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, SPLIT = SPLIT_, RING = RING_, BLOCKS = BLOCKS_, PANEL = PANEL_;
+    static constexpr int kThreads = 64 * WP * WQ * SPLIT, kLds = SPLIT * RING * (BP + BQ) * 128;
+};
+
+template <typename T, typename C>
+__global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear(Product a, Epilogue e) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
+    tile_product<T, kForward, C>(a, e, xcd_order(blockIdx.x, gridDim.x), lds);
+}
+
+// What k_linear_dz left of the bias's gradient: [blocks][n], summed in order by a block of 64 columns and 4 parts of the rows.
+struct BiasSums {
+    const float* sums;
+    void* db;
+    int blocks, n;
+};
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void sum_bias(const BiasSums& b, uint32_t item, float* lds) {
+    constexpr int kParts = THREADS / 64;
+    const int c = (int)item * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < b.n) {
+        const int from = (int)((int64_t)b.blocks * part / kParts), to = (int)((int64_t)b.blocks * (part + 1) / kParts);
+#pragma unroll 8
+        for (int i = from; i < to; ++i) s += b.sums[(int64_t)i * b.n + c];
+    }
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    if (part == 0 && c < b.n) {
+        for (int i = 1; i < kParts; ++i) s += lds[i * 64 + threadIdx.x];
+        ((T*)b.db)[c] = (T)s;
+    }
+}
+
+// All gradients behind dz in one launch: the tiles of dW (longer, as a rule) before those of dx, then the bias's.  A product of no
+// rows is not there.
+template <typename T, typename C>
+__global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear_grads(Product dw, Product dx, BiasSums b, int dw_f32) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
+    const uint32_t n_dw = (uint32_t)tiles_in<C::BP, C::BQ>(dw) * dw.parts, n_dx = (uint32_t)tiles_in<C::BP, C::BQ>(dx);
+    const uint32_t i = blockIdx.x;
+    Epilogue e = {};
+    e.out_f32 = dw_f32;
+    if (i < n_dw) tile_product<T, kDw, C>(dw, e, xcd_order(i, n_dw), lds);
+    else if (i < n_dw + n_dx) tile_product<T, kDx, C>(dx, e, xcd_order(i - n_dw, n_dx), lds);
+    else sum_bias<T, C::kThreads>(b, i - n_dw - n_dx, (float*)lds);
+}
+
+// dW from its parts, in their order, and behind those blocks the bias's gradient.
+struct Parts {
+    const float* sums;
+    void* dw;
+    int64_t n;                   // elements of dW, a multiple of 8
+    int parts, f32;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_parts(Parts p, uint32_t blocks, BiasSums b) {
+    __shared__ float lds[256];
+    if (blockIdx.x >= blocks) {
+        sum_bias<T, 256>(b, blockIdx.x - blocks, lds);
+        return;
+    }
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= p.n) return;
+    f32x4 s[2] = {};
+#pragma unroll 4
+    for (int k = 0; k < p.parts; ++k) {
+        s[0] += *(const f32x4*)(p.sums + k * p.n + i);
+        s[1] += *(const f32x4*)(p.sums + k * p.n + i + 4);
+    }
+    if (p.f32) {
+        *(f32x4*)((float*)p.dw + i) = s[0];
+        *(f32x4*)((float*)p.dw + i + 4) = s[1];
+    } else {
+        *(uint4*)((T*)p.dw + i) = round8<T>(s);
+    }
+}
+
+// Few results: a block has 16 x 16 of them, its waves take turns at the steps, and their sums meet in LDS.  Rows of both
+// operands come straight into the matrix unit's layout, four of a wave's steps under way at once, and no wave waits for another
+// before the end.
+constexpr int kFewWaves = 8;
+
+template <typename T>
+__global__ __launch_bounds__(64 * kFewWaves) void k_linear_few(Product a, Epilogue e) {
+    constexpr int kAhead = 4;
+    __shared__ f32x4 part[kFewWaves][64];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kq = lane >> 4;
+    const uint32_t item = xcd_order(blockIdx.x, gridDim.x), tp = (a.np + 15) / 16;
+    const int p0 = (int)(item % tp) * 16, q0 = (int)(item / tp) * 16, steps = (a.nc + kBC - 1) / kBC;
+    const T* W = (const T*)a.q + (int64_t)(q0 + n < a.nq ? q0 + n : a.nq - 1) * a.ldq + kq * 8;
+    const T* X = (const T*)a.p + (int64_t)(p0 + n < a.np ? p0 + n : a.np - 1) * a.ldp + kq * 8;
+    f32x4 acc = {};
+    const T* zero = (const T*)&g_zero16;
+    for (int s = wv; s < steps; s += kFewWaves * kAhead) {
+        uint4 w[kAhead][2], x[kAhead][2];
+        auto read = [&](auto inside) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const int c = (s + u * kFewWaves) * kBC + ks * 32;
+                    const bool in = decltype(inside)::value || c + kq * 8 < a.nc;
+                    w[u][ks] = *(const uint4*)(in ? W + c : zero);
+                    x[u][ks] = *(const uint4*)(in ? X + c : zero);
+                }
+        };
+        if ((s + (kAhead - 1) * kFewWaves + 1) * kBC <= a.nc) read(std::true_type());
+        else read(std::false_type());
+        __builtin_amdgcn_sched_barrier(0);                                     // all loads before the first wait
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) acc = mfma<T>(w[u][ks], x[u][ks], acc);
+    }
+    part[wv][lane] = acc;
+    __syncthreads();
+    // a thread has 8 columns of a row: lane (n, kq) of a result has columns 4 kq .. + 3 of row n
+    const int half = threadIdx.x & 1, row = threadIdx.x >> 1, c = q0 + half * 8;
+    if (row >= 16 || p0 + row >= a.np || c >= a.nq) return;
+    f32x4 sum[2] = {}, bias[2] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) sum[h] += part[w][(half * 2 + h) * 16 + row];
+    if (e.bias) widen8<T>(*(const uint4*)((const T*)e.bias + c), bias);
+    finish8<T>(a, e, p0 + row, c, sum, bias, e.res ? *(const uint4*)((const T*)e.res + (p0 + row) * e.ldr + c) : make_uint4(0, 0, 0, 0));
+}
+
 constexpr int kDzThreads = 256;
-constexpr int kDzRows = 64;                // tokens of a block, of 256 columns
 
 struct DzArgs {
     const void* dy;
@@ -25,6 +454,7 @@ struct DzArgs {
     float* sums;                 // [row blocks][n], null: none wanted
     int64_t lddy, ldz;
     int n_rows, n, act;
+    int rows;                    // of a block
 };
 
 // A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.
@@ -32,33 +462,27 @@ template <typename T, bool F32>
 __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
     __shared__ f32x4 part[8][32][2];
     const int t = threadIdx.x, u = t & 31, sub = t >> 5, c = (blockIdx.x * 32 + u) * 8;
-    const int r0 = (int)blockIdx.y * kDzRows;
+    const int64_t r0 = (int64_t)blockIdx.y * a.rows, r1 = r0 + a.rows < a.n_rows ? r0 + a.rows : a.n_rows;
     f32x4 sum[2] = {};
     if (c < a.n) {
-        for (int i = sub; i < kDzRows && r0 + i < a.n_rows; i += 8) {
-            const int64_t r = r0 + i;
+#pragma unroll 2
+        for (int64_t r = r0 + sub; r < r1; r += 8) {
             f32x4 d[2];
             if constexpr (F32) {
                 d[0] = *(const f32x4*)((const float*)a.dy + r * a.lddy + c);
                 d[1] = *(const f32x4*)((const float*)a.dy + r * a.lddy + c + 4);
             } else {
-                const uint4 v = *(const uint4*)((const T*)a.dy + r * a.lddy + c);
-                d[0] = widen4<T>(make_uint2(v.x, v.y));
-                d[1] = widen4<T>(make_uint2(v.z, v.w));
+                widen8<T>(*(const uint4*)((const T*)a.dy + r * a.lddy + c), d);
             }
             if (a.z) {
-                const uint4 v = *(const uint4*)((const T*)a.z + r * a.ldz + c);
-                const f32x4 z0 = widen4<T>(make_uint2(v.x, v.y)), z1 = widen4<T>(make_uint2(v.z, v.w));
+                f32x4 z[2];
+                widen8<T>(*(const uint4*)((const T*)a.z + r * a.ldz + c), z);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    d[0][e] *= slope(a.act, z0[e]);
-                    d[1][e] *= slope(a.act, z1[e]);
-                }
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[h][e] *= slope(a.act, z[h][e]);
             }
-            if (a.dz) {
-                const uint2 lo = round4<T>(d[0]), hi = round4<T>(d[1]);
-                *(uint4*)((T*)a.dz + r * a.n + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
+            if (a.dz) *(uint4*)((T*)a.dz + r * a.n + c) = round8<T>(d);
             sum[0] += d[0];
             sum[1] += d[1];
         }
@@ -77,14 +501,12 @@ __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void k_linear_db(const float* __restrict__ sums, int blocks, int n, T* __restrict__ db) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= n) return;
-    float s = 0.f;
-    for (int b = 0; b < blocks; ++b) s += sums[(int64_t)b * n + c];
-    db[c] = (T)s;
+// The rows of a block of k_linear_dz: about 1024 blocks, at most 256 of them below each other (what the bias's sums wait for).
+int dz_rows(int n_tok, int n) {
+    const int64_t cols = ((int64_t)n + 255) / 256, down = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / cols));
+    return (int)std::max<int64_t>(8, (n_tok + down * 8 - 1) / (down * 8) * 8);
 }
+int dz_blocks(int n_tok, int n) { return (int)(((int64_t)n_tok + dz_rows(n_tok, n) - 1) / dz_rows(n_tok, n)); }
 
 bool bad_matrix(const char* who, const char* name, const void* p, int64_t ld, int64_t width, int64_t rows) {
     if (ld % 8 || (rows > 1 && ld < width) || ld < 0) {
@@ -108,24 +530,133 @@ bool bad_sizes(const char* who, int n_tok, int n_in, int n_out, int act, int dty
     return false;
 }
 
+bool too_many(const char* who, int64_t blocks, int threads) {
+    if (blocks <= kMaxThreads / threads) return false;
+    moe_set_error("%s: %lld tiles are more than one launch takes", who, (long long)blocks);
+    return true;
+}
+
 uint64_t round_up(uint64_t v) { return (v + 255) / 256 * 256; }
 
-int row_blocks(int n_tok) { return (int)(((int64_t)n_tok + kDzRows - 1) / kDzRows); }
+#ifdef LINEAR_SWEEP
+int sweep() { const char* s = getenv("LINEAR_CFG"); return s ? atoi(s) : -1; }
+#endif
+
+// The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two.
+template <typename F>
+int each_tiles(const F& f) {
+    f(Tiles<64, 64, 2, 2, 2, 3, 2, 8>(), 24, 48);
+    f(Tiles<64, 64, 2, 2, 1, 4, 2, 8>(), 25, 45);
+    f(Tiles<128, 64, 2, 2, 1, 3, 2, 8>(), 42, 75);
+    f(Tiles<128, 128, 2, 4, 1, 4, 2, 6>(), 55, 110);
+    f(Tiles<128, 128, 2, 2, 1, 2, 2, 8>(), 90, 97);
+    f(Tiles<256, 256, 2, 4, 1, 2, 2, 4>(), 145, 290);
+    return 0;
+}
+
+// Calls run(tiles) with those that are done first: with one product, as many steps as a CU's blocks have; with two, which fill
+// each other's gaps, the sum of all steps over the CUs, but at least those of the longest tile.
+template <typename R>
+int best_tiles(const Product& a, const Product& b, const R& run) {
+    int64_t best = INT64_MAX;
+    int pick = 0, i = 0;
+    auto steps = [](const Product& p) { return (int64_t)(p.parts > 1 ? p.part_c : p.nc) / kBC + 1; };
+    each_tiles([&](auto tiles, int one, int two) {
+        using C = decltype(tiles);
+        const int64_t ta = tiles_in<C::BP, C::BQ>(a) * a.parts, tb = tiles_in<C::BP, C::BQ>(b) * b.parts;
+        int64_t cost;
+        if (ta == 0 || tb == 0) {
+            const int64_t n = (ta + tb + 255) / 256;
+            cost = (ta ? steps(a) : steps(b)) * (n / 2 * two + n % 2 * one);
+        } else {
+            cost = std::max((ta * steps(a) + tb * steps(b)) * two / 512, std::max(steps(a), steps(b)) * one);
+        }
+        if (cost < best) best = cost, pick = i;
+        ++i;
+    });
+#ifdef LINEAR_SWEEP
+    if (sweep() >= 0 && sweep() < 6) pick = sweep();
+#endif
+    int rc = -1;
+    i = 0;
+    each_tiles([&](auto tiles, int, int) {
+        if (i++ == pick) rc = run(tiles);
+    });
+    return rc;
+}
 
 template <typename T>
-int launch_dz(const DzArgs& a, int dy_f32, void* db, hipStream_t s) {
-    const int blocks = row_blocks(a.n_rows), cols = (a.n + 255) / 256;
-    if (blocks > 0) {
-        const dim3 grid(cols, blocks);
-        if (dy_f32) hipLaunchKernelGGL((k_linear_dz<T, true>), grid, dim3(kDzThreads), 0, s, a);
-        else hipLaunchKernelGGL((k_linear_dz<T, false>), grid, dim3(kDzThreads), 0, s, a);
+int forward(const Product& a, const Epilogue& e, hipStream_t s) {
+    const int64_t tiles16 = tiles_in<16, 16>(a);
+    bool few = a.np <= 16 || tiles16 <= 256;
+#ifdef LINEAR_SWEEP
+    if (sweep() >= 0) few = sweep() == 9;
+#endif
+    if (few) {
+        if (too_many("linear", tiles16, 64 * kFewWaves)) return -1;
+        hipLaunchKernelGGL((k_linear_few<T>), dim3((uint32_t)tiles16), dim3(64 * kFewWaves), 0, s, a, e);
         HIP_TRY(hipGetLastError());
+        return 0;
     }
-    if (db) {
-        hipLaunchKernelGGL((k_linear_db<T>), dim3((a.n + 63) / 64), dim3(64), 0, s, a.sums, blocks, a.n, (T*)db);
+    return best_tiles(a, Product{}, [&](auto tiles) {
+        using C = decltype(tiles);
+        const int64_t blocks = tiles_in<C::BP, C::BQ>(a);
+        if (too_many("linear", blocks, C::kThreads)) return -1;
+        hipLaunchKernelGGL((k_linear<T, C>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, a, e);
         HIP_TRY(hipGetLastError());
-    }
-    return 0;
+        return 0;
+    });
+}
+
+// The parts of dW's contraction, the tokens: as many as give every CU a tile of 64 x 64, of 16 steps or more.
+int dw_parts(int n_tok, int n_out, int n_in) {
+    const int64_t tiles = ((int64_t)n_out + 63) / 64 * (((int64_t)n_in + 63) / 64), steps = (int64_t)n_tok / kBC;
+    int64_t parts = std::min(256 / tiles, steps / 16);
+#ifdef LINEAR_SWEEP
+    if (const char* s = getenv("LINEAR_PARTS")) parts = atoi(s);
+#endif
+    return (int)std::max<int64_t>(1, parts);
+}
+
+template <typename T>
+int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const Product& dx, const BiasSums& b, const Parts& p, hipStream_t s) {
+    return best_tiles(dw, dx, [&](auto tiles) {
+        using C = decltype(tiles);
+        const bool parts = dw.parts > 1 && dw.np > 0;
+        // what one launch does not take is refused before anything is queued
+        const int64_t sums = b.db ? ((int64_t)b.n + 63) / 64 : 0, adds = parts ? (p.n / 8 + 255) / 256 : 0;
+        const int64_t blocks = tiles_in<C::BP, C::BQ>(dw) * dw.parts + tiles_in<C::BP, C::BQ>(dx) + (parts ? 0 : sums);
+        if (too_many("linear_grad", blocks, C::kThreads) || too_many("linear_grad", adds + sums, 256)) return -1;
+        if (dz && dz->n_rows > 0) {
+            const dim3 grid((dz->n + 255) / 256, dz_blocks(dz->n_rows, dz->n));
+            if (dy_f32) hipLaunchKernelGGL((k_linear_dz<T, true>), grid, dim3(kDzThreads), 0, s, *dz);
+            else hipLaunchKernelGGL((k_linear_dz<T, false>), grid, dim3(kDzThreads), 0, s, *dz);
+            HIP_TRY(hipGetLastError());
+        }
+        if (blocks > 0) {
+            hipLaunchKernelGGL((k_linear_grads<T, C>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, dw, dx, b, parts || dw_f32);
+            HIP_TRY(hipGetLastError());
+        }
+        if (parts) {
+            hipLaunchKernelGGL((k_linear_parts<T>), dim3((uint32_t)(adds + sums)), dim3(256), 0, s, p, (uint32_t)adds, b);
+            HIP_TRY(hipGetLastError());
+        }
+        return 0;
+    });
+}
+
+// The workspace: dz, the sums that the bias's gradient is made of, dW's parts.
+struct Layout {
+    uint64_t sums, parts, bytes;
+};
+
+Layout layout(int n_tok, int n_in, int n_out, bool own_dz, bool want_dw, bool want_db) {
+    Layout l;
+    l.sums = own_dz ? round_up(2 * (uint64_t)n_tok * n_out) : 0;
+    l.parts = l.sums + (want_db ? round_up(4 * (uint64_t)dz_blocks(n_tok, n_out) * n_out) : 0);
+    const int parts = want_dw ? dw_parts(n_tok, n_out, n_in) : 1;
+    l.bytes = l.parts + (parts > 1 ? 4 * (uint64_t)parts * n_out * n_in : 0);
+    return l;
 }
 
 }  // namespace
@@ -140,14 +671,14 @@ extern "C" int moe_linear(const void* x, int64_t ldx, const void* w, const void*
         (z && bad_matrix(who, "z", z, ldz, n_out, n_tok)) || bad_matrix(who, "y", y, ldy, n_out, n_tok))
         return -1;
     if (n_tok == 0) return 0;
-    const Linear l = {x, w, bias, residual, y, z, ldx, ldr, ldy, ldz, n_tok, n_out, n_in, act, out_f32};
-    return gmm::linear(l, dtype, (hipStream_t)stream);
+    const Product a = {x, w, y, ldx, n_in, ldy, n_tok, n_out, n_in, 1, 0};
+    const Epilogue e = {bias, residual, z, ldr, ldz, act, out_f32};
+    return dtype ? forward<__bf16>(a, e, (hipStream_t)stream) : forward<_Float16>(a, e, (hipStream_t)stream);
 }
 
-extern "C" uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_out, int act, int dy_f32, int want_db) {
-    if (n_tok < 0 || n_out < 0) return 0;
-    const uint64_t dz = act != kActNone || dy_f32 ? round_up(2 * (uint64_t)n_tok * n_out) : 0;
-    return dz + (want_db ? 4 * (uint64_t)row_blocks(n_tok) * n_out : 0);
+extern "C" uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_in, int n_out, int act, int dy_f32, int want_dw, int want_db) {
+    if (n_tok < 0 || n_in < 1 || n_out < 1) return 0;
+    return layout(n_tok, n_in, n_out, act != kActNone || dy_f32, want_dw, want_db).bytes;
 }
 
 extern "C" int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const void* x, int64_t ldx, const void* w, const void* z,
@@ -161,25 +692,22 @@ extern "C" int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const v
         (dx && (bad_matrix(who, "w", w, n_in, n_in, n_out) || bad_matrix(who, "dx", dx, n_in, n_in, n_tok))) ||
         (dw && bad_matrix(who, "dw", dw, n_in, n_in, n_out)))
         return -1;
-    if (moe_linear_grad_workspace_bytes(n_tok, n_out, act, dy_f32, db != nullptr) > 0 && (!workspace || (uintptr_t)workspace % 16)) {
+    const Layout at = layout(n_tok, n_in, n_out, own_dz, dw != nullptr, db != nullptr);
+    if (at.bytes > 0 && (!workspace || (uintptr_t)workspace % 16)) {
         moe_set_error("linear_grad: the workspace is null or not 16-byte aligned");
-        return -1;
-    }
-    if (row_blocks(n_tok) > 65535) {
-        moe_set_error("linear_grad: n_tok=%d (up to %d)", n_tok, 65535 * kDzRows);
         return -1;
     }
     void* dz = own_dz && (dx || dw) ? workspace : nullptr;
     const void* rows = own_dz ? dz : dy;
     const int64_t ld = own_dz ? n_out : lddy;
-    // what one launch does not take is refused before anything is queued
-    auto dx_of = [&](bool dry) { return !dx || n_tok == 0 ? 0 : linear_dx(rows, ld, w, dx, n_tok, n_out, n_in, dtype, dry, s); };
-    auto dw_of = [&](bool dry) { return !dw ? 0 : linear_dw(rows, ld, x, ldx, dw, n_tok, n_out, n_in, dw_f32, dtype, dry, s); };
-    if (dx_of(true) || dw_of(true)) return -1;
-    if (dz || db) {
-        const uint64_t skip = own_dz ? round_up(2 * (uint64_t)n_tok * n_out) : 0;
-        const DzArgs a = {dy, act != kActNone ? z : nullptr, dz, db ? (float*)((char*)workspace + skip) : nullptr, lddy, ldz, n_tok, n_out, act};
-        if (dtype ? launch_dz<__bf16>(a, dy_f32, db, s) : launch_dz<_Float16>(a, dy_f32, db, s)) return -1;
-    }
-    return dx_of(false) || dw_of(false) ? -1 : 0;
+    float* sums = db ? (float*)((char*)workspace + at.sums) : nullptr;
+    const DzArgs d = {dy, act != kActNone ? z : nullptr, dz, sums, lddy, ldz, n_tok, n_out, act, dz_rows(n_tok, n_out)};
+    const int parts = dw ? dw_parts(n_tok, n_out, n_in) : 1, part_c = (int)(((int64_t)n_tok + parts * kBC - 1) / (parts * kBC) * kBC);
+    void* into = parts > 1 ? (char*)workspace + at.parts : dw;
+    const Product gw = {rows, x, into, ld, ldx, n_in, dw ? n_out : 0, n_in, n_tok, parts, part_c};
+    const Product gx = {rows, w, dx, ld, n_in, n_in, dx ? n_tok : 0, n_in, n_out, 1, 0};
+    const BiasSums b = {sums, db, dz_blocks(n_tok, n_out), n_out};
+    const Parts p = {(const float*)into, dw, (int64_t)n_out * n_in, parts, dw_f32};
+    const DzArgs* need = dz || db ? &d : nullptr;
+    return dtype ? gradients<__bf16>(need, dy_f32, gw, dw_f32, gx, b, p, s) : gradients<_Float16>(need, dy_f32, gw, dw_f32, gx, b, p, s);
 }

@@ -133,7 +133,7 @@ SIGNATURES: dict[str, tuple] = {
     "moe_combine_grad": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_vp, _c_vp]),
     "moe_linear": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp,
                             _c_i64, _c_vp, _c_i64, _c_vp]),
-    "moe_linear_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "moe_linear_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "moe_linear_grad": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
                                  _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp]),
     "moe_clip_workspace_bytes": (_c_u64, [_c_int, _c_i64]),

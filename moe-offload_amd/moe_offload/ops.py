@@ -814,11 +814,11 @@ def linear_grad(dy, x, w, z=None, act=None, bias=False, want_dx=True, want_dw=Tr
     dw_dtype = dw_dtype or x.dtype
     if dw_dtype not in (x.dtype, torch.float32):
         raise TypeError(f"{who}: gradients of {x.dtype} come as {x.dtype} or torch.float32, not {dw_dtype}")
-    dx = torch.empty((n_tok, n_in), dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty((n_out, n_in), dtype=dw_dtype, device=x.device) if want_dw else None
-    db = torch.empty(n_out, dtype=x.dtype, device=x.device) if bias else None
+    dx = x.new_empty((n_tok, n_in)) if want_dx else None
+    dw = x.new_empty((n_out, n_in), dtype=dw_dtype) if want_dw else None
+    db = x.new_empty(n_out) if bias else None
     dy_f32 = int(dy.dtype == torch.float32)
-    nb = _lib.lib().moe_linear_grad_workspace_bytes(n_tok, n_out, act_id, dy_f32, int(bool(bias)))
+    nb = _lib.lib().moe_linear_grad_workspace_bytes(n_tok, n_in, n_out, act_id, dy_f32, int(want_dw), int(bool(bias)))
     ws = _scratch(nb, x, workspace, who) if nb else None
     _call("moe_linear_grad", dev, _p(dy), lddy, dy_f32, _p(x), ldx, _p(w), _p(z), ldz, n_tok, n_in, n_out, act_id, dt, _p(ws), _p(dx),
           _p(dw), int(dw_dtype == torch.float32), _p(db))

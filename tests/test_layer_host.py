@@ -132,12 +132,14 @@ def test_linear_arguments():
     assert "more than one launch" in refused("moe_linear", P, 8, P, None, None, 0, 1 << 30, 8, 1 << 30, 0, 1, 0, None, 0, P, 1 << 30, None)
     taken("moe_linear", *swapped(good, 6, 0))
     good = (P, 128, 0, P, 64, P, P, 128, 4, 64, 128, 1, 1, P, P, P, 0, P, None)
-    for i, bad in ((0, None), (1, 64), (3, None), (4, 60), (5, None), (6, None), (7, 64), (8, -1), (8, 1 << 22), (9, 12), (10, 12), (11, 4), (12, 2),
+    for i, bad in ((0, None), (1, 64), (3, None), (4, 60), (5, None), (6, None), (7, 64), (8, -1), (8, (1 << 30) + 8), (9, 12), (10, 12), (11, 4), (12, 2),
                    (13, None), (13, P + 8), (14, P + 8), (15, P + 8)):
         refused("moe_linear_grad", *swapped(good, i, bad))
     ws = _lib.lib().moe_linear_grad_workspace_bytes
-    assert ws(0, 128, 0, 0, 0) == 0 and ws(100, 128, 0, 0, 0) == 0 and ws(100, 128, 1, 0, 0) >= 2 * 100 * 128 and ws(100, 128, 0, 1, 0) >= 2 * 100 * 128
-    assert ws(100, 128, 0, 0, 1) >= 4 * 128 and ws(1 << 20, 4096, 1, 0, 0) >= 1 << 33
+    assert ws(0, 64, 128, 0, 0, 0, 0) == 0 and ws(100, 64, 128, 0, 0, 0, 0) == 0 and ws(100, 64, 128, 1, 0, 0, 0) >= 2 * 100 * 128
+    assert ws(100, 64, 128, 0, 1, 0, 0) >= 2 * 100 * 128 and ws(100, 64, 128, 0, 0, 0, 1) >= 4 * 128 and ws(1 << 20, 64, 4096, 1, 0, 0, 0) >= 1 << 33
+    # few tiles of a long contraction: parts of their own
+    assert ws(100, 64, 128, 0, 0, 1, 0) == 0 and ws(8192, 512, 64, 0, 0, 1, 0) >= 2 * 4 * 512 * 64
 
 
 def clip(grads, outs, sizes, types, limit=1.0, ws=P, norm=P):
