@@ -23,35 +23,52 @@ using namespace gmm;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu2 = 3 };
 
-// The normal distribution's integral up to -|z|, by Abramowitz and Stegun's 7.1.26 (Handbook of Mathematical Functions):
-// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most.
-__device__ __forceinline__ float normal_tail(float z) {
-    const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    return 0.5f * poly * __expf(-x * x);
+// The normal distribution's integral up to -m, m >= 0, by Abramowitz and Stegun's 7.1.26 (Handbook of Mathematical Functions):
+// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most; here x = m / sqrt(2), and half of it.
+__device__ __forceinline__ float normal_tail(float m) {
+    const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.70710678f) * m);
+    const float poly = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+    return poly * __builtin_amdgcn_exp2f(m * m * -0.72134752f);
 }
 
-// The activations, and their slopes.  Arguments past -200 are taken there, where both are their limits (0): an infinity
-// would meet a zero.  A NaN stays one.
-__device__ __forceinline__ float activation(int act, float z) {
-    if (act == kActNone) return z;
-    if (act == kActRelu2) return z < 0.f ? 0.f : z * z;
-    const float low = z < -200.f ? -200.f : z;
-    if (act == kActSilu) return low / (1.0f + __expf(-low));
-    const float tail = normal_tail(low);
-    return low < 0.f ? low * tail : low * (1.f - tail);
+// The activations, and their slopes.  Where exponentials have left fp32's range both are at their limits, taken from arguments
+// that are not infinite: an infinity would meet a zero.  A NaN stays one.
+template <int ACT>
+__device__ __forceinline__ float activation(float z) {
+    if constexpr (ACT == kActRelu2) return z < 0.f ? 0.f : z * z;
+    if constexpr (ACT == kActSilu) {
+        const float low = z < -200.f ? -200.f : z;
+        return low / (1.0f + __expf(-low));
+    }
+    if constexpr (ACT == kActGelu) {
+        const float m = fminf(fabsf(z), 200.f);                                // z N(z) = max(z, 0) - |z| N(-|z|)
+        return (z < 0.f ? 0.f : z) - m * normal_tail(m);
+    }
+    return z;
 }
 
-__device__ __forceinline__ float slope(int act, float z) {
-    if (act == kActNone) return 1.f;
-    if (act == kActRelu2) return z < 0.f ? 0.f : 2.f * z;
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == kActRelu2) return z < 0.f ? 0.f : 2.f * z;
     const float low = z < -200.f ? -200.f : z, both = low > 200.f ? 200.f : low;
-    if (act == kActSilu) {
+    if constexpr (ACT == kActSilu) {
         const float sg = 1.0f / (1.0f + __expf(-low));
         return sg * (1.0f + both * (1.0f - sg));
     }
-    const float tail = normal_tail(both);
-    return (both < 0.f ? tail : 1.f - tail) + both * 0.39894228f * __expf(-0.5f * both * both);
+    if constexpr (ACT == kActGelu) {
+        const float tail = normal_tail(fabsf(both));
+        return (both < 0.f ? tail : 1.f - tail) + both * 0.39894228f * __expf(-0.5f * both * both);
+    }
+    return 1.f;
+}
+
+// Calls f with the activation as a type: one branch for many values.
+template <typename F>
+__device__ __forceinline__ void by_act(int act, const F& f) {
+    if (act == kActNone) f(std::integral_constant<int, kActNone>());
+    else if (act == kActSilu) f(std::integral_constant<int, kActSilu>());
+    else if (act == kActGelu) f(std::integral_constant<int, kActGelu>());
+    else f(std::integral_constant<int, kActRelu2>());
 }
 
 // What a product does with its results: z = sum + bias, out = act(z) + res.
@@ -92,12 +109,14 @@ __device__ __forceinline__ void finish8(const Product& a, const Epilogue& e, int
                                         uint4 res) {
     f32x4 z[2], y[2], rs[2];
     widen8<T>(res, rs);
+    by_act(e.act, [&](auto act) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        z[h] = sum[h] + bias[h];
+        for (int h = 0; h < 2; ++h) {
+            z[h] = sum[h] + bias[h];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[h][i] = activation(e.act, z[h][i]) + rs[h][i];
-    }
+            for (int i = 0; i < 4; ++i) y[h][i] = activation<decltype(act)::value>(z[h][i]) + rs[h][i];
+        }
+    });
     if (e.z) store16((T*)e.z + r * e.ldz + c, round8<T>(z));
     if (e.out_f32) {
         float* d = (float*)a.out + r * a.ldo + c;
@@ -477,10 +496,12 @@ __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
             if (a.z) {
                 f32x4 z[2];
                 widen8<T>(*(const uint4*)((const T*)a.z + r * a.ldz + c), z);
+                by_act(a.act, [&](auto act) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[h][e] *= slope(a.act, z[h][e]);
+                        for (int e = 0; e < 4; ++e) d[h][e] *= slope<decltype(act)::value>(z[h][e]);
+                });
             }
             if (a.dz) *(uint4*)((T*)a.dz + r * a.n + c) = round8<T>(d);
             sum[0] += d[0];
