@@ -37,21 +37,35 @@ struct CombineArgs {
     int n_tok, k, hidden;
 };
 
-// A thread has 8 columns of a token.
+// A thread has 8 columns of a token, and kAtOnce of its rows under way at once.
 template <typename T, bool F32>
 __global__ __launch_bounds__(kCombineThreads) void k_combine(CombineArgs a) {
-    const int units = a.hidden / 8;
+    constexpr int kAtOnce = 5;
+    const uint32_t units = a.hidden / 8;
     const int64_t items = (int64_t)a.n_tok * units;
     for (int64_t i = (int64_t)blockIdx.x * kCombineThreads + threadIdx.x; i < items; i += (int64_t)gridDim.x * kCombineThreads) {
-        const int64_t t = i / units;
-        const int c = (int)(i % units) * 8;
+        // (a division of 64 bits is a loop of its own)
+        const int64_t t = items <= 0xFFFFFFFF ? (uint32_t)i / units : i / units;
+        const int c = (int)(i - t * units) * 8;
+        const T* y = (const T*)a.y + t * a.k * a.ldy + c;
+        const float* w = a.weights + t * a.k;
+        uint4 res = make_uint4(0, 0, 0, 0);
+        if (a.residual) res = *(const uint4*)((const T*)a.residual + t * a.ldr + c);
         f32x8 sum = {};
-        for (int j = 0; j < a.k; ++j) {
-            const float w = a.weights[t * a.k + j];
-            const f32x8 v = widen8<T>(*(const uint4*)((const T*)a.y + (t * a.k + j) * a.ldy + c));
-            if (w != 0.f) sum += w * v;
+        for (int j0 = 0; j0 < a.k; j0 += kAtOnce) {
+            uint4 v[kAtOnce];
+            float wj[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const bool in = j0 + j < a.k;
+                v[j] = *(const uint4*)(y + (in ? j0 + j : 0) * a.ldy);
+                wj[j] = in ? w[j0 + j] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+                if (wj[j] != 0.f) sum += wj[j] * widen8<T>(v[j]);
         }
-        if (a.residual) sum += widen8<T>(*(const uint4*)((const T*)a.residual + t * a.ldr + c));
+        sum += widen8<T>(res);
         if constexpr (F32) *(f32x8*)((float*)a.out + t * a.ldo + c) = sum;
         else *(uint4*)((T*)a.out + t * a.ldo + c) = round8<T>(sum);
     }
@@ -76,10 +90,12 @@ __global__ __launch_bounds__(kCombineThreads) void k_combine_grad(CombineGradArg
         const T* d = (const T*)a.dout + p / a.k * a.ldd;
         const float w = a.weights[p];
         float dot = 0.f;
+#pragma unroll 2
         for (int u = lane; u < units; u += 64) {
             const f32x8 dv = widen8<T>(*(const uint4*)(d + u * 8));
             const f32x8 v = widen8<T>(*(const uint4*)((const T*)a.y + p * a.ldy + u * 8));
-            *(uint4*)((T*)a.dy + p * a.lddy + u * 8) = round8<T>(w * dv);
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, round8<T>(w * dv)), (u32x4*)((T*)a.dy + p * a.lddy + u * 8));
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot += dv[e] * v[e];
         }
