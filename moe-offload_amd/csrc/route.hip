@@ -398,16 +398,15 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         nan |= l[i] != l[i];
-        top = fmaxf(top, l[i]);
     }
     nan = __any(nan);
-    if (!a.sigmoid) {
-        top = wave_max(top);
-        if (!a.renorm || GENERAL) {
+    if (!a.sigmoid && (!a.renorm || GENERAL)) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) sum += l[i] == top ? 1.f : l[i] > -kInf ? __expf(l[i] - top) : 0.f;
-            sum = lanes::group_sum<64>(sum);
-        }
+        for (int i = 0; i < P; ++i) top = fmaxf(top, l[i]);
+        top = wave_max(top);
+#pragma unroll
+        for (int i = 0; i < P; ++i) sum += l[i] == top ? 1.f : l[i] > -kInf ? __expf(l[i] - top) : 0.f;
+        sum = lanes::group_sum<64>(sum);
     }
     uint32_t key[P];
     float s_top = 0.f, c_top = 0.f, s_err = 0.f;
@@ -420,7 +419,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
             const bool in = l[i] > -kInf;
             float s = 0.f;
             if (a.bias || a.group_best > 1) {
-                s = a.sigmoid ? 1.f / (1.f + __expf(-l[i])) : (l[i] == top ? 1.f : __expf(l[i] - top)) * inv;
+                s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-l[i])) : (l[i] == top ? 1.f : __expf(l[i] - top)) * inv;
                 s_top = fmaxf(s_top, in ? s : 0.f);
             }
             float c = l[i];
@@ -465,7 +464,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
         if (c.has) {
             c.l = read_one(a.logits, t * a.ld + c.id, a.dtype);
             b = a.bias[c.id];
-            const float s = a.sigmoid ? 1.f / (1.f + __expf(-c.l)) : (c.l == top ? 1.f : __expf(c.l - top)) / sum;
+            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-c.l)) : (c.l == top ? 1.f : __expf(c.l - top)) / sum;
             const float x = a.sigmoid ? fabsf(c.l) * (1.f - s) : top - c.l;
             err = s * (fminf(x, 110.f) + (a.sigmoid ? 8.f : 24.f)) * 0x1p-22f + fabsf(v) * 0x1p-23f;
         }
