@@ -17,7 +17,7 @@
 //
 // A wave takes a token.  Comparisons are exact: logits as they come, and sums of a score and a bias in 64 bits, where
 // 32 would let experts trade places whose values differ by less than their rounding.  What the 64 bits cost is spent on few
-// tokens only: values in 32 bits, each with a bound of its error, decide unless two of them are closer than their bounds; then
+// tokens only: values in 32 bits, with a bound of their error, decide unless two of them are closer than twice that; then
 // those that are in question are computed in 64 bits.
 //
 // The k largest: the k-th largest of the 64 lanes' own maxima, rounded down to 16 bits by a search from bit 31 on (a
@@ -48,7 +48,7 @@ struct RouteArgs {
     int n_tok, n_exp, k, n_group, topk_group, group_best;
     int dtype, sigmoid, renorm;
     int wide;                    // rows may be read in pieces of a lane's adjacent values
-    int group_lanes;             // lanes that look through a group: a power of two
+    int group_size, group_shift; // experts of a group, lanes that look through it: 2^group_shift
     uint32_t group_div;          // e / (n_exp / n_group) = e * group_div >> 20
     float scale;
 };
@@ -295,25 +295,35 @@ __device__ __forceinline__ double exact_score(const RouteArgs& a, double l, floa
     return a.sigmoid ? sigmoid(l) : exp_below(l, (double)top) / sum;
 }
 
-// The lanes that a group's values are with: group g has lanes g L .. g L + L - 1.  Its largest and second largest value of those
+// The values of a lane that W lanes, or a mirror of the W next, are between: fit for sums and maxima over 16 lanes.
+template <int W>
+__device__ __forceinline__ float partner(float v) { return __uint_as_float(lanes::partner<W>(__float_as_uint(v))); }
+template <int W>
+__device__ __forceinline__ double partner(double v) { return lanes::partner_f64<W>(v); }
+
+// The lanes that a group's values are with: with L = 2^group_shift, group g has lanes g L .. g L + L - 1.  Its largest and second largest value of those
 // in LDS, in all of its lanes.
 template <typename F>
 __device__ __forceinline__ void best_two(const RouteArgs& a, const F* lds, int lane, F& first, F& second) {
-    const int per = a.n_exp / a.n_group, L = a.group_lanes, g = lane / L;
+    const int per = a.group_size, L = 1 << a.group_shift, g = lane >> a.group_shift;
     first = second = -(F)kInf;
     auto least = [](F x, F y) { return x < y ? x : y; };
     auto most = [](F x, F y) { return x > y ? x : y; };
     if (g < a.n_group)
-        for (int i = lane % L; i < per; i += L) {
+        for (int i = lane & (L - 1); i < per; i += L) {
             const F v = lds[g * per + i];
             second = most(second, least(v, first));
             first = most(first, v);
         }
-    for (int d = 1; d < L; d <<= 1) {
-        const F f = __shfl_xor(first, d, 64), s = __shfl_xor(second, d, 64);
+    auto merge = [&](F f, F s) {
         second = most(most(second, s), least(first, f));
         first = most(first, f);
-    }
+    };
+    if (L > 1) merge(partner<1>(first), partner<1>(second));
+    if (L > 2) merge(partner<2>(first), partner<2>(second));
+    if (L > 4) merge(partner<4>(first), partner<4>(second));
+    if (L > 8) merge(partner<8>(first), partner<8>(second));
+    for (int d = 16; d < L; d <<= 1) merge(__shfl_xor(first, d, 64), __shfl_xor(second, d, 64));
     if (a.group_best > 1 && second > -(F)kInf) first += second;
 }
 
@@ -322,8 +332,8 @@ __device__ __forceinline__ void best_two(const RouteArgs& a, const F* lds, int l
 template <int P>
 __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)[P], float top, const float (&value)[P], float err, bool exact,
                                             double* lds, int lane, uint32_t (&key)[P]) {
-    const int L = a.group_lanes, g = lane / L;
-    const bool one = g < a.n_group && lane % L == 0;
+    const int shift = a.group_shift, g = lane >> shift;
+    const bool one = g < a.n_group && g << shift == lane;
     float* lds32 = (float*)lds;
 #pragma unroll
     for (int i = 0; i < P; ++i) lds32[Row<P>::at(lane, i)] = value[i];
@@ -333,7 +343,7 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
     wave_lds_fence();
     int before = 0;
     for (int h = 0; h < a.n_group; ++h) {
-        const float o = lane_value(v, h * L);
+        const float o = lane_value(v, h << shift);
         before += o > v || (o == v && h < g);
     }
     bool stays = one && before < a.topk_group;
@@ -356,7 +366,7 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
             wave_lds_fence();
             before = 0;
             for (int h = 0; h < a.n_group; ++h) {
-                const double o = __shfl(w, h * L, 64);
+                const double o = __shfl(w, h << shift, 64);
                 before += o > w || (o == w && h < g);
             }
             stays = one && before < a.topk_group;
@@ -365,7 +375,7 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
     const uint64_t kept = __ballot(stays);
 #pragma unroll
     for (int i = 0; i < P; ++i)
-        if (!(kept >> ((Row<P>::at(lane, i) * a.group_div >> 20) * L & 63) & 1)) key[i] = 0;
+        if (!(kept >> ((Row<P>::at(lane, i) * a.group_div >> 20 << shift) & 63) & 1)) key[i] = 0;
 }
 
 // The k largest of more than 64 sums of a score and a bias that 32 bits do not tell apart, in 64 bits and k rounds.  key: 0 for
@@ -459,21 +469,19 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
         else c = in_rounds<P>(key, l, a.k, lane);
     } else if (GENERAL && a.bias) {
         const float v = order_value(mine);
-        float err = 0.f, b = 0.f;
+        int near = 0;                                                          // within both bounds of this lane's, itself among them
+        for (int j = 0; j < c.n; ++j) {
+            const float o = lane_value(v, j);
+            c.place += o > v;
+            near += !(fabsf(o - v) > 2 * s_err);
+        }
+        float b = 0.f;
         c.l = 0.f;
         if (c.has) {
             c.l = read_one(a.logits, t * a.ld + c.id, a.dtype);
             b = a.bias[c.id];
-            const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-c.l)) : (c.l == top ? 1.f : __expf(c.l - top)) / sum;
-            const float x = a.sigmoid ? fabsf(c.l) * (1.f - s) : top - c.l;
-            err = s * (fminf(x, 110.f) + (a.sigmoid ? 8.f : 24.f)) * 0x1p-22f + fabsf(v) * 0x1p-23f;
         }
-        bool close = false;
-        for (int j = 0; j < c.n; ++j) {
-            const float o = lane_value(v, j), oerr = lane_value(err, j);
-            c.place += o > v;
-            close |= j != lane && c.has && !(fabsf(o - v) > err + oerr);
-        }
+        const bool close = c.has && near > 1;
         if (__any(close)) {
             const double all = a.sigmoid ? 0.0 : exact_sum<P>(l, top);             // (by every lane, before any condition)
             const uint64_t key64 = c.has ? order_key(exact_score(a, (double)c.l, top, all) + (double)b) : 0;
@@ -650,8 +658,8 @@ extern "C" int moe_route(const void* logits, int64_t ld, int n_tok, int n_exp, i
         constexpr int P = decltype(width)::value;
         RouteArgs a = {logits, bias, ids, weights, ld, n_tok, n_exp, k, n_group, topk_group, group_best, dtype, score, renorm};
         a.wide = wide_rows(logits, ld, dtype, Row<P>::V);
-        a.group_lanes = 1;
-        while (2 * a.group_lanes * n_group <= 64) a.group_lanes *= 2;
+        a.group_size = n_exp / n_group;
+        while (n_group << (a.group_shift + 1) <= 64) ++a.group_shift;
         a.group_div = (1u << 20) / (uint32_t)(n_exp / n_group) + 1;
         a.scale = scale;
         return launch_tokens(a, ld * (dtype == 2 ? 4 : 2), 0, [&](const RouteArgs& part, dim3 grid) {
