@@ -559,15 +559,12 @@ bool too_many(const char* who, int64_t blocks, int threads) {
 
 uint64_t round_up(uint64_t v) { return (v + 255) / 256 * 256; }
 
-#ifdef LINEAR_SWEEP
-int sweep() { const char* s = getenv("LINEAR_CFG"); return s ? atoi(s) : -1; }
-#endif
-
 // The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two.
 template <typename F>
 int each_tiles(const F& f) {
     f(Tiles<64, 64, 2, 2, 2, 3, 2, 8>(), 24, 48);
     f(Tiles<64, 64, 2, 2, 1, 4, 2, 8>(), 25, 45);
+    f(Tiles<128, 64, 4, 2, 1, 4, 2, 8>(), 38, 80);
     f(Tiles<128, 64, 2, 2, 1, 3, 2, 8>(), 42, 75);
     f(Tiles<128, 128, 2, 4, 1, 4, 2, 6>(), 55, 110);
     f(Tiles<128, 128, 2, 2, 1, 2, 2, 8>(), 90, 97);
@@ -595,9 +592,6 @@ int best_tiles(const Product& a, const Product& b, const R& run) {
         if (cost < best) best = cost, pick = i;
         ++i;
     });
-#ifdef LINEAR_SWEEP
-    if (sweep() >= 0 && sweep() < 6) pick = sweep();
-#endif
     int rc = -1;
     i = 0;
     each_tiles([&](auto tiles, int, int) {
@@ -609,11 +603,7 @@ int best_tiles(const Product& a, const Product& b, const R& run) {
 template <typename T>
 int forward(const Product& a, const Epilogue& e, hipStream_t s) {
     const int64_t tiles16 = tiles_in<16, 16>(a);
-    bool few = a.np <= 16 || tiles16 <= 256;
-#ifdef LINEAR_SWEEP
-    if (sweep() >= 0) few = sweep() == 9;
-#endif
-    if (few) {
+    if (a.np <= 16 || tiles16 <= 256) {
         if (too_many("linear", tiles16, 64 * kFewWaves)) return -1;
         hipLaunchKernelGGL((k_linear_few<T>), dim3((uint32_t)tiles16), dim3(64 * kFewWaves), 0, s, a, e);
         HIP_TRY(hipGetLastError());
@@ -632,11 +622,7 @@ int forward(const Product& a, const Epilogue& e, hipStream_t s) {
 // The parts of dW's contraction, the tokens: as many as give every CU a tile of 64 x 64, of 16 steps or more.
 int dw_parts(int n_tok, int n_out, int n_in) {
     const int64_t tiles = ((int64_t)n_out + 63) / 64 * (((int64_t)n_in + 63) / 64), steps = (int64_t)n_tok / kBC;
-    int64_t parts = std::min(256 / tiles, steps / 16);
-#ifdef LINEAR_SWEEP
-    if (const char* s = getenv("LINEAR_PARTS")) parts = atoi(s);
-#endif
-    return (int)std::max<int64_t>(1, parts);
+    return (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
 }
 
 template <typename T>

@@ -317,12 +317,13 @@ def _half(who: str, t: torch.Tensor) -> int:
 
 # the current stream's handle without a Stream object around it, where torch has that (a microsecond per call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_gpu = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _call(name: str, dev: int, *args) -> None:
     """Calls an entry point on the tensors' own GPU and that GPU's current stream."""
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev:
+    if _current_gpu() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
