@@ -105,8 +105,8 @@ __device__ __forceinline__ void widen8(uint4 v, f32x4 (&f)[2]) {
 
 // 8 adjacent columns of a row out: act(sum + bias) + res, and z.
 template <typename T>
-__device__ __forceinline__ void finish8(const Product& a, const Epilogue& e, int64_t r, int c, const f32x4 (&sum)[2], const f32x4 (&bias)[2],
-                                        uint4 res) {
+__device__ __forceinline__ void finish8(const Product& a, const Epilogue& e, int64_t r, int c, const f32x4 (&sum)[2],
+                                        const f32x4 (&bias)[2], uint4 res) {
     f32x4 z[2], y[2], rs[2];
     widen8<T>(res, rs);
     by_act(e.act, [&](auto act) {
@@ -142,6 +142,10 @@ __device__ __forceinline__ void tile_at(const Product& a, uint32_t item, int& p0
     q0 = (int)(panel * PANEL + i % width) * BQ;
 }
 
+// What bounds it: full grids of large tiles the matrix unit (8192 x 4096 x 4096 bf16 in 256 x 256: 207-225 us, 54% busy, 1220-1330
+// TFLOP/s; the library's product 176-192), grids of one tile per CU the steps' latencies (4096 x 2048 x 512 in 128 x 64: 14.2 us, 0.37 us a
+// step; the library's 15).  In panels: 4096 x 4096 x 4096 in tiles of 64 205 us, 294 in lines, of 256 105 and 113.
+//
 // One tile of BP x BQ results by WP x WQ waves, or SPLIT = 2 times as many that take turns at the steps.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers, RING - 1 steps ahead of the one that is multiplied: with one
 // tile per block nothing else hides the way through memory.  One barrier per step (and two steps, of SPLIT = 2).
@@ -277,7 +281,9 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     if constexpr (SPLIT == 2) {
         // the waves of a turn hand the other's half of the rows over and add what they get
         static_assert(2 * kWaves * kOwn * SQ * 1024 <= SPLIT * RING * kStage, "");
-        auto box = [&](int turn, int i, int j) { return lds_all + (uint32_t)((((turn * kWaves + wv) * kOwn + i) * SQ + j) * 1024 + lane * 16); };
+        auto box = [&](int turn, int i, int j) {
+            return lds_all + (uint32_t)((((turn * kWaves + wv) * kOwn + i) * SQ + j) * 1024 + lane * 16);
+        };
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
 #pragma unroll
@@ -307,14 +313,16 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
         for (int it = 0; it < kIts; ++it) {
             const int r = p0 + wp * SP * 16 + (turn_of * kOwn + i) * 16 + it * kRowsPer + l / kUnits;
             row[it] = r < a.np && in ? r : -1;
-            rv[it] = KIND == kForward && e.res && row[it] >= 0 ? *(const uint4*)((const T*)e.res + row[it] * e.ldr + c) : make_uint4(0, 0, 0, 0);
+            rv[it] = make_uint4(0, 0, 0, 0);
+            if (KIND == kForward && e.res && row[it] >= 0) rv[it] = *(const uint4*)((const T*)e.res + row[it] * e.ldr + c);
         }
 #pragma unroll
         for (int j = 0; j < SQ; ++j) *(lds16)(uintptr_t)at(l16, 4 * j + lq) = __builtin_bit_cast(u32x4, acc[i][j]);
 #pragma unroll
         for (int it = 0; it < kIts; ++it) {
             const int m = it * kRowsPer + l / kUnits;
-            const f32x4 sum[2] = {__builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8)), __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + 1))};
+            const f32x4 sum[2] = {__builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8)),
+                                  __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + 1))};
             if (row[it] < 0) continue;
             if constexpr (KIND == kForward) {
                 finish8<T>(a, e, row[it], c, sum, bias, rv[it]);
@@ -413,6 +421,10 @@ __global__ __launch_bounds__(256) void k_linear_parts(Parts p, uint32_t blocks, 
     }
 }
 
+// Up to 256 tiles of 16 x 16, and up to 16 tokens, where a tile of 64 rows would be mostly empty.  us of these and of the tiles above:
+// 8 x 2048 x 2048 5.7 and 8.3, 24 x 2048 x 2048 (256 of them) 6.4 and 8.4, 64 x 2048 x 512 (128) 6.5 and 8.3; 48 x 2048 x 2048 (384)
+// 9.9 and 8.4, 512 x 2048 x 512 (1024) 17.8 and 8.6.  8 x 2048 x 2048: 8.5 MB at 1.5 TB/s, one run through memory and back.
+//
 // Few results: a block has 16 x 16 of them, its waves take turns at the steps, and their sums meet in LDS.  Rows of both
 // operands come straight into the matrix unit's layout, four of a wave's steps under way at once, and no wave waits for another
 // before the end.
@@ -476,7 +488,8 @@ struct DzArgs {
     int rows;                    // of a block
 };
 
-// A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.
+// A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.  1999 x 640 fp16 through silu 4.2-6.6 us:
+// 7.7 MB, a load, an exponential and a store after one another.
 template <typename T, bool F32>
 __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
     __shared__ f32x4 part[8][32][2];
@@ -531,7 +544,8 @@ int dz_blocks(int n_tok, int n) { return (int)(((int64_t)n_tok + dz_rows(n_tok, 
 
 bool bad_matrix(const char* who, const char* name, const void* p, int64_t ld, int64_t width, int64_t rows) {
     if (ld % 8 || (rows > 1 && ld < width) || ld < 0) {
-        moe_set_error("%s: %s: rows of %lld elements at a step of %lld (a multiple of 8 wanted)", who, name, (long long)width, (long long)ld);
+        moe_set_error("%s: %s: rows of %lld elements at a step of %lld (a multiple of 8 wanted)", who, name, (long long)width,
+                      (long long)ld);
         return true;
     }
     if (rows > 0 && (!p || (uintptr_t)p % 16)) {
@@ -559,7 +573,11 @@ bool too_many(const char* who, int64_t blocks, int threads) {
 
 uint64_t round_up(uint64_t v) { return (v + 255) / 256 * 256; }
 
-// The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two.
+// The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two, as measured.  us per forward product in
+// their order, chosen *: 1024 x 1024 x 1024 6.7* 7.3 - 9.9 11.5 14.6 29; 1030 x 72 x 1856 6.5 4.7* 7.4 5.7 5.6 7.4 12; 4096 x
+// 2048 x 512 17.4 15.2 13.4* 14.1 17.1 23.9 44; 2048 x 2048 x 2048 33 28 25.6 22.4 19.5* 27.9 44; 4096 x 4096 x 4096 229 199 174 159
+// 146 124 106*.  Both gradients: 333 x 640 x 2560 13.4* 12.3 14.5 14.5 18.4 26.7 48; 1999 x 2560 x 640 36 28 28 24 21.5* 27 44; 2048 x
+// 2048 x 2048 61 53 49 43 38 32* 44; 4096 x 2048 x 512 42 33 32 28* 33 49 81; 8192 x 4096 x 4096 864 1043 - 709 544 472 408*.
 template <typename F>
 int each_tiles(const F& f) {
     f(Tiles<64, 64, 2, 2, 2, 3, 2, 8>(), 24, 48);
@@ -619,14 +637,17 @@ int forward(const Product& a, const Epilogue& e, hipStream_t s) {
     });
 }
 
-// The parts of dW's contraction, the tokens: as many as give every CU a tile of 64 x 64, of 16 steps or more.
+// The parts of dW's contraction, the tokens: as many as give every CU a tile of 64 x 64, of 16 steps or more.  us of both gradients
+// with 1, 2, 4, 8, 16 parts: 8192 x 512 x 256 28.9 21.5 15.4 14.4* 15.7, 8192 x 2048 x 64 45 48 28 25* 22, 4096 x 2048 x 128 26.6 19.4
+// 16.0* 18 22, 4096 x 2048 x 512 32.2* 33.1 30.3 35 59.
 int dw_parts(int n_tok, int n_out, int n_in) {
     const int64_t tiles = ((int64_t)n_out + 63) / 64 * (((int64_t)n_in + 63) / 64), steps = (int64_t)n_tok / kBC;
     return (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
 }
 
 template <typename T>
-int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const Product& dx, const BiasSums& b, const Parts& p, hipStream_t s) {
+int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const Product& dx, const BiasSums& b, const Parts& p,
+              hipStream_t s) {
     return best_tiles(dw, dx, [&](auto tiles) {
         using C = decltype(tiles);
         const bool parts = dw.parts > 1 && dw.np > 0;

@@ -156,9 +156,9 @@ def combine(y, weights, residual=None):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, act, residual, dtype):
+    def forward(ctx, x, w, bias, act, residual, dtype, training):
         z = None
-        if act is not None and any(ctx.needs_input_grad[:3]):
+        if training and act is not None and any(ctx.needs_input_grad[:3]):
             z = torch.empty((x.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
         ctx.save_for_backward(x, w, z)
         ctx.act = act
@@ -169,18 +169,18 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         _refuse_capture("linear")
         x, w, z = ctx.saved_tensors
-        want_dx, want_dw, want_db, _, want_dr, _ = ctx.needs_input_grad
+        want_dx, want_dw, want_db, _, want_dr, _, _ = ctx.needs_input_grad
         dx = dw = db = None
         if want_dx or want_dw or want_db:
             dx, dw, db = ops.linear_grad(_operand(dy), x, w, z=z, act=ctx.act, bias=want_db, want_dx=want_dx, want_dw=want_dw)
-        return dx, dw, db, None, dy.to(x.dtype) if want_dr else None, None
+        return dx, dw, db, None, dy.to(x.dtype) if want_dr else None, None, None
 
 
 def linear(x, w, bias=None, act=None, residual=None, dtype=None):
     """ops.linear, differentiable in x, w, bias and residual; with an activation the pre-activations are kept in the
     inputs' type for the backward pass."""
     _refuse_capture("linear")
-    return _Linear.apply(x, w, bias, act, residual, dtype)
+    return _Linear.apply(x, w, bias, act, residual, dtype, torch.is_grad_enabled())
 
 
 def moe_layer(x, w_router, w_gate_up, w_down, k, score="softmax", bias=None, n_group=1, topk_group=1, group_best=1, renorm=True,
@@ -200,6 +200,10 @@ def moe_layer(x, w_router, w_gate_up, w_down, k, score="softmax", bias=None, n_g
 
 
 def clip_grad_norm(parameters, max_norm):
-    """ops.clip_grad_norm of the parameters' gradients, in place (those without one are left out); returns the norm before."""
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    return ops.clip_grad_norm([p.grad for p in parameters if p.grad is not None], max_norm)
+    """ops.clip_grad_norm of the parameters' gradients, in place (those without one are left out; 0 if all are); returns the norm
+    before."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device=parameters[0].device if parameters else None)
+    return ops.clip_grad_norm(grads, max_norm)

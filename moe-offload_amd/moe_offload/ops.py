@@ -756,8 +756,7 @@ def combine_grad(dout, y, weights):
     _per_place(who, "weights", weights, (n_tok, k), torch.float32)
     hidden, ldy = _pair_rows(who, "y", y, n_tok, k)
     ldd = _rows(who, "dout", dout, y.dtype, n_tok, hidden)
-    dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    dw = torch.empty((n_tok, k), dtype=torch.float32, device=y.device)
+    dy, dw = torch.empty_like(y, memory_format=torch.contiguous_format), torch.empty_like(weights)
     _call("moe_combine_grad", dev, _p(dout), ldd, _p(y), ldy, _p(weights), n_tok, k, hidden, dt, _p(dy), hidden, _p(dw))
     return dy, dw
 

@@ -97,6 +97,12 @@ def test_layer_shapes_and_constants_are_checked():
         dense.route(torch.zeros((4, 8)), 2, bias=torch.zeros(8, requires_grad=True))
 
 
+def test_parameters_without_gradients_have_the_norm_0():
+    for parameters in ([], torch.zeros(4, requires_grad=True), iter([torch.zeros(4, requires_grad=True)])):
+        norm = dense.clip_grad_norm(parameters, 1.0)
+        assert norm.shape == () and norm.dtype == torch.float32 and float(norm) == 0.0
+
+
 def test_route_arguments():
     good = (P, 512, 4, 512, 10, 0, 1, None, 8, 4, 2, 1.0, 2, P, P, None)
     for i, bad in ((0, None), (1, 511), (2, -1), (3, 0), (3, 1025), (4, 0), (4, 33), (5, 2), (5, -1), (6, 2), (8, 0), (8, 65), (8, 3), (9, 0),
