@@ -86,7 +86,7 @@ struct Product {
     void* out;
     int64_t ldp, ldq, ldo;       // elements from row to row of memory
     int np, nq, nc;              // extents: rows and columns of out, and the contraction
-    int parts, part_c;           // dW: the contraction in parts of part_c, each with results of its own (fp32, [parts][np][nq])
+    int parts, part_c;           // the contraction in parts of part_c, each with sums of its own (fp32, [parts][np][nq]; not dx)
 };
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
@@ -163,12 +163,12 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     const T* Q = (const T*)a.q;
     int nc = a.nc;
     int64_t part = 0;
-    if constexpr (KIND == kDw) {
+    if (KIND != kDx && a.parts > 1) {
         const uint32_t tiles = (uint32_t)tiles_in<BP, BQ>(a);
         part = item / tiles;
         item -= (uint32_t)part * tiles;
-        P += part * a.part_c * a.ldp;
-        Q += part * a.part_c * a.ldq;
+        P += part * a.part_c * (kAlongP ? a.ldp : 1);
+        Q += part * a.part_c * (kAlongQ ? a.ldq : 1);
         nc = nc - part * a.part_c < a.part_c ? (int)(nc - part * a.part_c) : a.part_c;
     }
     int p0, q0;
@@ -324,12 +324,12 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
             const f32x4 sum[2] = {__builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8)),
                                   __builtin_bit_cast(f32x4, *(lds16)(uintptr_t)at(m, 2 * u8 + 1))};
             if (row[it] < 0) continue;
-            if constexpr (KIND == kForward) {
-                finish8<T>(a, e, row[it], c, sum, bias, rv[it]);
-            } else if (KIND == kDw && e.out_f32) {
+            if ((KIND == kDw && e.out_f32) || (KIND == kForward && a.parts > 1)) {
                 float* d = (float*)a.out + (part * a.np + row[it]) * a.ldo + c;
                 store16(d, __builtin_bit_cast(uint4, sum[0]));
                 store16(d + 4, __builtin_bit_cast(uint4, sum[1]));
+            } else if constexpr (KIND == kForward) {
+                finish8<T>(a, e, row[it], c, sum, bias, rv[it]);
             } else {
                 store16((T*)a.out + row[it] * a.ldo + c, round8<T>(sum));
             }
@@ -349,6 +349,27 @@ template <typename T, typename C>
 __global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear(Product a, Epilogue e) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
     tile_product<T, kForward, C>(a, e, xcd_order(blockIdx.x, gridDim.x), lds);
+}
+
+// y from the parts of its contraction, in their order: a thread has 8 columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ sums, int parts, Product a, Epilogue e) {
+    const uint32_t units = a.nq / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / units;
+    const int c = (int)(i - r * units) * 8;
+    if (r >= a.np) return;
+    f32x4 s[2] = {}, bias[2] = {};
+    const float* from = sums + r * a.nq + c;
+    const int64_t step = (int64_t)a.np * a.nq;
+    uint4 res = make_uint4(0, 0, 0, 0);
+    if (e.res) res = *(const uint4*)((const T*)e.res + r * e.ldr + c);
+    if (e.bias) widen8<T>(*(const uint4*)((const T*)e.bias + c), bias);
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+        s[0] += *(const f32x4*)(from + k * step);
+        s[1] += *(const f32x4*)(from + k * step + 4);
+    }
+    finish8<T>(a, e, r, c, s, bias, res);
 }
 
 // What k_linear_dz left of the bias's gradient: [blocks][n], summed in order by a block of 64 columns and 4 parts of the rows.
@@ -618,21 +639,44 @@ int best_tiles(const Product& a, const Product& b, const R& run) {
     return rc;
 }
 
+// The length of a part, whole steps.
+int part_of(int64_t nc, int parts) { return (int)((nc + (int64_t)parts * kBC - 1) / ((int64_t)parts * kBC) * kBC); }
+
+// Results few enough for k_linear_few.
+bool few_results(int n_tok, int n_out) { return n_tok <= 16 || ((int64_t)n_tok + 15) / 16 * (((int64_t)n_out + 15) / 16) <= 256; }
+
+// The parts of a forward product's contraction: as many as give every CU a tile of 64 x 64, of 8 steps or more, if a tile is rid of
+// 30 steps that way, which pays for the second launch.  us with 1, 2, 4, 8 parts: 32 x 4096 x 4096 (64 steps) 14.2 12.7 10.5* 11.8, 256 x
+// 4096 x 1024 15.1 12.8 10.8* 12.9, 128 x 4096 x 1024 13.4 12.0 10.1 10.1*, 100 x 2560 x 640 (40) 9.5 9.8 8.4 8.9 (5: 8.6*), 128 x 2048
+// x 2048 (32) 8.6* 10.2 9.4 11.6.
+int forward_parts(int n_tok, int n_in, int n_out) {
+    if (n_tok < 1 || few_results(n_tok, n_out)) return 1;
+    const int64_t tiles = ((int64_t)n_tok + 63) / 64 * (((int64_t)n_out + 63) / 64), steps = (int64_t)n_in / kBC;
+    const int64_t parts = std::min(256 / tiles, steps / 8);
+    return parts < 2 || steps * (parts - 1) < 30 * parts ? 1 : (int)parts;
+}
+
 template <typename T>
-int forward(const Product& a, const Epilogue& e, hipStream_t s) {
+int forward(const Product& a, const Epilogue& e, void* workspace, hipStream_t s) {
     const int64_t tiles16 = tiles_in<16, 16>(a);
-    if (a.np <= 16 || tiles16 <= 256) {
+    if (few_results(a.np, a.nq)) {
         if (too_many("linear", tiles16, 64 * kFewWaves)) return -1;
         hipLaunchKernelGGL((k_linear_few<T>), dim3((uint32_t)tiles16), dim3(64 * kFewWaves), 0, s, a, e);
         HIP_TRY(hipGetLastError());
         return 0;
     }
-    return best_tiles(a, Product{}, [&](auto tiles) {
+    Product sums = a;
+    if (a.parts > 1) sums.out = workspace, sums.ldo = a.nq;
+    return best_tiles(sums, Product{}, [&](auto tiles) {
         using C = decltype(tiles);
-        const int64_t blocks = tiles_in<C::BP, C::BQ>(a);
-        if (too_many("linear", blocks, C::kThreads)) return -1;
-        hipLaunchKernelGGL((k_linear<T, C>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, a, e);
+        const int64_t blocks = tiles_in<C::BP, C::BQ>(a) * a.parts, joins = ((int64_t)a.np * (a.nq / 8) + 255) / 256;
+        if (too_many("linear", blocks, C::kThreads) || (a.parts > 1 && too_many("linear", joins, 256))) return -1;
+        hipLaunchKernelGGL((k_linear<T, C>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, sums, e);
         HIP_TRY(hipGetLastError());
+        if (a.parts > 1) {
+            hipLaunchKernelGGL((k_linear_join<T>), dim3((uint32_t)joins), dim3(256), 0, s, (const float*)workspace, a.parts, a, e);
+            HIP_TRY(hipGetLastError());
+        }
         return 0;
     });
 }
@@ -689,9 +733,15 @@ Layout layout(int n_tok, int n_in, int n_out, bool own_dz, bool want_dw, bool wa
 
 }  // namespace
 
+extern "C" uint64_t moe_linear_workspace_bytes(int n_tok, int n_in, int n_out) {
+    if (n_tok < 1 || n_in < 1 || n_out < 1) return 0;
+    const int parts = forward_parts(n_tok, n_in, n_out);
+    return parts > 1 ? 4 * (uint64_t)parts * n_tok * n_out : 0;
+}
+
 extern "C" int moe_linear(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual, int64_t ldr, int n_tok,
-                          int n_in, int n_out, int act, int dtype, int out_f32, void* z, int64_t ldz, void* y, int64_t ldy,
-                          void* stream) {
+                          int n_in, int n_out, int act, int dtype, int out_f32, void* workspace, void* z, int64_t ldz, void* y,
+                          int64_t ldy, void* stream) {
     const char* who = "linear";
     if (bad_sizes(who, n_tok, n_in, n_out, act, dtype) || bad_matrix(who, "x", x, ldx, n_in, n_tok) ||
         bad_matrix(who, "w", w, n_in, n_in, n_out) || (bias && bad_matrix(who, "bias", bias, n_out, n_out, 1)) ||
@@ -699,9 +749,15 @@ extern "C" int moe_linear(const void* x, int64_t ldx, const void* w, const void*
         (z && bad_matrix(who, "z", z, ldz, n_out, n_tok)) || bad_matrix(who, "y", y, ldy, n_out, n_tok))
         return -1;
     if (n_tok == 0) return 0;
-    const Product a = {x, w, y, ldx, n_in, ldy, n_tok, n_out, n_in, 1, 0};
+    const int parts = forward_parts(n_tok, n_in, n_out);
+    if (parts > 1 && (!workspace || (uintptr_t)workspace % 16)) {
+        moe_set_error("linear: the workspace is null or not 16-byte aligned");
+        return -1;
+    }
+    const Product a = {x, w, y, ldx, n_in, ldy, n_tok, n_out, n_in, parts, part_of(n_in, parts)};
     const Epilogue e = {bias, residual, z, ldr, ldz, act, out_f32};
-    return dtype ? forward<__bf16>(a, e, (hipStream_t)stream) : forward<_Float16>(a, e, (hipStream_t)stream);
+    const hipStream_t s = (hipStream_t)stream;
+    return dtype ? forward<__bf16>(a, e, workspace, s) : forward<_Float16>(a, e, workspace, s);
 }
 
 extern "C" uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_in, int n_out, int act, int dy_f32, int want_dw, int want_db) {
@@ -730,9 +786,9 @@ extern "C" int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const v
     const int64_t ld = own_dz ? n_out : lddy;
     float* sums = db ? (float*)((char*)workspace + at.sums) : nullptr;
     const DzArgs d = {dy, act != kActNone ? z : nullptr, dz, sums, lddy, ldz, n_tok, n_out, act, dz_rows(n_tok, n_out)};
-    const int parts = dw ? dw_parts(n_tok, n_out, n_in) : 1, part_c = (int)(((int64_t)n_tok + parts * kBC - 1) / (parts * kBC) * kBC);
+    const int parts = dw ? dw_parts(n_tok, n_out, n_in) : 1;
     void* into = parts > 1 ? (char*)workspace + at.parts : dw;
-    const Product gw = {rows, x, into, ld, ldx, n_in, dw ? n_out : 0, n_in, n_tok, parts, part_c};
+    const Product gw = {rows, x, into, ld, ldx, n_in, dw ? n_out : 0, n_in, n_tok, parts, part_of(n_tok, parts)};
     const Product gx = {rows, w, dx, ld, n_in, n_in, dx ? n_tok : 0, n_in, n_out, 1, 0};
     const BiasSums b = {sums, db, dz_blocks(n_tok, n_out), n_out};
     const Parts p = {(const float*)into, dw, (int64_t)n_out * n_in, parts, dw_f32};

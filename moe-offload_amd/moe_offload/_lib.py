@@ -131,8 +131,9 @@ SIGNATURES: dict[str, tuple] = {
                                 _c_vp]),
     "moe_combine": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_vp]),
     "moe_combine_grad": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_vp, _c_vp]),
+    "moe_linear_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int]),
     "moe_linear": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp,
-                            _c_i64, _c_vp, _c_i64, _c_vp]),
+                            _c_vp, _c_i64, _c_vp, _c_i64, _c_vp]),
     "moe_linear_grad_workspace_bytes": (_c_u64, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "moe_linear_grad": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
                                  _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp]),

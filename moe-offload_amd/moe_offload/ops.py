@@ -766,16 +766,17 @@ def _shared_weight(who: str, w: torch.Tensor, dtype: torch.dtype, n_in: int) -> 
         raise ValueError(f"{who}: w must be contiguous with a multiple of 8 rows, not {tuple(w.shape)} at {w.stride()}")
 
 
-def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out=None):
+def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out=None, workspace=None):
     """act(x @ w.T + bias) + residual: a projection that all tokens share (the router, a shared expert), in one launch.
 
     x: fp16 or bf16 [n_tok, n_in]; w: same type [n_out, n_in], contiguous; bias: same type [n_out] or None; act: None, "silu",
     "gelu" (exact, by the normal distribution's integral) or "relu2" (the squared relu); residual: same type [n_tok, n_out] or None.
     The result has the inputs' type, or fp32 with dtype=torch.float32 (router logits).  z_out, [n_tok, n_out] of the inputs'
-    type, receives x @ w.T + bias for linear_grad.  out=residual adds in place.
+    type, receives x @ w.T + bias for linear_grad.  out=residual adds in place.  workspace: scratch of
+    moe_linear_workspace_bytes.
     """
     who = "linear"
-    dev = _one_gpu(who, "x w bias residual z_out out", x, w, bias, residual, z_out, out)
+    dev = _one_gpu(who, "x w bias residual z_out out workspace", x, w, bias, residual, z_out, out, workspace)
     dt = _half(who, x)
     act = _choice(who, "act", act, _ACTS)
     ldx = _rows(who, "x", x, x.dtype, None, None)
@@ -787,8 +788,10 @@ def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out
     ldr = _rows(who, "residual", residual, x.dtype, n_tok, n_out) if residual is not None else 0
     ldz = _rows(who, "z_out", z_out, x.dtype, n_tok, n_out) if z_out is not None else 0
     out, ldy = _result(who, x, out, dtype, n_tok, n_out)
+    nb = _lib.lib().moe_linear_workspace_bytes(n_tok, n_in, n_out)
+    ws = _scratch(nb, x, workspace, who) if nb else None
     _call("moe_linear", dev, _p(x), ldx, _p(w), _p(bias), _p(residual), ldr, n_tok, n_in, n_out, act, dt,
-          int(out.dtype == torch.float32), _p(z_out), ldz, _p(out), ldy)
+          int(out.dtype == torch.float32), _p(ws), _p(z_out), ldz, _p(out), ldy)
     return out
 
 

@@ -22,7 +22,7 @@ def rnd(shape, dtype, seed, scale=1.0):
 # (tokens, n_in, n_out), one size at least for every kind of tile, with sides that end inside one
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n_tok,n_in,n_out", [(40, 200, 72), (600, 264, 520), (1030, 72, 1856), (513, 72, 2056), (513, 72, 4104), (2049, 136, 2056),
-                                              (2049, 72, 4104), (8192, 328, 4104)])
+                                              (2049, 72, 4104), (8192, 328, 4104), (70, 4104, 1032), (100, 2600, 328), (520, 4000, 200)])
 def test_every_tile_forward(dtype, n_tok, n_in, n_out):
     from moe_offload import ops
     x, w, b, res = rnd((n_tok, n_in), dtype, 1), rnd((n_out, n_in), dtype, 2, n_in ** -0.5), rnd((n_out,), dtype, 3), rnd((n_tok, n_out), dtype, 4)
@@ -151,6 +151,16 @@ def test_a_given_workspace_may_be_larger_and_hold_anything():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(ValueError, match="workspace"):
         ops.linear_grad(dy, x, w, z=z, act="relu2", bias=True, workspace=ws[:100])
+    # a long contraction over few tiles; with 512 columns it needs none
+    for n_out in (512, 1032):
+        a, b = rnd((70, 4096), torch.float16, 5), rnd((n_out, 4096), torch.float16, 6, 1 / 64)
+        out = torch.full((90, n_out + 8), 7.0, dtype=torch.float16, device=DEV)
+        want = ops.linear(a, b, act="gelu")
+        assert torch.equal(ops.linear(a, b, act="gelu", workspace=ws), want)
+        ops.linear(a, b, act="gelu", workspace=ws, out=out[:70, 8:])
+        assert torch.equal(out[:70, 8:], want) and bool((out[70:] == 7).all()) and bool((out[:, :8] == 7).all())
+    with pytest.raises(ValueError, match="workspace"):
+        ops.linear(a, b, workspace=ws[:100])
 
 
 def test_refusals_on_the_gpu():

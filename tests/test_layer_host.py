@@ -130,12 +130,17 @@ def test_combine_arguments():
 
 
 def test_linear_arguments():
-    good = (P, 64, P, P, P, 128, 4, 64, 128, 1, 1, 0, P, 128, P, 128, None)
+    good = (P, 64, P, P, P, 128, 4, 64, 128, 1, 1, 0, None, P, 128, P, 128, None)
     for i, bad in ((0, None), (0, P + 8), (1, 56), (1, 68), (2, None), (2, P + 2), (3, P + 8), (4, P + 8), (5, 64), (6, -1), (7, 0), (7, 12), (8, 0),
-                   (8, 12), (9, 4), (9, -1), (10, 2), (12, P + 8), (13, 64), (14, None), (14, P + 8), (15, 64)):
+                   (8, 12), (9, 4), (9, -1), (10, 2), (13, P + 8), (14, 64), (15, None), (15, P + 8), (16, 64)):
         refused("moe_linear", *swapped(good, i, bad))
-    refused("moe_linear", P, 64, P, None, None, 0, (1 << 30) + 8, 64, 128, 0, 1, 0, None, 0, P, 128, None)
-    assert "more than one launch" in refused("moe_linear", P, 8, P, None, None, 0, 1 << 30, 8, 1 << 30, 0, 1, 0, None, 0, P, 1 << 30, None)
+    refused("moe_linear", P, 64, P, None, None, 0, (1 << 30) + 8, 64, 128, 0, 1, 0, None, None, 0, P, 128, None)
+    assert "more than one launch" in refused("moe_linear", P, 8, P, None, None, 0, 1 << 30, 8, 1 << 30, 0, 1, 0, None, None, 0, P, 1 << 30, None)
+    # few tiles of a long contraction take a workspace
+    ws = _lib.lib().moe_linear_workspace_bytes
+    assert ws(64, 4096, 4096) >= 2 * 4 * 64 * 4096 and ws(1, 4096, 4096) == 0 and ws(4096, 4096, 4096) == 0 and ws(0, 64, 64) == 0
+    for bad in (None, P + 8):
+        refused("moe_linear", P, 4096, P, None, None, 0, 64, 4096, 4096, 0, 1, 0, bad, None, 0, P, 4096, None)
     taken("moe_linear", *swapped(good, 6, 0))
     good = (P, 128, 0, P, 64, P, P, 128, 4, 64, 128, 1, 1, P, P, P, 0, P, None)
     for i, bad in ((0, None), (1, 64), (3, None), (4, 60), (5, None), (6, None), (7, 64), (8, -1), (8, (1 << 30) + 8), (9, 12), (10, 12), (11, 4), (12, 2),
