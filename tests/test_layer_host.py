@@ -103,6 +103,74 @@ def test_parameters_without_gradients_have_the_norm_0():
         assert norm.shape == () and norm.dtype == torch.float32 and float(norm) == 0.0
 
 
+# ---- the reference that the GPU tests compare with, against loops over its definition ---------------------
+
+def looped_route(row, k, score, bias, n_group, topk_group, group_best):
+    """[(id, score)] of one token, by sorting tuples."""
+    import math
+    live = [not math.isnan(v) and v > -math.inf for v in row]
+    top = max([v for v, ok in zip(row, live) if ok], default=0.0)
+    e = [(1.0 if v == top else math.exp(v - top)) if ok else 0.0 for v, ok in zip(row, live)]
+    s = [1 / (1 + math.exp(-v)) if ok else 0.0 for v, ok in zip(row, live)] if score == "sigmoid" else [v / (sum(e) or 1.0) for v in e]
+    c = [v + b for v, b in zip(s, bias)] if bias is not None else list(row)
+    live = [ok and not math.isnan(v) and v > -math.inf for ok, v in zip(live, c)]
+    per, stay = len(row) // n_group, set(range(n_group))
+    if n_group > 1:
+        of = c if bias is not None or group_best == 1 else s
+        value = []
+        for g in range(n_group):
+            best = sorted((of[i] for i in range(g * per, (g + 1) * per) if live[i]), reverse=True)[:group_best]
+            value.append(sum(best) if best else -math.inf)
+        stay = set(sorted(range(n_group), key=lambda g: (-value[g], g))[:topk_group])
+    order = sorted((i for i in range(len(row)) if live[i] and i // per in stay), key=lambda i: (-c[i], i))
+    return [(i, s[i]) for i in order[:k]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_reference_against_loops(score):
+    import math
+
+    import layer_ref as ref
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn((30, 24), generator=g, dtype=torch.float64)
+    logits[3] = logits[3].round()
+    logits[4, ::2] = -math.inf
+    logits[5] = -math.inf
+    logits[6, 3:] = -math.inf
+    bias = torch.randn(24, generator=g) * 0.2
+    bias[7] = -math.inf
+    for b in (None, bias):
+        for n_group, topk_group, best in ((1, 1, 1), (4, 2, 1), (4, 2, 2), (24, 5, 2), (3, 3, 2)):
+            for renorm in (True, False):
+                ids, w = ref.route(logits, 5, score, b, n_group, topk_group, best, renorm, 1.5)
+                for t, row in enumerate(logits.tolist()):
+                    want = looped_route(row, 5, score, None if b is None else b.tolist(), n_group, topk_group, best)
+                    total = sum(v for _, v in want) if renorm else 1.0
+                    assert ids[t].tolist() == [i for i, _ in want] + [-1] * (5 - len(want))
+                    assert w[t].tolist() == pytest.approx([1.5 * v / total for _, v in want] + [0.0] * (5 - len(want)), rel=1e-12)
+    # a mistake in the rule shows: equals by the highest index, groups by one score where two are asked for
+    flipped = 23 - ref.route(logits.flip(1), 5, score)[0]
+    assert not torch.equal(flipped.clamp(max=23)[3], ref.route(logits, 5, score)[0][3])
+    assert not torch.equal(ref.route(logits, 5, score, bias, 4, 2, 1)[0], ref.route(logits, 5, score, bias, 4, 2, 2)[0])
+
+
+def test_the_reference_gradients_against_differences():
+    import layer_ref as ref
+    g = torch.Generator().manual_seed(2)
+    logits, dw, v = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((8, 12), (8, 3), (8, 12)))
+    ids = ref.route(logits, 3)[0]
+    h = 1e-5
+    for score in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            d, _ = ref.route_grad(dw, logits, ids, score, renorm, 2.0)
+            f = [(ref.chosen_weights(logits + s * h * v, ids, ids >= 0, score, renorm, 2.0) * dw).sum() for s in (1, -1)]
+            assert float((d * v).sum()) == pytest.approx(float(f[0] - f[1]) / (2 * h), rel=1e-7, abs=1e-9)
+    x, w, z, dy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 8), (16, 8), (5, 16), (5, 16)))
+    for act in (None, "silu", "gelu", "relu2"):
+        diff = (ref.activation(z + h, act) - ref.activation(z - h, act)) / (2 * h)
+        assert torch.allclose(ref.slope(z, act), diff, rtol=1e-6, atol=1e-6)
+
+
 def test_route_arguments():
     good = (P, 512, 4, 512, 10, 0, 1, None, 8, 4, 2, 1.0, 2, P, P, None)
     for i, bad in ((0, None), (1, 511), (2, -1), (3, 0), (3, 1025), (4, 0), (4, 33), (5, 2), (5, -1), (6, 2), (8, 0), (8, 65), (8, 3), (9, 0),
