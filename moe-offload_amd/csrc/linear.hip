@@ -142,13 +142,16 @@ __device__ __forceinline__ void tile_at(const Product& a, uint32_t item, int& p0
     q0 = (int)(panel * PANEL + i % width) * BQ;
 }
 
-// What bounds it: full grids of large tiles the matrix unit (8192 x 4096 x 4096 bf16 in 256 x 256: 207-225 us, 54% busy, 1220-1330
-// TFLOP/s; the library's product 176-192), grids of one tile per CU the steps' latencies (4096 x 2048 x 512 in 128 x 64: 14.2 us, 0.37 us a
-// step; the library's 15).  In panels: 4096 x 4096 x 4096 in tiles of 64 205 us, 294 in lines, of 256 105 and 113.
+// What bounds it: full grids of large tiles the matrix unit and what feeds it (8192 x 4096 x 4096 bf16 in 256 x 256: 194-205 us, 1340-1420
+// TFLOP/s, 1.4 us a step and 8 at a tile's ends; the library's product 177-185), grids of one tile per CU the steps' latencies (4096 x 2048 x
+// 512 in 128 x 64: 14.1 us, 0.32 us a step; the library's 15).  In panels: 4096 x 4096 x 4096 in tiles of 64 205 us, 294 in lines, of 256
+// 105 and 113.  Tiles of 256 x 256 by four waves of 128 x 128, which read LDS less, took 106-121 for it: a wave alone on its SIMD
+// waits for every load that it issues.
 //
 // One tile of BP x BQ results by WP x WQ waves, or SPLIT = 2 times as many that take turns at the steps.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers, RING - 1 steps ahead of the one that is multiplied: with one
-// tile per block nothing else hides the way through memory.  One barrier per step (and two steps, of SPLIT = 2).
+// tile per block nothing else hides the way through memory.  One barrier per step (and two steps, of SPLIT = 2), at its start or,
+// in large tiles, in its middle, where half of the next step's operands are read from LDS behind this one's products.
 template <typename T, int KIND, typename C>
 __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e, uint32_t item, uint8_t* lds) {
     constexpr int BP = C::BP, BQ = C::BQ, WP = C::WP, WQ = C::WQ, RING = C::RING, SPLIT = C::SPLIT;
@@ -156,7 +159,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     constexpr bool kAlongP = KIND == kDw, kAlongQ = KIND != kForward;
     constexpr int kLoadsP = BP / 8 / kWaves, kLoadsQ = BQ / 8 / kWaves, kLoads = kLoadsP + kLoadsQ;   // 1 KiB each
     constexpr uint32_t kStageP = BP * 128, kStage = (BP + BQ) * 128;
-    static_assert(SQ % 2 == 0 && kLoadsP >= 1 && kLoadsQ >= 1 && RING * kStage / kWaves >= SQ * 1024, "");
+    static_assert((SQ == 2 || SQ == 4) && BP % (8 * kWaves) == 0 && BQ % (8 * kWaves) == 0 && RING * kStage / kWaves >= SQ * 1024, "");
     const int t = threadIdx.x, lane = t & 63, all = __builtin_amdgcn_readfirstlane(t >> 6), turn_of = all / kWaves, wv = all % kWaves;
     const uint32_t lds_all = (uint32_t)(uintptr_t)(lds_u8*)lds, lds0 = lds_all + turn_of * RING * kStage;
     const T* P = (const T*)a.p;
@@ -222,51 +225,103 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     fq.init(lds0 + kStageP, wq * SQ * 16, lane);
     f32x4 acc[SP][SQ] = {};
     place();
+    auto wait = [&](auto outstanding) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(outstanding)::value * kLoads) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto after = [](uint32_t stage) { return stage + kStage == RING * kStage ? 0 : stage + kStage; };
+    // Both loops: us of forward products of 4096 x 4096 x 4096 in 256 x 256 100 and 104, 2048 x 2048 x 2048 in 128 x 128 20.8 and
+    // 21.7, 4096 x 2048 x 512 in 128 x 64 13.3 and 13.0, 1024 x 1024 x 1024 in 64 x 64 7.2 and 6.6; of both gradients, which read LDS
+    // with twice as many instructions, 8192 x 2048 x 2048 in 256 x 128 117 and 120, 2048 x 2048 x 1024 in 128 x 128, four steps in the
+    // ring, 23.6 and 21.2.
+    constexpr bool kHalfAhead = BP * BQ >= 128 * 128 && (KIND == kForward || RING < 4);
+    static_assert(!kHalfAhead || SPLIT == 1, "");
+    constexpr int kAhead = kHalfAhead ? RING : RING - 1;                       // steps that are loaded before the first product
+    uint4 vp[2][SP], vq[2][SQ];
+    uint32_t stage = 0;
 #pragma unroll
-    for (int s = 0; s < RING - 1; ++s) {
+    for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
         for (int d = 0; d < kLoads; ++d) load(d, s * kStage);
         advance();
     }
-    uint32_t stage = 0, fill = (RING - 1) * kStage;
+    if constexpr (kHalfAhead) {
+        // One barrier, in the middle of a step: past it everyone's loads of the next step have landed, and everyone's reads of this
+        // one are done, so that the loads of the step RING on go where it was.  The reads and loads come one by one between the
+        // products: a wave that issues many together waits for the unit that takes them, and its products with it.
+        auto read_some = [&](auto half, uint32_t from, int i) {
+            constexpr int H = decltype(half)::value, kReads = SP + SQ;
+#pragma unroll
+            for (int x = 0; x < kReads; ++x) {
+                if (x < i * kReads / (SP - 1) || x >= (i + 1) * kReads / (SP - 1)) continue;
+                if (x > 0 && x <= SQ) vq[H][x - 1] = fq.read(from, x - 1, H);
+                else vp[H][x == 0 ? 0 : x - SQ] = fp.read(from, x == 0 ? 0 : x - SQ, H);
+            }
+        };
+        const std::integral_constant<int, 0> first;
+        const std::integral_constant<int, 1> second;
+        wait(std::integral_constant<int, RING - 1>());
+#pragma unroll
+        for (int i = 0; i < SP - 1; ++i) read_some(first, stage, i);
 #pragma unroll 1
-    for (int c0 = 0; c0 < nc; c0 += SPLIT * kBC) {
-        // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
-        // everyone's
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * kLoads) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        uint4 vp[2][SP], vq[2][SQ];
-#pragma unroll
-        for (int j = 0; j < SQ; ++j) vq[0][j] = fq.read(stage, j, 0);
-#pragma unroll
-        for (int i = 0; i < SP; ++i) vp[0][i] = fp.read(stage, i, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        // the step's second half is read from LDS, and the loads ahead are issued, between the first half's products
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            constexpr int kFrom = SP > 4 ? SP / 2 : 0, kEach = SP > 4 ? 2 : 1;
-            if (i == kFrom) {
-#pragma unroll
-                for (int j = 0; j < SQ; ++j) vq[1][j] = fq.read(stage, j, 1);
-            }
-            if (i >= kFrom) {
-#pragma unroll
-                for (int x = (i - kFrom) * kEach; x < (i - kFrom + 1) * kEach; ++x) vp[1][x] = fp.read(stage, x, 1);
-            }
-#pragma unroll
-            for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
-#pragma unroll
-            for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
+        for (int c0 = 0; c0 < nc; c0 += kBC) {
+            const uint32_t next = after(stage);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < SP; ++i) {
+                if (i < SP - 1) read_some(second, stage, i);
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            wait(std::integral_constant<int, RING - 2>());
+#pragma unroll
+            for (int i = 0; i < SP; ++i) {
+                if (i < SP - 1) read_some(first, next, i);
+#pragma unroll
+                for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, stage);
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance();
+            stage = next;
         }
-        advance();
+    } else {
+        uint32_t fill = (RING - 1) * kStage;
+#pragma unroll 1
+        for (int c0 = 0; c0 < nc; c0 += SPLIT * kBC) {
+            // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
+            // everyone's
+            wait(std::integral_constant<int, RING - 2>());
 #pragma unroll
-        for (int i = 0; i < SP; ++i)
+            for (int j = 0; j < SQ; ++j) vq[0][j] = fq.read(stage, j, 0);
 #pragma unroll
-            for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
-        stage = stage + kStage == RING * kStage ? 0 : stage + kStage;
-        fill = fill + kStage == RING * kStage ? 0 : fill + kStage;
+            for (int i = 0; i < SP; ++i) vp[0][i] = fp.read(stage, i, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            // the step's second half is read from LDS, and the loads ahead are issued, between the first half's products
+#pragma unroll
+            for (int i = 0; i < SP; ++i) {
+                if (i == 0) {
+#pragma unroll
+                    for (int j = 0; j < SQ; ++j) vq[1][j] = fq.read(stage, j, 1);
+                }
+                vp[1][i] = fp.read(stage, i, 1);
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+#pragma unroll
+                for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance();
+#pragma unroll
+            for (int i = 0; i < SP; ++i)
+#pragma unroll
+                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+            stage = after(stage);
+            fill = after(fill);
+        }
     }
     // The results go through LDS, one of a wave's subtile rows at a time: a lane of the matrix unit's result has 4 columns of
     // a row and its neighbour another row's; out of LDS 8 columns, and whole lines side by side.  (The loads past the last
@@ -595,30 +650,34 @@ bool too_many(const char* who, int64_t blocks, int threads) {
 uint64_t round_up(uint64_t v) { return (v + 255) / 256 * 256; }
 
 // The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two, as measured.  us per forward product in
-// their order, chosen *: 1024 x 1024 x 1024 6.7* 7.3 - 9.9 11.5 14.6 29; 1030 x 72 x 1856 6.5 4.7* 7.4 5.7 5.6 7.4 12; 4096 x
-// 2048 x 512 17.4 15.2 13.4* 14.1 17.1 23.9 44; 2048 x 2048 x 2048 33 28 25.6 22.4 19.5* 27.9 44; 4096 x 4096 x 4096 229 199 174 159
-// 146 124 106*.  Both gradients: 333 x 640 x 2560 13.4* 12.3 14.5 14.5 18.4 26.7 48; 1999 x 2560 x 640 36 28 28 24 21.5* 27 44; 2048 x
-// 2048 x 2048 61 53 49 43 38 32* 44; 4096 x 2048 x 512 42 33 32 28* 33 49 81; 8192 x 4096 x 4096 864 1043 - 709 544 472 408*.
-template <typename F>
+// their order, chosen *: 1024 x 1024 x 1024 6.8* 7.0 8.4 9.2 10.5 12.3 15.4 20 26; 1030 x 72 x 1856 6.9 5.1* 7.5 6.1 6.2 8.1 8.5 10.5
+// 13; 4096 x 2048 x 512 17.6 15.1 14.0* 15.1 16.9 20 25 35 42; 2048 x 2048 x 2048 35 29 26.7 23.8 20.5* 26.5 27.5 36 42; 3000 x 2048 x 2048
+// 47 39 36 34 37 29 28.4* 36 42; 5000 x 4096 x 2056 158 131 131 110 95 101 101 75.6* 86; 4096 x 4096 x 4096 228 190 178 148 131 118 113 135
+// 99.7*.  Both gradients, without 192 x 256: 333 x 640 x 2560 13.6* 12.7 15 15 19 24 28 47; 1999 x 2560 x 640 37 28 29 25 22.9* 26 28 42;
+// 2048 x 2048 x 2048 65 53 53 44 40 34 33.2* 46; 4096 x 2048 x 512 44 33 33 30* 34 46 47 76; 8192 x 4096 x 4096 882 1050 734 716 563 480 455
+// 393*.
+template <bool FORWARD, typename F>
 int each_tiles(const F& f) {
-    f(Tiles<64, 64, 2, 2, 2, 3, 2, 8>(), 24, 48);
-    f(Tiles<64, 64, 2, 2, 1, 4, 2, 8>(), 25, 45);
-    f(Tiles<128, 64, 4, 2, 1, 4, 2, 8>(), 38, 80);
-    f(Tiles<128, 64, 2, 2, 1, 3, 2, 8>(), 42, 75);
-    f(Tiles<128, 128, 2, 4, 1, 4, 2, 6>(), 55, 110);
-    f(Tiles<128, 128, 2, 2, 1, 2, 2, 8>(), 90, 97);
-    f(Tiles<256, 256, 2, 4, 1, 2, 2, 4>(), 145, 290);
+    f(Tiles<64, 64, 2, 2, 2, 3, 2, 8>(), 21, 40);
+    f(Tiles<64, 64, 2, 2, 1, 4, 2, 8>(), 22, 37);
+    f(Tiles<128, 64, 4, 2, 1, 4, 2, 8>(), 32, 63);
+    f(Tiles<128, 64, 2, 2, 1, 3, 2, 8>(), 32, 54);
+    f(Tiles<128, 128, 2, 4, 1, 4, 2, 6>(), 44, 89);
+    f(Tiles<128, 128, 2, 2, 1, 2, 2, 8>(), 60, 85);
+    f(Tiles<256, 128, 4, 2, 1, 3, 2, 6>(), 80, 163);
+    if constexpr (FORWARD) f(Tiles<192, 256, 2, 4, 1, 2, 2, 4>(), 107, 213);   // (an image along the other index has a power of two)
+    f(Tiles<256, 256, 2, 4, 1, 2, 2, 4>(), 138, 273);
     return 0;
 }
 
 // Calls run(tiles) with those that are done first: with one product, as many steps as a CU's blocks have; with two, which fill
 // each other's gaps, the sum of all steps over the CUs, but at least those of the longest tile.
-template <typename R>
+template <bool FORWARD, typename R>
 int best_tiles(const Product& a, const Product& b, const R& run) {
     int64_t best = INT64_MAX;
     int pick = 0, i = 0;
     auto steps = [](const Product& p) { return (int64_t)(p.parts > 1 ? p.part_c : p.nc) / kBC + 1; };
-    each_tiles([&](auto tiles, int one, int two) {
+    each_tiles<FORWARD>([&](auto tiles, int one, int two) {
         using C = decltype(tiles);
         const int64_t ta = tiles_in<C::BP, C::BQ>(a) * a.parts, tb = tiles_in<C::BP, C::BQ>(b) * b.parts;
         int64_t cost;
@@ -633,7 +692,7 @@ int best_tiles(const Product& a, const Product& b, const R& run) {
     });
     int rc = -1;
     i = 0;
-    each_tiles([&](auto tiles, int, int) {
+    each_tiles<FORWARD>([&](auto tiles, int, int) {
         if (i++ == pick) rc = run(tiles);
     });
     return rc;
@@ -667,7 +726,7 @@ int forward(const Product& a, const Epilogue& e, void* workspace, hipStream_t s)
     }
     Product sums = a;
     if (a.parts > 1) sums.out = workspace, sums.ldo = a.nq;
-    return best_tiles(sums, Product{}, [&](auto tiles) {
+    return best_tiles<true>(sums, Product{}, [&](auto tiles) {
         using C = decltype(tiles);
         const int64_t blocks = tiles_in<C::BP, C::BQ>(a) * a.parts, joins = ((int64_t)a.np * (a.nq / 8) + 255) / 256;
         if (too_many("linear", blocks, C::kThreads) || (a.parts > 1 && too_many("linear", joins, 256))) return -1;
@@ -692,7 +751,7 @@ int dw_parts(int n_tok, int n_out, int n_in) {
 template <typename T>
 int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const Product& dx, const BiasSums& b, const Parts& p,
               hipStream_t s) {
-    return best_tiles(dw, dx, [&](auto tiles) {
+    return best_tiles<false>(dw, dx, [&](auto tiles) {
         using C = decltype(tiles);
         const bool parts = dw.parts > 1 && dw.np > 0;
         // what one launch does not take is refused before anything is queued

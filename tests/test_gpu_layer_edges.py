@@ -48,6 +48,36 @@ def test_every_tile_backward(dtype, n_tok, n_in, n_out):
     check(ops.linear_grad(dy, x, w, z=z, act="silu", want_dx=False, dw_dtype=torch.float32)[1], *want[1], "dw alone")
 
 
+# large tiles over contractions of a part of a step, of one, and of few more than are under way at once; the kinds that the sizes above
+# leave out
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_tok,n_in,n_out", [(3000, 8, 4104), (3000, 72, 4104), (2900, 328, 4104), (5000, 64, 776), (5000, 200, 776), (2049, 8, 4104),
+                                              (2100, 264, 4104), (777, 8, 2568), (777, 392, 2568), (564, 8, 10904), (564, 136, 10904), (12000, 72, 264),
+                                              (131, 72, 8264)])
+def test_large_tiles_short_contractions(dtype, n_tok, n_in, n_out):
+    from moe_offload import ops
+    x, w, b, res = rnd((n_tok, n_in), dtype, 1), rnd((n_out, n_in), dtype, 2, n_in ** -0.5), rnd((n_out,), dtype, 3), rnd((n_tok, n_out), dtype, 4)
+    want, slack, wz, sz = ref.linear(x, w, b, "silu", res)
+    z = torch.empty((n_tok, n_out), dtype=dtype, device=DEV)
+    check(ops.linear(x, w, bias=b, act="silu", residual=res, z_out=z), want, slack)
+    check(z, wz, sz, "z")
+    check(ops.linear(x, w, bias=b, act="silu", residual=res, dtype=torch.float32), want, slack, "fp32")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_tok,n_in,n_out", [(1500, 4104, 1544), (2049, 4104, 1544), (300, 4104, 264), (777, 4104, 776), (513, 4104, 520), (8192, 72, 1032),
+                                              (40, 4104, 4104), (8200, 4104, 8)])
+def test_large_tiles_backward(dtype, n_tok, n_in, n_out):
+    from moe_offload import ops
+    dy, x, w, z = rnd((n_tok, n_out), dtype, 1), rnd((n_tok, n_in), dtype, 2), rnd((n_out, n_in), dtype, 3, n_out ** -0.5), rnd((n_tok, n_out), dtype, 4)
+    want = ref.linear_grad(dy, x, w, z, "gelu")
+    got = ops.linear_grad(dy, x, w, z=z, act="gelu", bias=True)
+    for g, (v, slack), name in zip(got, want, ("dx", "dw", "db")):
+        check(g, v, slack, name)
+    check(ops.linear_grad(dy, x, w, z=z, act="gelu", want_dw=False)[0], *want[0], "dx alone")
+    check(ops.linear_grad(dy, x, w, z=z, act="gelu", want_dx=False, dw_dtype=torch.float32)[1], *want[1], "dw alone")
+
+
 def test_offsets_past_32_bits():
     """x and y of more than 2^32 bytes, the rows that count at their end."""
     from moe_offload import ops
