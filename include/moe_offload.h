@@ -385,9 +385,11 @@ int moe_combine_grad(const void* dout, int64_t ldd, const void* y, int64_t ldy, 
 uint64_t moe_linear_workspace_bytes(int n_tok, int n_in, int n_out);
 int moe_linear(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual, int64_t ldr, int n_tok, int n_in,
                int n_out, int act, int dtype, int out_f32, void* workspace, void* z, int64_t ldz, void* y, int64_t ldy, void* stream);
-/* Its gradients from dy (of the inputs' type, or fp32: dy_f32 != 0) and the z it kept (act != 0): dz = dy act'(z), rounded to
- * the inputs' type, dx [n_tok][n_in] = dz W, dw [n_out][n_in] = dz^T x (fp32 if dw_f32 != 0), db [n_out] = the sum of dz over
- * the tokens; the residual's is dy.  Those that are null are not computed; outputs are contiguous.
+/* Its gradients from dy (of the inputs' type, or fp32: dy_f32 != 0) and the z it kept (act != 0): dz = dy act'(z),
+ * dx [n_tok][n_in] = dz W, dw [n_out][n_in] = dz^T x (fp32 if dw_f32 != 0), db [n_out] = the sum of dz over
+ * the tokens; the residual's is dy.  Where dz is not dy as it came, the products take it with a relative error of 2^-15 at most and
+ * fp32's range, and for an fp32 dw with all of its bits; through silu or gelu of an fp16 dy, for an fp16 dw, with 2^-21 of it, or
+ * 2^-33 in its place.  Those that are null are not computed; outputs are contiguous.
  * workspace: moe_linear_grad_workspace_bytes bytes, 16-byte aligned, any contents, one per call in flight. */
 uint64_t moe_linear_grad_workspace_bytes(int n_tok, int n_in, int n_out, int act, int dy_f32, int want_dw, int want_db);
 int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const void* x, int64_t ldx, const void* w, const void* z, int64_t ldz,

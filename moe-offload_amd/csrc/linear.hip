@@ -9,8 +9,15 @@
 // (grouped_mm.h: loads straight into LDS, operands along or across a row of memory), without rows to look up: x and W have c
 // along a row, W for dx has it along the column, dz and x for dW both.
 //
-// dz is rounded to the inputs' type before the matrix unit takes it, unless it is dy as it came: half a step of each
-// value, the same as that of the products' own results, and independent from value to value.
+// dz goes to the matrix unit as it came where it is dy itself, in the inputs' type.  Where it is computed, or dy is fp32, one value of
+// 16 bits would add an error as large as the results' own rounding (fp16, 1999 x 2560 x 640 through silu: 2.9e-4 of the norm
+// for 2.1e-4), and fp16 has no place for all that dy may hold.  So it goes in parts, images one after another in the contraction:
+//   kParts   bf16 values, each with the next 8 of its bits, over fp32's range: two for results of 16 bits (2^-15 of a value is lost at
+//            most), three for fp32 ones (nothing is).  fp16's x and W, two bf16 values each, take every product twice.
+//   kHalves  for fp16 dy through slopes that are never above 1.13, and results of 16 bits: dz / 2 as two fp16 values, the
+//            second times 2^10 (2^-21 of a value is lost, or 2^-33), half the products of kParts.
+// us of both gradients through silu, fp16, as one value, in kHalves and in kParts: 1999 x 2560 x 640 28 43 80, 8192 x 4096 x 4096 440 841
+// 1554; bf16, as one value and in kParts: 28 45, 430 801.
 #include <algorithm>
 #include <type_traits>
 
@@ -87,9 +94,14 @@ struct Product {
     int64_t ldp, ldq, ldo;       // elements from row to row of memory
     int np, nq, nc;              // extents: rows and columns of out, and the contraction
     int parts, part_c;           // the contraction in parts of part_c, each with sums of its own (fp32, [parts][np][nq]; not dx)
+    int terms;                   // gradients: P is the sum of so many images, one after another from p on,
+    int64_t term_p;              // so many elements apart; the contraction goes over all of them
 };
 
 enum { kForward = 0, kDx = 1, kDw = 2 };
+enum { kWhole = 0, kParts = 1, kHalves = 2 };                                  // how P comes
+
+constexpr float kSecondHalf = 0x1p-10f;                                        // of kHalves, the first image
 
 template <typename T>
 __device__ __forceinline__ uint4 round8(const f32x4 (&v)[2]) {
@@ -127,6 +139,36 @@ __device__ __forceinline__ void finish8(const Product& a, const Epilogue& e, int
     }
 }
 
+// c + q p, and in kParts p, a bf16 part of a value, goes with q of T: fp16's 11 bits are two bf16 values, the upper 8 and
+// the other 3.  An infinite q is infinite in both, and of one that the first holds whole the second is as good as nothing, but not
+// zero: so the sum is infinite where q p is, and a NaN only where that is one.
+template <typename T, int MODE>
+__device__ __forceinline__ f32x4 multiply(uint4 q, uint4 p, f32x4 c) {
+    if constexpr (MODE == kParts && __is_same(T, _Float16)) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f16x2 both = __builtin_bit_cast(f16x2, v[e]), top = __builtin_bit_cast(f16x2, v[e] & 0xFFF8FFF8u);
+            // up to 7 of the value's last steps, 32 at most; of an infinity -256, which the infinity below outweighs
+            const f16x2 rest = __builtin_elementwise_max(both - top, (f16x2)(-256.f));
+            uint32_t t[2], r[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                t[k] = __builtin_bit_cast(uint32_t, (float)top[k]);
+                r[k] = __builtin_bit_cast(uint32_t, __builtin_fmaf((float)both[k], 0x1p-40f, (float)rest[k]));
+            }
+            hi[e] = __builtin_amdgcn_perm(t[1], t[0], 0x07060302);             // upper halves (a NaN's quiet bit is among them)
+            lo[e] = __builtin_amdgcn_perm(r[1], r[0], 0x07060302);
+        }
+        c = mfma<__bf16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), p, c);
+        return mfma<__bf16>(make_uint4(lo[0], lo[1], lo[2], lo[3]), p, c);
+    } else {
+        return mfma<T>(q, p, c);
+    }
+}
+
 template <int BP, int BQ>
 __host__ __device__ inline int64_t tiles_in(const Product& a) {
     return ((int64_t)a.np + BP - 1) / BP * (((int64_t)a.nq + BQ - 1) / BQ);
@@ -152,7 +194,7 @@ __device__ __forceinline__ void tile_at(const Product& a, uint32_t item, int& p0
 // indexes goes from global memory to LDS without passing registers, RING - 1 steps ahead of the one that is multiplied: with one
 // tile per block nothing else hides the way through memory.  One barrier per step (and two steps, of SPLIT = 2), at its start or,
 // in large tiles, in its middle, where half of the next step's operands are read from LDS behind this one's products.
-template <typename T, int KIND, typename C>
+template <typename T, int KIND, typename C, int MODE = kWhole>
 __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e, uint32_t item, uint8_t* lds) {
     constexpr int BP = C::BP, BQ = C::BQ, WP = C::WP, WQ = C::WQ, RING = C::RING, SPLIT = C::SPLIT;
     constexpr int kWaves = WP * WQ, SP = BP / WP / 16, SQ = BQ / WQ / 16;
@@ -172,8 +214,12 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
         item -= (uint32_t)part * tiles;
         P += part * a.part_c * (kAlongP ? a.ldp : 1);
         Q += part * a.part_c * (kAlongQ ? a.ldq : 1);
-        nc = nc - part * a.part_c < a.part_c ? (int)(nc - part * a.part_c) : a.part_c;
+        nc = (int)std::clamp<int64_t>(nc - part * a.part_c, 0, a.part_c);
     }
+    // P's images follow each other in the contraction, each as whole steps
+    int term = 0;
+    const int whole = (nc + kBC - 1) / kBC * kBC;
+    const uint32_t all_c = KIND == kForward ? nc : (uint32_t)a.terms * whole;
     int p0, q0;
     tile_at<BP, BQ, C::PANEL>(a, item, p0, q0);
     const T* zero = (const T*)&g_zero16;
@@ -196,6 +242,13 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
         }
     };
     auto place = [&]() {
+        if constexpr (KIND != kForward) {
+            for (; load_c >= whole && term < a.terms; ++term) {
+                load_c -= whole;
+                P += a.term_p;
+            }
+            if (term == a.terms) nc = 0;
+        }
 #pragma unroll
         for (int j = 0; j < kLoadsP; ++j)
             pp[j] = place_one(std::integral_constant<bool, kAlongP>(), std::integral_constant<int, BP>(), P, a.ldp, p0, a.np, kLoadsP, j);
@@ -240,6 +293,19 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     constexpr int kAhead = kHalfAhead ? RING : RING - 1;                       // steps that are loaded before the first product
     uint4 vp[2][SP], vq[2][SQ];
     uint32_t stage = 0;
+    bool second = MODE == kHalves;                                             // the sums are those of the second halves
+    auto scale_sums = [&](float by) {
+#pragma unroll
+        for (int i = 0; i < SP; ++i)
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) acc[i][j] *= by;
+    };
+    auto first_halves_from = [&](uint32_t c) {
+        if (MODE == kHalves && second && c >= (uint32_t)whole) {
+            scale_sums(kSecondHalf);
+            second = false;
+        }
+    };
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
@@ -265,14 +331,15 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
 #pragma unroll
         for (int i = 0; i < SP - 1; ++i) read_some(first, stage, i);
 #pragma unroll 1
-        for (int c0 = 0; c0 < nc; c0 += kBC) {
+        for (uint32_t c0 = 0; c0 < all_c; c0 += kBC) {
             const uint32_t next = after(stage);
+            first_halves_from(c0);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < SP; ++i) {
                 if (i < SP - 1) read_some(second, stage, i);
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply<T, MODE>(vq[0][j], vp[0][i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             wait(std::integral_constant<int, RING - 2>());
@@ -282,7 +349,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
 #pragma unroll
                 for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, stage);
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply<T, MODE>(vq[1][j], vp[1][i], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             advance();
@@ -291,10 +358,11 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     } else {
         uint32_t fill = (RING - 1) * kStage;
 #pragma unroll 1
-        for (int c0 = 0; c0 < nc; c0 += SPLIT * kBC) {
+        for (uint32_t c0 = 0; c0 < all_c; c0 += SPLIT * kBC) {
             // this wave's loads of the step have landed and its reads of the step before are done; past the barrier, so are
             // everyone's
             wait(std::integral_constant<int, RING - 2>());
+            first_halves_from(c0 + turn_of * kBC);
 #pragma unroll
             for (int j = 0; j < SQ; ++j) vq[0][j] = fq.read(stage, j, 0);
 #pragma unroll
@@ -309,7 +377,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
                 }
                 vp[1][i] = fp.read(stage, i, 1);
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[0][j], vp[0][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply<T, MODE>(vq[0][j], vp[0][i], acc[i][j]);
 #pragma unroll
                 for (int d = i * kLoads / SP; d < (i + 1) * kLoads / SP; ++d) load(d, fill);
                 __builtin_amdgcn_sched_barrier(0);
@@ -318,11 +386,12 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
 #pragma unroll
             for (int i = 0; i < SP; ++i)
 #pragma unroll
-                for (int j = 0; j < SQ; ++j) acc[i][j] = mfma<T>(vq[1][j], vp[1][i], acc[i][j]);
+                for (int j = 0; j < SQ; ++j) acc[i][j] = multiply<T, MODE>(vq[1][j], vp[1][i], acc[i][j]);
             stage = after(stage);
             fill = after(fill);
         }
     }
+    if constexpr (MODE == kHalves) scale_sums(second ? 2.f * kSecondHalf : 2.f);
     // The results go through LDS, one of a wave's subtile rows at a time: a lane of the matrix unit's result has 4 columns of
     // a row and its neighbour another row's; out of LDS 8 columns, and whole lines side by side.  (The loads past the last
     // step write there too, so they are waited for.)
@@ -454,15 +523,15 @@ __device__ __forceinline__ void sum_bias(const BiasSums& b, uint32_t item, float
 
 // All gradients behind dz in one launch: the tiles of dW (longer, as a rule) before those of dx, then the bias's.  A product of no
 // rows is not there.
-template <typename T, typename C>
+template <typename T, typename C, int MODE>
 __global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear_grads(Product dw, Product dx, BiasSums b, int dw_f32) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
     const uint32_t n_dw = (uint32_t)tiles_in<C::BP, C::BQ>(dw) * dw.parts, n_dx = (uint32_t)tiles_in<C::BP, C::BQ>(dx);
     const uint32_t i = blockIdx.x;
     Epilogue e = {};
     e.out_f32 = dw_f32;
-    if (i < n_dw) tile_product<T, kDw, C>(dw, e, xcd_order(i, n_dw), lds);
-    else if (i < n_dw + n_dx) tile_product<T, kDx, C>(dx, e, xcd_order(i - n_dw, n_dx), lds);
+    if (i < n_dw) tile_product<T, kDw, C, MODE>(dw, e, xcd_order(i, n_dw), lds);
+    else if (i < n_dw + n_dx) tile_product<T, kDx, C, MODE>(dx, e, xcd_order(i - n_dw, n_dx), lds);
     else sum_bias<T, C::kThreads>(b, i - n_dw - n_dx, (float*)lds);
 }
 
@@ -558,6 +627,7 @@ struct DzArgs {
     const void* dy;
     const void* z;               // null: dz = dy
     void* dz;                    // null: only the sums
+    int parts, halves;           // images of dz, 2 or 3, one after another; those of kHalves
     float* sums;                 // [row blocks][n], null: none wanted
     int64_t lddy, ldz;
     int n_rows, n, act;
@@ -566,6 +636,30 @@ struct DzArgs {
 
 // A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.  1999 x 640 fp16 through silu 4.2-6.6 us:
 // 7.7 MB, a load, an exponential and a store after one another.
+//
+// The images of kParts: a value's upper 16 bits, then those of what is left, the last one rounded; of kHalves: the rest of the rounding
+// below, then that.  All have the value's sign, and none is zero unless it is, or is below 2^-23 of kHalves (the smallest there
+// is stands for nothing): an infinity that they meet in a product stays one.
+__device__ __forceinline__ void dz_parts(float v, int parts, __bf16 (&p)[3]) {
+    const bool fine = fabsf(v) < __builtin_inff();
+    const uint32_t sign = __float_as_uint(v) & 1u << 31;
+    const bool any = v != 0.f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        p[k] = fine && k + 1 < parts ? __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(v) >> 16)) : (__bf16)v;
+        if (fine) v -= (float)p[k];
+        if (any && fabsf(v) < 0x1p-126f) v = __uint_as_float(sign | 1u << 23);
+    }
+}
+
+__device__ __forceinline__ void dz_halves(float v, _Float16 (&p)[3]) {
+    const float u = 0.5f * v;
+    p[1] = (_Float16)__builtin_amdgcn_cvt_pkrtz(u, 0.f)[0];
+    p[0] = fabsf(u) < __builtin_inff() ? (_Float16)((u - (float)p[1]) * (1.f / kSecondHalf)) : p[1];
+    const uint16_t tiny = (uint16_t)((__float_as_uint(v) >> 16 & 0x8000u) | 1u);
+    if (v != 0.f && p[0] == (_Float16)0.f) p[0] = __builtin_bit_cast(_Float16, tiny);
+}
+
 template <typename T, bool F32>
 __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
     __shared__ f32x4 part[8][32][2];
@@ -592,7 +686,25 @@ __global__ __launch_bounds__(kDzThreads) void k_linear_dz(DzArgs a) {
                         for (int e = 0; e < 4; ++e) d[h][e] *= slope<decltype(act)::value>(z[h][e]);
                 });
             }
-            if (a.dz) *(uint4*)((T*)a.dz + r * a.n + c) = round8<T>(d);
+            if (a.dz) {
+                auto images = [&](auto type, auto&& split) {
+                    using I = decltype(type);
+                    typedef I i8 __attribute__((ext_vector_type(8)));
+                    i8 image[3];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        I p[3];
+                        split(d[e / 4][e % 4], p);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) image[k][e] = p[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        if (k < a.parts) *(i8*)((I*)a.dz + ((int64_t)k * a.n_rows + r) * a.n + c) = image[k];
+                };
+                if (__is_same(T, _Float16) && a.halves) images(_Float16(), [](float v, _Float16 (&p)[3]) { dz_halves(v, p); p[2] = p[0]; });
+                else images(__bf16(), [&](float v, __bf16 (&p)[3]) { dz_parts(v, a.parts, p); });
+            }
             sum[0] += d[0];
             sum[1] += d[1];
         }
@@ -672,13 +784,16 @@ int each_tiles(const F& f) {
 
 // Calls run(tiles) with those that are done first: with one product, as many steps as a CU's blocks have; with two, which fill
 // each other's gaps, the sum of all steps over the CUs, but at least those of the longest tile.
+// split: fp16's values are taken apart on the way to the matrix unit, by every wave for its own columns: a step has WP BQ / 8 subtiles of
+// them for a CU's four vector units, of 36 operations each.
 template <bool FORWARD, typename R>
-int best_tiles(const Product& a, const Product& b, const R& run) {
+int best_tiles(const Product& a, const Product& b, bool split, const R& run) {
     int64_t best = INT64_MAX;
     int pick = 0, i = 0;
-    auto steps = [](const Product& p) { return (int64_t)(p.parts > 1 ? p.part_c : p.nc) / kBC + 1; };
+    auto steps = [](const Product& p) { return ((int64_t)(p.parts > 1 ? p.part_c : p.nc) / kBC + 1) * p.terms; };
     each_tiles<FORWARD>([&](auto tiles, int one, int two) {
         using C = decltype(tiles);
+        if (split) one += C::WP * C::BQ / 5, two += C::WP * C::BQ / 5 * 2;
         const int64_t ta = tiles_in<C::BP, C::BQ>(a) * a.parts, tb = tiles_in<C::BP, C::BQ>(b) * b.parts;
         int64_t cost;
         if (ta == 0 || tb == 0) {
@@ -726,7 +841,7 @@ int forward(const Product& a, const Epilogue& e, void* workspace, hipStream_t s)
     }
     Product sums = a;
     if (a.parts > 1) sums.out = workspace, sums.ldo = a.nq;
-    return best_tiles<true>(sums, Product{}, [&](auto tiles) {
+    return best_tiles<true>(sums, Product{}, false, [&](auto tiles) {
         using C = decltype(tiles);
         const int64_t blocks = tiles_in<C::BP, C::BQ>(a) * a.parts, joins = ((int64_t)a.np * (a.nq / 8) + 255) / 256;
         if (too_many("linear", blocks, C::kThreads) || (a.parts > 1 && too_many("linear", joins, 256))) return -1;
@@ -748,10 +863,10 @@ int dw_parts(int n_tok, int n_out, int n_in) {
     return (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
 }
 
-template <typename T>
+template <typename T, int MODE>
 int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const Product& dx, const BiasSums& b, const Parts& p,
               hipStream_t s) {
-    return best_tiles<false>(dw, dx, [&](auto tiles) {
+    return best_tiles<false>(dw, dx, __is_same(T, _Float16) && MODE == kParts, [&](auto tiles) {
         using C = decltype(tiles);
         const bool parts = dw.parts > 1 && dw.np > 0;
         // what one launch does not take is refused before anything is queued
@@ -765,7 +880,7 @@ int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const
             HIP_TRY(hipGetLastError());
         }
         if (blocks > 0) {
-            hipLaunchKernelGGL((k_linear_grads<T, C>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, dw, dx, b, parts || dw_f32);
+            hipLaunchKernelGGL((k_linear_grads<T, C, MODE>), dim3((uint32_t)blocks), dim3(C::kThreads), 0, s, dw, dx, b, parts || dw_f32);
             HIP_TRY(hipGetLastError());
         }
         if (parts) {
@@ -776,14 +891,17 @@ int gradients(const DzArgs* dz, int dy_f32, const Product& dw, int dw_f32, const
     });
 }
 
-// The workspace: dz, the sums that the bias's gradient is made of, dW's parts.
+// Images of dz for a dW of 16 bits or of fp32; dx, always of 16 bits, takes the first two.
+constexpr int kDzParts = 2, kDzPartsF32 = 3;
+
+// The workspace: dz (as a dW of fp32 takes it), the sums that the bias's gradient is made of, dW's parts.
 struct Layout {
     uint64_t sums, parts, bytes;
 };
 
 Layout layout(int n_tok, int n_in, int n_out, bool own_dz, bool want_dw, bool want_db) {
     Layout l;
-    l.sums = own_dz ? round_up(2 * (uint64_t)n_tok * n_out) : 0;
+    l.sums = own_dz ? round_up(2 * (uint64_t)(want_dw ? kDzPartsF32 : kDzParts) * n_tok * n_out) : 0;
     l.parts = l.sums + (want_db ? round_up(4 * (uint64_t)dz_blocks(n_tok, n_out) * n_out) : 0);
     const int parts = want_dw ? dw_parts(n_tok, n_out, n_in) : 1;
     l.bytes = l.parts + (parts > 1 ? 4 * (uint64_t)parts * n_out * n_in : 0);
@@ -813,7 +931,7 @@ extern "C" int moe_linear(const void* x, int64_t ldx, const void* w, const void*
         moe_set_error("linear: the workspace is null or not 16-byte aligned");
         return -1;
     }
-    const Product a = {x, w, y, ldx, n_in, ldy, n_tok, n_out, n_in, parts, part_of(n_in, parts)};
+    const Product a = {x, w, y, ldx, n_in, ldy, n_tok, n_out, n_in, parts, part_of(n_in, parts), 1, 0};
     const Epilogue e = {bias, residual, z, ldr, ldz, act, out_f32};
     const hipStream_t s = (hipStream_t)stream;
     return dtype ? forward<__bf16>(a, e, workspace, s) : forward<_Float16>(a, e, workspace, s);
@@ -844,13 +962,21 @@ extern "C" int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const v
     const void* rows = own_dz ? dz : dy;
     const int64_t ld = own_dz ? n_out : lddy;
     float* sums = db ? (float*)((char*)workspace + at.sums) : nullptr;
-    const DzArgs d = {dy, act != kActNone ? z : nullptr, dz, sums, lddy, ldz, n_tok, n_out, act, dz_rows(n_tok, n_out)};
+    const int images = dw && dw_f32 ? kDzPartsF32 : kDzParts;
+    const bool halves = dtype == 0 && !dy_f32 && (act == kActSilu || act == kActGelu) && images == kDzParts;
+    const DzArgs d = {dy, act != kActNone ? z : nullptr, dz, images, halves, sums, lddy, ldz, n_tok, n_out, act, dz_rows(n_tok, n_out)};
     const int parts = dw ? dw_parts(n_tok, n_out, n_in) : 1;
     void* into = parts > 1 ? (char*)workspace + at.parts : dw;
-    const Product gw = {rows, x, into, ld, ldx, n_in, dw ? n_out : 0, n_in, n_tok, parts, part_of(n_tok, parts)};
-    const Product gx = {rows, w, dx, ld, n_in, n_in, dx ? n_tok : 0, n_in, n_out, 1, 0};
+    const Product gw = {rows, x, into, ld, ldx, n_in, dw ? n_out : 0, n_in, n_tok, parts, part_of(n_tok, parts),
+                        own_dz ? images : 1, (int64_t)n_tok * n_out};
+    const Product gx = {rows, w, dx, ld, n_in, n_in, dx ? n_tok : 0, n_in, n_out, 1, 0, own_dz ? kDzParts : 1,
+                        (int64_t)n_tok * n_out};
     const BiasSums b = {sums, db, dz_blocks(n_tok, n_out), n_out};
     const Parts p = {(const float*)into, dw, (int64_t)n_out * n_in, parts, dw_f32};
     const DzArgs* need = dz || db ? &d : nullptr;
-    return dtype ? gradients<__bf16>(need, dy_f32, gw, dw_f32, gx, b, p, s) : gradients<_Float16>(need, dy_f32, gw, dw_f32, gx, b, p, s);
+    // (bf16's parts are values like any)
+    if (dtype) return gradients<__bf16, kWhole>(need, dy_f32, gw, dw_f32, gx, b, p, s);
+    if (!own_dz) return gradients<_Float16, kWhole>(need, dy_f32, gw, dw_f32, gx, b, p, s);
+    return halves ? gradients<_Float16, kHalves>(need, dy_f32, gw, dw_f32, gx, b, p, s)
+                  : gradients<_Float16, kParts>(need, dy_f32, gw, dw_f32, gx, b, p, s);
 }

@@ -799,8 +799,9 @@ def linear_grad(dy, x, w, z=None, act=None, bias=False, want_dx=True, want_dw=Tr
     """linear's gradients (dx, dw, dbias), None for those that are not wanted; the residual's is dy.
 
     dy: x's type, or fp32, [n_tok, n_out]; z: what linear wrote to z_out, where act is not None; bias: whether the bias's
-    gradient is wanted.  dw in x's type, or fp32 with dw_dtype=torch.float32.  dz = dy act'(z) is rounded to x's type before
-    the products (dy alone too, where it is fp32).  workspace: scratch of moe_linear_grad_workspace_bytes.
+    gradient is wanted.  dw in x's type, or fp32 with dw_dtype=torch.float32.  dz = dy act'(z) (dy alone too, where it is fp32) goes
+    through the products in parts, with more bits than 16-bit results show, for an fp32 dw with all of its own.  workspace:
+    scratch of moe_linear_grad_workspace_bytes.
     """
     who = "linear_grad"
     dev = _one_gpu(who, "dy x w z workspace", dy, x, w, z, workspace)
