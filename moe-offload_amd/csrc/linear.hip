@@ -94,7 +94,7 @@ struct Product {
     int64_t ldp, ldq, ldo;       // elements from row to row of memory
     int np, nq, nc;              // extents: rows and columns of out, and the contraction
     int parts, part_c;           // the contraction in parts of part_c, each with sums of its own (fp32, [parts][np][nq]; not dx)
-    int terms;                   // gradients: P is the sum of so many images, one after another from p on,
+    int terms;                   // kParts, kHalves: P is the sum of so many images, one after another from p on,
     int64_t term_p;              // so many elements apart; the contraction goes over all of them
 };
 
@@ -219,7 +219,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     // P's images follow each other in the contraction, each as whole steps
     int term = 0;
     const int whole = (nc + kBC - 1) / kBC * kBC;
-    const uint32_t all_c = KIND == kForward ? nc : (uint32_t)a.terms * whole;
+    const uint32_t all_c = MODE == kWhole ? nc : (uint32_t)a.terms * whole;
     int p0, q0;
     tile_at<BP, BQ, C::PANEL>(a, item, p0, q0);
     const T* zero = (const T*)&g_zero16;
@@ -242,7 +242,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
         }
     };
     auto place = [&]() {
-        if constexpr (KIND != kForward) {
+        if constexpr (MODE != kWhole) {
             for (; load_c >= whole && term < a.terms; ++term) {
                 load_c -= whole;
                 P += a.term_p;
@@ -974,8 +974,8 @@ extern "C" int moe_linear_grad(const void* dy, int64_t lddy, int dy_f32, const v
     const BiasSums b = {sums, db, dz_blocks(n_tok, n_out), n_out};
     const Parts p = {(const float*)into, dw, (int64_t)n_out * n_in, parts, dw_f32};
     const DzArgs* need = dz || db ? &d : nullptr;
-    // (bf16's parts are values like any)
-    if (dtype) return gradients<__bf16, kWhole>(need, dy_f32, gw, dw_f32, gx, b, p, s);
+    if (dtype) return own_dz ? gradients<__bf16, kParts>(need, dy_f32, gw, dw_f32, gx, b, p, s)
+                             : gradients<__bf16, kWhole>(need, dy_f32, gw, dw_f32, gx, b, p, s);
     if (!own_dz) return gradients<_Float16, kWhole>(need, dy_f32, gw, dw_f32, gx, b, p, s);
     return halves ? gradients<_Float16, kHalves>(need, dy_f32, gw, dw_f32, gx, b, p, s)
                   : gradients<_Float16, kParts>(need, dy_f32, gw, dw_f32, gx, b, p, s);
