@@ -374,7 +374,8 @@ int moe_route_grad(const float* dweights, const void* logits, int64_t ld, const 
  * multiples of 8; n_tok * k up to 2^30. */
 int moe_combine(const void* y, int64_t ldy, const float* weights, const void* residual, int64_t ldr, int n_tok, int k, int hidden,
                 int dtype, int out_f32, void* out, int64_t ldo, void* stream);
-/* Its gradients: dy[t * k + j] = weights[t][j] * dout[t], dweights[t][j] = <dout[t], y[t * k + j]> (the residual's is dout). */
+/* Its gradients: dy[t * k + j] = weights[t][j] * dout[t], dweights[t][j] = <dout[t], y[t * k + j]> (the residual's is dout).  Of a
+ * weight of 0 dy is 0 whatever dout holds, and dweights is 0 where it would be infinite or NaN. */
 int moe_combine_grad(const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* weights, int n_tok, int k, int hidden,
                      int dtype, void* dy, int64_t lddy, float* dweights, void* stream);
 /* y = act(z) + residual, z = x W^T + bias: x [n_tok][n_in], W [n_out][n_in] contiguous, bias [n_out], residual [n_tok][n_out]

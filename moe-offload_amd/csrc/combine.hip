@@ -2,7 +2,8 @@
 //     out[t] = residual[t] + sum over j of w[t][j] y[t k + j]         (the residual may be absent)
 //     dy[t k + j] = w[t][j] dout[t],     dw[t][j] = <dout[t], y[t k + j]>
 // y, residual, dout and dy fp16 or bf16, out too or fp32, w and dw fp32; sums in fp32, in the order of j, one rounding at
-// the end.  A place of weight 0 adds nothing whatever its row holds.  moe_pair_combine (mlx-qwen38/loader.py:964-965) is
+// the end.  A place of weight 0 adds nothing whatever its row holds, and so do its gradients: dy is 0, and dw, which a
+// weight that happens to be 0 has too, is 0 where it would not be finite.  moe_pair_combine (mlx-qwen38/loader.py:964-965) is
 // the sum of fp16 rows by fp16 scores, of inference.
 #include <hip/hip_fp16.h>
 
@@ -91,17 +92,19 @@ __global__ __launch_bounds__(kCombineThreads) void k_combine_grad(CombineGradArg
     for (int64_t p = (int64_t)blockIdx.x * (kCombineThreads / 64) + (threadIdx.x >> 6); p < pairs; p += step) {
         const T* d = (const T*)a.dout + p / a.k * a.ldd;
         const float w = a.weights[p];
+        const bool none = w == 0.f;
         float dot = 0.f;
 #pragma unroll 2
         for (int u = lane; u < units; u += 64) {
             const f32x8 dv = widen8<T>(*(const uint4*)(d + u * 8));
             const f32x8 v = widen8<T>(*(const uint4*)((const T*)a.y + p * a.ldy + u * 8));
             typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, round8<T>(w * dv)), (u32x4*)((T*)a.dy + p * a.lddy + u * 8));
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, round8<T>(none ? (f32x8)(0.f) : w * dv)), (u32x4*)((T*)a.dy + p * a.lddy + u * 8));
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot += dv[e] * v[e];
         }
         dot = lanes::group_sum<64>(dot);
+        if (none && !(fabsf(dot) < __builtin_inff())) dot = 0.f;
         if (lane == 0) a.dweights[p] = dot;
     }
 }

@@ -746,7 +746,10 @@ def combine(y, weights, residual=None, dtype=None, out=None):
 
 
 def combine_grad(dout, y, weights):
-    """combine's gradients: dy, of y's shape and type, and fp32 dweights [n_tok, k] (the residual's is dout, of y's type)."""
+    """combine's gradients: dy, of y's shape and type, and fp32 dweights [n_tok, k] (the residual's is dout, of y's type).
+
+    Of a weight of 0 dy is 0 whatever dout holds, and dweights is 0 where it would be infinite or NaN.
+    """
     who = "combine_grad"
     dev = _one_gpu(who, "dout y weights", dout, y, weights)
     dt = _half(who, y)
