@@ -30,12 +30,16 @@ using namespace gmm;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu2 = 3 };
 
-// The normal distribution's integral up to -m, m >= 0, by Abramowitz and Stegun's 7.1.26 (Handbook of Mathematical Functions):
-// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most; here x = m / sqrt(2), and half of it.
+// The normal distribution's integral up to -m, m >= 0, times exp(m^2 / 2), as a polynomial in t = 1 / (1 + 0.27 m): fitted to its relative
+// error for m up to 20 (least squares over 4000 Chebyshev points, weighted anew until the largest was least), 2.4e-8 of the value;
+// in fp32, with the exponential, (m^2 / 2 + 4) steps of 2^-23 of it.
 __device__ __forceinline__ float normal_tail(float m) {
-    const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.70710678f) * m);
-    const float poly = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-    return poly * __builtin_amdgcn_exp2f(m * m * -0.72134752f);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.27f * m);
+    constexpr float c[] = {0.10772167f, 0.107526444f, 0.10192253f, 0.071631186f, 0.10876759f, -0.070522137f, 0.17089182f, -0.12700342f, 0.029064333f};
+    float poly = c[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) poly = c[i] + t * poly;
+    return t * poly * __builtin_amdgcn_exp2f(m * m * -0.72134752f);
 }
 
 // The activations, and their slopes.  Where exponentials have left fp32's range both are at their limits, taken from arguments
