@@ -218,7 +218,7 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
         item -= (uint32_t)part * tiles;
         P += part * a.part_c * (kAlongP ? a.ldp : 1);
         Q += part * a.part_c * (kAlongQ ? a.ldq : 1);
-        nc = (int)std::clamp<int64_t>(nc - part * a.part_c, 0, a.part_c);
+        nc = (int)std::min<int64_t>(nc - part * a.part_c, a.part_c);
     }
     // P's images follow each other in the contraction, each as whole steps
     int term = 0;
@@ -817,8 +817,9 @@ int best_tiles(const Product& a, const Product& b, bool split, const R& run) {
     return rc;
 }
 
-// The length of a part, whole steps.
-int part_of(int64_t nc, int parts) { return (int)((nc + (int64_t)parts * kBC - 1) / ((int64_t)parts * kBC) * kBC); }
+// The length of a part, whole steps, and the parts of up to so many that have something then.
+int part_of(int64_t nc, int64_t parts) { return (int)((nc + parts * kBC - 1) / (parts * kBC) * kBC); }
+int parts_of(int64_t nc, int64_t parts) { return parts < 2 || nc < 1 ? 1 : (int)((nc - 1) / part_of(nc, parts) + 1); }
 
 // Results few enough for k_linear_few.
 bool few_results(int n_tok, int n_out) { return n_tok <= 16 || ((int64_t)n_tok + 15) / 16 * (((int64_t)n_out + 15) / 16) <= 256; }
@@ -831,7 +832,7 @@ int forward_parts(int n_tok, int n_in, int n_out) {
     if (n_tok < 1 || few_results(n_tok, n_out)) return 1;
     const int64_t tiles = ((int64_t)n_tok + 63) / 64 * (((int64_t)n_out + 63) / 64), steps = (int64_t)n_in / kBC;
     const int64_t parts = std::min(256 / tiles, steps / 8);
-    return parts < 2 || steps * (parts - 1) < 30 * parts ? 1 : (int)parts;
+    return parts < 2 || steps * (parts - 1) < 30 * parts ? 1 : parts_of(n_in, parts);
 }
 
 template <typename T>
@@ -864,7 +865,7 @@ int forward(const Product& a, const Epilogue& e, void* workspace, hipStream_t s)
 // 16.0* 18 22, 4096 x 2048 x 512 32.2* 33.1 30.3 35 59.
 int dw_parts(int n_tok, int n_out, int n_in) {
     const int64_t tiles = ((int64_t)n_out + 63) / 64 * (((int64_t)n_in + 63) / 64), steps = (int64_t)n_tok / kBC;
-    return (int)std::max<int64_t>(1, std::min(256 / tiles, steps / 16));
+    return parts_of(n_tok, std::min(256 / tiles, steps / 16));
 }
 
 template <typename T, int MODE>
