@@ -306,9 +306,9 @@ template <int W>
 __device__ __forceinline__ double partner(double v) { return lanes::partner_f64<W>(v); }
 
 // With L = 2^group_shift, the values of group g are lanes g L .. g L + L - 1's to look through.  first: the largest of those in LDS,
-// and for group_best = 2 the second largest added, in all of its lanes.
+// and for group_best = 2 the second largest added, in all of its lanes.  size: the magnitudes of those that are finite.
 template <typename F>
-__device__ __forceinline__ F best_of_group(const RouteArgs& a, const F* lds, int lane) {
+__device__ __forceinline__ F best_of_group(const RouteArgs& a, const F* lds, int lane, F& size) {
     const int per = a.group_size, L = 1 << a.group_shift, g = lane >> a.group_shift;
     F first = -(F)kInf, second = first;
     auto least = [](F x, F y) { return x < y ? x : y; };
@@ -328,11 +328,15 @@ __device__ __forceinline__ F best_of_group(const RouteArgs& a, const F* lds, int
     if (L > 4) merge(partner<4>(first), partner<4>(second));
     if (L > 8) merge(partner<8>(first), partner<8>(second));
     for (int d = 16; d < L; d <<= 1) merge(__shfl_xor(first, d, 64), __shfl_xor(second, d, 64));
-    return a.group_best > 1 && second > -(F)kInf ? first + second : first;
+    const bool both = a.group_best > 1 && second > -(F)kInf;
+    const F f = first < 0 ? -first : first, s = second < 0 ? -second : second;
+    size = (f < (F)kInf ? f : 0) + (both && s < (F)kInf ? s : 0);
+    return both ? first + second : first;
 }
 
 // Experts of the groups that stay keep their keys.  value[i]: what the groups are compared by, -inf for experts that are never
-// chosen; err: a bound of its error, of a sum of two of them too.  Where that does not decide, the values in 64 bits do.
+// chosen; err: a bound of its score's error.  The group's own magnitudes bound the rounding of its sums: an expert that a bias of -1e9 keeps
+// out leaves the others' bounds alone.  Where that does not decide, the values in 64 bits do.
 template <int P>
 __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)[P], float top, const float (&value)[P], float err,
                                             bool exact, double* lds, int lane, uint32_t (&key)[P]) {
@@ -342,7 +346,8 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
 #pragma unroll
     for (int i = 0; i < P; ++i) lds32[Row<P>::at(lane, i)] = value[i];
     wave_lds_fence();
-    const float v = best_of_group(a, (const float*)lds32, lane);
+    float size;
+    const float v = best_of_group(a, (const float*)lds32, lane, size);
     wave_lds_fence();
     int before = 0;
     for (int h = 0; h < a.n_group; ++h) {
@@ -351,9 +356,9 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
     }
     bool stays = one && before < a.topk_group;
     if (!exact) {
-        const float least = -wave_max(stays ? -v : -kInf), most = wave_max(one && !stays ? v : -kInf);
-        const float room = 2 * err + (fabsf(least) + fabsf(most)) * 0x1p-21f;
-        if (most > -kInf && !(least - most > room)) {
+        const float off = (float)a.group_best * err + size * 0x1p-21f;
+        const float least = -wave_max(stays ? off - v : -kInf), most = wave_max(one && !stays ? v + off : -kInf);
+        if (most > -kInf && !(least > most)) {
             const double sum = a.sigmoid ? 0.0 : exact_sum<P>(l, top);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -364,7 +369,8 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)
                 __builtin_amdgcn_sched_barrier(0);
             }
             wave_lds_fence();
-            const double w = best_of_group(a, (const double*)lds, lane);
+            double none;
+            const double w = best_of_group(a, (const double*)lds, lane, none);
             wave_lds_fence();
             before = 0;
             for (int h = 0; h < a.n_group; ++h) {
@@ -421,7 +427,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
         sum = lanes::group_sum<64>(sum);
     }
     uint32_t key[P];
-    float s_top = 0.f, c_top = 0.f, s_err = 0.f;
+    float s_top = 0.f, s_err = 0.f;
     if constexpr (GENERAL) {
         float value[P];
         const float inv = 1.f / sum;
@@ -435,19 +441,15 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
                 s_top = fmaxf(s_top, in ? s : 0.f);
             }
             float c = l[i];
-            if (a.bias) {
-                c = in ? s + a.bias[e] : -kInf;
-                c_top = fmaxf(c_top, fabsf(c) < kInf ? fabsf(c) : 0.f);
-            }
+            if (a.bias) c = in ? s + a.bias[e] : -kInf;
             key[i] = order_key(c);
             value[i] = key[i] == 0 ? -kInf : a.bias || a.group_best == 1 ? c : s;
         }
         s_top = wave_max(s_top);
-        c_top = wave_max(c_top);
         // an exponential's argument x is rounded, which its value shows |x| times: at most 0.4 of what x exp(-x) can be (times 1 - s
-        // in a sigmoid); the sums and functions around it, of s itself
-        s_err = ((a.sigmoid ? 8.f : 24.f) * s_top + 0.4f) * 0x1p-22f + c_top * 0x1p-23f;
-        if (a.n_group > 1) keep_groups<P>(a, l, top, value, 2 * s_err, !a.bias && a.group_best == 1, lds, lane, key);
+        // in a sigmoid); the sums and functions around it, of s itself.  The sum with a bias adds half a step of its own.
+        s_err = ((a.sigmoid ? 8.f : 24.f) * s_top + 0.4f) * 0x1p-22f;
+        if (a.n_group > 1) keep_groups<P>(a, l, top, value, s_err, !a.bias && a.group_best == 1, lds, lane, key);
     } else {
 #pragma unroll
         for (int i = 0; i < P; ++i) key[i] = order_key(l[i]);
@@ -458,8 +460,10 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
     for (int i = 1; i < P; ++i) lane_max = key[i] > lane_max ? key[i] : lane_max;
     uint32_t from = not_above_kth(lane_max, a.k);
     if (GENERAL && a.bias && from > 1) {
-        // what may be above it in truth
-        const uint32_t lower = order_key(order_value(from) - 4 * s_err);
+        // what may be above it in truth: a value further below is also larger in magnitude, by no more than it is further, so the
+        // threshold's own magnitude bounds both roundings
+        const float at = order_value(from);
+        const uint32_t lower = fabsf(at) < kInf ? order_key(at - (4 * s_err + fabsf(at) * 0x1p-21f)) : from;
         from = lower ? lower : 1u;
     }
     uint32_t mine;
@@ -471,11 +475,13 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
         else c = in_rounds<P>(key, l, a.k, lane);
     } else if (GENERAL && a.bias) {
         const float v = order_value(mine);
+        // (the candidates' magnitudes: the others do not meet here)
+        const float off = 2 * (s_err + wave_max(c.has && fabsf(v) < kInf ? fabsf(v) : 0.f) * 0x1p-23f);
         int near = 0;                                                          // within both bounds of this lane's, itself among them
         for (int j = 0; j < c.n; ++j) {
             const float o = lane_value(v, j);
             c.place += o > v;
-            near += !(fabsf(o - v) > 2 * s_err);
+            near += !(fabsf(o - v) > off);
         }
         float b = 0.f;
         c.l = 0.f;
