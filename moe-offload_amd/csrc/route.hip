@@ -330,8 +330,13 @@ __device__ __forceinline__ F best_of_group(const RouteArgs& a, const F* lds, int
     for (int d = 16; d < L; d <<= 1) merge(__shfl_xor(first, d, 64), __shfl_xor(second, d, 64));
     const bool both = a.group_best > 1 && second > -(F)kInf;
     const F f = first < 0 ? -first : first, s = second < 0 ? -second : second;
-    size = (f < (F)kInf ? f : 0) + (both && s < (F)kInf ? s : 0);
-    return both ? first + second : first;
+    size = f < (F)kInf ? f : 0;
+    if (!both) return first;
+    if (!(f < (F)kInf && s < (F)kInf)) return first + second;
+    // the sum of two finite values is more than no value, and less than an infinite one, also where 32 bits do not hold it
+    const F limit = sizeof(F) == 4 ? (F)0x1.fffffep127f : (F)kInf;
+    size = least(f + s, limit);
+    return least(most(first + second, -limit), limit);
 }
 
 // Experts of the groups that stay keep their keys.  value[i]: what the groups are compared by, -inf for experts that are never

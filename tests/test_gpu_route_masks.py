@@ -53,3 +53,18 @@ def test_values_a_step_apart_beside_far_ones(score, n_exp, k, n_group, topk_grou
             compare(logits, k, score=score, bias=bias, n_group=n_group, topk_group=topk_group, group_best=group_best)
         bias = torch.where(torch.rand(n_exp, device=DEV, generator=g) < 0.5, -1e9, -1e9 - 64)
         compare(logits, k, score=score, bias=bias, n_group=n_group, topk_group=topk_group, group_best=group_best)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("large", [LOWEST, 3e38])
+def test_group_sums_past_fp32(score, large):
+    """Two values of a group whose sum fp32 does not hold: still more than a group that has none, and in the order of the 64-bit sums."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    logits = torch.randn((50, 32), device=DEV, generator=g)
+    bias = torch.zeros(32, device=DEV)
+    bias[:12] = -math.inf                              # groups 0 to 2 have nobody
+    bias[20:24], bias[24:28] = large, large * 0.9
+    for topk_group in (1, 2, 3, 4, 5, 6, 8):
+        for k in (4, 20):
+            compare(logits, k, score=score, bias=bias, n_group=8, topk_group=topk_group, group_best=2)
+            compare(logits, k, score=score, bias=-bias.clamp(min=-3e38), n_group=8, topk_group=topk_group, group_best=2)
