@@ -380,8 +380,8 @@ int moe_combine_grad(const void* dout, int64_t ldd, const void* y, int64_t ldy, 
                      int dtype, void* dy, int64_t lddy, float* dweights, void* stream);
 /* y = act(z) + residual, z = x W^T + bias: x [n_tok][n_in], W [n_out][n_in] contiguous, bias [n_out], residual [n_tok][n_out]
  * (either may be null) of fp16 or bf16 (dtype 0, 1), y of that type or fp32 (out_f32 != 0).  act: 0 none, 1 silu, 2 gelu (z
- * times the normal distribution's integral, within z^2 / 2 + 10 steps of 2^-23 of its value), 3 the squared relu.  z, where it is not null, receives the pre-activations in
- * the inputs' type.  y may be residual (of its type and step).  Matrices 16-byte aligned; n_in, n_out and steps multiples of 8.
+ * times the normal distribution's integral, within z^2 / 2 + 10 steps of 2^-23 of its value), 3 the squared relu.  z, where it is
+ * not null, receives the pre-activations in the inputs' type.  y may be residual (of its type and step).  Matrices 16-byte aligned; n_in, n_out and steps multiples of 8.
  * workspace: moe_linear_workspace_bytes bytes (0: may be null), 16-byte aligned, any contents, one per call in flight. */
 uint64_t moe_linear_workspace_bytes(int n_tok, int n_in, int n_out);
 int moe_linear(const void* x, int64_t ldx, const void* w, const void* bias, const void* residual, int64_t ldr, int n_tok, int n_in,

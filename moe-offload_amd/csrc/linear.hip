@@ -35,7 +35,8 @@ enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu2 = 3 };
 // in fp32, with the exponential, (m^2 / 2 + 4) steps of 2^-23 of it.
 __device__ __forceinline__ float normal_tail(float m) {
     const float t = __builtin_amdgcn_rcpf(1.f + 0.27f * m);
-    constexpr float c[] = {0.10772167f, 0.107526444f, 0.10192253f, 0.071631186f, 0.10876759f, -0.070522137f, 0.17089182f, -0.12700342f, 0.029064333f};
+    constexpr float c[] = {0.10772167f, 0.107526444f, 0.10192253f, 0.071631186f, 0.10876759f, -0.070522137f, 0.17089182f, -0.12700342f,
+                           0.029064333f};
     float poly = c[8];
 #pragma unroll
     for (int i = 7; i >= 0; --i) poly = c[i] + t * poly;
@@ -188,11 +189,11 @@ __device__ __forceinline__ void tile_at(const Product& a, uint32_t item, int& p0
     q0 = (int)(panel * PANEL + i % width) * BQ;
 }
 
-// What bounds it: full grids of large tiles the matrix unit and what feeds it (8192 x 4096 x 4096 bf16 in 256 x 256: 194-205 us, 1340-1420
+// What bounds it: full grids of large tiles the matrix unit and what feeds it (8192 x 4096 x 4096 bf16 in 256 x 256: 190-205 us, 1340-1450
 // TFLOP/s, 1.4 us a step and 8 at a tile's ends; the library's product 177-185), grids of one tile per CU the steps' latencies (4096 x 2048 x
-// 512 in 128 x 64: 14.1 us, 0.32 us a step; the library's 15).  In panels: 4096 x 4096 x 4096 in tiles of 64 205 us, 294 in lines, of 256
-// 105 and 113.  Tiles of 256 x 256 by four waves of 128 x 128, which read LDS less, took 106-121 for it: a wave alone on its SIMD
-// waits for every load that it issues.
+// 512 in 128 x 64: 12.5-14.3 us on one box and another, 0.3 us a step, the waves waiting for 48% of it, the matrix unit busy for 28%, LDS for
+// 30%; the library's 15).  In panels: 4096 x 4096 x 4096 in tiles of 64 205 us, 294 in lines, of 256 105 and 113.  Tiles of 256 x 256 by
+// four waves of 128 x 128, which read LDS less, took 106-121 for it: a wave alone on its SIMD waits for every load that it issues.
 //
 // One tile of BP x BQ results by WP x WQ waves, or SPLIT = 2 times as many that take turns at the steps.  A step of 64 contraction
 // indexes goes from global memory to LDS without passing registers, RING - 1 steps ahead of the one that is multiplied: with one
@@ -466,15 +467,16 @@ __device__ __forceinline__ void tile_product(const Product& a, const Epilogue& e
     }
 }
 
-// A tile's sides, its waves, how many share the steps, its ring, the blocks per CU that registers are kept for, the panel.
-template <int BP_, int BQ_, int WP_, int WQ_, int SPLIT_, int RING_, int BLOCKS_, int PANEL_>
+// A tile's sides, its waves, how many share the steps, its ring, the waves per SIMD that registers are kept for (of one block of eight
+// waves, as LDS holds no second, or of two blocks of four), the panel.
+template <int BP_, int BQ_, int WP_, int WQ_, int SPLIT_, int RING_, int PER_SIMD_, int PANEL_>
 struct Tiles {
-    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, SPLIT = SPLIT_, RING = RING_, BLOCKS = BLOCKS_, PANEL = PANEL_;
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, SPLIT = SPLIT_, RING = RING_, PER_SIMD = PER_SIMD_, PANEL = PANEL_;
     static constexpr int kThreads = 64 * WP * WQ * SPLIT, kLds = SPLIT * RING * (BP + BQ) * 128;
 };
 
 template <typename T, typename C>
-__global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear(Product a, Epilogue e) {
+__global__ __launch_bounds__(C::kThreads, C::PER_SIMD) void k_linear(Product a, Epilogue e) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
     tile_product<T, kForward, C>(a, e, xcd_order(blockIdx.x, gridDim.x), lds);
 }
@@ -528,7 +530,7 @@ __device__ __forceinline__ void sum_bias(const BiasSums& b, uint32_t item, float
 // All gradients behind dz in one launch: the tiles of dW (longer, as a rule) before those of dx, then the bias's.  A product of no
 // rows is not there.
 template <typename T, typename C, int MODE>
-__global__ __launch_bounds__(C::kThreads, C::BLOCKS) void k_linear_grads(Product dw, Product dx, BiasSums b, int dw_f32) {
+__global__ __launch_bounds__(C::kThreads, C::PER_SIMD) void k_linear_grads(Product dw, Product dx, BiasSums b, int dw_f32) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
     const uint32_t n_dw = (uint32_t)tiles_in<C::BP, C::BQ>(dw) * dw.parts, n_dx = (uint32_t)tiles_in<C::BP, C::BQ>(dx);
     const uint32_t i = blockIdx.x;
@@ -638,12 +640,12 @@ struct DzArgs {
     int rows;                    // of a block
 };
 
-// A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.  1999 x 640 fp16 through silu 4.2-6.6 us:
-// 7.7 MB, a load, an exponential and a store after one another.
+// A thread has 8 columns of every eighth row of its block; the rows' sums meet in LDS.  1999 x 640 fp16 through silu 6.4-7.0 us
+// (4.2-6.6 with one image): 10.2 MB, a load, an exponential and stores after one another.
 //
 // The images of kParts: a value's upper 16 bits, then those of what is left, the last one rounded; of kHalves: the rest of the rounding
-// below, then that.  All have the value's sign, and none is zero unless it is, or is below 2^-23 of kHalves (the smallest there
-// is stands for nothing): an infinity that they meet in a product stays one.
+// below, then that.  All have the value's sign, and none is zero (the smallest there is stands for nothing) unless the value is,
+// or is below the type's range, 2^-23 of kHalves: an infinity that they meet in a product stays one.
 __device__ __forceinline__ void dz_parts(float v, int parts, __bf16 (&p)[3]) {
     const bool fine = fabsf(v) < __builtin_inff();
     const uint32_t sign = __float_as_uint(v) & 1u << 31;
@@ -765,7 +767,8 @@ bool too_many(const char* who, int64_t blocks, int threads) {
 
 uint64_t round_up(uint64_t v) { return (v + 255) / 256 * 256; }
 
-// The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two, as measured.  us per forward product in
+// The tiles there are, with 0.01 us of a step where a CU has one of their blocks, and two (side by side those of four waves, one after the
+// other those of eight), as measured, of dz as it came.  us per forward product in
 // their order, chosen *: 1024 x 1024 x 1024 6.8* 7.0 8.4 9.2 10.5 12.3 15.4 20 26; 1030 x 72 x 1856 6.9 5.1* 7.5 6.1 6.2 8.1 8.5 10.5
 // 13; 4096 x 2048 x 512 17.6 15.1 14.0* 15.1 16.9 20 25 35 42; 2048 x 2048 x 2048 35 29 26.7 23.8 20.5* 26.5 27.5 36 42; 3000 x 2048 x 2048
 // 47 39 36 34 37 29 28.4* 36 42; 5000 x 4096 x 2056 158 131 131 110 95 101 101 75.6* 86; 4096 x 4096 x 4096 228 190 178 148 131 118 113 135
@@ -786,8 +789,8 @@ int each_tiles(const F& f) {
     return 0;
 }
 
-// Calls run(tiles) with those that are done first: with one product, as many steps as a CU's blocks have; with two, which fill
-// each other's gaps, the sum of all steps over the CUs, but at least those of the longest tile.
+// Calls run(tiles) with those that are done first: with one product, as many steps as a CU's blocks have; with two, whose blocks follow
+// each other as CUs get free, the sum of all steps over the CUs, but at least those of the longest tile.
 // split: fp16's values are taken apart on the way to the matrix unit, by every wave for its own columns: a step has WP BQ / 8 subtiles of
 // them for a CU's four vector units, of 36 operations each.
 template <bool FORWARD, typename R>

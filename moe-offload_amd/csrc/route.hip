@@ -26,8 +26,9 @@
 // rounds of a maximum over the wave find them (k rounds for all: 108 us for 16384 tokens of 512, 12 this way).
 //
 // The vector unit bounds it: 16384 tokens of 512 fp32 logits, top-10, 11.8 us (79% busy, some 310 operations per token; 35 MB at
-// 3 TB/s), of 1024 17.5, of 64 7.0, which is what so many waves take to come and go; top-32 of 512 18. 5001 tokens of 240 with a bias and
-// groups 10.5. Several tokens per wave, the next one's row read ahead, took 13.5 for the first: more registers, no fewer operations.
+// 3 TB/s), of 1024 17.5, of 64 7.0, which is what so many waves take to come and go; top-32 of 512 18; of 512 with a bias 20 (sigmoid) and
+// 24 (softmax), whatever its size. 5001 tokens of 240 with a bias and groups 10.5 (74% busy).
+// Several tokens per wave, the next one's row read ahead, took 13.5 for the first: more registers, no fewer operations.
 #include <hip/hip_fp16.h>
 
 #include "lane_reduce.h"
@@ -340,8 +341,8 @@ __device__ __forceinline__ F best_of_group(const RouteArgs& a, const F* lds, int
 }
 
 // Experts of the groups that stay keep their keys.  value[i]: what the groups are compared by, -inf for experts that are never
-// chosen; err: a bound of its score's error.  The group's own magnitudes bound the rounding of its sums: an expert that a bias of -1e9 keeps
-// out leaves the others' bounds alone.  Where that does not decide, the values in 64 bits do.
+// chosen; err: a bound of its score's error.  The group's own magnitudes bound the rounding of its sums: an expert that a bias of
+// -1e9 keeps out leaves the others' bounds alone.  Where that does not decide, the values in 64 bits do.
 template <int P>
 __device__ __forceinline__ void keep_groups(const RouteArgs& a, const float (&l)[P], float top, const float (&value)[P], float err,
                                             bool exact, double* lds, int lane, uint32_t (&key)[P]) {
@@ -427,6 +428,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
 #pragma unroll
         for (int i = 0; i < P; ++i) top = fmaxf(top, l[i]);
         top = wave_max(top);
+        // (__expf: 16384 x 512 13.0 us, weights 6.1e-8 of their norm from 64 bits; expf 14.9 and 5.2e-8)
 #pragma unroll
         for (int i = 0; i < P; ++i) sum += l[i] == top ? 1.f : l[i] > -kInf ? __expf(l[i] - top) : 0.f;
         sum = lanes::group_sum<64>(sum);
@@ -561,6 +563,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_grad(RouteGradArgs a) {
 #pragma unroll
         for (int i = 0; i < P; ++i) top = fmaxf(top, x[i]);
         top = wave_max(top);
+        // (__expf: 8192 x 512 9.5 us, 7.1e-8 of the norm from 64 bits; expf 10.4 and 6.5e-8)
 #pragma unroll
         for (int i = 0; i < P; ++i) sum += x[i] = x[i] == -kInf ? 0.f : x[i] == top ? 1.f : __expf(x[i] - top);
         sum = lanes::group_sum<64>(sum);

@@ -773,8 +773,8 @@ def linear(x, w, bias=None, act=None, residual=None, z_out=None, dtype=None, out
     """act(x @ w.T + bias) + residual: a projection that all tokens share (the router, a shared expert), in one launch.
 
     x: fp16 or bf16 [n_tok, n_in]; w: same type [n_out, n_in], contiguous; bias: same type [n_out] or None; act: None, "silu",
-    "gelu" (z times the normal distribution's integral, within z^2 / 2 + 10 steps of 2^-23 of its value) or "relu2" (the squared relu); residual: same type [n_tok, n_out] or None.
-    The result has the inputs' type, or fp32 with dtype=torch.float32 (router logits).  z_out, [n_tok, n_out] of the inputs'
+    "gelu" (z times the normal distribution's integral, within z^2 / 2 + 10 steps of 2^-23 of its value) or "relu2" (the squared
+    relu); residual: same type [n_tok, n_out] or None.  The result has the inputs' type, or fp32 with dtype=torch.float32 (router logits).  z_out, [n_tok, n_out] of the inputs'
     type, receives x @ w.T + bias for linear_grad.  out=residual adds in place.  workspace: scratch of
     moe_linear_workspace_bytes.
     """
