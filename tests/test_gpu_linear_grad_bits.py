@@ -163,3 +163,57 @@ def test_the_router_of_a_layer_gets_its_logits_gradient_whole():
     check(x.grad, want_dx, sx)
     check(w.grad, want_dw, sw)
     assert bool(w.grad.any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_images_past_32_bits(dtype):
+    """Images of dz of 2^30 elements and more, the rows that count at their end."""
+    from moe_offload import ops
+    n_tok, n_in, n_out = (1 << 20) + 24, 64, 1032
+    x, w = torch.zeros((n_tok, n_in), dtype=dtype, device=DEV), rnd((n_out, n_in), dtype, 1, n_out ** -0.5)
+    dy, z = torch.zeros((n_tok, n_out), dtype=dtype, device=DEV), torch.zeros((n_tok, n_out), dtype=dtype, device=DEV)
+    x[-40:], dy[-40:], z[-40:] = rnd((40, n_in), dtype, 2), rnd((40, n_out), dtype, 3), rnd((40, n_out), dtype, 4)
+    for dw_type, lose in ((None, lost(dtype, dtype, "silu")), (torch.float32, (THREE,))):
+        dx, dw, _ = ops.linear_grad(dy, x, w, z=z, act="silu", dw_dtype=dw_type)
+        want_dx = exact(dy[-40:], x[-40:], w, z[-40:], "silu", *(lose if dw_type is None else (TWO,)))[0]
+        check(dx[-40:], *want_dx, "dx")
+        check(dw, *exact(dy[-40:], x[-40:], w, z[-40:], "silu", *lose)[1], "dw")
+        assert not bool(dx[:-40].any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_replayed_and_side_by_side(dtype):
+    """Every form of dz in a graph, replayed with other inputs between eager calls, and on two streams at once."""
+    from moe_offload import ops
+    x, w = rnd((300, 136), dtype, 1), rnd((72, 136), dtype, 2)
+    z, dy, wide = rnd((300, 72), dtype, 3), rnd((300, 72), dtype, 4), rnd((300, 72), torch.float32, 5)
+    forms = [lambda: ops.linear_grad(dy, x, w, z=z, act="silu", bias=True), lambda: ops.linear_grad(dy, x, w, z=z, act="relu2"),
+             lambda: ops.linear_grad(wide, x, w, dw_dtype=torch.float32), lambda: ops.linear_grad(wide, x, w, z=z, act="gelu")]
+    graphs, held = [], []
+    for form in forms:
+        form()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(form())
+    for seed in (1, 2, 3):
+        dy.copy_(rnd(dy.shape, dtype, seed + 10))
+        wide.copy_(rnd(wide.shape, torch.float32, seed + 20))
+        for i in (0, 1, 2, 3, 3, 1, 2, 0):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for h, form in zip(held, forms):
+            assert all(torch.equal(a, b) for a, b in zip(h, form()) if a is not None)
+    want = [form() for form in forms]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append([form() for form in forms])
+    torch.cuda.synchronize()
+    for runs in got:
+        for run in runs:
+            for r, v in zip(run, want):
+                assert all(torch.equal(a, b) for a, b in zip(r, v) if a is not None)
